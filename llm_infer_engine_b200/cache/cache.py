@@ -7,6 +7,10 @@ ask for the same thing (KV heads, head sizes, window or chunk, kept first positi
     k, v          [units, pages + 1, kv_heads, page_size, head_dim]   keys are stored rotated
     block_table   [slots + 1, max_pages_per_seq] int32                logical page -> page
 
+With `kv_dtype` torch.float8_e4m3fn, k and v hold 8-bit codes and each 16 positions of a head have an exponent, int8
+`k_exp`, `v_exp` [units, pages + 1, kv_heads, page_size / 16]: a number is code * 2^exponent (csrc/fp8.cuh). Every mixer
+must have said that its kernels know such a cache (`KVRequest.eight_bit`).
+
 Pages hold `page_size` (64) consecutive positions of one sequence; a sequence holds only the
 pages it has reached, so memory follows the tokens held, not slots x longest length. A group
 with a window or chunks gives pages back once no later token can read them (the pages of the first
@@ -23,7 +27,7 @@ slot and one shared position (src/kv_cache.py:4-57).
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -31,6 +35,7 @@ import torch
 from .allocator import CacheError, FreeList, PageTableHost
 
 PAGE_SIZE = 64
+EXP_BLOCK = 16          # positions of a head that share an exponent in a cache in 8 bits
 
 
 @dataclass(frozen=True)
@@ -50,6 +55,8 @@ class KVRequest:
     # n > 0: the values ARE the first n columns of the key rows (a latent that serves as key and value at once);
     # no value storage is made, `v` is a view into `k`, and v_head_dim is n
     values_in_keys: int = 0
+    # the mixer's kernels can work with keys and values in 8 bits (says nothing about the storage's layout)
+    eight_bit: bool = field(default=False, compare=False)
 
     @property
     def value_dim(self) -> int:
@@ -86,6 +93,9 @@ class KVUnit:
     page_size: int
     window: int
     keep_first: int = 0
+    # a cache in 8 bits: the exponents of k and v, [pages + 1, kv_heads, page_size / 16] int8
+    k_exp: Optional[torch.Tensor] = None
+    v_exp: Optional[torch.Tensor] = None
 
 
 class CacheUnit:
@@ -119,17 +129,27 @@ class _KVGroup:
             self.v = self.k[..., :req.values_in_keys]
         else:
             self.v = torch.zeros(shape + (req.value_dim,), dtype=dtype, device=device)
+        self.k_exp = self.v_exp = None
+        if dtype == torch.float8_e4m3fn:
+            exps = shape[:3] + (PAGE_SIZE // EXP_BLOCK,)
+            self.k_exp = torch.zeros(exps, dtype=torch.int8, device=device)
+            self.v_exp = torch.zeros(exps, dtype=torch.int8, device=device)
         self.block_table = torch.full((n_slots + 1, max_pages_per_seq), n_pages, dtype=torch.int32, device=device)
 
     def bytes(self) -> int:
-        return (self.k.numel() + (0 if self.req.values_in_keys else self.v.numel())) * self.k.element_size()
+        held = (self.k.numel() + (0 if self.req.values_in_keys else self.v.numel())) * self.k.element_size()
+        return held + (0 if self.k_exp is None else self.k_exp.numel() + self.v_exp.numel())
 
 
 class Cache:
     def __init__(self, unit_requests: Sequence[Sequence[object]], n_slots: int, max_tokens: int,
-                 max_seq_len: int, dtype: torch.dtype, device):
+                 max_seq_len: int, dtype: torch.dtype, device, kv_dtype: Optional[torch.dtype] = None):
         """unit_requests[u] lists what unit u's mixer asked for. `max_tokens` is the number of
-        positions all live sequences may hold together, each rounded up to whole pages."""
+        positions all live sequences may hold together, each rounded up to whole pages. `kv_dtype`: what keys and
+        values are held in, `dtype` (the default) or torch.float8_e4m3fn."""
+        kv_dtype = dtype if kv_dtype is None else kv_dtype
+        if kv_dtype not in (dtype, torch.float8_e4m3fn):
+            raise ValueError(f"keys and values are held in {dtype} or float8_e4m3fn, not in {kv_dtype}")
         if n_slots <= 0 or max_tokens <= 0 or max_seq_len <= 0:
             raise ValueError("n_slots, max_tokens and max_seq_len must be positive")
         self.page_size = PAGE_SIZE
@@ -139,6 +159,7 @@ class Cache:
         self.max_seq_len = max_seq_len
         self.max_pages_per_seq = min(self.n_pages, (max_seq_len + PAGE_SIZE - 1) // PAGE_SIZE)
         self.dtype = dtype
+        self.kv_dtype = kv_dtype
         self.device = torch.device(device)
         self.slots = FreeList(n_slots, "slot")
         self.lengths: List[int] = [0] * (n_slots + 1)          # host mirror of seq_lens
@@ -159,6 +180,10 @@ class Cache:
                     raise ValueError(f"cache unit {u}: two {type(r).__name__}s are named {r.name!r}; give them "
                                      "different names")
                 names.add((type(r), r.name))
+                if isinstance(r, KVRequest) and kv_dtype == torch.float8_e4m3fn and (not r.eight_bit or r.values_in_keys
+                                                                                    or r.value_dim != r.head_dim or r.keep_first):
+                    raise ValueError(f"cache unit {u}: the keys and values of {r.name!r} cannot be held in 8 bits (its mixer's "
+                                     "kernels do not know such a cache)")
                 if isinstance(r, KVRequest):
                     by_geometry.setdefault(r.geometry(), []).append((u, r.name))
                     first_request.setdefault(r.geometry(), r)
@@ -166,7 +191,7 @@ class Cache:
                     state_specs.setdefault((r.name, tuple(r.shape), r.dtype), []).append(u)
         for geo, members in by_geometry.items():
             self._groups[geo] = _KVGroup(first_request[geo], members, self.n_pages, n_slots, self.max_pages_per_seq,
-                                         dtype, device)
+                                         kv_dtype, device)
         self._state: Dict[Tuple[str, Tuple[int, ...], torch.dtype], Tuple[List[int], torch.Tensor]] = {}
         for (name, shape, sdtype), units in state_specs.items():
             self._state[(name, shape, sdtype)] = (units, torch.zeros((len(units), n_slots + 1) + shape,
@@ -178,7 +203,8 @@ class Cache:
                 if isinstance(r, KVRequest):
                     g = self._groups[r.geometry()]
                     i = g.units.index((u, r.name))
-                    kvs[r.name] = KVUnit(g.k[i], g.v[i], g.block_table, PAGE_SIZE, r.window, r.keep_first if r.window else 0)
+                    kvs[r.name] = KVUnit(g.k[i], g.v[i], g.block_table, PAGE_SIZE, r.window, r.keep_first if r.window else 0,
+                                         None if g.k_exp is None else g.k_exp[i], None if g.v_exp is None else g.v_exp[i])
                 else:
                     units, store = self._state[(r.name, tuple(r.shape), r.dtype)]
                     state[r.name] = store[units.index(u)]

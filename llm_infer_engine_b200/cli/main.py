@@ -5,7 +5,8 @@ default (main.py:73-87), the same printed stages (main.py:243,297,457).
 Differences that follow from this library's design: model sizes come from config.json (found
 in --model, or in --tokenizer as the reference does, main.py:374); the size flags --dim,
 --n-layers, ... are read only in random-weights mode when there is no config.json;
---quantization is not offered; --dtype chooses the bfloat16 or the true float32 path;
+--quantization is not offered; --dtype chooses the bfloat16 or the true float32 path, --cache-dtype what keys and values
+are held in;
 --prompt-ids and --prompt-ids-file run without a tokenizer; --init-std sets the spread of random
 weights; stop ids come from config.json, generation_config.json and the tokenizer together.
 """
@@ -48,6 +49,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--max-batch", type=int, default=None, help="Sequences held at once")
     p.add_argument("--cuda-graph", type=str, default=None, choices=["on", "off"], help="CUDA Graph for decode")
     p.add_argument("--dtype", type=str, default=None, choices=["bfloat16", "float32"])
+    p.add_argument("--cache-dtype", type=str, default=None, choices=["auto", "float8_e4m3"],
+                   help="What keys and values are held in: the dtype (auto), or 8 bits a number")
     p.add_argument("--nvtx", action="store_true", help="Mark the stages of every step with NVTX ranges")
     return p
 
@@ -90,6 +93,7 @@ OPTIONS = {
     "n_kv_heads": ("LLM_N_KV_HEADS", None, int), "hidden_dim": ("LLM_HIDDEN_DIM", None, int),
     "vocab_size": ("LLM_VOCAB_SIZE", None, int), "max_seq_len": ("LLM_MAX_SEQ_LEN", 4096, int),
     "max_batch": ("LLM_MAX_BATCH", 1, int), "dtype": ("LLM_DTYPE", "bfloat16", str),
+    "cache_dtype": ("LLM_CACHE_DTYPE", "auto", str),
 }
 
 
@@ -233,7 +237,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     print("=" * 70)
     print(f"Device: cuda:{device}")
     print(f"CUDA Graph: {opts['cuda_graph']}")
-    print(f"Dtype: {opts['dtype']}")
+    print(f"Dtype: {opts['dtype']}" + ("" if opts["cache_dtype"] == "auto" else f", cache {opts['cache_dtype']}"))
     if opts["prompt"]:
         shown = opts["system_prompt"]
         print(f"System Prompt: {shown[:100] + '...' if len(shown) > 100 else shown}")
@@ -254,7 +258,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         parser.error(str(e))
     t0 = time.time()
     engine = Engine(folder, dtype=opts["dtype"], device=device, max_batch=opts["max_batch"],
-                    max_seq_len=opts["max_seq_len"], cuda_graph=opts["cuda_graph"] == "on", nvtx=args.nvtx)
+                    max_seq_len=opts["max_seq_len"], cuda_graph=opts["cuda_graph"] == "on", nvtx=args.nvtx,
+                    cache_dtype=opts["cache_dtype"])
     report = engine.model.load_report
     print(f"    Model: loaded={report['tensors']} tensors, {report['bytes'] / 1e9:.3f} GB in {time.time() - t0:.4f}s")
 

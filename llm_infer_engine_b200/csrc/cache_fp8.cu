@@ -1,0 +1,162 @@
+// Keys and values of a step go into a paged cache in 8 bits, with the position rotation on the way.
+//
+//   (y_i, y_{i + R/2}) = (x_i c_i - x_{i + R/2} s_i,  x_{i + R/2} c_i + x_i s_i)        i < R/2, R the rotated size
+//
+// for queries and keys, (c, s) the cosine and sine of the token's position from a float32 table; every product and every
+// sum is rounded once to float32 (no fused multiply-add: keys then have the same codes wherever they are made). Queries go
+// out in their own type; keys and values become codes of their block of 16 positions (fp8.cuh).
+//
+// A block of positions and a KV head is one thread block's work, with the query heads that belong to it: it knows all of
+// the block's new numbers, so the block's exponent needs no atomics and comes out the same in any order. A block that
+// already holds earlier positions keeps the larger of its own exponent and the new numbers'; if that raises it, the earlier
+// codes are rounded to it. Rows behind the sequence's last one are left as they are.
+#include "fp8.cuh"
+
+namespace llmie {
+
+constexpr int kStoreThreads = 128;
+
+struct StoreArgs {
+  unsigned char* k;                  // [pages, n_kv, 64, hd] codes
+  unsigned char* v;
+  signed char* k_exp;                // [pages, n_kv, 4]
+  signed char* v_exp;
+  const int* cu_q;
+  const int* seq_slot;
+  const int* seq_start;
+  const int* block_table;
+  int max_pages, n_q, n_kv, hd, rot_dim, table_len, write_kv;
+};
+
+// What a thread block works on: positions [p0, p1) of sequence `seq`, all in one block of 16.
+struct StoreBlock {
+  int p0, p1, tok0;                  // tok0: row of p0 in the packed step
+  int lead;                          // positions of the block that were there before
+  size_t row;                        // page * n_kv + head, the page that holds the block
+  int in_page;                       // row of the block's first position in its page
+};
+__device__ __forceinline__ bool store_block(const StoreArgs& a, int hk, StoreBlock& b) {
+  const int seq = blockIdx.z;
+  const int start = a.seq_start[seq], t0 = a.cu_q[seq], n_new = a.cu_q[seq + 1] - t0;
+  const int first = (start / kExpBlock + (int)blockIdx.x) * kExpBlock;
+  b.p0 = max(start, first);
+  b.p1 = min(start + n_new, first + kExpBlock);
+  if (b.p0 >= b.p1) return false;
+  b.tok0 = t0 + b.p0 - start;
+  b.lead = b.p0 - first;
+  b.in_page = first % kFp8Page;
+  b.row = 0;
+  if (a.write_kv) {
+    const int page = a.block_table[(size_t)a.seq_slot[seq] * a.max_pages + first / kFp8Page];
+    b.row = (size_t)page * a.n_kv + hk;
+  }
+  return true;
+}
+
+// The exponent of a block that holds `lead` earlier positions at `at`; raises it, and lowers the earlier codes, if need be.
+// All threads of the block call it; `need`: the bits of the new numbers' largest magnitude.
+__device__ __forceinline__ int settle_exponent(signed char* at, unsigned char* codes, int lead, int hd, unsigned need) {
+  int e = exponent_for(need);
+  if (lead > 0) {
+    const int before = clamp_exponent(*at);
+    e = max(e, before);
+    if (e > before) {
+      const float f = lower_factor(before, e);
+      for (int i = threadIdx.x; i < lead * hd / 4; i += kStoreThreads) {
+        unsigned* w = reinterpret_cast<unsigned*>(codes) + i;
+        *w = lower_codes(*w, f);
+      }
+    }
+  }
+  return e;
+}
+
+// Every size: any even rotation up to the head size (or none), one number at a time through shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kStoreThreads)
+rope_store_fp8_kernel(const T* qkv, T* __restrict__ q_out, const float2* LLMIE_WEIGHT table, const StoreArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ float staged[];  // [2][16][hd]: the block's new keys and values
+  __shared__ unsigned largest[2];
+  const int hk = blockIdx.y, G = a.n_q / a.n_kv, hd = a.hd, half = a.rot_dim >> 1;
+  StoreBlock b;
+  if (!store_block(a, hk, b)) return;
+  const int n = b.p1 - b.p0;
+  const size_t row_w = (size_t)(a.n_q + 2 * a.n_kv) * hd;
+  if (threadIdx.x < 2) largest[threadIdx.x] = 0u;
+  __syncthreads();
+  // rotated number i of the row x at position p
+  auto turned = [&](const T* x, int i, int p) {
+    if (!table || i >= a.rot_dim) return to_f32(x[i]);
+    const float2 c = table[(size_t)min(p, a.table_len - 1) * half + (i < half ? i : i - half)];
+    const float x1 = to_f32(x[i < half ? i : i - half]), x2 = to_f32(x[i < half ? i + half : i]);
+    return i < half ? __fsub_rn(__fmul_rn(x1, c.x), __fmul_rn(x2, c.y)) : __fadd_rn(__fmul_rn(x2, c.x), __fmul_rn(x1, c.y));
+  };
+  for (int it = threadIdx.x; it < n * G * hd; it += kStoreThreads) {
+    const int i = it % hd, g = it / hd % G, r = it / hd / G;
+    const size_t col = (size_t)(hk * G + g) * hd;
+    q_out[(size_t)(b.tok0 + r) * a.n_q * hd + col + i] = from_f32<T>(turned(qkv + (b.tok0 + r) * row_w + col, i, b.p0 + r));
+  }
+  if (!a.write_kv) return;
+  for (int which = 0; which < 2; ++which) {
+    unsigned big = 0u;
+    for (int it = threadIdx.x; it < n * hd; it += kStoreThreads) {
+      const int i = it % hd, r = it / hd;
+      const T* x = qkv + (b.tok0 + r) * row_w + (size_t)(a.n_q + which * a.n_kv + hk) * hd;
+      const float y = which ? to_f32(x[i]) : turned(x, i, b.p0 + r);
+      staged[which * kExpBlock * hd + it] = y;
+      big = max(big, finite_magnitude(y));
+    }
+    atomicMax(&largest[which], big);
+  }
+  __syncthreads();
+  for (int which = 0; which < 2; ++which) {
+    signed char* at = (which ? a.v_exp : a.k_exp) + b.row * kPageExps + b.in_page / kExpBlock;
+    unsigned char* codes = (which ? a.v : a.k) + (b.row * kFp8Page + b.in_page) * hd;
+    const int e = settle_exponent(at, codes, b.lead, hd, largest[which]);
+    const float f = pow2_of(-e);
+    unsigned short* dst = reinterpret_cast<unsigned short*>(codes + (size_t)b.lead * hd);
+    const float* src = staged + which * kExpBlock * hd;
+    for (int it = threadIdx.x; it < n * hd / 2; it += kStoreThreads) dst[it] = to_e4m3x2(src[2 * it] * f, src[2 * it + 1] * f);
+    __syncthreads();                 // everyone has read the old exponent
+    if (threadIdx.x == 0) *at = (signed char)e;
+  }
+}
+
+template <typename T>
+static int launch_store(const void* qkv, void* q_out, const float2* table, const StoreArgs& a, int blocks, int n_seqs,
+                        cudaStream_t stream) {
+  const size_t smem = (size_t)2 * kExpBlock * a.hd * sizeof(float);
+  launch_k(rope_store_fp8_kernel<T>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), smem, stream, (const T*)qkv, (T*)q_out,
+           table, a);
+  LLMIE_LAUNCH_CHECK();
+  return LLMIE_OK;
+}
+
+}  // namespace llmie
+
+using namespace llmie;
+
+// qkv [T, (n_q + 2 n_kv) hd], q_out [T, n_q hd] of one type; caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv,
+// 4]; table float32 [table_len, rot_dim / 2, 2] or null (no rotation). cu_q [n_seqs + 1], seq_slot, seq_start [n_seqs]:
+// sequence i brings rows cu_q[i] .. cu_q[i + 1] - 1, at positions from seq_start[i] on. max_q_len: the most that one brings.
+extern "C" int llmie_rope_store_fp8(const void* qkv, void* q_out, void* k_cache, void* v_cache, void* k_exp, void* v_exp,
+                                    const float* table, const int* cu_q, const int* seq_slot, const int* seq_start,
+                                    const int* block_table, int max_pages, int n_seqs, int max_q_len, int n_q, int n_kv,
+                                    int hd, int rot_dim, int table_len, int write_kv, int dtype, cudaStream_t stream) {
+  if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0) return LLMIE_ERR_BAD_ARG;
+  if (hd < 16 || hd > 256 || hd % 16) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  if (table && (rot_dim <= 0 || rot_dim % 2 || rot_dim > hd || table_len <= 0)) return LLMIE_ERR_BAD_ARG;
+  if (write_kv && (!aligned16(k_cache) || !aligned16(v_cache))) return LLMIE_ERR_ALIGNMENT;
+  if (table && (reinterpret_cast<uintptr_t>(table) & 7u)) return LLMIE_ERR_ALIGNMENT;
+  if (n_seqs == 0 || max_q_len <= 0) return LLMIE_OK;
+  if (n_seqs > 65535 || n_kv > 65535) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  const StoreArgs a{(unsigned char*)k_cache, (unsigned char*)v_cache, (signed char*)k_exp, (signed char*)v_exp, cu_q, seq_slot,
+                    seq_start, block_table, max_pages, n_q, n_kv, hd, table ? rot_dim : 0, table_len, write_kv ? 1 : 0};
+  // a run of L positions lies in at most (L + 14) / 16 + 1 blocks of 16
+  const int blocks = (max_q_len + kExpBlock - 2) / kExpBlock + 1;
+  if (dtype == LLMIE_F32) return launch_store<float>(qkv, q_out, (const float2*)table, a, blocks, n_seqs, stream);
+  if (dtype == LLMIE_BF16) return launch_store<__nv_bfloat16>(qkv, q_out, (const float2*)table, a, blocks, n_seqs, stream);
+  return LLMIE_ERR_DTYPE;
+}

@@ -64,6 +64,14 @@ class StepContext:
         plan = self.kernels
         if plan is not None and plan.attention(self, q, kv, out, n_q, n_kv, head_dim, options, gate):
             return
+        if kv.k_exp is not None:
+            if not options.plain:
+                raise ops.KernelError("attention over a cache in 8 bits knows a scale, a window and chunks, no other option")
+            ops.attention_paged_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, self.tok_pos, self.tok_seq, self.seq_slot,
+                                    kv.block_table, n_q, n_kv, head_dim, options.scale, options.reach)
+            if gate is not None:
+                ops.sigmoid_gate(out, gate)
+            return
         ops.attention_paged(q, kv.k, kv.v, out, self.tok_pos, self.tok_seq, self.seq_slot, kv.block_table,
                             kv.page_size, n_q, n_kv, head_dim, options.scale, options.reach, options.keep_first,
                             options.sink, gate, options.softcap, options.distance_bias, options.sink_values,

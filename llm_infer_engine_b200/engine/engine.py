@@ -21,7 +21,7 @@ from typing import Dict, List, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from ..cache.cache import Cache
+from ..cache.cache import EXP_BLOCK, Cache
 from ..kernels import ops, trace
 from ..weights.loader import build_model
 from .context import StepContext
@@ -44,6 +44,15 @@ def resolve_dtype(dtype: Union[str, torch.dtype]) -> torch.dtype:
     if dtype not in _DTYPES:
         raise EngineError(f"dtype {dtype!r} is not supported (bfloat16, float32)")
     return _DTYPES[dtype]
+
+
+def resolve_cache_dtype(cache_dtype: Union[str, torch.dtype], dtype: torch.dtype) -> torch.dtype:
+    """What keys and values are held in: the engine's own dtype ("auto", or its name) or float8_e4m3."""
+    if cache_dtype in ("auto", None) or cache_dtype is dtype or _DTYPES.get(cache_dtype) is dtype:
+        return dtype
+    if cache_dtype in ("float8_e4m3", "float8_e4m3fn", "fp8", torch.float8_e4m3fn):
+        return torch.float8_e4m3fn
+    raise EngineError(f"cache_dtype {cache_dtype!r} is not supported (auto, float8_e4m3)")
 
 
 def _round_up(x: int, m: int) -> int:
@@ -75,14 +84,17 @@ def _flatten_tokens(tokens, lens) -> np.ndarray:
 class Engine:
     def __init__(self, model_dir: str, dtype: Union[str, torch.dtype] = "bfloat16", device: Union[str, int] = 0,
                  max_batch: int = 8, max_seq_len: Optional[int] = None, max_tokens: Optional[int] = None,
-                 cuda_graph: bool = True, nvtx: bool = False, decode_attention: str = "auto"):
+                 cuda_graph: bool = True, nvtx: bool = False, decode_attention: str = "auto",
+                 cache_dtype: Union[str, torch.dtype] = "auto"):
         """max_batch: sequences held at once (slots). max_seq_len: longest sequence; the upper bound is the
         model's max_position_embeddings, the default is that bound but at most DEFAULT_MAX_SEQ_LEN (4096, the
         reference's default, main.py:40): a real checkpoint allows 131,072 positions, and a cache sized for
         that by default would take tens of gigabytes. max_tokens: positions all live sequences may hold
         together, in whole pages of 64 (default: max_batch * max_seq_len). nvtx: mark the stages of every
         step with NVTX ranges under the reference's names. decode_attention: "auto", or "split" to keep
-        the CUDA-core split-KV kernel for every one-token step (for comparisons)."""
+        the CUDA-core split-KV kernel for every one-token step (for comparisons). cache_dtype: what keys and values
+        are held in, "auto" (the engine's dtype) or "float8_e4m3": 8 bits a number and an exponent for each 16
+        positions of a head, half the memory and half the reads of bfloat16 (models of plain grouped-query attention)."""
         if not torch.cuda.is_available():
             raise EngineError("no CUDA device: this library runs on a GPU only (there is no CPU path)")
         self.device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
@@ -93,6 +105,7 @@ class Engine:
         if decode_attention not in ("auto", "split"):
             raise EngineError(f"decode_attention must be 'auto' or 'split', got {decode_attention!r}")
         self.decode_attention = decode_attention
+        self.cache_dtype = resolve_cache_dtype(cache_dtype, self.dtype)
         if nvtx:
             trace.enable_ranges(True)
         self.model, self.config = build_model(model_dir, self.dtype, self.device,
@@ -102,8 +115,13 @@ class Engine:
         page = 64
         if max_tokens is None:
             max_tokens = self.max_batch * _round_up(self.max_seq_len, page)
-        self.cache = Cache(self.model.unit_requests, self.max_batch, int(max_tokens), self.max_seq_len, self.dtype,
-                           self.device)
+        try:
+            self.cache = Cache(self.model.unit_requests, self.max_batch, int(max_tokens), self.max_seq_len, self.dtype,
+                               self.device, self.cache_dtype)
+        except ValueError as exc:
+            if self.cache_dtype == self.dtype:
+                raise
+            raise EngineError(f"cache_dtype {cache_dtype!r}: {exc}") from None
         self.vocab_size = self.model.vocab_size
         self.use_cuda_graph = bool(cuda_graph)
         from .plan import KernelPlan
@@ -298,13 +316,15 @@ class Engine:
 
     def kv_bytes_per_token(self) -> int:
         """Cache bytes one position of one sequence occupies, over all units."""
-        esize = 2 if self.dtype == torch.bfloat16 else 4
-        total = 0
+        eight = self.cache_dtype == torch.float8_e4m3fn
+        esize = 1 if eight else 2 if self.dtype == torch.bfloat16 else 4
+        total = exps = 0
         for reqs in self.model.unit_requests:
             for r in reqs:
                 if hasattr(r, "n_kv_heads"):
                     total += r.stored_per_position * esize
-        return total
+                    exps += 2 * r.n_kv_heads if eight else 0
+        return total + (exps + EXP_BLOCK - 1) // EXP_BLOCK
 
 
 BUCKETS = (1, 2, 4, 8, 16, 32, 64, 128, 256)

@@ -43,6 +43,14 @@ class KernelPlan:
         size exists. Returns False (and does nothing) otherwise; the caller then rotates and stores first."""
         if not write_kv:
             return False       # a borrowed cache already holds the owner's new key: it must be read, not replaced
+        if kv.k_exp is not None:
+            # the same over a cache in 8 bits (where query heads do not need two passes over a key/value head)
+            if not (ctx.decode and table is not None and options.plain
+                    and ops.attention_decode_fp8_rope_supported(n_q, n_kv, head_dim, qkv.dtype)):
+                return False
+            ops.attention_decode_fp8_rope(qkv, kv.k, kv.v, kv.k_exp, kv.v_exp, out, table, ctx.seq_slot, ctx.seq_kvlen,
+                                          kv.block_table, n_q, n_kv, head_dim, options.scale, options.reach, ctx.max_kv_len)
+            return True
         if not (ctx.decode and self.decode_attention != "split" and qkv.dtype == torch.bfloat16
                 and table is not None and ops.attention_decode_mma_supported(head_dim, qkv.dtype, kv.page_size)):
             return False
@@ -59,6 +67,8 @@ class KernelPlan:
         every option (scale, window, kept first keys, sink, gate); the CUDA-core split-KV kernel knows scale and
         window. A value head size that differs from the key head size is the plain kernel's alone."""
         scale, window = options.scale, options.reach
+        if kv.k_exp is not None:
+            return self._attention_fp8(ctx, q, kv, out, n_q, n_kv, head_dim, options, gate)
         if options.sigmoid_bias is not None:
             return self._sigmoid_attention(ctx, q, kv, out, n_q, n_kv, head_dim, options, gate)
         if kv.v.shape[-1] != head_dim or not kv.v.is_contiguous():
@@ -112,6 +122,24 @@ class KernelPlan:
             # head sizes that none of the kernels above takes
             return self._attention_by_rows(ctx, q, kv, out, n_q, n_kv, head_dim, options, gate)
         return False
+
+    def _attention_fp8(self, ctx, q, kv, out, n_q, n_kv, head_dim, options, gate) -> bool:
+        """A cache in 8 bits: bfloat16 with head size 64 or 128 has kernels of its own for one-token steps and for prompts;
+        other sizes and float32 are the plain kernel's."""
+        if not options.plain or not ops.attention_decode_fp8_supported(head_dim, q.dtype):
+            return False
+        if ctx.decode:
+            ops.attention_decode_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, ctx.seq_slot, ctx.seq_kvlen, kv.block_table, n_q,
+                                     n_kv, head_dim, options.scale, options.reach, ctx.max_kv_len)
+        elif options.scale > 0:
+            ops.attention_prefill_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, ctx.cu_q, ctx.seq_slot, ctx.seq_start,
+                                      kv.block_table, ctx.n_seqs, ctx.max_q_len, n_q, n_kv, head_dim, options.scale,
+                                      options.reach)
+        else:
+            return False
+        if gate is not None:
+            ops.sigmoid_gate(out, gate)
+        return True
 
     def _sigmoid_attention(self, ctx, q, kv, out, n_q, n_kv, head_dim, options, gate) -> bool:
         """Attention without a softmax (weights sigmoid(score + a number per head), not normalised). Prompts of the

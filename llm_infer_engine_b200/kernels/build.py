@@ -45,6 +45,9 @@ FAMILIES: Dict[str, tuple] = {
     "attention_decode_mma": ("attention_decode_mma.cu", [], []),
     "attention_prefill_tc": ("attention_prefill_tc.cu", [], []),
     "attention_latent_tc": ("attention_latent_tc.cu", [], []),
+    "cache_fp8": ("cache_fp8.cu", [], []),
+    "attention_fp8": ("attention_fp8.cu", [], []),
+    "attention_decode_fp8": ("attention_decode_fp8.cu", [], []),
     "attention_rows_mma": ("attention_rows_mma.cu", [], []),
     "gemm_simt": ("gemm_simt.cu", [], []),
     "gemm_f32_tc": ("gemm_f32_tc.cu", [], []),

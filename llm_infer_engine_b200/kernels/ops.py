@@ -1627,6 +1627,192 @@ def latent_prepare(proj, q_off: int, dkv_off: int, q_out, cache, norm_w, eps: fl
 
 
 # ------------------------------------------------------------------------------------------ attention by rows
+# ------------------------------------------------------------------------------------------ a cache in 8 bits
+FP8 = torch.float8_e4m3fn
+FP8_PAGE = 64            # positions of a page
+FP8_BLOCK = 16           # positions that share an exponent
+
+
+def _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv: int, head_dim: int) -> None:
+    """The checks of a cache in 8 bits: codes [pages, n_kv, 64, head_dim] float8_e4m3fn, exponents [pages, n_kv, 4] int8."""
+    _need(k_cache, "k_cache", FP8, (None, n_kv, FP8_PAGE, head_dim))
+    _need(v_cache, "v_cache", FP8, tuple(k_cache.shape))
+    _need(k_exp, "k_exp", torch.int8, (k_cache.shape[0], n_kv, FP8_PAGE // FP8_BLOCK))
+    _need(v_exp, "v_exp", torch.int8, tuple(k_exp.shape))
+
+
+def _need_heads(name: str, n_q: int, n_kv: int) -> None:
+    if n_q <= 0 or n_kv <= 0 or n_q % n_kv:
+        raise KernelError(f"{name}: {n_q} query heads are no multiple of {n_kv} key/value heads")
+
+
+def _need_arrays(name: str, n: int, device, **arrays) -> None:
+    """int32 arrays of at least n entries each (two-dimensional ones of any size), on the call's device."""
+    for what, t in arrays.items():
+        _need(t, what, torch.int32)
+        if t.device != device:
+            raise KernelError(f"{name}: {what} is on {t.device}, the call on {device}")
+        if t.dim() == 1 and t.numel() < n:
+            raise KernelError(f"{name}: {what} has {t.numel()} entries, {n} are needed")
+        if t.dim() > 2 or (t.dim() == 2 and what != "block_table"):
+            raise KernelError(f"{name}: {what} has {t.dim()} dimensions")
+    if "block_table" in arrays and (arrays["block_table"].dim() != 2 or arrays["block_table"].shape[1] < 1):
+        raise KernelError(f"{name}: block_table must be [slots, pages of a sequence]")
+
+
+def _need_here(name: str, *tensors) -> None:
+    """All tensors on one device, and that the current one: launches go to the current device's current stream."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise KernelError(f"{name}: tensors on {device} and on {t.device}")
+    if device.index != torch.cuda.current_device():
+        raise KernelError(f"{name}: the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_slot, seq_start, block_table, n_seqs: int,
+                   max_q_len: int, n_q: int, n_kv: int, head_dim: int, rot_dim: int, write_kv: bool = True):
+    """Rotates q and k by position and writes k, v into a paged cache in 8 bits (rope_store for such a cache).
+
+    qkv [T, (n_q + 2 n_kv) hd] and q_out [T, n_q hd] float32 or bfloat16; caches float8_e4m3fn [pages, n_kv, 64, hd] with
+    exponents int8 [pages, n_kv, 4]: each 16 positions of a head are held as code * 2^exponent, with the smallest exponent
+    that keeps the codes within 448 (csrc/fp8.cuh). table float32 [max_pos, rot_dim / 2, 2] of (cos, sin), or None for no
+    rotation. Sequence i (of n_seqs) brings rows cu_q[i] .. cu_q[i + 1] - 1, at positions from seq_start[i] on, none more than
+    max_q_len. A slot may appear once. Where a block already holds earlier positions its exponent only rises, and their codes
+    are rounded to it. head_dim: a multiple of 16 up to 256. With write_kv False only the queries are rotated."""
+    T = qkv.shape[0]
+    _need_heads("rope_store_fp8", n_q, n_kv)
+    _need(qkv, "qkv", None, (T, (n_q + 2 * n_kv) * head_dim))
+    _need(q_out, "q_out", qkv.dtype, (T, n_q * head_dim))
+    _need_arrays("rope_store_fp8", n_seqs, qkv.device, cu_q=cu_q, seq_slot=seq_slot, seq_start=seq_start, block_table=block_table)
+    if cu_q.numel() < n_seqs + 1:
+        raise KernelError(f"rope_store_fp8: cu_q has {cu_q.numel()} entries, {n_seqs + 1} are needed")
+    if n_seqs < 0 or (T > 0 and max_q_len <= 0):
+        raise KernelError(f"rope_store_fp8: {n_seqs} sequences with at most {max_q_len} new tokens each")
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise KernelError(f"rope_store_fp8: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
+    table_len = 0
+    if table is not None:
+        if rot_dim <= 0 or rot_dim % 2 or rot_dim > head_dim:
+            raise KernelError(f"rope_store_fp8: {rot_dim} of {head_dim} columns cannot be rotated")
+        _need(table, "table", torch.float32, (None, rot_dim // 2, 2))
+        table_len = table.shape[0]
+        if table_len < 1:
+            raise KernelError("rope_store_fp8: the table of angles is empty")
+    if write_kv:
+        _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _need_here("rope_store_fp8", qkv, q_out, table, *((k_cache, v_cache, k_exp, v_exp) if write_kv else ()))
+    _work(_nbytes(qkv, q_out) + (2 * T * n_kv * head_dim if write_kv else 0))
+    f = _fn("cache_fp8", "llmie_rope_store_fp8", [_c_void_p] * 11 + [_c_int] * 10 + [_c_void_p])
+    _check(f(qkv.data_ptr(), q_out.data_ptr(), _ptr(k_cache) if write_kv else None, _ptr(v_cache) if write_kv else None,
+             _ptr(k_exp) if write_kv else None, _ptr(v_exp) if write_kv else None, _ptr(table), cu_q.data_ptr(),
+             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], int(n_seqs),
+             int(max_q_len), n_q, n_kv, head_dim, int(rot_dim), table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()),
+           "rope_store_fp8")
+    return q_out
+
+
+def attention_paged_fp8(q, k_cache, v_cache, k_exp, v_exp, out, tok_pos, tok_seq, seq_slot, block_table, n_q: int, n_kv: int,
+                        head_dim: int, scale: float, window: int = 0):
+    """Plain attention over a paged cache in 8 bits, one warp per (token, query head): q, out [T, n_q hd] float32 or bfloat16,
+    the cache as in rope_store_fp8, the rest as in attention_paged. Every head size that is a multiple of 16 up to 256."""
+    T = q.shape[0]
+    _need_heads("attention_paged_fp8", n_q, n_kv)
+    _need(q, "q", None, (T, n_q * head_dim))
+    _need(out, "out", q.dtype, (T, n_q * head_dim))
+    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _need_arrays("attention_paged_fp8", 0, q.device, tok_pos=tok_pos, tok_seq=tok_seq, seq_slot=seq_slot, block_table=block_table)
+    if tok_pos.numel() < T or tok_seq.numel() < T:
+        raise KernelError("attention_paged_fp8: tok_pos / tok_seq shorter than the token count")
+    if head_dim % 16 or not 16 <= head_dim <= 256:
+        raise KernelError(f"attention_paged_fp8: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
+    _need_here("attention_paged_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
+    _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_fp8", "llmie_attention_paged_fp8", [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p])
+    _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
+             tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, n_q,
+             n_kv, head_dim, float(scale), int(window), _dt(q, "q"), _stream()), "attention_paged_fp8")
+    return out
+
+
+def attention_decode_fp8_supported(head_dim: int, dtype: torch.dtype) -> bool:
+    """The sizes attention_decode_fp8.cu is instantiated for (answered without loading the library)."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128)
+
+
+def attention_decode_fp8_rope_supported(n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> bool:
+    """Whether attention_decode_fp8_rope takes a step."""
+    return attention_decode_fp8_supported(head_dim, dtype)
+
+
+_fp8_scratch_floats = {}
+
+
+def _decode_fp8_scratch(n_q: int, n_kv: int, head_dim: int, device) -> torch.Tensor:
+    key = (n_q, n_kv, head_dim)
+    floats = _fp8_scratch_floats.get(key)
+    if floats is None:
+        f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_scratch", [_c_int] * 3, query=True)
+        floats = _fp8_scratch_floats[key] = int(f(n_q, n_kv, head_dim))
+    return torch.empty(floats, dtype=torch.float32, device=device)
+
+
+def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_kvlen, block_table, n_q: int, n_kv: int,
+                         head_dim: int, scale: float, window: int = 0, max_kv_len: int = 0):
+    """Attention for a one-token step over a paged cache in 8 bits, on the tensor cores: q, out bfloat16 [n, n_q hd], the cache
+    as in rope_store_fp8 (it holds the step's keys and values already), seq_kvlen int32 [n] the keys each sequence holds (0:
+    its rows of out become zeros), window as in attention_paged. head_dim 64 or 128. max_kv_len: no sequence is longer (0: not
+    known; nothing but launch sizes depends on it)."""
+    n = q.shape[0]
+    _need_heads("attention_decode_fp8", n_q, n_kv)
+    if not attention_decode_fp8_supported(head_dim, q.dtype):
+        raise KernelError(f"attention_decode_fp8: head_dim {head_dim}, {q.dtype} is not supported (bfloat16, 64 or 128)")
+    _need(q, "q", torch.bfloat16, (n, n_q * head_dim))
+    _need(out, "out", torch.bfloat16, (n, n_q * head_dim))
+    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _need_arrays("attention_decode_fp8", n, q.device, seq_slot=seq_slot, seq_kvlen=seq_kvlen, block_table=block_table)
+    _need_here("attention_decode_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
+    scratch = _decode_fp8_scratch(n_q, n_kv, head_dim, q.device)
+    _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8", [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_void_p])
+    _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
+             scratch.data_ptr(), seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), block_table.shape[1], n, n_q,
+             n_kv, head_dim, float(scale), int(window), _stream()), "attention_decode_fp8")
+    return out
+
+
+def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, seq_slot, seq_kvlen, block_table, n_q: int,
+                              n_kv: int, head_dim: int, scale: float, window: int = 0, max_kv_len: int = 0):
+    """What a one-token step does with its projections over a cache in 8 bits: qkv bfloat16 [n, (n_q + 2 n_kv) hd], rotated by
+    table (float32 [max_pos, hd / 2, 2], the whole head), the new key and value written for position seq_kvlen[i] - 1 as
+    rope_store_fp8 does it, and attention_decode_fp8 over the cache with them."""
+    n = qkv.shape[0]
+    _need_heads("attention_decode_fp8_rope", n_q, n_kv)
+    if not attention_decode_fp8_supported(head_dim, qkv.dtype):
+        raise KernelError(f"attention_decode_fp8_rope: head_dim {head_dim}, {qkv.dtype} is not supported (bfloat16, 64 or 128)")
+    q = torch.empty((n, n_q * head_dim), dtype=qkv.dtype, device=qkv.device)
+    cu = torch.arange(n + 1, dtype=torch.int32, device=qkv.device)
+    rope_store_fp8(qkv, q, k_cache, v_cache, k_exp, v_exp, table, cu, seq_slot, seq_kvlen[:n] - 1, block_table, n, 1, n_q, n_kv,
+                   head_dim, head_dim)
+    return attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_kvlen, block_table, n_q, n_kv, head_dim,
+                                scale, window, max_kv_len)
+
+
+def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot, seq_start, block_table, n_seqs: int,
+                          max_q_len: int, n_q: int, n_kv: int, head_dim: int, scale: float, window: int = 0):
+    """Causal attention of runs of new tokens over a paged cache in 8 bits: q, out [T, n_q hd] with the sequences packed (cu_q),
+    seq_start the tokens each held before."""
+    _need_heads("attention_prefill_fp8", n_q, n_kv)
+    if not attention_decode_fp8_supported(head_dim, q.dtype):
+        raise KernelError(f"attention_prefill_fp8: head_dim {head_dim}, {q.dtype} is not supported (bfloat16, 64 or 128)")
+    _need(q, "q", torch.bfloat16, (None, n_q * head_dim))
+    lens = (cu_q[1:n_seqs + 1] - cu_q[:n_seqs]).long()
+    tok_seq = torch.repeat_interleave(torch.arange(n_seqs, dtype=torch.int32, device=q.device), lens)
+    tok_pos = (torch.arange(q.shape[0], dtype=torch.int32, device=q.device) + (seq_start[:n_seqs] - cu_q[:n_seqs])[tok_seq.long()])
+    return attention_paged_fp8(q, k_cache, v_cache, k_exp, v_exp, out, tok_pos, tok_seq, seq_slot, block_table, n_q, n_kv,
+                               head_dim, scale, window)
+
+
 def attention_rows_mma_supported(head_dim: int, v_head_dim: int, page_size: int, dtype: torch.dtype,
                                  shared_rows: bool) -> bool:
     """The sizes attention_rows_mma.cu takes (answered without loading the library): bfloat16, a head size that is a

@@ -61,6 +61,12 @@ def yarn_frequencies(dims: int, base: float, factor: float, original: float, fas
     return f / factor * ramp + f * (1.0 - ramp), 0.1 * math.log(factor) + 1.0
 
 
+def _store_fp8(qkv, q, ctx, kv, table, n_q, n_kv, head_dim, rot_dim, write_kv):
+    """encode_and_store for a cache in 8 bits: the whole step's tokens, block by block of 16 positions."""
+    return ops.rope_store_fp8(qkv, q, kv.k, kv.v, kv.k_exp, kv.v_exp, table, ctx.cu_q, ctx.seq_slot, ctx.seq_start,
+                              kv.block_table, ctx.n_seqs, ctx.max_q_len, n_q, n_kv, head_dim, rot_dim, write_kv)
+
+
 class RotaryEncoding(PositionEncoding):
     """params: rot_dim (how many leading elements of a head are rotated), theta, scaling
     (None or {"rope_type": "llama3", factor, low_freq_factor, high_freq_factor,
@@ -96,6 +102,8 @@ class RotaryEncoding(PositionEncoding):
         """`v_head_dim`: the size of a value head where it differs from head_dim (the packed row then ends with
         n_kv * v_head_dim value columns)."""
         q = torch.empty((qkv.shape[0], n_q * head_dim), dtype=qkv.dtype, device=qkv.device)
+        if kv is not None and kv.k_exp is not None:
+            return _store_fp8(qkv, q, ctx, kv, self.table, n_q, n_kv, head_dim, self.rot_dim, write_kv)
         ops.rope_store(qkv, q, kv.k if kv is not None else None, kv.v if kv is not None else None, self.table,
                        ctx.tok_pos, ctx.tok_seq, ctx.seq_slot, kv.block_table, kv.page_size, n_q, n_kv, head_dim,
                        self.rot_dim, write_kv, v_head_dim=v_head_dim)
@@ -107,6 +115,8 @@ class NoEncoding(PositionEncoding):
 
     def encode_and_store(self, qkv, ctx, kv, n_q, n_kv, head_dim, write_kv):
         q = torch.empty((qkv.shape[0], n_q * head_dim), dtype=qkv.dtype, device=qkv.device)
+        if kv.k_exp is not None:
+            return _store_fp8(qkv, q, ctx, kv, None, n_q, n_kv, head_dim, 0, write_kv)
         ops.rope_store(qkv, q, kv.k, kv.v, None, ctx.tok_pos, ctx.tok_seq, ctx.seq_slot, kv.block_table,
                        kv.page_size, n_q, n_kv, head_dim, 0, write_kv)
         return q

@@ -1,0 +1,346 @@
+"""The kernels of a cache in 8 bits against tests/fp8_cache.py: what an append leaves, bit for bit, and attention against
+64-bit arithmetic over what the cache holds.
+
+Bounds on attention. The kernels read exact numbers (codes, exponents, bfloat16 queries); what they round is the weights
+(the tensor-core kernels: half precision, 2^-11 relative), the exponentials (2^-21 relative, and an argument of up to 2^7 in
+units of log2 that carries 2^-24 of itself, 2^-17), sums over up to 2^11 keys in float32 (2^-24 a step, 2^-13 together at
+worst) and the output (bfloat16: 2^-8; float32: 2^-24). So |error| <= half step of the output + w sum_j p_j |v_j| with
+w = 2^-11 + 2^-12 for the tensor cores and 2^-12 for float32 arithmetic: `allowed`."""
+import math
+
+import pytest
+import torch
+
+import fp8_cache
+from fp8_cache import F8, PlainCache
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def ops():
+    from llm_infer_engine_b200.kernels import ops as o
+    return o
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def angles(n, rot, seed=0):
+    if rot == 0:
+        return None
+    a = torch.outer(torch.arange(n).double(), 10000.0 ** (-torch.arange(0, rot, 2).double() / rot))
+    return torch.stack([torch.cos(a), torch.sin(a)], -1).float().contiguous()
+
+
+def allowed(want, size, dtype, tensor_cores):
+    half = torch.finfo(dtype).eps / 2
+    return half * want.abs() + (2.0 ** -11 + 2.0 ** -12 if tensor_cores else 2.0 ** -12) * size + 1e-30
+
+
+def same_bits(a, b):
+    return torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def store(pc, qkv, table, starts, news, n_q, n_kv, hd, rot, write_kv=True, cache=None):
+    """One call for sequences that bring news[i] tokens behind starts[i]; returns the rotated queries and the device cache."""
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    cache = pc.dev() if cache is None else cache
+    q = torch.empty(cu[-1], n_q * hd, dtype=qkv.dtype, device=DEV)
+    ops().rope_store_fp8(qkv.to(DEV), q, *cache, None if table is None else table.to(DEV), i32(cu), i32(pc.slots), i32(starts),
+                         pc.table.to(DEV), len(news), max(news), n_q, n_kv, hd, rot, write_kv)
+    return q, cache
+
+
+def plain_store(pc, qkv, table, starts, news, n_q, n_kv, hd, rot):
+    row, queries = 0, []
+    for i, (st, m) in enumerate(zip(starts, news)):
+        x = qkv[row:row + m].float().view(m, n_q + 2 * n_kv, hd)
+        t = table[st:st + m] if table is not None else None
+        turned = fp8_cache.rotate(x[:, :n_q + n_kv], t, rot)
+        queries.append(turned[:, :n_q].reshape(m, n_q * hd).to(qkv.dtype))
+        if m:
+            pc.append(i, st, turned[:, n_q:], x[:, n_q + n_kv:])
+        row += m
+    return torch.cat(queries)
+
+
+def check_cache(pc, cache, what=""):
+    k, v, ke, ve = (t.cpu() for t in cache)
+    assert torch.equal(ke, pc.ke) and torch.equal(ve, pc.ve), what
+    assert same_bits(k, pc.k), (what, int((k.view(torch.uint8) != pc.k.view(torch.uint8)).sum()))
+    assert same_bits(v, pc.v), what
+
+
+# ------------------------------------------------------------------------------------------ append
+LAYOUTS = [(4, 2, 16, 16), (3, 1, 32, 20), (6, 2, 48, 48), (8, 8, 64, 64), (4, 4, 64, 0), (5, 5, 80, 80), (4, 1, 96, 32),
+           (16, 2, 128, 128), (20, 1, 128, 128), (2, 1, 256, 256)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n_q,n_kv,hd,rot", LAYOUTS)
+def test_append_bit_for_bit(dtype, n_q, n_kv, hd, rot):
+    """Runs that begin and end inside blocks, at block and page borders, of one token and of several pages; one sequence brings
+    nothing. Queries, codes and exponents are what the plain form gives; every other byte of the pages is as it was."""
+    starts, news = [0, 3, 16, 70, 63, 15, 5, 128], [1, 13, 16, 9, 130, 1, 0, 33]
+    pc = PlainCache([s + m for s, m in zip(starts, news)], n_kv, hd, seed=hd + n_q, nan_stale=True)
+    for i, st in enumerate(starts):                    # what earlier steps left: finite
+        if st:
+            g = torch.Generator().manual_seed(i)
+            pc.append(i, 0, torch.randn(st, n_kv, hd, generator=g), 0.1 * torch.randn(st, n_kv, hd, generator=g))
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(sum(news), (n_q + 2 * n_kv) * hd, generator=g)
+    qkv *= torch.exp(2 * torch.randn(sum(news), 1, generator=g))       # some tokens raise their block's exponent, some do not
+    qkv = qkv.to(dtype)
+    table = angles(256, rot)
+    q, cache = store(pc, qkv, table, starts, news, n_q, n_kv, hd, rot)
+    want = plain_store(pc, qkv, table, starts, news, n_q, n_kv, hd, rot)
+    assert torch.equal(q.cpu(), want)
+    check_cache(pc, cache)
+    # a step that is run again leaves what it left
+    q2, cache = store(pc, qkv, table, starts, news, n_q, n_kv, hd, rot, cache=cache)
+    assert torch.equal(q2, q)
+    check_cache(pc, cache, "again")
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 2, 64), (4, 2, 128), (2, 1, 32)])
+def test_append_holds_numbers_to_half_a_step(n_q, n_kv, hd):
+    """|held - x| <= 2^-4 |x|, or half the smallest step of the block (2^-10 2^e) where x is small for its block. One call."""
+    n = 77
+    pc = PlainCache([n], n_kv, hd, seed=1)
+    g = torch.Generator().manual_seed(2)
+    qkv = (torch.randn(n, (n_q + 2 * n_kv) * hd, generator=g) * torch.exp(3 * torch.randn(n, 1, generator=g))).to(BF)
+    _, cache = store(pc, qkv, angles(128, hd), [0], [n], n_q, n_kv, hd, hd)
+    pc.k, pc.v, pc.ke, pc.ve = (t.cpu() for t in cache)
+    x = qkv.double().view(n, n_q + 2 * n_kv, hd)
+    t = angles(128, hd)[:n].double()
+    a, b = x[..., :hd // 2], x[..., hd // 2:]
+    c, s = t[:, None, :, 0], t[:, None, :, 1]
+    turned = torch.cat([a * c - b * s, b * c + a * s], -1)[:, n_q:n_q + n_kv]
+    for got, want, exps in zip(pc.held(0, n), (turned, x[:, n_q + n_kv:]), (pc.ke, pc.ve)):
+        at = torch.arange(n)
+        e = exps[pc.table[pc.slots[0]].long()[at // 64], :, at % 64 // 16].double()[..., None]
+        # rotation in float32: three roundings of numbers up to sqrt(2) max(|a|, |b|)
+        slack = 2.0 ** -22 * want.abs().amax(-1, keepdim=True) * 2
+        assert bool(((got - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * 2.0 ** e + slack).all())
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_append_in_pieces(hd):
+    """The same tokens one by one, in pieces and at once: the same exponents, and numbers that differ at most by the second
+    rounding of codes that were small for their block (half a smallest step)."""
+    n_q, n_kv, n = 2, 2, 75
+    g = torch.Generator().manual_seed(3)
+    qkv = (torch.randn(n, (n_q + 2 * n_kv) * hd, generator=g) * torch.exp(2 * torch.randn(n, 1, generator=g))).to(BF)
+    table = angles(128, hd)
+    got = []
+    for cuts in ([n], [1] * n, [5, 1, 30, 12, 27]):
+        pc = PlainCache([n], n_kv, hd, seed=4)
+        cache, at = pc.dev(), 0
+        for m in cuts:
+            _, cache = store(pc, qkv[at:at + m], table, [at], [m], n_q, n_kv, hd, hd, cache=cache)
+            at += m
+        pc.k, pc.v, pc.ke, pc.ve = (t.cpu() for t in cache)
+        got.append((pc.held(0, n), pc))
+    rows = torch.arange(n)
+    for (k, v), pc in got[1:]:
+        pages = pc.table[pc.slots[0]].long()
+        for a, b, ea, eb in ((k, got[0][0][0], pc.ke, got[0][1].ke), (v, got[0][0][1], pc.ve, got[0][1].ve)):
+            ea, eb = ea[pages[rows // 64], :, rows % 64 // 16], eb[pages[rows // 64], :, rows % 64 // 16]
+            assert torch.equal(ea, eb)
+            assert bool(((a - b).abs() <= 2.0 ** -9 * 2.0 ** eb.double()[..., None]).all())
+            assert float((a != b).double().mean()) < 0.02
+
+
+@pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_append_of_extreme_numbers(hd, dtype):
+    """Zeros, the smallest and largest numbers of the type, and numbers that are not finite, each in a block of its own and next
+    to ordinary ones; then a token that raises a block's exponent by more than its codes' range."""
+    n_q, n_kv, n = 1, 1, 96
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(n, 3 * hd, generator=g)
+    x[0:16] = 0.0
+    x[16:32] = torch.finfo(dtype).tiny / 4
+    x[32:48, ::3] = torch.finfo(dtype).max
+    x[48:64, 5::hd] = math.inf
+    x[50, 6::hd] = math.nan
+    x[64:80] *= 1e-25
+    x = x.to(dtype)
+    pc = PlainCache([n + 8], n_kv, hd, seed=4)
+    q, cache = store(pc, x, None, [0], [n], n_q, n_kv, hd, 0)
+    plain_store(pc, x, None, [0], [n], n_q, n_kv, hd, 0)
+    check_cache(pc, cache)
+    for start, size in ((90, 1e30), (91, 1e-30)):      # as if the sequence had been cut there
+        y = (torch.randn(2, 3 * hd, generator=g) * size).to(dtype)
+        _, cache = store(pc, y, None, [start], [2], n_q, n_kv, hd, 0, cache=cache)
+        plain_store(pc, y, None, [start], [2], n_q, n_kv, hd, 0)
+        check_cache(pc, cache, size)
+
+
+def test_append_without_writing_rotates_the_queries_alone():
+    n_q, n_kv, hd = 4, 2, 64
+    pc = PlainCache([40], n_kv, hd, seed=1)
+    qkv = torch.randn(9, (n_q + 2 * n_kv) * hd).to(BF)
+    before = [t.clone() for t in pc.dev()]
+    q, cache = store(pc, qkv, angles(64, hd), [31], [9], n_q, n_kv, hd, hd, write_kv=False)
+    for a, b in zip(before, cache):
+        assert same_bits(a, b)
+    want = fp8_cache.rotate(qkv.float().view(9, -1, hd)[:, :n_q], angles(64, hd)[31:40], hd)
+    assert torch.equal(q.cpu(), want.reshape(9, -1).to(BF))
+
+
+@pytest.mark.parametrize("hd", [32, 64])
+def test_append_from_rows_that_start_anywhere(hd):
+    """A step's projections that do not start on 16 bytes."""
+    n_q, n_kv, n = 2, 1, 21
+    pc = PlainCache([n], n_kv, hd, seed=1)
+    flat = torch.randn(n * (n_q + 2 * n_kv) * hd + 1).to(BF).to(DEV)
+    qkv = flat[1:].view(n, -1)
+    q, cache = store(pc, qkv, angles(64, hd), [0], [n], n_q, n_kv, hd, hd)
+    want = plain_store(pc, qkv.cpu(), angles(64, hd), [0], [n], n_q, n_kv, hd, hd)
+    assert torch.equal(q.cpu(), want)
+    check_cache(pc, cache)
+
+
+# ------------------------------------------------------------------------------------------ attention
+def filled(lens, n_kv, hd, seed, nan_stale=True, spread=1.0):
+    """A cache whose sequences hold lens[i] positions; every other row holds what former owners left, NaN among it."""
+    pc = PlainCache(lens, n_kv, hd, seed=seed, nan_stale=nan_stale)
+    g = torch.Generator().manual_seed(seed)
+    for i, l in enumerate(lens):
+        if l:
+            size = torch.exp(spread * torch.randn((l + 15) // 16, 1, 1, generator=g)).repeat_interleave(16, 0)[:l]
+            pc.append(i, 0, torch.randn(l, n_kv, hd, generator=g) * size, torch.randn(l, n_kv, hd, generator=g) * size)
+    return pc
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 2, 16), (3, 1, 48), (8, 8, 64), (6, 2, 80), (4, 1, 128), (2, 1, 256)])
+def test_plain_attention(dtype, n_q, n_kv, hd):
+    starts, news = [0, 70, 3, 150], [33, 9, 1, 64]
+    lens = [s + m for s, m in zip(starts, news)]
+    pc = filled(lens, n_kv, hd, seed=hd)
+    q = torch.randn(sum(news), n_q * hd, generator=torch.Generator().manual_seed(1)).to(dtype)
+    tok_seq = [i for i, m in enumerate(news) for _ in range(m)]
+    tok_pos = [s + j for s, m in zip(starts, news) for j in range(m)]
+    for window in (0, 20, -32):
+        out = torch.full((sum(news), n_q * hd), math.nan, dtype=dtype, device=DEV)
+        ops().attention_paged_fp8(q.to(DEV), *pc.dev(), out, i32(tok_pos), i32(tok_seq), i32(pc.slots), pc.table.to(DEV), n_q,
+                                  n_kv, hd, hd ** -0.5, window)
+        row = 0
+        for i, m in enumerate(news):
+            k, v = pc.held(i, lens[i])
+            want, size = fp8_cache.attention(q[row:row + m].double().view(m, n_q, hd), k, v, tok_pos[row:row + m], hd ** -0.5, window)
+            err = (out[row:row + m].cpu().double().view(m, n_q, hd) - want).abs()
+            assert bool((err <= allowed(want, size, dtype, False)).all()), (window, i, float((err / allowed(want, size, dtype, False)).max()))
+            row += m
+
+
+DECODE_LENS = [1, 15, 16, 17, 0, 63, 64, 65, 300, 777, 1024]
+
+
+@pytest.mark.parametrize("window", [0, 40, 1000, -64])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 4, 64), (12, 4, 64), (8, 1, 64), (13, 1, 64), (32, 8, 128), (40, 8, 128), (16, 1, 128),
+                                         (20, 1, 128), (20, 1, 64)])
+def test_decode(n_q, n_kv, hd, window):
+    """Lengths around blocks and pages, a sequence that holds nothing, groups of 1 to 20 query heads."""
+    pc = filled(DECODE_LENS, n_kv, hd, seed=hd + n_q)
+    n = len(DECODE_LENS)
+    q = torch.randn(n, n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = torch.full((n, n_q * hd), math.nan, dtype=BF, device=DEV)
+    ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32(DECODE_LENS), pc.table.to(DEV), n_q, n_kv, hd,
+                               hd ** -0.5, window, 1024)
+    for i, l in enumerate(DECODE_LENS):
+        if l == 0:
+            assert bool((out[i] == 0).all())
+            continue
+        want, size = fp8_cache.attention(q[i:i + 1].double().view(1, n_q, hd), *pc.held(i, l), [l - 1], hd ** -0.5, window)
+        err = (out[i].cpu().double().view(1, n_q, hd) - want).abs()
+        assert bool((err <= allowed(want, size, BF, True)).all()), (l, float((err / allowed(want, size, BF, True)).max()))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("case", ["large keys", "small queries", "large queries", "values apart", "zero values", "negative scale"])
+def test_decode_far_ranges(hd, case):
+    """Scores, queries and values far from 1: the sum over the values is in half precision inside, the ranges are not."""
+    n_q, n_kv, lens = 8, 2, [200, 333]
+    g = torch.Generator().manual_seed(3)
+    pc = PlainCache(lens, n_kv, hd, seed=5)
+    q = torch.randn(2, n_q * hd, generator=g)
+    scale = hd ** -0.5
+    k_size = v_size = None
+    if case == "large keys":
+        k_size, scale = 1e18, 1e-18 * hd ** -0.5
+    elif case == "small queries":
+        q, scale = q * 1e-20, 1e20 * hd ** -0.5
+    elif case == "large queries":
+        q, scale = q * 1e20, 1e-20 * hd ** -0.5
+    elif case == "negative scale":
+        scale = -scale
+    for i, l in enumerate(lens):
+        k, v = torch.randn(l, n_kv, hd, generator=g), torch.randn(l, n_kv, hd, generator=g)
+        if k_size:
+            k = k * k_size
+        if case == "values apart":                     # blocks of values from 1e-12 to 1e12
+            v = v * (10.0 ** torch.linspace(-12, 12, (l + 15) // 16).repeat_interleave(16)[:l, None, None])
+        if case == "zero values":
+            v[16:l - 20] = 0.0
+        pc.append(i, 0, k, v)
+    q = q.to(BF)
+    out = torch.empty(2, n_q * hd, dtype=BF, device=DEV)
+    ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, scale, 0, 333)
+    for i, l in enumerate(lens):
+        want, size = fp8_cache.attention(q[i:i + 1].double().view(1, n_q, hd), *pc.held(i, l), [l - 1], scale, 0)
+        err = (out[i].cpu().double().view(1, n_q, hd) - want).abs()
+        assert bool((err <= allowed(want, size, BF, True)).all()), float((err / allowed(want, size, BF, True)).max())
+
+
+def test_decode_numbers_that_are_not_finite_stay_with_the_rows_that_see_them():
+    """A key or value that is NaN, a query head that is: NaN where they are seen, nothing elsewhere."""
+    n_q, n_kv, hd, lens = 8, 2, 64, [100, 100, 100, 100]
+    pc = filled(lens, n_kv, hd, seed=8)
+    g = torch.Generator().manual_seed(8)
+    k, v = torch.randn(1, n_kv, hd, generator=g), torch.randn(1, n_kv, hd, generator=g)
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[0, 1, 3], bad_v[0, 1, 5] = math.inf, math.nan
+    pc.append(0, 50, bad_k, v)                         # sequence 0: a key of KV head 1 is not finite
+    pc.append(1, 50, k, bad_v)                         # sequence 1: one column of a value of KV head 1
+    q = torch.randn(4, n_q * hd, generator=g).to(BF)
+    q[2, 3 * hd + 1] = math.inf                        # sequence 2: query head 3
+    out = torch.empty(4, n_q * hd, dtype=BF, device=DEV)
+    for window, seen in ((0, True), (40, False)):
+        ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, 0.125,
+                                   window, 100)
+        bad = torch.isnan(out.cpu()).view(4, n_q, hd)
+        want = torch.zeros_like(bad)
+        if seen:
+            want[0, 4:] = True
+            want[1, 4:, 5] = True
+        want[2, 3] = True
+        assert torch.equal(bad, want), window
+
+
+def test_decode_of_one_long_sequence_among_short_ones():
+    """A sequence that is cut into many shares, beside ones of a block: a needle far back must come through."""
+    n_q, n_kv, hd = 8, 2, 128
+    lens = [5, 20000, 1, 40]
+    pc = filled(lens, n_kv, hd, seed=2, spread=0.3)
+    q = torch.randn(4, n_q * hd, generator=torch.Generator().manual_seed(2)).to(BF)
+    needle = q[1].float().view(n_q, hd)[::n_q // n_kv]
+    needle = needle * (24.0 / ((needle * needle).sum(-1, keepdim=True) * hd ** -0.5))
+    pc.append(1, 1234, needle[None], torch.full((1, n_kv, hd), 5.0))
+    out = torch.empty(4, n_q * hd, dtype=BF, device=DEV)
+    for max_len in (20000, 0):
+        ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd,
+                                   hd ** -0.5, 0, max_len)
+        for i, l in enumerate(lens):
+            want, size = fp8_cache.attention(q[i:i + 1].double().view(1, n_q, hd), *pc.held(i, l), [l - 1], hd ** -0.5, 0)
+            err = (out[i].cpu().double().view(1, n_q, hd) - want).abs()
+            # 20,000 keys: eight times the keys that `allowed` counts float32 sums for
+            assert bool((err <= allowed(want, size, BF, True) + 2.0 ** -10 * size).all()), l
+        assert float(out[1].float().view(n_q, hd)[::n_q // n_kv].mean()) > 4.0
