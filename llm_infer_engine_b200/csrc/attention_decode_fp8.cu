@@ -78,12 +78,13 @@ struct DecodeArgs {
 };
 
 // Blocks of 16 positions that a sequence's newest token sees: [first, first + count).
-__device__ __forceinline__ void df_units(int len, int window, int& first, int& count) {
+__device__ __forceinline__ void df_units(const DecodeArgs& a, int len, int& first, int& count) {
+  len = min(len, a.max_pages * kFp8Page);              // what the table has room for
   if (len <= 0) {
     first = count = 0;
     return;
   }
-  first = first_visible_key(len - 1, window) / kExpBlock;
+  first = first_visible_key(len - 1, a.window) / kExpBlock;
   count = (len - 1) / kExpBlock - first + 1;
 }
 
@@ -93,7 +94,7 @@ __device__ __forceinline__ long long df_total(const DecodeArgs& a) {
   long long t = 0;
   for (int s = lane; s < a.n_seqs; s += 32) {
     int f, c;
-    df_units(a.seq_kvlen[s], a.window, f, c);
+    df_units(a, a.seq_kvlen[s], f, c);
     t += c;
   }
 #pragma unroll
@@ -159,7 +160,7 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a) {
     long long before = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
       int f, c = 0;
-      if (s0 + lane < a.n_seqs) df_units(a.seq_kvlen[s0 + lane], a.window, f, c);
+      if (s0 + lane < a.n_seqs) df_units(a, a.seq_kvlen[s0 + lane], f, c);
       long long incl = (long long)c * per_seq;
       const long long own = incl;
 #pragma unroll
@@ -179,8 +180,8 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a) {
   }
 
   while (cur < end) {
-    const int len = a.seq_kvlen[seq];
-    df_units(len, a.window, first, count);
+    const int len = min(a.seq_kvlen[seq], a.max_pages * kFp8Page);
+    df_units(a, len, first, count);
     if (count == 0) {
       ++seq;
       continue;
@@ -435,12 +436,12 @@ __global__ void __launch_bounds__(HD) decode_fp8_join_kernel(const DecodeArgs a,
   if (h >= min(Cfg::kHeads, G - g0)) return;
   const int lane = threadIdx.x & 31;
   int first, count;
-  df_units(a.seq_kvlen[seq], a.window, first, count);
+  df_units(a, a.seq_kvlen[seq], first, count);
   if (count == 0) return;
   long long all = 0, ahead = 0;
   for (int s = lane; s < a.n_seqs; s += 32) {
     int f, c;
-    df_units(a.seq_kvlen[s], a.window, f, c);
+    df_units(a, a.seq_kvlen[s], f, c);
     all += c;
     ahead += s < seq ? c : 0;
   }

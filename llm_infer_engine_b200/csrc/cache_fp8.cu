@@ -41,7 +41,7 @@ __device__ __forceinline__ bool store_block(const StoreArgs& a, int hk, StoreBlo
   const int first = (start / kExpBlock + (int)blockIdx.x) * kExpBlock;
   b.p0 = max(start, first);
   b.p1 = min(start + n_new, first + kExpBlock);
-  if (b.p0 >= b.p1) return false;
+  if (b.p0 >= b.p1 || first / kFp8Page >= a.max_pages) return false;
   b.tok0 = t0 + b.p0 - start;
   b.lead = b.p0 - first;
   b.in_page = first % kFp8Page;

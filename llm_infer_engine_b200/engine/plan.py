@@ -131,7 +131,7 @@ class KernelPlan:
         if ctx.decode:
             ops.attention_decode_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, ctx.seq_slot, ctx.seq_kvlen, kv.block_table, n_q,
                                      n_kv, head_dim, options.scale, options.reach, ctx.max_kv_len)
-        elif options.scale > 0:
+        elif options.scale > 0 and ops.attention_prefill_fp8_supported(n_q, n_kv, head_dim, q.dtype):
             ops.attention_prefill_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, ctx.cu_q, ctx.seq_slot, ctx.seq_start,
                                       kv.block_table, ctx.n_seqs, ctx.max_q_len, n_q, n_kv, head_dim, options.scale,
                                       options.reach)

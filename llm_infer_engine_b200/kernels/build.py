@@ -47,6 +47,7 @@ FAMILIES: Dict[str, tuple] = {
     "attention_latent_tc": ("attention_latent_tc.cu", [], []),
     "cache_fp8": ("cache_fp8.cu", [], []),
     "attention_fp8": ("attention_fp8.cu", [], []),
+    "attention_prefill_fp8": ("attention_prefill_fp8.cu", [], []),
     "attention_decode_fp8": ("attention_decode_fp8.cu", [], []),
     "attention_rows_mma": ("attention_rows_mma.cu", [], []),
     "gemm_simt": ("gemm_simt.cu", [], []),

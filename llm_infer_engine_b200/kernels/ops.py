@@ -1798,19 +1798,44 @@ def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, s
                                 scale, window, max_kv_len)
 
 
+def attention_prefill_fp8_supported(n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> bool:
+    """The sizes attention_prefill_fp8.cu takes (answered without loading the library): bfloat16, head size 64 or 128, at most
+    128 query heads a key/value head."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128) and n_kv > 0 and n_q // n_kv <= 128
+
+
 def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot, seq_start, block_table, n_seqs: int,
                           max_q_len: int, n_q: int, n_kv: int, head_dim: int, scale: float, window: int = 0):
-    """Causal attention of runs of new tokens over a paged cache in 8 bits: q, out [T, n_q hd] with the sequences packed (cu_q),
-    seq_start the tokens each held before."""
+    """Causal attention of runs of new tokens over a paged cache in 8 bits, on the tcgen05 tensor cores: q, out bfloat16
+    [T, n_q hd] with the sequences packed (cu_q int32 [n + 1]), the cache as in rope_store_fp8 (it holds the step's keys and
+    values already), seq_start int32 [n] the tokens each sequence held before this step, window as in attention_paged.
+    head_dim 64 or 128, scale > 0. A block whose waits run out leaves NaN in its rows, and check_tc_status raises."""
     _need_heads("attention_prefill_fp8", n_q, n_kv)
-    if not attention_decode_fp8_supported(head_dim, q.dtype):
-        raise KernelError(f"attention_prefill_fp8: head_dim {head_dim}, {q.dtype} is not supported (bfloat16, 64 or 128)")
-    _need(q, "q", torch.bfloat16, (None, n_q * head_dim))
-    lens = (cu_q[1:n_seqs + 1] - cu_q[:n_seqs]).long()
-    tok_seq = torch.repeat_interleave(torch.arange(n_seqs, dtype=torch.int32, device=q.device), lens)
-    tok_pos = (torch.arange(q.shape[0], dtype=torch.int32, device=q.device) + (seq_start[:n_seqs] - cu_q[:n_seqs])[tok_seq.long()])
-    return attention_paged_fp8(q, k_cache, v_cache, k_exp, v_exp, out, tok_pos, tok_seq, seq_slot, block_table, n_q, n_kv,
-                               head_dim, scale, window)
+    if not attention_prefill_fp8_supported(n_q, n_kv, head_dim, q.dtype):
+        raise KernelError(f"attention_prefill_fp8: {n_q} / {n_kv} heads of {head_dim}, {q.dtype} are not supported (bfloat16, "
+                          "64 or 128, at most 128 query heads a key/value head)")
+    if not scale > 0:
+        raise KernelError(f"attention_prefill_fp8: the scale must be positive, got {scale}")
+    T = q.shape[0]
+    _need(q, "q", torch.bfloat16, (T, n_q * head_dim))
+    _need(out, "out", torch.bfloat16, (T, n_q * head_dim))
+    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _need_arrays("attention_prefill_fp8", n_seqs, q.device, cu_q=cu_q, seq_slot=seq_slot, seq_start=seq_start, block_table=block_table)
+    if cu_q.numel() < n_seqs + 1:
+        raise KernelError(f"attention_prefill_fp8: cu_q has {cu_q.numel()} entries, {n_seqs + 1} are needed")
+    _need_here("attention_prefill_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
+    floats = _fp8_scratch_floats.get(head_dim)
+    if floats is None:
+        f = _fn("attention_prefill_fp8", "llmie_attention_prefill_fp8_scratch", [_c_int], query=True)
+        floats = _fp8_scratch_floats[head_dim] = int(f(head_dim))
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
+    _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_prefill_fp8", "llmie_attention_prefill_fp8", [_c_void_p] * 12 + [_c_int] * 6 + [_c_float, _c_int, _c_void_p])
+    _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
+             scratch.data_ptr(), tc_status_word(q.device).data_ptr(), cu_q.data_ptr(), seq_slot.data_ptr(), seq_start.data_ptr(),
+             block_table.data_ptr(), block_table.shape[1], T, int(n_seqs), n_q, n_kv, head_dim, float(scale), int(window),
+             _stream()), "attention_prefill_fp8")
+    return out
 
 
 def attention_rows_mma_supported(head_dim: int, v_head_dim: int, page_size: int, dtype: torch.dtype,

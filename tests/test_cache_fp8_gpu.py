@@ -344,3 +344,120 @@ def test_decode_of_one_long_sequence_among_short_ones():
             # 20,000 keys: eight times the keys that `allowed` counts float32 sums for
             assert bool((err <= allowed(want, size, BF, True) + 2.0 ** -10 * size).all()), l
         assert float(out[1].float().view(n_q, hd)[::n_q // n_kv].mean()) > 4.0
+
+
+# ------------------------------------------------------------------------------------------ prompts
+def prompt(pc, q, starts, news, n_q, n_kv, hd, scale, window, cache=None):
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    out = torch.full((cu[-1], n_q * hd), math.nan, dtype=BF, device=DEV)
+    ops().attention_prefill_fp8(q.to(DEV), *(pc.dev() if cache is None else cache), out, i32(cu), i32(pc.slots), i32(starts),
+                                pc.table.to(DEV), len(news), max(news), n_q, n_kv, hd, scale, window)
+    ops().check_tc_status(DEV)
+    return out.cpu().double()
+
+
+def check_prompt(pc, out, q, starts, news, n_q, n_kv, hd, scale, window, rows=None):
+    """Every row, or `rows` of each sequence's."""
+    row = 0
+    for i, (st, m) in enumerate(zip(starts, news)):
+        pick = list(range(m)) if rows is None else sorted({r for r in rows if r < m} | ({m - 1} if m else set()))
+        if pick:
+            want, size = fp8_cache.attention(q[row:row + m].double().view(m, n_q, hd)[pick], *pc.held(i, st + m),
+                                             [st + r for r in pick], scale, window)
+            err = (out[row:row + m].view(m, n_q, hd)[pick] - want).abs()
+            bound = allowed(want, size, BF, True)
+            assert bool((err <= bound).all()), (i, st, m, float((err / bound).max()), int((err > bound).sum()))
+        row += m
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 1, 64), (4, 1, 128)])
+@pytest.mark.parametrize("start,new", [(0, 2), (0, 33), (100, 28)])
+def test_prompt_small(n_q, n_kv, hd, start, new):
+    pc = filled([start + new], n_kv, hd, seed=hd)
+    q = torch.randn(new, n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = prompt(pc, q, [start], [new], n_q, n_kv, hd, hd ** -0.5, 0)
+    check_prompt(pc, out, q, [start], [new], n_q, n_kv, hd, hd ** -0.5, 0)
+
+
+@pytest.mark.parametrize("window", [0, 40, 200, -64, -300])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(2, 2, 64), (12, 4, 64), (7, 1, 128), (8, 2, 128), (16, 1, 64), (40, 1, 64)])
+def test_prompt(n_q, n_kv, hd, window):
+    """Ragged pieces at odd places, one of a token, one of none; groups of 1 to 40 query heads."""
+    starts, news = [0, 70, 3, 700, 130, 63], [33, 9, 1, 40, 300, 0]
+    pc = filled([s + m for s, m in zip(starts, news)], n_kv, hd, seed=hd + n_q)
+    q = torch.randn(sum(news), n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = prompt(pc, q, starts, news, n_q, n_kv, hd, hd ** -0.5, window)
+    check_prompt(pc, out, q, starts, news, n_q, n_kv, hd, hd ** -0.5, window, rows=[0, 1, 15, 16, 31, 32, 63, 64, 127, 128, 129, 255])
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd,start,new", [(4, 1, 64, 0, 1500), (8, 2, 128, 400, 1100), (4, 4, 64, 0, 700), (8, 1, 128, 3000, 5)])
+def test_prompt_long(n_q, n_kv, hd, start, new):
+    """Many key tiles: the bound moves, the sums are rescaled, tiles are cut into runs and joined. A needle early on."""
+    pc = filled([start + new], n_kv, hd, seed=3, spread=0.5)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(new, n_q * hd, generator=g).to(BF)
+    needle = q[-1].float().view(n_q, hd)[::n_q // n_kv]
+    needle = needle * (24.0 / ((needle * needle).sum(-1, keepdim=True) * hd ** -0.5))
+    pc.append(0, 7, needle[None], torch.full((1, n_kv, hd), 5.0))
+    out = prompt(pc, q, [start], [new], n_q, n_kv, hd, hd ** -0.5, 0)
+    check_prompt(pc, out, q, [start], [new], n_q, n_kv, hd, hd ** -0.5, 0, rows=[0, 1, 100, 127, 128, 511, 512, 640, 1000])
+    assert float(out[-1].view(n_q, hd)[::n_q // n_kv].mean()) > 4.0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("case", ["large keys", "small queries", "large queries", "values apart", "zero values", "zero queries",
+                                  "growing scores"])
+def test_prompt_far_ranges(hd, case):
+    n_q, n_kv, starts, news = 4, 2, [150, 0], [40, 300]
+    g = torch.Generator().manual_seed(3)
+    pc = PlainCache([s + m for s, m in zip(starts, news)], n_kv, hd, seed=5, nan_stale=True)
+    q = torch.randn(sum(news), n_q * hd, generator=g)
+    scale = hd ** -0.5
+    for i, l in enumerate(s + m for s, m in zip(starts, news)):
+        k, v = torch.randn(l, n_kv, hd, generator=g), torch.randn(l, n_kv, hd, generator=g)
+        if case == "large keys":
+            k = k * 1e18
+        if case == "values apart":
+            v = v * (10.0 ** torch.linspace(-12, 12, (l + 15) // 16).repeat_interleave(16)[:l, None, None])
+        if case == "zero values":
+            v[16:l - 20] = 0.0
+        if case == "zero queries":
+            k[:64] = 0.0
+        if case == "growing scores":                   # every key tile has larger scores than the one before
+            k = k * torch.linspace(0.1, 12.0, l)[:, None, None]
+        pc.append(i, 0, k, v)
+    if case == "large keys":
+        scale *= 1e-18
+    elif case == "small queries":
+        q, scale = q * 1e-20, scale * 1e20
+    elif case == "large queries":
+        q, scale = q * 1e20, scale * 1e-20
+    elif case == "zero queries":
+        q[:] = 0.0
+    q = q.to(BF)
+    out = prompt(pc, q, starts, news, n_q, n_kv, hd, scale, 0)
+    check_prompt(pc, out, q, starts, news, n_q, n_kv, hd, scale, 0, rows=[0, 1, 17, 100, 128, 200])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_numbers_that_are_not_finite_stay_with_the_rows_that_see_them(hd):
+    n_q, n_kv, new = 4, 2, 200
+    pc = filled([new], n_kv, hd, seed=8)
+    g = torch.Generator().manual_seed(8)
+    k, v = torch.randn(1, n_kv, hd, generator=g), torch.randn(1, n_kv, hd, generator=g)
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[0, 1, 3], bad_v[0, 0, 5] = math.inf, math.nan
+    pc.append(0, 60, k, bad_v)                         # position 60: column 5 of KV head 0's value
+    pc.append(0, 130, bad_k, v)                        # position 130: the key of KV head 1
+    q = torch.randn(new, n_q * hd, generator=g).to(BF)
+    q[20, 3 * hd + 1] = math.nan                       # one query head of one token
+    for window in (0, 30):
+        bad = torch.isnan(prompt(pc, q, [0], [new], n_q, n_kv, hd, hd ** -0.5, window)).view(new, n_q, hd)
+        want = torch.zeros_like(bad)
+        last = new if window == 0 else None
+        want[60:last or 90, :2, 5] = True
+        want[130:last or 160, 2:] = True
+        want[20, 3] = True
+        assert torch.equal(bad, want), window
