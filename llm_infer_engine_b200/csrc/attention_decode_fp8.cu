@@ -130,9 +130,78 @@ template <int HD> struct DfUnit {
   int ke, ve;
 };
 
-template <int HD, int NH>
+// A step's projections as they come, [n_seqs, (n_q + 2 n_kv) HD], and what the new key and value need (rope == null: q is
+// rotated already, and the cache holds the step's keys and values).
+struct DecodeStep {
+  const float4* rope;                // (cos, sin) [table_len, HD / 2]
+  int table_len;
+  unsigned char* k;                  // the cache, to be written
+  unsigned char* v;
+  signed char* k_exp;
+  signed char* v_exp;
+};
+
+// Writes position len - 1 of (sequence, KV head) into its block: rotated key and value, the block's exponents, the earlier codes
+// lowered where an exponent rises (cache_fp8.cu has the rules; the numbers are the same bit for bit). One warp; what it wrote
+// is there for the whole warp when it returns.
+template <int HD>
+__device__ __forceinline__ void df_append(const __nv_bfloat16* qkv_row, const DecodeArgs& a, const DecodeStep& st, int hk, int len, int page) {
+  const int lane = threadIdx.x & 31;
+  const int pos = len - 1, in = pos % kExpBlock;
+  const size_t head = (size_t)page * a.n_kv + hk;
+  const size_t at = head * kPageExps + pos % kFp8Page / kExpBlock;
+  const size_t row = (head * kFp8Page + pos % kFp8Page) * HD;
+  constexpr int kN = HD / 64;        // neighbouring columns a lane has in each half of the head
+  const int d = lane * kN;
+  const float2* cs = reinterpret_cast<const float2*>(st.rope) + (size_t)min(pos, st.table_len - 1) * (HD / 2) + d;
+  const __nv_bfloat16* kp = qkv_row + (size_t)(a.n_q + hk) * HD + d;
+  const __nv_bfloat16* vp = kp + (size_t)a.n_kv * HD;
+  float x[2][2][kN];
+  unsigned big[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const float2 c = cs[i];
+    const float k0 = __bfloat162float(kp[i]), k1 = __bfloat162float(kp[i + HD / 2]);
+    x[0][0][i] = __fsub_rn(__fmul_rn(k0, c.x), __fmul_rn(k1, c.y));
+    x[0][1][i] = __fadd_rn(__fmul_rn(k1, c.x), __fmul_rn(k0, c.y));
+    x[1][0][i] = __bfloat162float(vp[i]);
+    x[1][1][i] = __bfloat162float(vp[i + HD / 2]);
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) big[w] = max(big[w], max(finite_magnitude(x[w][0][i]), finite_magnitude(x[w][1][i])));
+    big[w] = __reduce_max_sync(0xffffffffu, big[w]);
+    signed char* exp_at = (w ? st.v_exp : st.k_exp) + at;
+    unsigned char* codes = (w ? st.v : st.k) + row;
+    int e = exponent_for(big[w]);
+    if (in > 0) {
+      const int before = clamp_exponent(*exp_at);
+      e = max(e, before);
+      if (e > before) {
+        const float f = lower_factor(before, e);
+        unsigned* old = reinterpret_cast<unsigned*>(codes - (size_t)in * HD);
+        for (int i = lane; i < in * HD / 4; i += 32) old[i] = lower_codes(old[i], f);
+      }
+    }
+    const float f = pow2_of(-e);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (kN == 2) {
+        *reinterpret_cast<unsigned short*>(codes + d + h * (HD / 2)) = to_e4m3x2(x[w][h][0] * f, x[w][h][kN - 1] * f);
+      } else {
+        codes[d + h * (HD / 2)] = (unsigned char)(to_e4m3x2(x[w][h][0] * f, 0.f) & 0xffu);
+      }
+    }
+    __syncwarp();                    // every lane has read the old exponent
+    if (lane == 0) *exp_at = (signed char)e;
+  }
+  __syncwarp();
+}
+
+template <int HD, int NH, bool ROPE>
 __global__ void __launch_bounds__(kDfThreads, df_per_sm<HD, NH>())
-decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a) {
+decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep st) {
   pdl_launch_dependents();
   pdl_wait();
   using Cfg = DfCfg<HD, NH>;
@@ -222,6 +291,9 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a) {
     const int u_stop = first + u_end;
     DfUnit<HD> x0, x1;
     int pg_next = 0;
+    const size_t q_pitch = (size_t)(ROPE ? a.n_q + 2 * a.n_kv : a.n_q) * HD;
+    if (ROPE && u_begin + 1 <= count && u_end == count && (count - 1 - u_begin) % kDfWarps == warp)
+      df_append<HD>(q + seq * q_pitch, a, st, hk, len, page_of(first + count - 1));     // this warp reads that block itself
     if (u < u_stop) load(x0, u, page_of(u));
     if (u + kDfWarps < u_stop) pg_next = page_of(u + kDfWarps);
 
@@ -231,12 +303,29 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a) {
 #pragma unroll
     for (int nh = 0; nh < NH; ++nh) {
       const bool there = nh * 8 + g < ng;
-      const __nv_bfloat16* row = q + (size_t)seq * a.n_q * HD + (size_t)(hk * G + g0 + (there ? nh * 8 + g : 0)) * HD;
+      const __nv_bfloat16* row = q + seq * q_pitch + (size_t)(hk * G + g0 + (there ? nh * 8 + g : 0)) * HD;
       uint2 raw[KS];
       float big = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        raw[ks] = there ? *reinterpret_cast<const uint2*>(row + (ks >> 2) * 64 + t * 16 + (ks & 3) * 4) : make_uint2(0u, 0u);
+        const int col = (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;
+        raw[ks] = there ? *reinterpret_cast<const uint2*>(row + col) : make_uint2(0u, 0u);
+        if (ROPE) {
+          // four columns and the four that they are rotated with, half a head away
+          const bool upper = col >= HD / 2;
+          const uint2 other = there ? *reinterpret_cast<const uint2*>(row + (upper ? col - HD / 2 : col + HD / 2)) : make_uint2(0u, 0u);
+          const float4* cs = st.rope + ((size_t)min(len - 1, st.table_len - 1) * (HD / 2) + (upper ? col - HD / 2 : col)) / 2;
+          const float4 c0 = cs[0], c1 = cs[1];
+          auto turned = [&](unsigned x, unsigned y, const float4& c) {
+            const float2 u2 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+            const float2 v2 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y));
+            const float p0 = __fmul_rn(u2.x, c.x), p1 = __fmul_rn(u2.y, c.z), r0 = __fmul_rn(v2.x, c.y), r1 = __fmul_rn(v2.y, c.w);
+            const __nv_bfloat162 z = upper ? __floats2bfloat162_rn(__fadd_rn(p0, r0), __fadd_rn(p1, r1))
+                                           : __floats2bfloat162_rn(__fsub_rn(p0, r0), __fsub_rn(p1, r1));
+            return *reinterpret_cast<const unsigned*>(&z);
+          };
+          raw[ks] = make_uint2(turned(raw[ks].x, other.x, c0), turned(raw[ks].y, other.y, c1));
+        }
         const float2 y0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
         const float2 y1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
         big = fmaxf(big, fmaxf(fmaxf(fabsf(y0.x), fabsf(y0.y)), fmaxf(fabsf(y1.x), fabsf(y1.y))));
@@ -480,9 +569,10 @@ __global__ void __launch_bounds__(HD) decode_fp8_join_kernel(const DecodeArgs a,
 }
 
 template <int HD, int NH>
-static int launch_decode(const void* q, const DecodeArgs& a, cudaStream_t stream) {
+static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& st, cudaStream_t stream) {
   constexpr int blocks = df_blocks<HD, NH>();
-  launch_k(decode_fp8_kernel<HD, NH>, dim3(blocks), dim3(kDfThreads), 0, stream, (const __nv_bfloat16*)q, a);
+  if (st.rope) launch_k(decode_fp8_kernel<HD, NH, true>, dim3(blocks), dim3(kDfThreads), 0, stream, (const __nv_bfloat16*)q, a, st);
+  else launch_k(decode_fp8_kernel<HD, NH, false>, dim3(blocks), dim3(kDfThreads), 0, stream, (const __nv_bfloat16*)q, a, st);
   LLMIE_LAUNCH_CHECK();
   const int G = a.n_q / a.n_kv, chunks = (G + 8 * NH - 1) / (8 * NH);
   launch_k(decode_fp8_join_kernel<HD, NH>, dim3((unsigned)(a.n_seqs * a.n_kv * chunks), min(G, 8 * NH)), dim3(HD), 0, stream, a, blocks);
@@ -502,14 +592,11 @@ extern "C" int llmie_attention_decode_fp8_scratch(int n_q, int n_kv, int hd) {
   return one ? 2 * df_blocks<128, 1>() * DfCfg<128, 1>::kRecord : 2 * df_blocks<128, 2>() * DfCfg<128, 2>::kRecord;
 }
 
-// q, out bfloat16 [n_seqs, n_q hd], hd 64 or 128; caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv, 4];
-// seq_kvlen: keys that each sequence holds, this step's among them (0: its rows become zeros). window as in the other attention
-// kernels. scratch: llmie_attention_decode_fp8_scratch floats, 16-byte aligned.
-extern "C" int llmie_attention_decode_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_exp,
-                                          const void* v_exp, void* out, float* scratch, const int* seq_slot, const int* seq_kvlen,
-                                          const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd,
-                                          float scale, int window, cudaStream_t stream) {
-  if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || !scratch) return LLMIE_ERR_BAD_ARG;
+static int decode_fp8_entry(const void* q, const void* k_cache, const void* v_cache, const void* k_exp, const void* v_exp, void* out,
+                            float* scratch, const float* rope, int table_len, const int* seq_slot, const int* seq_kvlen,
+                            const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd, float scale, int window,
+                            cudaStream_t stream) {
+  if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || max_pages > (1 << 24) || !scratch) return LLMIE_ERR_BAD_ARG;
   if (hd != 64 && hd != 128) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache)) return LLMIE_ERR_ALIGNMENT;
   if (n_seqs == 0) return LLMIE_OK;
@@ -517,7 +604,32 @@ extern "C" int llmie_attention_decode_fp8(const void* q, const void* k_cache, co
   const DecodeArgs a{(const unsigned char*)k_cache, (const unsigned char*)v_cache, (const signed char*)k_exp, (const signed char*)v_exp,
                      (__nv_bfloat16*)out, scratch, seq_slot, seq_kvlen, block_table, max_pages, n_seqs, n_q, n_kv,
                      scale * 1.4426950408889634f, window};
+  const DecodeStep st{(const float4*)rope, table_len, (unsigned char*)k_cache, (unsigned char*)v_cache, (signed char*)k_exp, (signed char*)v_exp};
   const bool one = n_q / n_kv <= 8;
-  if (hd == 64) return one ? launch_decode<64, 1>(q, a, stream) : launch_decode<64, 2>(q, a, stream);
-  return one ? launch_decode<128, 1>(q, a, stream) : launch_decode<128, 2>(q, a, stream);
+  if (hd == 64) return one ? launch_decode<64, 1>(q, a, st, stream) : launch_decode<64, 2>(q, a, st, stream);
+  return one ? launch_decode<128, 1>(q, a, st, stream) : launch_decode<128, 2>(q, a, st, stream);
+}
+
+// q, out bfloat16 [n_seqs, n_q hd], hd 64 or 128; caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv, 4];
+// seq_kvlen: keys that each sequence holds, this step's among them (0: its rows become zeros). window as in the other attention
+// kernels. scratch: llmie_attention_decode_fp8_scratch floats, 16-byte aligned.
+extern "C" int llmie_attention_decode_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_exp,
+                                          const void* v_exp, void* out, float* scratch, const int* seq_slot, const int* seq_kvlen,
+                                          const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd,
+                                          float scale, int window, cudaStream_t stream) {
+  return decode_fp8_entry(q, k_cache, v_cache, k_exp, v_exp, out, scratch, nullptr, 0, seq_slot, seq_kvlen, block_table, max_pages,
+                          n_seqs, n_q, n_kv, hd, scale, window, stream);
+}
+
+// The same from a step's projections: qkv bfloat16 [n_seqs, (n_q + 2 n_kv) hd], rope float32 [table_len, hd / 2, 2] the (cos, sin) of
+// every position; the new key (rotated) and value of sequence i are written for position seq_kvlen[i] - 1 and read with the rest. A
+// KV head must be one block's work (at most 16 query heads): the others would read what one of them writes.
+extern "C" int llmie_attention_decode_fp8_rope(const void* qkv, void* k_cache, void* v_cache, void* k_exp, void* v_exp, void* out,
+                                               float* scratch, const float* rope, int table_len, const int* seq_slot,
+                                               const int* seq_kvlen, const int* block_table, int max_pages, int n_seqs, int n_q,
+                                               int n_kv, int hd, float scale, int window, cudaStream_t stream) {
+  if (!rope || table_len <= 0 || n_kv <= 0 || n_q / n_kv > 16) return LLMIE_ERR_BAD_ARG;
+  if (!aligned16(rope)) return LLMIE_ERR_ALIGNMENT;
+  return decode_fp8_entry(qkv, k_cache, v_cache, k_exp, v_exp, out, scratch, rope, table_len, seq_slot, seq_kvlen, block_table,
+                          max_pages, n_seqs, n_q, n_kv, hd, scale, window, stream);
 }

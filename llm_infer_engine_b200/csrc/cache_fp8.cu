@@ -124,9 +124,125 @@ rope_store_fp8_kernel(const T* qkv, T* __restrict__ q_out, const float2* LLMIE_W
   }
 }
 
+// Head size 64 or 128, the whole head rotated (or none), rows on 16 bytes: a thread has eight neighbouring columns and their
+// partners half a head on, of one position, for all the heads there are; the angles are read once for all of them.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kStoreThreads)
+rope_store_fp8_vec_kernel(const T* qkv, T* __restrict__ q_out, const float4* LLMIE_WEIGHT table, const StoreArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int kLanes = HD / 16;                            // threads a row
+  constexpr int kParts = kStoreThreads / (kExpBlock * kLanes);         // 1: a thread has keys and values; 2: one of them
+  __shared__ unsigned largest[2];
+  const int hk = blockIdx.y, G = a.n_q / a.n_kv;
+  StoreBlock b;
+  if (!store_block(a, hk, b)) return;
+  const int n = b.p1 - b.p0;
+  if (threadIdx.x < 2) largest[threadIdx.x] = 0u;
+  __syncthreads();
+  const int lane = threadIdx.x % kLanes, row = threadIdx.x / kLanes % kExpBlock, part = threadIdx.x / (kLanes * kExpBlock);
+  const bool active = row < n;
+  const size_t row_w = (size_t)(a.n_q + 2 * a.n_kv) * HD;
+  const T* src = qkv + (size_t)(b.tok0 + (active ? row : 0)) * row_w + lane * 8;
+  float c[8], s[8];
+  if (table) {
+    const float4* cs = table + ((size_t)min(b.p0 + row, a.table_len - 1) * (HD / 2) + lane * 8) / 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 v = cs[i];
+      c[2 * i] = v.x;
+      s[2 * i] = v.y;
+      c[2 * i + 1] = v.z;
+      s[2 * i + 1] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = 1.f;
+      s[i] = 0.f;
+    }
+  }
+  auto turn = [&](float (&x)[8], float (&y)[8]) {
+    if (!table) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float u = x[i], v = y[i];
+      x[i] = __fsub_rn(__fmul_rn(u, c[i]), __fmul_rn(v, s[i]));
+      y[i] = __fadd_rn(__fmul_rn(v, c[i]), __fmul_rn(u, s[i]));
+    }
+  };
+  // keys and values: which of them this thread has, as numbers
+  float x[3 - kParts][2][8];
+  if (a.write_kv) {
+#pragma unroll
+    for (int i = 0; i < 3 - kParts; ++i) {
+      const int which = kParts == 1 ? i : part;
+      const T* p = src + (size_t)(a.n_q + which * a.n_kv + hk) * HD;
+      load8(p, x[i][0]);
+      load8(p + HD / 2, x[i][1]);
+      if (which == 0) turn(x[i][0], x[i][1]);
+      unsigned big = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = max(big, max(finite_magnitude(x[i][0][e]), finite_magnitude(x[i][1][e])));
+      big = __reduce_max_sync(0xffffffffu, active ? big : 0u);
+      if ((threadIdx.x & 31) == 0) atomicMax(&largest[which], big);
+    }
+  }
+  if (active) {
+    T* dst = q_out + (size_t)(b.tok0 + row) * a.n_q * HD + lane * 8;
+#pragma unroll 4
+    for (int g = part; g < G; g += kParts) {
+      const size_t col = (size_t)(hk * G + g) * HD;
+      float u[8], v[8];
+      load8(src + col, u);
+      load8(src + col + HD / 2, v);
+      turn(u, v);
+      store8(dst + col, u);
+      store8(dst + col + HD / 2, v);
+    }
+  }
+  if (!a.write_kv) return;
+  __syncthreads();
+  int e[2];
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
+    e[which] = settle_exponent((which ? a.v_exp : a.k_exp) + b.row * kPageExps + b.in_page / kExpBlock,
+                               (which ? a.v : a.k) + (b.row * kFp8Page + b.in_page) * HD, b.lead, HD, largest[which]);
+  if (active) {
+#pragma unroll
+    for (int i = 0; i < 3 - kParts; ++i) {
+      const int which = kParts == 1 ? i : part;
+      const float f = pow2_of(-(which ? e[1] : e[0]));
+      unsigned char* dst = (which ? a.v : a.k) + (b.row * kFp8Page + b.in_page + b.lead + row) * HD + lane * 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        unsigned w[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          w[j] = (unsigned)to_e4m3x2(x[i][h][4 * j] * f, x[i][h][4 * j + 1] * f) |
+                 ((unsigned)to_e4m3x2(x[i][h][4 * j + 2] * f, x[i][h][4 * j + 3] * f) << 16);
+        *reinterpret_cast<uint2*>(dst + h * (HD / 2)) = make_uint2(w[0], w[1]);
+      }
+    }
+  }
+  if (b.lead > 0) __syncthreads();   // everyone has read the old exponents
+  if (threadIdx.x < 2) (threadIdx.x ? a.v_exp : a.k_exp)[b.row * kPageExps + b.in_page / kExpBlock] = (signed char)(threadIdx.x ? e[1] : e[0]);
+}
+
 template <typename T>
 static int launch_store(const void* qkv, void* q_out, const float2* table, const StoreArgs& a, int blocks, int n_seqs,
                         cudaStream_t stream) {
+  const bool vec = (a.rot_dim == a.hd || !table) && aligned16(qkv) && aligned16(q_out) && aligned16(table);
+  if (vec && (a.hd == 64 || a.hd == 128)) {
+    if (a.hd == 64)
+      launch_k(rope_store_fp8_vec_kernel<T, 64>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), 0, stream, (const T*)qkv,
+               (T*)q_out, (const float4*)table, a);
+    else
+      launch_k(rope_store_fp8_vec_kernel<T, 128>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), 0, stream, (const T*)qkv,
+               (T*)q_out, (const float4*)table, a);
+    LLMIE_LAUNCH_CHECK();
+    return LLMIE_OK;
+  }
   const size_t smem = (size_t)2 * kExpBlock * a.hd * sizeof(float);
   launch_k(rope_store_fp8_kernel<T>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), smem, stream, (const T*)qkv, (T*)q_out,
            table, a);

@@ -1741,8 +1741,8 @@ def attention_decode_fp8_supported(head_dim: int, dtype: torch.dtype) -> bool:
 
 
 def attention_decode_fp8_rope_supported(n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> bool:
-    """Whether attention_decode_fp8_rope takes a step."""
-    return attention_decode_fp8_supported(head_dim, dtype)
+    """Whether attention_decode_fp8_rope takes a step: one block has all the query heads of a key/value head."""
+    return attention_decode_fp8_supported(head_dim, dtype) and n_kv > 0 and n_q // n_kv <= 16
 
 
 _fp8_scratch_floats = {}
@@ -1783,19 +1783,30 @@ def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_k
 
 def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, seq_slot, seq_kvlen, block_table, n_q: int,
                               n_kv: int, head_dim: int, scale: float, window: int = 0, max_kv_len: int = 0):
-    """What a one-token step does with its projections over a cache in 8 bits: qkv bfloat16 [n, (n_q + 2 n_kv) hd], rotated by
-    table (float32 [max_pos, hd / 2, 2], the whole head), the new key and value written for position seq_kvlen[i] - 1 as
-    rope_store_fp8 does it, and attention_decode_fp8 over the cache with them."""
+    """What a one-token step does with its projections over a cache in 8 bits, in one kernel: qkv bfloat16
+    [n, (n_q + 2 n_kv) hd] rotated by table (float32 [max_pos, hd / 2, 2], the whole head), the new key and value written for
+    position seq_kvlen[i] - 1 as rope_store_fp8 does it, and attention_decode_fp8 over the cache with them. At most 16 query
+    heads a key/value head. A slot may appear once."""
     n = qkv.shape[0]
     _need_heads("attention_decode_fp8_rope", n_q, n_kv)
-    if not attention_decode_fp8_supported(head_dim, qkv.dtype):
-        raise KernelError(f"attention_decode_fp8_rope: head_dim {head_dim}, {qkv.dtype} is not supported (bfloat16, 64 or 128)")
-    q = torch.empty((n, n_q * head_dim), dtype=qkv.dtype, device=qkv.device)
-    cu = torch.arange(n + 1, dtype=torch.int32, device=qkv.device)
-    rope_store_fp8(qkv, q, k_cache, v_cache, k_exp, v_exp, table, cu, seq_slot, seq_kvlen[:n] - 1, block_table, n, 1, n_q, n_kv,
-                   head_dim, head_dim)
-    return attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_kvlen, block_table, n_q, n_kv, head_dim,
-                                scale, window, max_kv_len)
+    if not attention_decode_fp8_rope_supported(n_q, n_kv, head_dim, qkv.dtype):
+        raise KernelError(f"attention_decode_fp8_rope: {n_q} / {n_kv} heads of {head_dim}, {qkv.dtype} are not supported (bfloat16, "
+                          "64 or 128, at most 16 query heads a key/value head)")
+    _need(qkv, "qkv", torch.bfloat16, (n, (n_q + 2 * n_kv) * head_dim))
+    _need(out, "out", torch.bfloat16, (n, n_q * head_dim))
+    _need(table, "table", torch.float32, (None, head_dim // 2, 2))
+    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _need_arrays("attention_decode_fp8_rope", n, qkv.device, seq_slot=seq_slot, seq_kvlen=seq_kvlen, block_table=block_table)
+    _need_here("attention_decode_fp8_rope", qkv, out, table, k_cache, v_cache, k_exp, v_exp)
+    scratch = _decode_fp8_scratch(n_q, n_kv, head_dim, qkv.device)
+    _work(_nbytes(qkv, out) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_rope",
+            [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_void_p])
+    _check(f(qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
+             scratch.data_ptr(), table.data_ptr(), table.shape[0], seq_slot.data_ptr(), seq_kvlen.data_ptr(),
+             block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv, head_dim, float(scale), int(window), _stream()),
+           "attention_decode_fp8_rope")
+    return out
 
 
 def attention_prefill_fp8_supported(n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> bool:

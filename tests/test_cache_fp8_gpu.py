@@ -461,3 +461,47 @@ def test_prompt_numbers_that_are_not_finite_stay_with_the_rows_that_see_them(hd)
         want[130:last or 160, 2:] = True
         want[20, 3] = True
         assert torch.equal(bad, want), window
+
+
+# ------------------------------------------------------------------------------------------ one-token steps in one kernel
+@pytest.mark.parametrize("window", [0, 40, -64])
+@pytest.mark.parametrize("n_q,n_kv,hd", [(4, 4, 64), (12, 4, 64), (32, 8, 128), (7, 1, 128), (16, 1, 64), (32, 2, 128)])
+def test_step(n_q, n_kv, hd, window):
+    """The new key and value go into the cache bit for bit as rope_store_fp8 leaves them (blocks that begin, go on, raise their
+    exponent), and attention sees them; a lane without a sequence writes nothing. Run twice: the same."""
+    lens = [1, 16, 17, 64, 65, 300, 0, 777, 48]
+    n = len(lens)
+    pc = PlainCache(lens, n_kv, hd, seed=hd + n_q, nan_stale=True)
+    g = torch.Generator().manual_seed(3)
+    for i, l in enumerate(lens):
+        if l > 1:
+            pc.append(i, 0, torch.randn(l - 1, n_kv, hd, generator=g), torch.randn(l - 1, n_kv, hd, generator=g))
+    qkv = torch.randn(n, (n_q + 2 * n_kv) * hd, generator=g)
+    qkv[2] *= 40.0                                     # position 16 begins a block
+    qkv[5] *= 40.0                                     # position 299 raises its block's exponents
+    qkv[8] *= 1e-3                                     # position 47 does not
+    qkv = qkv.to(BF)
+    table = angles(1024, hd)
+    cache = pc.dev()
+    before = [t.clone() for t in cache]
+    outs = []
+    for _ in range(2):
+        out = torch.full((n, n_q * hd), math.nan, dtype=BF, device=DEV)
+        ops().attention_decode_fp8_rope(qkv.to(DEV), *cache, out, table.to(DEV), i32(pc.slots), i32(lens), pc.table.to(DEV), n_q,
+                                        n_kv, hd, hd ** -0.5, window, 1024)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1])
+    starts, news = [max(l - 1, 0) for l in lens], [min(l, 1) for l in lens]
+    keep = torch.tensor([m > 0 for m in news])
+    q = plain_store(pc, qkv[keep], table, starts, news, n_q, n_kv, hd, hd)
+    check_cache(pc, cache)
+    assert not same_bits(before[0], cache[0])
+    row = 0
+    for i, l in enumerate(lens):
+        if l == 0:
+            assert bool((outs[0][i] == 0).all())
+            continue
+        want, size = fp8_cache.attention(q[row:row + 1].double().view(1, n_q, hd), *pc.held(i, l), [l - 1], hd ** -0.5, window)
+        err = (outs[0][i].cpu().double().view(1, n_q, hd) - want).abs()
+        assert bool((err <= allowed(want, size, BF, True)).all()), (l, float((err / allowed(want, size, BF, True)).max()))
+        row += 1
