@@ -2,16 +2,17 @@
 //
 //   o = sum_j 2^(s_j) c_j 2^(ev_j) / sum_j 2^(s_j),     s_j = scale log2(e) (q . k_j) 2^(ek_j)      (k, c: codes of keys, values)
 //
-// A warp works on 16 positions of a KV head at a time, which is one block of the cache: its keys have one exponent, its
+// A warp works on 32 positions of a KV head at a time, which are two blocks of the cache: a block's keys have one exponent, its
 // values another. A value's exponent is added to the score, so that one exponential gives the weight that its codes get:
-// with R >= s_j + ev_j a running bound, w_j = 2^(s_j + ev_j - R + 15) lies in (0, 2^15] and goes into the second product
-// in half precision (its normal range reaches 2^-29 below the largest weight), and the softmax's denominator is sum_j w_j
-// 2^(-ev_j), kept in float32 relative to the same R.
+// with R a running bound, w_j = 2^(s_j + ev_j - R + 7) goes into the second product in half precision, and the softmax's
+// denominator is sum_j w_j 2^(-ev_j), kept in float32 relative to the same R. R follows the largest s_j + ev_j only when that
+// has outgrown it by 8, so that w_j stays below 2^15 (half precision then holds what is within 2^-21 of the largest weight with
+// 11 digits) and the sums have to be rescaled a few times in a sequence, not with every block.
 //
 // Both products are mma.sync.m16n8k16 with the cache as the 16-row operand and the query heads of the KV head as the 8
-// columns: S^T = K Q^T and O^T = V^T W^T. Codes become half-precision numbers (exactly) in registers, so the cache goes from
-// global memory to the multiplier without shared memory: which k index stands for which column of a head is free as long as
-// both operands agree, so a lane reads 16 neighbouring codes of a key (and 8 or 16 of a value), whole sectors every time.
+// columns: S^T = K Q^T and O^T = V^T W^T. Codes become half-precision numbers (exactly) in registers, and which k
+// index stands for which column of a head is free as long as both operands agree: a lane reads 16 neighbouring codes of a key
+// (and 8 or 16 of a value), whole sectors every time, through a ring of asynchronous copies of its own.
 // W^T comes out of S^T's accumulators by one 8x8 transpose between lanes (movmatrix). Queries are brought to half precision
 // with a power of two per head (their largest number in [2^14, 2^15)), which keeps every digit of bfloat16.
 //
@@ -20,13 +21,18 @@
 // a captured step costs what its sequences hold. An item that lies in several shares leaves partial results, and a second
 // small kernel joins them in the order of the shares: no atomics, no counters, nothing kept between calls.
 #include "fp8.cuh"
+#include "tcgen05.cuh"
 #include <math.h>
 
 namespace llmie {
 
 constexpr int kDfWarps = 4;
+constexpr int kDfUnit = 2 * kExpBlock;
 constexpr int kDfThreads = kDfWarps * 32;
 constexpr int kSms = 148;
+constexpr float kDfSlack = 8.f;      // how far scores may outgrow a head's bound, in units of log2
+constexpr float kDfTop = 7.f;        // the bound's own weight is 2^7: none is above 2^15
+constexpr int kDfFew = 12;           // units a warp up to which an item is one cluster's
 
 __device__ __forceinline__ float df_exp2(float x) {
   float y;
@@ -50,18 +56,6 @@ __device__ __forceinline__ unsigned df_half2(float a, float b) {
 }
 __device__ __forceinline__ unsigned df_lo(unsigned w) { return e4m3x2_to_half2((unsigned short)(w & 0xffffu)); }
 __device__ __forceinline__ unsigned df_hi(unsigned w) { return e4m3x2_to_half2((unsigned short)(w >> 16)); }
-// The cache is read once: past the first-level cache.
-__device__ __forceinline__ uint4 df_load16(const unsigned char* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 df_load8(const unsigned char* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-  return v;
-}
-
 struct DecodeArgs {
   const unsigned char* k;            // [pages, n_kv, 64, HD] codes
   const unsigned char* v;
@@ -77,21 +71,21 @@ struct DecodeArgs {
   int window;
 };
 
-// Blocks of 16 positions that a sequence's newest token sees: [first, first + count).
+// Units of 32 positions (two blocks of the cache) in which a sequence's newest token sees some: [first, first + count).
 __device__ __forceinline__ void df_units(const DecodeArgs& a, int len, int& first, int& count) {
   len = min(len, a.max_pages * kFp8Page);              // what the table has room for
   if (len <= 0) {
     first = count = 0;
     return;
   }
-  first = first_visible_key(len - 1, a.window) / kExpBlock;
-  count = (len - 1) / kExpBlock - first + 1;
+  first = first_visible_key(len - 1, a.window) / kDfUnit;
+  count = (len - 1) / kDfUnit - first + 1;
 }
 
 // Units of all sequences together (every item of a sequence has as many as the sequence). All lanes of a warp call it.
-__device__ __forceinline__ long long df_total(const DecodeArgs& a) {
+__device__ __forceinline__ int df_total(const DecodeArgs& a) {
   const int lane = threadIdx.x & 31;
-  long long t = 0;
+  int t = 0;
   for (int s = lane; s < a.n_seqs; s += 32) {
     int f, c;
     df_units(a, a.seq_kvlen[s], f, c);
@@ -103,8 +97,8 @@ __device__ __forceinline__ long long df_total(const DecodeArgs& a) {
 }
 
 // Units that a thread block takes: an equal share, and four at least (one a warp).
-__device__ __forceinline__ long long df_share(long long total_units, int blocks) {
-  const long long s = (total_units + blocks - 1) / blocks;
+__device__ __forceinline__ int df_share(int total_units, int blocks) {
+  const int s = (total_units + blocks - 1) / blocks;
   return s < kDfWarps ? kDfWarps : s;
 }
 
@@ -114,21 +108,13 @@ template <int HD, int NH> struct DfCfg {
   static constexpr int kRecord = kHeads * (HD + 2);              // floats of a partial result: sums, then bounds and denominators
 };
 // Thread blocks that an SM holds at once.
-template <int HD, int NH> __host__ __device__ constexpr int df_per_sm() { return HD == 64 ? (NH == 1 ? 4 : 3) : NH == 1 ? 3 : 2; }
+template <int HD, int NH> __host__ __device__ constexpr int df_per_sm() { return HD == 64 ? (NH == 1 ? 5 : 3) : NH == 1 ? 3 : 2; }
 template <int HD, int NH> constexpr int df_blocks() { return kSms * df_per_sm<HD, NH>(); }
 // Where column d of a head stands among a head's sums: as the second product's accumulators hold them.
 template <int HD> __device__ __forceinline__ int df_place(int d) {
   constexpr int R = HD / 8;
   return (d % R / 2) * 16 + (d & 1) * 8 + d / R;
 }
-
-// One unit as a warp's lanes hold it: lane (g, t) has keys g and g + 8, 16 columns from 16 t on of every 64; and the values
-// of positions 2t, 2t + 1, 2t + 8, 2t + 9, HD / 8 columns from g HD / 8 on.
-template <int HD> struct DfUnit {
-  uint4 k[2][HD / 64];
-  uint2 v[4][HD / 64];
-  int ke, ve;
-};
 
 // A step's projections as they come, [n_seqs, (n_q + 2 n_kv) HD], and what the new key and value need (rope == null: q is
 // rotated already, and the cache holds the step's keys and values).
@@ -199,22 +185,350 @@ __device__ __forceinline__ void df_append(const __nv_bfloat16* qkv_row, const De
   __syncwarp();
 }
 
+// A warp's pipeline of units: a ring of stages in shared memory, filled by asynchronous copies of whole lines. A unit's keys are one
+// run of memory, its values another; 16-byte pieces lie in lines of 128 bytes, their places in a line permuted so that no two
+// lanes of a quarter warp meet in a bank when the fragments are read: keys by 4 neighbouring pieces of 2 rows, values by one piece
+// of 4 rows 2 apart. Fragments: lane (g, t) reads, of keys g, g + 8, g + 16 and g + 24, 16 codes from column 16 t on of every
+// 64; of the values of positions 2t, 2t + 1, 2t + 8, 2t + 9 and those 16 on, HD / 8 codes from column g HD / 8 on.
+// (Lanes that copied what they read themselves, 64 bytes of a line at a time, needed no barrier but reached 64 % of the copy
+// bandwidth at head size 128 with the arithmetic left out.)
+template <int HD> __device__ __forceinline__ int df_swizzle(int line) {
+  return HD == 64 ? (line & 3) << 1 : ((line >> 1 & 3) << 1) ^ ((line & 1) << 2);
+}
+// byte offset of piece p of row r in a unit
+template <int HD> __device__ __forceinline__ int df_at(int r, int p) {
+  const int l = r * (HD / 16) + p, line = l >> 3;
+  return line * 128 + ((l & 7) ^ df_swizzle<HD>(line)) * 16;
+}
+template <int HD, int NH> struct DfPipe {
+  static constexpr int kStages = 2;
+  static constexpr int kHalf = kDfUnit * HD;                 // bytes of a unit's keys, or values
+  static constexpr int kUnit = 2 * kHalf + 128;              // and the exponents; whole lines
+
+  static constexpr int kWarp = kStages * kUnit;
+  static constexpr int kSums = DfCfg<HD, NH>::kHeads * (DfCfg<HD, NH>::kPitch + 2) * 4;        // a warp's results, in the same place afterwards
+  static constexpr int kPerWarp = ((kWarp > kSums ? kWarp : kSums) + 127) / 128 * 128;
+  static constexpr int kSmem = kDfWarps * kPerWarp;
+};
+__device__ __forceinline__ void df_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void df_copy4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// A piece of an item: units [u_begin, u_end) of the `count` that sequence seq's newest token sees (unit 0 of them is `first`),
+// KV head hk, ng query heads from g0 of its group on. All warps of the block; each leaves its sums (df_place), bounds and
+// denominators in its own part of shared memory: [heads][pitch], [heads], [heads] floats.
+template <int HD, int NH, bool ROPE>
+__device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArgs& a, const DecodeStep& st, unsigned char* smem, int seq,
+                                         int len, int hk, int g0, int ng, int first, int count, int u_begin, int u_end) {
+  using Cfg = DfCfg<HD, NH>;
+  using Pipe = DfPipe<HD, NH>;
+  constexpr int KS = HD / 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int G = a.n_q / a.n_kv;
+  const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.max_pages;
+  const int lo = first_visible_key(len - 1, a.window);
+  unsigned char* mine = smem + warp * Pipe::kPerWarp;
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(mine);
+
+  int u = first + u_begin + warp;
+  const int u_stop = first + u_end;
+  auto page_of = [&](int v) { return v < u_stop ? pages[v >> 1] : 0; };
+  auto issue = [&](int v, int page, int stage) {
+    if (v < u_stop) {
+      const size_t row = (size_t)page * a.n_kv + hk;
+      const size_t off = (row * kFp8Page + (v & 1) * kDfUnit) * HD + lane * 16;
+      const uint32_t dst = ring + stage * Pipe::kUnit;
+#pragma unroll
+      for (int i = 0; i < Pipe::kHalf / 512; ++i) {
+        const int line = i * 4 + (lane >> 3), to = line * 128 + ((lane & 7) ^ df_swizzle<HD>(line)) * 16;
+        df_copy16(dst + to, a.k + off + i * 512);
+        df_copy16(dst + Pipe::kHalf + to, a.v + off + i * 512);
+      }
+      if (lane < 2) df_copy4(dst + 2 * Pipe::kHalf + lane * 4, (lane ? a.v_exp : a.k_exp) + row * kPageExps);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  const size_t q_pitch = (size_t)(ROPE ? a.n_q + 2 * a.n_kv : a.n_q) * HD;
+  if (ROPE && u_end == count && u_begin < count && (count - 1 - u_begin) % kDfWarps == warp)
+    df_append<HD>(q + seq * q_pitch, a, st, hk, len, pages[(first + count - 1) >> 1]);            // this warp reads that block itself
+  int pg_next;                       // page of the next unit to be asked for
+  {
+    int pg[Pipe::kStages];
+#pragma unroll
+    for (int i = 0; i < Pipe::kStages; ++i) pg[i] = page_of(u + i * kDfWarps);
+#pragma unroll
+    for (int i = 0; i < Pipe::kStages - 1; ++i) issue(u + i * kDfWarps, pg[i], i);
+    pg_next = pg[Pipe::kStages - 1];
+  }
+
+  // the queries: for head g of each group of 8, columns in the order of the keys' codes
+  unsigned qb[NH][KS][2];
+  float q_scale[NH][2];              // of heads 2t, 2t + 1: scale log2(e) 2^(what the queries were shifted by)
+#pragma unroll
+  for (int nh = 0; nh < NH; ++nh) {
+    const bool there = nh * 8 + g < ng;
+    const __nv_bfloat16* row = q + seq * q_pitch + (size_t)(hk * G + g0 + (there ? nh * 8 + g : 0)) * HD;
+    uint2 raw[KS];
+    float big = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int col = (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;
+      raw[ks] = there ? *reinterpret_cast<const uint2*>(row + col) : make_uint2(0u, 0u);
+      if (ROPE) {
+        // four columns and the four that they are rotated with, half a head away
+        const bool upper = col >= HD / 2;
+        const uint2 other = there ? *reinterpret_cast<const uint2*>(row + (upper ? col - HD / 2 : col + HD / 2)) : make_uint2(0u, 0u);
+        const float4* cs = st.rope + ((size_t)min(len - 1, st.table_len - 1) * (HD / 2) + (upper ? col - HD / 2 : col)) / 2;
+        const float4 c0 = cs[0], c1 = cs[1];
+        auto turned = [&](unsigned x, unsigned y, const float4& c) {
+          const float2 u2 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+          const float2 v2 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y));
+          const float p0 = __fmul_rn(u2.x, c.x), p1 = __fmul_rn(u2.y, c.z), r0 = __fmul_rn(v2.x, c.y), r1 = __fmul_rn(v2.y, c.w);
+          const __nv_bfloat162 z = upper ? __floats2bfloat162_rn(__fadd_rn(p0, r0), __fadd_rn(p1, r1))
+                                         : __floats2bfloat162_rn(__fsub_rn(p0, r0), __fsub_rn(p1, r1));
+          return *reinterpret_cast<const unsigned*>(&z);
+        };
+        raw[ks] = make_uint2(turned(raw[ks].x, other.x, c0), turned(raw[ks].y, other.y, c1));
+      }
+      const float2 y0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
+      const float2 y1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
+      big = fmaxf(big, fmaxf(fmaxf(fabsf(y0.x), fabsf(y0.y)), fmaxf(fabsf(y1.x), fabsf(y1.y))));
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // the exponent that brings the largest number into [2^14, 2^15); a head that is not finite stays as it is
+    const int eb = (int)(__float_as_uint(big) >> 23);
+    const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);
+    const float f = pow2_of(shift);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const float2 y0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
+      const float2 y1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
+      qb[nh][ks][0] = df_half2(y0.x * f, y0.y * f);
+      qb[nh][ks][1] = df_half2(y1.x * f, y1.y * f);
+    }
+    const float back = a.scale2 * pow2_of(-shift);
+    q_scale[nh][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+    q_scale[nh][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
+  }
+  float o[NH][KS][4];
+  float R[NH][2], l[NH][2];          // a head's bound, and this lane's share of its denominator
+#pragma unroll
+  for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+    for (int i = 0; i < KS; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.f;
+    R[nh][0] = R[nh][1] = -INFINITY;
+    l[nh][0] = l[nh][1] = 0.f;
+  }
+
+  int stage = 0, ahead = Pipe::kStages - 1;                  // where this unit lies, and where the one to be asked for goes
+  for (; u < u_stop; u += kDfWarps) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(Pipe::kStages - 2) : "memory");
+    __syncwarp();                    // everyone's share of the unit is there, and everyone has read the unit before
+    issue(u + (Pipe::kStages - 1) * kDfWarps, pg_next, ahead);
+    pg_next = page_of(u + Pipe::kStages * kDfWarps);
+    const unsigned char* at = mine + stage * Pipe::kUnit;
+    ahead = stage;
+    stage = stage + 1 == Pipe::kStages ? 0 : stage + 1;
+    // S^T = K Q^T, block by block
+    float s[2][NH][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh) s[b][nh][0] = s[b][nh][1] = s[b][nh][2] = s[b][nh][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < HD / 64; ++c) {
+      uint4 k4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k4[i] = *reinterpret_cast<const uint4*>(at + df_at<HD>(g + 8 * i, c * 4 + t));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const unsigned ka = w == 0 ? k4[2 * b].x : w == 1 ? k4[2 * b].y : w == 2 ? k4[2 * b].z : k4[2 * b].w;
+          const unsigned kb = w == 0 ? k4[2 * b + 1].x : w == 1 ? k4[2 * b + 1].y : w == 2 ? k4[2 * b + 1].z : k4[2 * b + 1].w;
+          const unsigned a0 = df_lo(ka), a1 = df_lo(kb), a2 = df_hi(ka), a3 = df_hi(kb);
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) df_mma(s[b][nh], a0, a1, a2, a3, qb[nh][c * 4 + w][0], qb[nh][c * 4 + w][1]);
+        }
+      }
+    }
+    unsigned exps = lane < 2 ? *reinterpret_cast<const unsigned*>(at + 2 * Pipe::kHalf + lane * 4) : 0u;
+    exps >>= (u & 1) * 16;
+    const unsigned kes = __shfl_sync(0xffffffffu, exps, 0), ves = __shfl_sync(0xffffffffu, exps, 1);
+    const int p0 = u * kDfUnit;
+    const bool edge = p0 < lo || p0 + kDfUnit > len;
+    float back[2];
+    bool grow = false;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int ke = clamp_exponent((int)(signed char)(kes >> (8 * b) & 0xffu)), ve = clamp_exponent((int)(signed char)(ves >> (8 * b) & 0xffu));
+      const float kf = pow2_of(ke), add = (float)ve;
+      back[b] = pow2_of(-ve);
+      const int p = p0 + b * kExpBlock + g;
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh) {
+        const float f0 = q_scale[nh][0] * kf, f1 = q_scale[nh][1] * kf;
+        float* x = s[b][nh];
+        x[0] = fmaf(x[0], f0, add);
+        x[1] = fmaf(x[1], f1, add);
+        x[2] = fmaf(x[2], f0, add);
+        x[3] = fmaf(x[3], f1, add);
+        if (edge) {
+          if (p < lo || p >= len) x[0] = x[1] = -INFINITY;
+          if (p + 8 < lo || p + 8 >= len) x[2] = x[3] = -INFINITY;
+        }
+        grow |= fmaxf(x[0], x[2]) > R[nh][0] + kDfSlack || fmaxf(x[1], x[3]) > R[nh][1] + kDfSlack;
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+      // a head has outgrown its bound: all of them follow their largest score
+#pragma unroll
+      for (int nh = 0; nh < NH; ++nh) {
+        float mx0 = fmaxf(fmaxf(s[0][nh][0], s[0][nh][2]), fmaxf(s[1][nh][0], s[1][nh][2]));
+        float mx1 = fmaxf(fmaxf(s[0][nh][1], s[0][nh][3]), fmaxf(s[1][nh][1], s[1][nh][3]));
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
+          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
+        }
+        const float r0 = fmaxf(R[nh][0], mx0), r1 = fmaxf(R[nh][1], mx1);
+        const float al0 = R[nh][0] == -INFINITY ? 0.f : df_exp2(R[nh][0] - r0), al1 = R[nh][1] == -INFINITY ? 0.f : df_exp2(R[nh][1] - r1);
+        R[nh][0] = r0;
+        R[nh][1] = r1;
+        l[nh][0] *= al0;
+        l[nh][1] *= al1;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          o[nh][i][0] *= al0;
+          o[nh][i][1] *= al1;
+          o[nh][i][2] *= al0;
+          o[nh][i][3] *= al1;
+        }
+      }
+    }
+    unsigned wb[2][NH][2];
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh) {
+      const float c0 = (R[nh][0] == -INFINITY ? 0.f : R[nh][0]) - kDfTop, c1 = (R[nh][1] == -INFINITY ? 0.f : R[nh][1]) - kDfTop;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const float* x = s[b][nh];
+        const float w0 = df_exp2(x[0] - c0), w1 = df_exp2(x[1] - c1), w2 = df_exp2(x[2] - c0), w3 = df_exp2(x[3] - c1);
+        l[nh][0] = fmaf(w0 + w2, back[b], l[nh][0]);
+        l[nh][1] = fmaf(w1 + w3, back[b], l[nh][1]);
+        wb[b][nh][0] = df_transpose(df_half2(w0, w1));
+        wb[b][nh][1] = df_transpose(df_half2(w2, w3));
+      }
+    }
+    // O^T += V^T W^T
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      unsigned v[4][HD / 32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned char* p = at + Pipe::kHalf + df_at<HD>(b * kExpBlock + 2 * t + (i & 1) + (i >> 1) * 8, HD == 64 ? g >> 1 : g) +
+                                 (HD == 64 ? (g & 1) * 8 : 0);
+        if (HD == 64) {
+          const uint2 w = *reinterpret_cast<const uint2*>(p);
+          v[i][0] = w.x;
+          v[i][1] = w.y;
+        } else {
+          const uint4 w = *reinterpret_cast<const uint4*>(p);
+          v[i][0] = w.x;
+          v[i][1] = w.y;
+          v[i][HD / 32 - 2] = w.z;
+          v[i][HD / 32 - 1] = w.w;
+        }
+        if (edge) {
+          // values that nobody sees may be anything (a page has had other owners): they must not meet a weight, not even zero
+          const int pos = p0 + b * kExpBlock + 2 * t + (i & 1) + (i >> 1) * 8;
+          if (pos < lo || pos >= len) {
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) v[i][c] = 0u;
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        // four columns of two positions each, interleaved into pairs of neighbouring positions
+        const unsigned e0 = __byte_perm(v[0][c], v[1][c], 0x5140), e1 = __byte_perm(v[0][c], v[1][c], 0x7362);
+        const unsigned h0 = __byte_perm(v[2][c], v[3][c], 0x5140), h1 = __byte_perm(v[2][c], v[3][c], 0x7362);
+        const unsigned b0 = df_lo(e0), b1 = df_hi(e0), b2 = df_lo(h0), b3 = df_hi(h0);
+        const unsigned d0 = df_lo(e1), d1 = df_hi(e1), d2 = df_lo(h1), d3 = df_hi(h1);
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+          df_mma(o[nh][2 * c], b0, b1, b2, b3, wb[b][nh][0], wb[b][nh][1]);
+          df_mma(o[nh][2 * c + 1], d0, d1, d2, d3, wb[b][nh][0], wb[b][nh][1]);
+        }
+      }
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();                      // no lane reads its units any more: the place becomes the results'
+  float* sums = reinterpret_cast<float*>(mine);
+  float* bounds = sums + Cfg::kHeads * Cfg::kPitch;
+#pragma unroll
+  for (int nh = 0; nh < NH; ++nh) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) {
+      l[nh][0] += __shfl_xor_sync(0xffffffffu, l[nh][0], d);
+      l[nh][1] += __shfl_xor_sync(0xffffffffu, l[nh][1], d);
+    }
+    if (g == 0) {
+      bounds[nh * 8 + 2 * t] = R[nh][0];
+      bounds[nh * 8 + 2 * t + 1] = R[nh][1];
+      bounds[Cfg::kHeads + nh * 8 + 2 * t] = l[nh][0];
+      bounds[Cfg::kHeads + nh * 8 + 2 * t + 1] = l[nh][1];
+    }
+    float* dst = sums + (nh * 8 + 2 * t) * Cfg::kPitch + g;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      dst[i * 16] = o[nh][i][0];
+      dst[i * 16 + Cfg::kPitch] = o[nh][i][1];
+      dst[i * 16 + 8] = o[nh][i][2];
+      dst[i * 16 + 8 + Cfg::kPitch] = o[nh][i][3];
+    }
+  }
+}
+
+// One number of a block's result: head h, place `at` of its sums; its bound and denominator with it. Behind a barrier.
+template <int HD, int NH>
+__device__ __forceinline__ void df_of_warps(const unsigned char* smem, int h, int at, float& M, float& num, float& den) {
+  using Cfg = DfCfg<HD, NH>;
+  const float* s[kDfWarps];
+#pragma unroll
+  for (int w = 0; w < kDfWarps; ++w) s[w] = reinterpret_cast<const float*>(smem + w * DfPipe<HD, NH>::kPerWarp);
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kDfWarps; ++w) M = fmaxf(M, s[w][Cfg::kHeads * Cfg::kPitch + h]);
+  const float Mu = M == -INFINITY ? 0.f : M;
+  num = den = 0.f;
+#pragma unroll
+  for (int w = 0; w < kDfWarps; ++w) {
+    const float f = df_exp2(s[w][Cfg::kHeads * Cfg::kPitch + h] - Mu);
+    num = fmaf(f, s[w][h * Cfg::kPitch + at], num);
+    den = fmaf(f, s[w][Cfg::kHeads * (Cfg::kPitch + 1) + h], den);
+  }
+}
+
+// Equal shares of the line of all units.
 template <int HD, int NH, bool ROPE>
 __global__ void __launch_bounds__(kDfThreads, df_per_sm<HD, NH>())
 decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep st) {
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   using Cfg = DfCfg<HD, NH>;
-  constexpr int KS = HD / 16;
-  __shared__ float sums[kDfWarps][Cfg::kHeads * Cfg::kPitch];
-  __shared__ float bound_[kDfWarps][Cfg::kHeads], denom_[kDfWarps][Cfg::kHeads];
+  extern __shared__ __align__(16) unsigned char df_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
   const int G = a.n_q / a.n_kv, chunks = (G + Cfg::kHeads - 1) / Cfg::kHeads, per_seq = a.n_kv * chunks;
-  const long long total = df_total(a) * per_seq;
-  const long long share = df_share(total, gridDim.x);
-  long long cur = (long long)blockIdx.x * share;
-  const long long end = min(cur + share, total);
+  const int total = df_total(a) * per_seq, share = df_share(total, gridDim.x);
+  int cur = blockIdx.x * share;
+  const int end = min(cur + share, total);
   if (blockIdx.x == 0) {
     // sequences that hold nothing: zeros
     for (int s = warp; s < a.n_seqs; s += kDfWarps)
@@ -224,17 +538,17 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
   if (cur >= end) return;
   // the sequence in which the share begins
   int seq = 0, first, count;
-  long long begin = 0;               // where the sequence's units begin on the line
+  int begin = 0;                     // where the sequence's units begin on the line
   {
-    long long before = 0;
+    int before = 0;
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
       int f, c = 0;
       if (s0 + lane < a.n_seqs) df_units(a, a.seq_kvlen[s0 + lane], f, c);
-      long long incl = (long long)c * per_seq;
-      const long long own = incl;
+      int incl = c * per_seq;
+      const int own = incl;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += up;
       }
       const unsigned here = __ballot_sync(0xffffffffu, before + incl > cur);
@@ -247,7 +561,6 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
-
   while (cur < end) {
     const int len = min(a.seq_kvlen[seq], a.max_pages * kFp8Page);
     df_units(a, len, first, count);
@@ -255,246 +568,19 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
       ++seq;
       continue;
     }
-    const int item = (int)((cur - begin) / count);               // (KV head, chunk of query heads)
-    const int u_begin = (int)((cur - begin) - (long long)item * count);
-    const int u_end = (int)min((long long)count, u_begin + (end - cur));
+    const int item = (cur - begin) / count;                      // (KV head, chunk of query heads)
+    const int u_begin = cur - begin - item * count;
+    const int u_end = min(count, u_begin + (end - cur));
     const int hk = item / chunks, g0 = item % chunks * Cfg::kHeads, ng = min(Cfg::kHeads, G - g0);
-    const int* pages = a.block_table + (size_t)a.seq_slot[seq] * a.max_pages;
-    const int lo = first_visible_key(len - 1, a.window);
-
-    auto load = [&](DfUnit<HD>& x, int u, int page) {
-      const size_t row = (size_t)page * a.n_kv + hk;
-      const int b = u & (kPageExps - 1);
-      const unsigned char* kp = a.k + (row * kFp8Page + b * kExpBlock) * HD;
-      const unsigned char* vp = a.v + (row * kFp8Page + b * kExpBlock) * HD;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < HD / 64; ++c) x.k[i][c] = df_load16(kp + (g + 8 * i) * HD + c * 64 + t * 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned char* p = vp + (2 * t + (i & 1) + (i >> 1) * 8) * HD + g * (HD / 8);
-        if (HD == 64) {
-          x.v[i][0] = df_load8(p);
-        } else {
-          const uint4 w = df_load16(p);
-          x.v[i][0] = make_uint2(w.x, w.y);
-          x.v[i][HD / 64 - 1] = make_uint2(w.z, w.w);
-        }
-      }
-      x.ke = clamp_exponent(a.k_exp[row * kPageExps + b]);
-      x.ve = clamp_exponent(a.v_exp[row * kPageExps + b]);
-    };
-    auto page_of = [&](int u) { return pages[u / kPageExps]; };
-
-    int u = first + u_begin + warp;
-    const int u_stop = first + u_end;
-    DfUnit<HD> x0, x1;
-    int pg_next = 0;
-    const size_t q_pitch = (size_t)(ROPE ? a.n_q + 2 * a.n_kv : a.n_q) * HD;
-    if (ROPE && u_begin + 1 <= count && u_end == count && (count - 1 - u_begin) % kDfWarps == warp)
-      df_append<HD>(q + seq * q_pitch, a, st, hk, len, page_of(first + count - 1));     // this warp reads that block itself
-    if (u < u_stop) load(x0, u, page_of(u));
-    if (u + kDfWarps < u_stop) pg_next = page_of(u + kDfWarps);
-
-    // the queries: for head g of each group of 8, columns in the order of the keys' codes
-    unsigned qb[NH][KS][2];
-    float q_scale[NH][2];            // of heads 2t, 2t + 1: scale log2(e) 2^(what the queries were shifted by)
-#pragma unroll
-    for (int nh = 0; nh < NH; ++nh) {
-      const bool there = nh * 8 + g < ng;
-      const __nv_bfloat16* row = q + seq * q_pitch + (size_t)(hk * G + g0 + (there ? nh * 8 + g : 0)) * HD;
-      uint2 raw[KS];
-      float big = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int col = (ks >> 2) * 64 + t * 16 + (ks & 3) * 4;
-        raw[ks] = there ? *reinterpret_cast<const uint2*>(row + col) : make_uint2(0u, 0u);
-        if (ROPE) {
-          // four columns and the four that they are rotated with, half a head away
-          const bool upper = col >= HD / 2;
-          const uint2 other = there ? *reinterpret_cast<const uint2*>(row + (upper ? col - HD / 2 : col + HD / 2)) : make_uint2(0u, 0u);
-          const float4* cs = st.rope + ((size_t)min(len - 1, st.table_len - 1) * (HD / 2) + (upper ? col - HD / 2 : col)) / 2;
-          const float4 c0 = cs[0], c1 = cs[1];
-          auto turned = [&](unsigned x, unsigned y, const float4& c) {
-            const float2 u2 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
-            const float2 v2 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y));
-            const float p0 = __fmul_rn(u2.x, c.x), p1 = __fmul_rn(u2.y, c.z), r0 = __fmul_rn(v2.x, c.y), r1 = __fmul_rn(v2.y, c.w);
-            const __nv_bfloat162 z = upper ? __floats2bfloat162_rn(__fadd_rn(p0, r0), __fadd_rn(p1, r1))
-                                           : __floats2bfloat162_rn(__fsub_rn(p0, r0), __fsub_rn(p1, r1));
-            return *reinterpret_cast<const unsigned*>(&z);
-          };
-          raw[ks] = make_uint2(turned(raw[ks].x, other.x, c0), turned(raw[ks].y, other.y, c1));
-        }
-        const float2 y0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
-        const float2 y1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
-        big = fmaxf(big, fmaxf(fmaxf(fabsf(y0.x), fabsf(y0.y)), fmaxf(fabsf(y1.x), fabsf(y1.y))));
-      }
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // the exponent that brings the largest number into [2^14, 2^15); a head that is not finite stays as it is
-      const int eb = (int)(__float_as_uint(big) >> 23);
-      const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);
-      const float f = pow2_of(shift);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const float2 y0 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
-        const float2 y1 = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
-        qb[nh][ks][0] = df_half2(y0.x * f, y0.y * f);
-        qb[nh][ks][1] = df_half2(y1.x * f, y1.y * f);
-      }
-      const float back = a.scale2 * pow2_of(-shift);
-      q_scale[nh][0] = __shfl_sync(0xffffffffu, back, 8 * t);
-      q_scale[nh][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
-    }
-    float o[NH][KS][4];
-    float R[NH][2], l[NH][2];
-#pragma unroll
-    for (int nh = 0; nh < NH; ++nh) {
-#pragma unroll
-      for (int i = 0; i < KS; ++i) o[nh][i][0] = o[nh][i][1] = o[nh][i][2] = o[nh][i][3] = 0.f;
-      R[nh][0] = R[nh][1] = -INFINITY;
-      l[nh][0] = l[nh][1] = 0.f;
-    }
-
-    auto work = [&](DfUnit<HD>& x, int uu) {
-      float s[NH][4];
-#pragma unroll
-      for (int nh = 0; nh < NH; ++nh) s[nh][0] = s[nh][1] = s[nh][2] = s[nh][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-        const unsigned ka[4] = {x.k[0][c].x, x.k[0][c].y, x.k[0][c].z, x.k[0][c].w};
-        const unsigned kb[4] = {x.k[1][c].x, x.k[1][c].y, x.k[1][c].z, x.k[1][c].w};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const unsigned a0 = df_lo(ka[w]), a1 = df_lo(kb[w]), a2 = df_hi(ka[w]), a3 = df_hi(kb[w]);
-#pragma unroll
-          for (int nh = 0; nh < NH; ++nh) df_mma(s[nh], a0, a1, a2, a3, qb[nh][c * 4 + w][0], qb[nh][c * 4 + w][1]);
-        }
-      }
-      const int p0 = uu * kExpBlock;
-      const bool edge = p0 < lo || p0 + kExpBlock > len;
-      const bool see_a = p0 + g >= lo && p0 + g < len, see_b = p0 + g + 8 >= lo && p0 + g + 8 < len;
-      if (edge) {
-        // values that nobody sees may be anything (a page has had other owners): they must not meet a weight, not even zero
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int p = p0 + 2 * t + (i & 1) + (i >> 1) * 8;
-          if (p < lo || p >= len) {
-#pragma unroll
-            for (int c = 0; c < HD / 64; ++c) x.v[i][c] = make_uint2(0u, 0u);
-          }
-        }
-      }
-      const float kf = pow2_of(x.ke), ve = (float)x.ve, back = pow2_of(-x.ve);
-      unsigned wb[NH][2];
-#pragma unroll
-      for (int nh = 0; nh < NH; ++nh) {
-        const float f0 = q_scale[nh][0] * kf, f1 = q_scale[nh][1] * kf;
-        s[nh][0] = fmaf(s[nh][0], f0, ve);
-        s[nh][1] = fmaf(s[nh][1], f1, ve);
-        s[nh][2] = fmaf(s[nh][2], f0, ve);
-        s[nh][3] = fmaf(s[nh][3], f1, ve);
-        if (edge) {
-          if (!see_a) s[nh][0] = s[nh][1] = -INFINITY;
-          if (!see_b) s[nh][2] = s[nh][3] = -INFINITY;
-        }
-        float mx0 = fmaxf(s[nh][0], s[nh][2]), mx1 = fmaxf(s[nh][1], s[nh][3]);
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) {
-          mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, d));
-          mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, d));
-        }
-        const float r0 = fmaxf(R[nh][0], mx0), r1 = fmaxf(R[nh][1], mx1);
-        const float c0 = r0 == -INFINITY ? 0.f : r0 - 15.f, c1 = r1 == -INFINITY ? 0.f : r1 - 15.f;
-        const float al0 = df_exp2(R[nh][0] - 15.f - c0), al1 = df_exp2(R[nh][1] - 15.f - c1);   // 0 while R is -inf
-        R[nh][0] = r0;
-        R[nh][1] = r1;
-        const float w0 = df_exp2(s[nh][0] - c0), w1 = df_exp2(s[nh][1] - c1), w2 = df_exp2(s[nh][2] - c0), w3 = df_exp2(s[nh][3] - c1);
-        l[nh][0] = fmaf(l[nh][0], al0, (w0 + w2) * back);
-        l[nh][1] = fmaf(l[nh][1], al1, (w1 + w3) * back);
-        wb[nh][0] = df_transpose(df_half2(w0, w1));
-        wb[nh][1] = df_transpose(df_half2(w2, w3));
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-          o[nh][i][0] *= al0;
-          o[nh][i][1] *= al1;
-          o[nh][i][2] *= al0;
-          o[nh][i][3] *= al1;
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < HD / 64; ++c) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          // four columns of two positions each, interleaved into pairs of neighbouring positions
-          const unsigned va = w ? x.v[0][c].y : x.v[0][c].x, vb = w ? x.v[1][c].y : x.v[1][c].x;
-          const unsigned vc = w ? x.v[2][c].y : x.v[2][c].x, vd = w ? x.v[3][c].y : x.v[3][c].x;
-          const unsigned e0 = __byte_perm(va, vb, 0x5140), e1 = __byte_perm(va, vb, 0x7362);
-          const unsigned h0 = __byte_perm(vc, vd, 0x5140), h1 = __byte_perm(vc, vd, 0x7362);
-          const int i = (c * 2 + w) * 2;
-#pragma unroll
-          for (int nh = 0; nh < NH; ++nh) {
-            df_mma(o[nh][i], df_lo(e0), df_hi(e0), df_lo(h0), df_hi(h0), wb[nh][0], wb[nh][1]);
-            df_mma(o[nh][i + 1], df_lo(e1), df_hi(e1), df_lo(h1), df_hi(h1), wb[nh][0], wb[nh][1]);
-          }
-        }
-      }
-    };
-
-    while (u < u_stop) {
-      if (u + kDfWarps < u_stop) load(x1, u + kDfWarps, pg_next);
-      if (u + 2 * kDfWarps < u_stop) pg_next = page_of(u + 2 * kDfWarps);
-      work(x0, u);
-      u += kDfWarps;
-      if (u >= u_stop) break;
-      if (u + kDfWarps < u_stop) load(x0, u + kDfWarps, pg_next);
-      if (u + 2 * kDfWarps < u_stop) pg_next = page_of(u + 2 * kDfWarps);
-      work(x1, u);
-      u += kDfWarps;
-    }
-
-    // ---- the warps' results meet
-#pragma unroll
-    for (int nh = 0; nh < NH; ++nh) {
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        l[nh][0] += __shfl_xor_sync(0xffffffffu, l[nh][0], d);
-        l[nh][1] += __shfl_xor_sync(0xffffffffu, l[nh][1], d);
-      }
-      if (g == 0) {
-        bound_[warp][nh * 8 + 2 * t] = R[nh][0];
-        bound_[warp][nh * 8 + 2 * t + 1] = R[nh][1];
-        denom_[warp][nh * 8 + 2 * t] = l[nh][0];
-        denom_[warp][nh * 8 + 2 * t + 1] = l[nh][1];
-      }
-      float* mine = sums[warp] + (nh * 8 + 2 * t) * Cfg::kPitch + g;
-#pragma unroll
-      for (int i = 0; i < KS; ++i) {
-        mine[i * 16] = o[nh][i][0];
-        mine[i * 16 + Cfg::kPitch] = o[nh][i][1];
-        mine[i * 16 + 8] = o[nh][i][2];
-        mine[i * 16 + 8 + Cfg::kPitch] = o[nh][i][3];
-      }
-    }
+    df_piece<HD, NH, ROPE>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
     __syncthreads();
-    const bool starts = u_begin == 0, ends = u_end == count;
+    const bool starts = u_begin == 0, whole = starts && u_end == count;
     float* rec = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Cfg::kRecord;
     for (int i = threadIdx.x; i < ng * HD; i += kDfThreads) {
       const int h = i / HD, d = i % HD;
-      const int at = (starts && ends) ? df_place<HD>(d) : d;     // a partial result stays in the order of the sums
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kDfWarps; ++w) M = fmaxf(M, bound_[w][h]);
-      const float Mu = M == -INFINITY ? 0.f : M;
-      float num = 0.f, den = 0.f;
-#pragma unroll
-      for (int w = 0; w < kDfWarps; ++w) {
-        const float f = df_exp2(bound_[w][h] - Mu);
-        num = fmaf(f, sums[w][h * Cfg::kPitch + at], num);
-        den = fmaf(f, denom_[w][h], den);
-      }
-      if (starts && ends) {
+      float M, num, den;
+      df_of_warps<HD, NH>(df_smem, h, whole ? df_place<HD>(d) : d, M, num, den);      // a partial result stays in the order of the sums
+      if (whole) {
         a.out[((size_t)seq * a.n_q + hk * G + g0 + h) * HD + d] = __float2bfloat16_rn(num / den);
       } else {
         rec[h * HD + d] = num;
@@ -506,76 +592,224 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
     }
     __syncthreads();                 // shared memory may be written again
     cur += u_end - u_begin;
-    if (item + 1 == per_seq && ends) {
-      begin += (long long)count * per_seq;
+    if (item + 1 == per_seq && u_end == count) {
+      begin += count * per_seq;
       ++seq;
     }
   }
 }
 
-// Joins the partial results of the items that lie in several shares. grid (n_seqs * items of a sequence, heads of an item); HD threads.
-template <int HD, int NH>
-__global__ void __launch_bounds__(HD) decode_fp8_join_kernel(const DecodeArgs a, int blocks) {
+// Few short sequences: an item is one cluster's, its units in equal runs over the cluster's blocks, which read one another's
+// results from shared memory. grid (blocks of a cluster, items of a sequence, sequences). One launch, no partial results.
+template <int HD, int NH, bool ROPE>
+__global__ void __launch_bounds__(kDfThreads, df_per_sm<HD, NH>())
+decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep st) {
   pdl_launch_dependents();
   pdl_wait();
   using Cfg = DfCfg<HD, NH>;
+  extern __shared__ __align__(16) unsigned char df_smem[];
+  __shared__ float joined[Cfg::kHeads * (HD + 2)];           // this block's result: sums, bounds, denominators
+  const int G = a.n_q / a.n_kv, chunks = (G + Cfg::kHeads - 1) / Cfg::kHeads;
+  const int seq = blockIdx.z, hk = blockIdx.y / chunks, g0 = blockIdx.y % chunks * Cfg::kHeads, ng = min(Cfg::kHeads, G - g0);
+  const int len = min(a.seq_kvlen[seq], a.max_pages * kFp8Page);
+  int first, count;
+  df_units(a, len, first, count);
+  __nv_bfloat16* out = a.out + ((size_t)seq * a.n_q + hk * G + g0) * HD;
+  if (count == 0) {                  // the whole cluster alike
+    for (int i = blockIdx.x * kDfThreads + threadIdx.x; i < ng * HD; i += gridDim.x * kDfThreads) out[i] = __float2bfloat16_rn(0.f);
+    return;
+  }
+  const int u_begin = count * blockIdx.x / gridDim.x, u_end = count * (blockIdx.x + 1) / gridDim.x;
+  df_piece<HD, NH, ROPE>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
+  __syncthreads();
+  for (int i = threadIdx.x; i < ng * HD; i += kDfThreads) {
+    const int h = i / HD, d = i % HD;
+    float M, num, den;
+    df_of_warps<HD, NH>(df_smem, h, df_place<HD>(d), M, num, den);
+    if (gridDim.x == 1) {
+      out[i] = __float2bfloat16_rn(num / den);
+      continue;
+    }
+    joined[i] = num;
+    if (d == 0) {
+      joined[Cfg::kHeads * HD + h] = M;
+      joined[Cfg::kHeads * (HD + 1) + h] = den;
+    }
+  }
+  if (gridDim.x == 1) return;
+  tc::cluster_sync_all();
+  const uint32_t here = (uint32_t)__cvta_generic_to_shared(joined);
+  for (int i = blockIdx.x * kDfThreads + threadIdx.x; i < ng * HD; i += gridDim.x * kDfThreads) {
+    const int h = i / HD;
+    float m[8], n[8], l[8], M = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      if (b >= gridDim.x) continue;
+      const uint32_t there = tc::map_to_block(here, b);
+      m[b] = tc::ld_cluster_f32(there + (Cfg::kHeads * HD + h) * 4);
+      n[b] = tc::ld_cluster_f32(there + i * 4);
+      l[b] = tc::ld_cluster_f32(there + (Cfg::kHeads * (HD + 1) + h) * 4);
+    }
+#pragma unroll
+    for (int b = 0; b < 8; ++b)
+      if (b < gridDim.x) M = fmaxf(M, m[b]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      if (b >= gridDim.x) continue;
+      const float f = df_exp2(m[b] - Mu);
+      num = fmaf(f, n[b], num);
+      den = fmaf(f, l[b], den);
+    }
+    out[i] = __float2bfloat16_rn(num / den);
+  }
+  tc::cluster_sync_all();            // nobody's shared memory goes before everyone has read it
+}
+
+// Joins the partial results of the items that lie in several shares. grid (items of all sequences, heads side by side); four threads
+// a column, a quarter of the partial results each.
+constexpr int kDfSlices = 4;
+template <int HD, int NH>
+__global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const DecodeArgs a, int blocks) {
+  pdl_launch_dependents();
+  using Cfg = DfCfg<HD, NH>;
+  __shared__ float factor[kSms * 6], denom[kSms * 6], part_num[kDfSlices][HD], part_den[kDfSlices * HD / 32], top[kDfSlices * HD / 32];
   const int G = a.n_q / a.n_kv, chunks = (G + Cfg::kHeads - 1) / Cfg::kHeads, per_seq = a.n_kv * chunks;
   const int seq = blockIdx.x / per_seq, item = blockIdx.x % per_seq;
-  const int hk = item / chunks, g0 = item % chunks * Cfg::kHeads, h = blockIdx.y;
-  if (h >= min(Cfg::kHeads, G - g0)) return;
-  const int lane = threadIdx.x & 31;
+  const int hk = item / chunks, g0 = item % chunks * Cfg::kHeads, ng = min(Cfg::kHeads, G - g0);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int first, count;
-  df_units(a, a.seq_kvlen[seq], first, count);
-  if (count == 0) return;
-  long long all = 0, ahead = 0;
+  int all = 0, ahead = 0;
   for (int s = lane; s < a.n_seqs; s += 32) {
     int f, c;
     df_units(a, a.seq_kvlen[s], f, c);
     all += c;
     ahead += s < seq ? c : 0;
   }
+  df_units(a, a.seq_kvlen[seq], first, count);
+  if (count == 0) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     all += __shfl_xor_sync(0xffffffffu, all, o);
     ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
   }
-  const long long share = df_share(all * per_seq, blocks);
-  const long long begin = ahead * per_seq + (long long)item * count;
-  const int c0 = (int)(begin / share), c1 = (int)((begin + count - 1) / share);
-  if (c0 == c1) return;
-  auto record = [&](int c) { return a.part + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * Cfg::kRecord; };
-  float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(record(c) + Cfg::kHeads * HD + h));
-  M = warp_max(M);
-  const float Mu = M == -INFINITY ? 0.f : M;
-  const int d = threadIdx.x;
-  float num = 0.f, den = 0.f;
-  for (int b = c0; b <= c1; b += 32) {
-    float f = 0.f;
-    if (b + lane <= c1) {
-      const float* r = record(b + lane) + Cfg::kHeads * HD;
-      f = df_exp2(__ldcg(r + h) - Mu);
-      den = fmaf(f, __ldcg(r + Cfg::kHeads + h), den);
+  const int share = df_share(all * per_seq, blocks);
+  const int begin = ahead * per_seq + item * count;
+  const int c0 = begin / share, n = (begin + count - 1) / share - c0 + 1;
+  if (n == 1) return;
+  // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait).
+  pdl_wait();
+  // partial result i: the first lies where a piece begins with its item, the others where one goes on
+  const float* base = a.part + (size_t)c0 * 2 * Cfg::kRecord;
+  auto record = [&](int i) { return base + (size_t)(i == 0 ? 1 : 2 * i) * Cfg::kRecord; };
+  __nv_bfloat16* out = a.out + ((size_t)seq * a.n_q + hk * G + g0) * HD;
+  // the column whose sum is at place d
+  auto column = [](int d) { return (d % 8) * (HD / 8) + (d / 16) * 2 + (d / 8 & 1); };
+  if (n <= 4) {
+    // few of them (many sequences): a thread a column, everything asked for at once
+    for (int x = blockIdx.y * kDfSlices * HD + threadIdx.x; x < ng * HD; x += gridDim.y * kDfSlices * HD) {
+      const int h = x / HD;
+      float m[4], l[4], v[4], M = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] = i < n ? __ldcg(record(i) + Cfg::kHeads * HD + h) : -INFINITY;
+        l[i] = i < n ? __ldcg(record(i) + Cfg::kHeads * (HD + 1) + h) : 0.f;
+        v[i] = i < n ? __ldcg(record(i) + x) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) M = fmaxf(M, m[i]);
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float num = 0.f, den = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = df_exp2(m[i] - Mu);
+        num = fmaf(f, v[i], num);
+        den = fmaf(f, l[i], den);
+      }
+      out[h * HD + column(x % HD)] = __float2bfloat16_rn(num / den);
     }
-    const int n = min(32, c1 - b + 1);
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) num = fmaf(__shfl_sync(0xffffffffu, f, i), __ldcg(record(b + i) + h * HD + d), num);
+    return;
   }
-  den = warp_sum(den);
-  // this thread's sum stands for the column whose place it is
-  constexpr int R = HD / 8;
-  const int col = (d % 8) * R + (d / 16) * 2 + (d / 8 & 1);
-  a.out[((size_t)seq * a.n_q + hk * G + g0 + h) * HD + col] = __float2bfloat16_rn(num / den);
+  const int d = threadIdx.x % HD, slice = threadIdx.x / HD;
+  for (int h = blockIdx.y; h < ng; h += gridDim.y) {
+    // the first numbers are asked for before their factors are known
+    float v[8];
+    int i = slice;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = i + e * kDfSlices < n ? __ldcg(record(i + e * kDfSlices) + h * HD + d) : 0.f;
+    float M = -INFINITY;
+    for (int k = threadIdx.x; k < n; k += kDfSlices * HD) {
+      const float m = __ldcg(record(k) + Cfg::kHeads * HD + h);
+      factor[k] = m;
+      denom[k] = __ldcg(record(k) + Cfg::kHeads * (HD + 1) + h);
+      M = fmaxf(M, m);
+    }
+    M = warp_max(M);
+    if (lane == 0) top[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kDfSlices * HD / 32; ++w) M = fmaxf(M, top[w]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float den = 0.f;
+    for (int k = threadIdx.x; k < n; k += kDfSlices * HD) {
+      const float f = df_exp2(factor[k] - Mu);
+      factor[k] = f;
+      den = fmaf(f, denom[k], den);
+    }
+    den = warp_sum(den);
+    if (lane == 0) part_den[warp] = den;
+    __syncthreads();
+    float num = 0.f;
+    while (i < n) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e * kDfSlices < n) num = fmaf(factor[i + e * kDfSlices], v[e], num);
+      i += 8 * kDfSlices;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = i + e * kDfSlices < n ? __ldcg(record(i + e * kDfSlices) + h * HD + d) : 0.f;
+    }
+    part_num[slice][d] = num;
+    __syncthreads();
+    if (slice == 0) {
+      den = 0.f;
+#pragma unroll
+      for (int w = 0; w < kDfSlices * HD / 32; ++w) den += part_den[w];
+#pragma unroll
+      for (int e = 1; e < kDfSlices; ++e) num += part_num[e][d];
+      out[h * HD + column(d)] = __float2bfloat16_rn(num / den);
+    }
+    __syncthreads();
+  }
 }
 
-template <int HD, int NH>
-static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& st, cudaStream_t stream) {
-  constexpr int blocks = df_blocks<HD, NH>();
-  if (st.rope) launch_k(decode_fp8_kernel<HD, NH, true>, dim3(blocks), dim3(kDfThreads), 0, stream, (const __nv_bfloat16*)q, a, st);
-  else launch_k(decode_fp8_kernel<HD, NH, false>, dim3(blocks), dim3(kDfThreads), 0, stream, (const __nv_bfloat16*)q, a, st);
-  LLMIE_LAUNCH_CHECK();
+template <int HD, int NH, bool ROPE>
+static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& st, int max_kv_len, cudaStream_t stream) {
+  constexpr int smem = DfPipe<HD, NH>::kSmem;
   const int G = a.n_q / a.n_kv, chunks = (G + 8 * NH - 1) / (8 * NH);
-  launch_k(decode_fp8_join_kernel<HD, NH>, dim3((unsigned)(a.n_seqs * a.n_kv * chunks), min(G, 8 * NH)), dim3(HD), 0, stream, a, blocks);
+  const long long items = (long long)a.n_seqs * a.n_kv * chunks;
+  // units of the longest sequence, as far as the caller knows
+  long long units = max_kv_len > 0 ? max_kv_len : (long long)a.max_pages * kFp8Page;
+  if (a.window > 0 && a.window + kDfUnit < units) units = a.window + kDfUnit;
+  if (a.window < 0 && -(long long)a.window < units) units = -(long long)a.window;
+  units = (units + kDfUnit - 1) / kDfUnit;
+  int cluster = 1;
+  while (cluster < 8 && 2 * cluster * items <= df_blocks<HD, NH>() && 2 * cluster * kDfWarps <= units) cluster *= 2;
+  if (units <= (long long)cluster * kDfWarps * kDfFew && items <= df_blocks<HD, NH>() && items <= 65535) {
+    cudaError_t e = cudaFuncSetAttribute(decode_fp8_cluster_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    launch_k_cluster(decode_fp8_cluster_kernel<HD, NH, ROPE>, dim3(cluster, a.n_kv * chunks, a.n_seqs), dim3(kDfThreads), smem, stream,
+                     cluster, (const __nv_bfloat16*)q, a, st);
+    LLMIE_LAUNCH_CHECK();
+    return LLMIE_OK;
+  }
+  cudaError_t e = cudaFuncSetAttribute(decode_fp8_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return (int)e;
+  constexpr int blocks = df_blocks<HD, NH>();
+  launch_k(decode_fp8_kernel<HD, NH, ROPE>, dim3(blocks), dim3(kDfThreads), smem, stream, (const __nv_bfloat16*)q, a, st);
+  LLMIE_LAUNCH_CHECK();
+  const int side = (int)max(1LL, min((long long)min(G, 8 * NH), 4 * kSms / items));
+  launch_k(decode_fp8_join_kernel<HD, NH>, dim3((unsigned)items, side), dim3(kDfSlices * HD), 0, stream, a, blocks);
   LLMIE_LAUNCH_CHECK();
   return LLMIE_OK;
 }
@@ -595,30 +829,36 @@ extern "C" int llmie_attention_decode_fp8_scratch(int n_q, int n_kv, int hd) {
 static int decode_fp8_entry(const void* q, const void* k_cache, const void* v_cache, const void* k_exp, const void* v_exp, void* out,
                             float* scratch, const float* rope, int table_len, const int* seq_slot, const int* seq_kvlen,
                             const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd, float scale, int window,
-                            cudaStream_t stream) {
+                            int max_kv_len, cudaStream_t stream) {
   if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || max_pages > (1 << 24) || !scratch) return LLMIE_ERR_BAD_ARG;
   if (hd != 64 && hd != 128) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache)) return LLMIE_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 3u) return LLMIE_ERR_ALIGNMENT;   // a page's four at once
   if (n_seqs == 0) return LLMIE_OK;
-  if ((long long)n_seqs * n_q > 0x7fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  if ((double)n_seqs * n_q * max_pages * 2 > 1.0e9) return LLMIE_ERR_UNSUPPORTED_SIZE;       // the line of units is counted in 32 bits
   const DecodeArgs a{(const unsigned char*)k_cache, (const unsigned char*)v_cache, (const signed char*)k_exp, (const signed char*)v_exp,
                      (__nv_bfloat16*)out, scratch, seq_slot, seq_kvlen, block_table, max_pages, n_seqs, n_q, n_kv,
                      scale * 1.4426950408889634f, window};
   const DecodeStep st{(const float4*)rope, table_len, (unsigned char*)k_cache, (unsigned char*)v_cache, (signed char*)k_exp, (signed char*)v_exp};
   const bool one = n_q / n_kv <= 8;
-  if (hd == 64) return one ? launch_decode<64, 1>(q, a, st, stream) : launch_decode<64, 2>(q, a, st, stream);
-  return one ? launch_decode<128, 1>(q, a, st, stream) : launch_decode<128, 2>(q, a, st, stream);
+#define LLMIE_DECODE(HD, NH) return rope ? launch_decode<HD, NH, true>(q, a, st, max_kv_len, stream) : launch_decode<HD, NH, false>(q, a, st, max_kv_len, stream)
+  if (hd == 64 && one) LLMIE_DECODE(64, 1);
+  if (hd == 64) LLMIE_DECODE(64, 2);
+  if (one) LLMIE_DECODE(128, 1);
+  LLMIE_DECODE(128, 2);
+#undef LLMIE_DECODE
 }
 
 // q, out bfloat16 [n_seqs, n_q hd], hd 64 or 128; caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv, 4];
 // seq_kvlen: keys that each sequence holds, this step's among them (0: its rows become zeros). window as in the other attention
-// kernels. scratch: llmie_attention_decode_fp8_scratch floats, 16-byte aligned.
+// kernels. max_kv_len: no sequence is longer (0: not known); the choice of the kernel goes by it, not its result.
+// scratch: llmie_attention_decode_fp8_scratch floats, 16-byte aligned.
 extern "C" int llmie_attention_decode_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_exp,
                                           const void* v_exp, void* out, float* scratch, const int* seq_slot, const int* seq_kvlen,
                                           const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd,
-                                          float scale, int window, cudaStream_t stream) {
+                                          float scale, int window, int max_kv_len, cudaStream_t stream) {
   return decode_fp8_entry(q, k_cache, v_cache, k_exp, v_exp, out, scratch, nullptr, 0, seq_slot, seq_kvlen, block_table, max_pages,
-                          n_seqs, n_q, n_kv, hd, scale, window, stream);
+                          n_seqs, n_q, n_kv, hd, scale, window, max_kv_len, stream);
 }
 
 // The same from a step's projections: qkv bfloat16 [n_seqs, (n_q + 2 n_kv) hd], rope float32 [table_len, hd / 2, 2] the (cos, sin) of
@@ -627,9 +867,9 @@ extern "C" int llmie_attention_decode_fp8(const void* q, const void* k_cache, co
 extern "C" int llmie_attention_decode_fp8_rope(const void* qkv, void* k_cache, void* v_cache, void* k_exp, void* v_exp, void* out,
                                                float* scratch, const float* rope, int table_len, const int* seq_slot,
                                                const int* seq_kvlen, const int* block_table, int max_pages, int n_seqs, int n_q,
-                                               int n_kv, int hd, float scale, int window, cudaStream_t stream) {
+                                               int n_kv, int hd, float scale, int window, int max_kv_len, cudaStream_t stream) {
   if (!rope || table_len <= 0 || n_kv <= 0 || n_q / n_kv > 16) return LLMIE_ERR_BAD_ARG;
   if (!aligned16(rope)) return LLMIE_ERR_ALIGNMENT;
   return decode_fp8_entry(qkv, k_cache, v_cache, k_exp, v_exp, out, scratch, rope, table_len, seq_slot, seq_kvlen, block_table,
-                          max_pages, n_seqs, n_q, n_kv, hd, scale, window, stream);
+                          max_pages, n_seqs, n_q, n_kv, hd, scale, window, max_kv_len, stream);
 }

@@ -1774,10 +1774,10 @@ def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_k
     _need_here("attention_decode_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
     scratch = _decode_fp8_scratch(n_q, n_kv, head_dim, q.device)
     _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8", [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_void_p])
+    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8", [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p])
     _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
              scratch.data_ptr(), seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), block_table.shape[1], n, n_q,
-             n_kv, head_dim, float(scale), int(window), _stream()), "attention_decode_fp8")
+             n_kv, head_dim, float(scale), int(window), int(max_kv_len), _stream()), "attention_decode_fp8")
     return out
 
 
@@ -1801,11 +1801,11 @@ def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, s
     scratch = _decode_fp8_scratch(n_q, n_kv, head_dim, qkv.device)
     _work(_nbytes(qkv, out) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
     f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_rope",
-            [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_void_p])
+            [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p])
     _check(f(qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
              scratch.data_ptr(), table.data_ptr(), table.shape[0], seq_slot.data_ptr(), seq_kvlen.data_ptr(),
-             block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv, head_dim, float(scale), int(window), _stream()),
-           "attention_decode_fp8_rope")
+             block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv, head_dim, float(scale), int(window), int(max_kv_len),
+             _stream()), "attention_decode_fp8_rope")
     return out
 
 
