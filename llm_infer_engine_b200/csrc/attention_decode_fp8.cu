@@ -30,6 +30,7 @@ constexpr int kDfWarps = 4;
 constexpr int kDfUnit = 2 * kExpBlock;
 constexpr int kDfThreads = kDfWarps * 32;
 constexpr int kSms = 148;
+constexpr int kNeedsScratch = -5;    // the answer to a call without scratch that cannot do without
 constexpr float kDfSlack = 8.f;      // how far scores may outgrow a head's bound, in units of log2
 constexpr float kDfTop = 7.f;        // the bound's own weight is 2^7: none is above 2^15
 constexpr int kDfFew = 12;           // units a warp up to which an item is one cluster's
@@ -803,6 +804,7 @@ static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& s
     LLMIE_LAUNCH_CHECK();
     return LLMIE_OK;
   }
+  if (!a.part) return kNeedsScratch;
   cudaError_t e = cudaFuncSetAttribute(decode_fp8_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return (int)e;
   constexpr int blocks = df_blocks<HD, NH>();
@@ -830,7 +832,7 @@ static int decode_fp8_entry(const void* q, const void* k_cache, const void* v_ca
                             float* scratch, const float* rope, int table_len, const int* seq_slot, const int* seq_kvlen,
                             const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd, float scale, int window,
                             int max_kv_len, cudaStream_t stream) {
-  if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || max_pages > (1 << 24) || !scratch) return LLMIE_ERR_BAD_ARG;
+  if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || max_pages > (1 << 24)) return LLMIE_ERR_BAD_ARG;
   if (hd != 64 && hd != 128) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache)) return LLMIE_ERR_ALIGNMENT;
   if ((reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 3u) return LLMIE_ERR_ALIGNMENT;   // a page's four at once
@@ -852,7 +854,7 @@ static int decode_fp8_entry(const void* q, const void* k_cache, const void* v_ca
 // q, out bfloat16 [n_seqs, n_q hd], hd 64 or 128; caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv, 4];
 // seq_kvlen: keys that each sequence holds, this step's among them (0: its rows become zeros). window as in the other attention
 // kernels. max_kv_len: no sequence is longer (0: not known); the choice of the kernel goes by it, not its result.
-// scratch: llmie_attention_decode_fp8_scratch floats, 16-byte aligned.
+// scratch: llmie_attention_decode_fp8_scratch floats, 16-byte aligned; null: a call that needs it launches nothing and returns -5.
 extern "C" int llmie_attention_decode_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_exp,
                                           const void* v_exp, void* out, float* scratch, const int* seq_slot, const int* seq_kvlen,
                                           const int* block_table, int max_pages, int n_seqs, int n_q, int n_kv, int hd,

@@ -34,6 +34,7 @@ constexpr int kPfKeys = 128;         // keys of a step
 constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B; 8-11: conversion; 12: the tensor core; 13-15 idle
 constexpr int kPfSub = kPfRows * 128;        // bytes of 128 rows of 64 half-precision numbers
 constexpr int kPfSms = 148;
+constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
 constexpr int kPfLeast = 4;          // key tiles that a run has at least, on average
 constexpr int kPfSlots = 400;        // partial results at once (see pf_plan)
 constexpr float kPfSlack = 8.f;      // how far scores may outgrow R, in units of log2
@@ -740,6 +741,7 @@ static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, cudaStream_t s
   if (run < kPfLeast) run = kPfLeast;
   const long long parts = (most_tiles + run / 2) / run;
   const bool cut = parts > 1;
+  if (cut && !a.part) return kPfNeedsScratch;
   const long long blocks = cut ? min(items * parts, items + kPfSlots) : items;
   if (blocks > 0x7fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
   launch_k(prefill_fp8_kernel<HD>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
@@ -763,13 +765,13 @@ extern "C" int llmie_attention_prefill_fp8_scratch(int hd) {
 // q, out bfloat16 [n_tokens, n_q hd], hd 64 or 128, at most 128 query heads a key/value head; sequences packed one after another
 // (cu_q [n_seqs + 1]); caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv, 4]; seq_start[i]: tokens that sequence i
 // held before this step, whose keys are in the cache already. scale > 0. window: as in the other attention kernels.
-// scratch: llmie_attention_prefill_fp8_scratch floats, 16-byte aligned.
+// scratch: llmie_attention_prefill_fp8_scratch floats, 16-byte aligned; null: a call that needs it launches nothing and returns -5.
 extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_exp,
                                            const void* v_exp, void* out, float* scratch, int* status, const int* cu_q,
                                            const int* seq_slot, const int* seq_start, const int* block_table, int max_pages,
                                            int n_tokens, int n_seqs, int n_q, int n_kv, int hd, float scale, int window,
                                            cudaStream_t stream) {
-  if (n_tokens < 0 || n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || !scratch || !status) return LLMIE_ERR_BAD_ARG;
+  if (n_tokens < 0 || n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || !status) return LLMIE_ERR_BAD_ARG;
   if (!(scale > 0.f)) return LLMIE_ERR_BAD_ARG;              // a row's bound is taken before scores are scaled
   if ((hd != 64 && hd != 128) || n_q / n_kv > kPfRows || (n_q + 3) / 4 > 65535) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(scratch)) return LLMIE_ERR_ALIGNMENT;

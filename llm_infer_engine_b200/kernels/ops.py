@@ -1633,12 +1633,10 @@ FP8_PAGE = 64            # positions of a page
 FP8_BLOCK = 16           # positions that share an exponent
 
 
-def _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv: int, head_dim: int) -> None:
-    """The checks of a cache in 8 bits: codes [pages, n_kv, 64, head_dim] float8_e4m3fn, exponents [pages, n_kv, 4] int8."""
-    _need(k_cache, "k_cache", FP8, (None, n_kv, FP8_PAGE, head_dim))
-    _need(v_cache, "v_cache", FP8, tuple(k_cache.shape))
-    _need(k_exp, "k_exp", torch.int8, (k_cache.shape[0], n_kv, FP8_PAGE // FP8_BLOCK))
-    _need(v_exp, "v_exp", torch.int8, tuple(k_exp.shape))
+_FP8_STORE_ARGS = [_c_void_p] * 11 + [_c_int] * 10 + [_c_void_p]
+_FP8_ATTENTION_ARGS = [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
+_FP8_STEP_ARGS = [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
+_FP8_PROMPT_ARGS = [_c_void_p] * 12 + [_c_int] * 6 + [_c_float, _c_int, _c_void_p]
 
 
 def _need_heads(name: str, n_q: int, n_kv: int) -> None:
@@ -1646,28 +1644,47 @@ def _need_heads(name: str, n_q: int, n_kv: int) -> None:
         raise KernelError(f"{name}: {n_q} query heads are no multiple of {n_kv} key/value heads")
 
 
-def _need_arrays(name: str, n: int, device, **arrays) -> None:
-    """int32 arrays of at least n entries each (two-dimensional ones of any size), on the call's device."""
-    for what, t in arrays.items():
-        _need(t, what, torch.int32)
-        if t.device != device:
-            raise KernelError(f"{name}: {what} is on {t.device}, the call on {device}")
-        if t.dim() == 1 and t.numel() < n:
-            raise KernelError(f"{name}: {what} has {t.numel()} entries, {n} are needed")
-        if t.dim() > 2 or (t.dim() == 2 and what != "block_table"):
-            raise KernelError(f"{name}: {what} has {t.dim()} dimensions")
-    if "block_table" in arrays and (arrays["block_table"].dim() != 2 or arrays["block_table"].shape[1] < 1):
-        raise KernelError(f"{name}: block_table must be [slots, pages of a sequence]")
+def _index_of(name: str, t) -> int:
+    """The number of the device that a call's first tensor is on: it has to be the current one, whose current stream launches go to."""
+    index = t.get_device()
+    if index < 0:
+        raise KernelError(f"{name}: must be a CUDA tensor (this library has no CPU path)")
+    current = _get_device() if _get_device is not None else torch.cuda.current_device()
+    if index != current:
+        raise KernelError(f"{name}: a tensor is on {t.device}, the current device is cuda:{current}")
+    return index
 
 
-def _need_here(name: str, *tensors) -> None:
-    """All tensors on one device, and that the current one: launches go to the current device's current stream."""
-    device = tensors[0].device
+def _all_here(name: str, index: int, dtype, *tensors) -> None:
+    """Contiguous tensors of one type on device `index`. Written for speed: a call has ten tensors, and a one-token step's kernel
+    takes as long as a dozen Python calls."""
     for t in tensors:
-        if t is not None and t.device != device:
-            raise KernelError(f"{name}: tensors on {device} and on {t.device}")
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"{name}: the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t.get_device() != index or t.dtype is not dtype or not t.is_contiguous():
+            if not t.is_cuda:
+                raise KernelError(f"{name}: must be a CUDA tensor (this library has no CPU path)")
+            if t.get_device() != index:
+                raise KernelError(f"{name}: a tensor is on {t.device}, others are on cuda:{index}")
+            raise KernelError(f"{name}: a contiguous tensor of {dtype} is needed, got {t.dtype}, shape {tuple(t.shape)}, "
+                              f"strides {t.stride()}")
+
+
+def _fp8_shapes(name: str, k_cache, v_cache, k_exp, v_exp, n_kv: int, head_dim: int) -> None:
+    """Codes [pages, n_kv, 64, head_dim], exponents [pages, n_kv, 4]."""
+    pages = k_cache.shape[0] if k_cache.dim() else 0
+    codes, exps = (pages, n_kv, FP8_PAGE, head_dim), (pages, n_kv, FP8_PAGE // FP8_BLOCK)
+    if not (k_cache.shape == codes and v_cache.shape == codes and k_exp.shape == exps and v_exp.shape == exps):
+        raise KernelError(f"{name}: caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)} with exponents {tuple(k_exp.shape)}, "
+                          f"{tuple(v_exp.shape)}; [pages, {n_kv}, {FP8_PAGE}, {head_dim}] and [pages, {n_kv}, "
+                          f"{FP8_PAGE // FP8_BLOCK}] are expected")
+
+
+def _fp8_arrays(name: str, block_table, *counted) -> None:
+    """block_table [slots, pages of a sequence]; `counted`: an index array and the entries it must have, in turn."""
+    if block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise KernelError(f"{name}: block_table has shape {tuple(block_table.shape)}, [slots, pages of a sequence] is expected")
+    for t, n in zip(counted[::2], counted[1::2]):
+        if t.dim() != 1 or t.shape[0] < n:
+            raise KernelError(f"{name}: an index array of shape {tuple(t.shape)}, {n} entries are needed")
 
 
 def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_slot, seq_start, block_table, n_seqs: int,
@@ -1680,35 +1697,36 @@ def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_
     rotation. Sequence i (of n_seqs) brings rows cu_q[i] .. cu_q[i + 1] - 1, at positions from seq_start[i] on, none more than
     max_q_len. A slot may appear once. Where a block already holds earlier positions its exponent only rises, and their codes
     are rounded to it. head_dim: a multiple of 16 up to 256. With write_kv False only the queries are rotated."""
+    name = "rope_store_fp8"
+    _need_heads(name, n_q, n_kv)
+    index = _index_of(name, qkv)
+    _all_here(name, index, qkv.dtype, qkv, q_out)
+    _all_here(name, index, torch.int32, cu_q, seq_slot, seq_start, block_table)
     T = qkv.shape[0]
-    _need_heads("rope_store_fp8", n_q, n_kv)
-    _need(qkv, "qkv", None, (T, (n_q + 2 * n_kv) * head_dim))
-    _need(q_out, "q_out", qkv.dtype, (T, n_q * head_dim))
-    _need_arrays("rope_store_fp8", n_seqs, qkv.device, cu_q=cu_q, seq_slot=seq_slot, seq_start=seq_start, block_table=block_table)
-    if cu_q.numel() < n_seqs + 1:
-        raise KernelError(f"rope_store_fp8: cu_q has {cu_q.numel()} entries, {n_seqs + 1} are needed")
+    if qkv.shape != (T, (n_q + 2 * n_kv) * head_dim) or q_out.shape != (T, n_q * head_dim):
+        raise KernelError(f"{name}: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)} for {n_q} / {n_kv} heads of {head_dim}")
+    _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
     if n_seqs < 0 or (T > 0 and max_q_len <= 0):
-        raise KernelError(f"rope_store_fp8: {n_seqs} sequences with at most {max_q_len} new tokens each")
+        raise KernelError(f"{name}: {n_seqs} sequences with at most {max_q_len} new tokens each")
     if head_dim % 16 or not 16 <= head_dim <= 256:
-        raise KernelError(f"rope_store_fp8: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
+        raise KernelError(f"{name}: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
     table_len = 0
     if table is not None:
-        if rot_dim <= 0 or rot_dim % 2 or rot_dim > head_dim:
-            raise KernelError(f"rope_store_fp8: {rot_dim} of {head_dim} columns cannot be rotated")
-        _need(table, "table", torch.float32, (None, rot_dim // 2, 2))
+        _all_here(name, index, torch.float32, table)
         table_len = table.shape[0]
-        if table_len < 1:
-            raise KernelError("rope_store_fp8: the table of angles is empty")
+        if rot_dim <= 0 or rot_dim % 2 or rot_dim > head_dim or table.shape != (table_len, rot_dim // 2, 2) or table_len < 1:
+            raise KernelError(f"{name}: {rot_dim} of {head_dim} columns by a table of shape {tuple(table.shape)}")
     if write_kv:
-        _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _need_here("rope_store_fp8", qkv, q_out, table, *((k_cache, v_cache, k_exp, v_exp) if write_kv else ()))
-    _work(_nbytes(qkv, q_out) + (2 * T * n_kv * head_dim if write_kv else 0))
-    f = _fn("cache_fp8", "llmie_rope_store_fp8", [_c_void_p] * 11 + [_c_int] * 10 + [_c_void_p])
-    _check(f(qkv.data_ptr(), q_out.data_ptr(), _ptr(k_cache) if write_kv else None, _ptr(v_cache) if write_kv else None,
-             _ptr(k_exp) if write_kv else None, _ptr(v_exp) if write_kv else None, _ptr(table), cu_q.data_ptr(),
-             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], int(n_seqs),
-             int(max_q_len), n_q, n_kv, head_dim, int(rot_dim), table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()),
-           "rope_store_fp8")
+        _all_here(name, index, FP8, k_cache, v_cache)
+        _all_here(name, index, torch.int8, k_exp, v_exp)
+        _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    if trace.timer is not None:
+        _work(_nbytes(qkv, q_out) + (2 * T * n_kv * head_dim if write_kv else 0))
+    f = _fn("cache_fp8", "llmie_rope_store_fp8", _FP8_STORE_ARGS)
+    _check(f(qkv.data_ptr(), q_out.data_ptr(), k_cache.data_ptr() if write_kv else None, v_cache.data_ptr() if write_kv else None,
+             k_exp.data_ptr() if write_kv else None, v_exp.data_ptr() if write_kv else None, _ptr(table), cu_q.data_ptr(),
+             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], n_seqs, max_q_len, n_q, n_kv,
+             head_dim, rot_dim, table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()), name)
     return q_out
 
 
@@ -1716,28 +1734,31 @@ def attention_paged_fp8(q, k_cache, v_cache, k_exp, v_exp, out, tok_pos, tok_seq
                         head_dim: int, scale: float, window: int = 0):
     """Plain attention over a paged cache in 8 bits, one warp per (token, query head): q, out [T, n_q hd] float32 or bfloat16,
     the cache as in rope_store_fp8, the rest as in attention_paged. Every head size that is a multiple of 16 up to 256."""
+    name = "attention_paged_fp8"
+    _need_heads(name, n_q, n_kv)
+    index = _index_of(name, q)
+    _all_here(name, index, q.dtype, q, out)
+    _all_here(name, index, FP8, k_cache, v_cache)
+    _all_here(name, index, torch.int8, k_exp, v_exp)
+    _all_here(name, index, torch.int32, tok_pos, tok_seq, seq_slot, block_table)
     T = q.shape[0]
-    _need_heads("attention_paged_fp8", n_q, n_kv)
-    _need(q, "q", None, (T, n_q * head_dim))
-    _need(out, "out", q.dtype, (T, n_q * head_dim))
-    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _need_arrays("attention_paged_fp8", 0, q.device, tok_pos=tok_pos, tok_seq=tok_seq, seq_slot=seq_slot, block_table=block_table)
-    if tok_pos.numel() < T or tok_seq.numel() < T:
-        raise KernelError("attention_paged_fp8: tok_pos / tok_seq shorter than the token count")
+    if q.shape != (T, n_q * head_dim) or out.shape != q.shape:
+        raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_q} heads of {head_dim}")
+    _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _fp8_arrays(name, block_table, tok_pos, T, tok_seq, T, seq_slot, 0)
     if head_dim % 16 or not 16 <= head_dim <= 256:
-        raise KernelError(f"attention_paged_fp8: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
-    _need_here("attention_paged_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
+        raise KernelError(f"{name}: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
     _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_fp8", "llmie_attention_paged_fp8", [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p])
+    f = _fn("attention_fp8", "llmie_attention_paged_fp8", _FP8_ATTENTION_ARGS)
     _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
              tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, n_q,
-             n_kv, head_dim, float(scale), int(window), _dt(q, "q"), _stream()), "attention_paged_fp8")
+             n_kv, head_dim, scale, window, _dt(q, "q"), _stream()), name)
     return out
 
 
 def attention_decode_fp8_supported(head_dim: int, dtype: torch.dtype) -> bool:
     """The sizes attention_decode_fp8.cu is instantiated for (answered without loading the library)."""
-    return dtype == torch.bfloat16 and head_dim in (64, 128)
+    return dtype is torch.bfloat16 and head_dim in (64, 128)
 
 
 def attention_decode_fp8_rope_supported(n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> bool:
@@ -1745,16 +1766,21 @@ def attention_decode_fp8_rope_supported(n_q: int, n_kv: int, head_dim: int, dtyp
     return attention_decode_fp8_supported(head_dim, dtype) and n_kv > 0 and n_q // n_kv <= 16
 
 
+_NEEDS_SCRATCH = -5          # a launcher's answer to a call without scratch whose work is cut: nothing was launched
 _fp8_scratch_floats = {}
 
 
-def _decode_fp8_scratch(n_q: int, n_kv: int, head_dim: int, device) -> torch.Tensor:
-    key = (n_q, n_kv, head_dim)
-    floats = _fp8_scratch_floats.get(key)
-    if floats is None:
-        f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_scratch", [_c_int] * 3, query=True)
-        floats = _fp8_scratch_floats[key] = int(f(n_q, n_kv, head_dim))
-    return torch.empty(floats, dtype=torch.float32, device=device)
+def _with_scratch(name: str, family: str, f, args_before, args_after, key, device) -> None:
+    """A launch that needs scratch for partial results where its work is cut, which the launcher decides: asked without scratch
+    first, since small calls, where a microsecond counts, do not need any."""
+    status = f(*args_before, None, *args_after)
+    if status == _NEEDS_SCRATCH:
+        floats = _fp8_scratch_floats.get((family, key))
+        if floats is None:
+            ask = _fn(family, f"llmie_{family}_scratch", [_c_int] * len(key), query=True)
+            floats = _fp8_scratch_floats[family, key] = int(ask(*key))
+        status = f(*args_before, torch.empty(floats, dtype=torch.float32, device=device).data_ptr(), *args_after)
+    _check(status, name)
 
 
 def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_kvlen, block_table, n_q: int, n_kv: int,
@@ -1762,22 +1788,28 @@ def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_k
     """Attention for a one-token step over a paged cache in 8 bits, on the tensor cores: q, out bfloat16 [n, n_q hd], the cache
     as in rope_store_fp8 (it holds the step's keys and values already), seq_kvlen int32 [n] the keys each sequence holds (0:
     its rows of out become zeros), window as in attention_paged. head_dim 64 or 128. max_kv_len: no sequence is longer (0: not
-    known; nothing but launch sizes depends on it)."""
-    n = q.shape[0]
-    _need_heads("attention_decode_fp8", n_q, n_kv)
+    known; only the choice of the kernel goes by it)."""
+    name = "attention_decode_fp8"
+    _need_heads(name, n_q, n_kv)
     if not attention_decode_fp8_supported(head_dim, q.dtype):
-        raise KernelError(f"attention_decode_fp8: head_dim {head_dim}, {q.dtype} is not supported (bfloat16, 64 or 128)")
-    _need(q, "q", torch.bfloat16, (n, n_q * head_dim))
-    _need(out, "out", torch.bfloat16, (n, n_q * head_dim))
-    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _need_arrays("attention_decode_fp8", n, q.device, seq_slot=seq_slot, seq_kvlen=seq_kvlen, block_table=block_table)
-    _need_here("attention_decode_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
-    scratch = _decode_fp8_scratch(n_q, n_kv, head_dim, q.device)
-    _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8", [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p])
-    _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
-             scratch.data_ptr(), seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), block_table.shape[1], n, n_q,
-             n_kv, head_dim, float(scale), int(window), int(max_kv_len), _stream()), "attention_decode_fp8")
+        raise KernelError(f"{name}: head_dim {head_dim}, {q.dtype} is not supported (bfloat16, 64 or 128)")
+    index = _index_of(name, q)
+    _all_here(name, index, torch.bfloat16, q, out)
+    _all_here(name, index, FP8, k_cache, v_cache)
+    _all_here(name, index, torch.int8, k_exp, v_exp)
+    _all_here(name, index, torch.int32, seq_slot, seq_kvlen, block_table)
+    n = q.shape[0]
+    if q.shape != (n, n_q * head_dim) or out.shape != q.shape:
+        raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_q} heads of {head_dim}")
+    _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
+    if trace.timer is not None:
+        _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8", _FP8_ATTENTION_ARGS)
+    _with_scratch(name, "attention_decode_fp8", f,
+                  (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
+                  (seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv,
+                   head_dim, scale, window, max_kv_len, _stream()), (n_q, n_kv, head_dim), q.device)
     return out
 
 
@@ -1787,32 +1819,40 @@ def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, s
     [n, (n_q + 2 n_kv) hd] rotated by table (float32 [max_pos, hd / 2, 2], the whole head), the new key and value written for
     position seq_kvlen[i] - 1 as rope_store_fp8 does it, and attention_decode_fp8 over the cache with them. At most 16 query
     heads a key/value head. A slot may appear once."""
-    n = qkv.shape[0]
-    _need_heads("attention_decode_fp8_rope", n_q, n_kv)
+    name = "attention_decode_fp8_rope"
+    _need_heads(name, n_q, n_kv)
     if not attention_decode_fp8_rope_supported(n_q, n_kv, head_dim, qkv.dtype):
-        raise KernelError(f"attention_decode_fp8_rope: {n_q} / {n_kv} heads of {head_dim}, {qkv.dtype} are not supported (bfloat16, "
-                          "64 or 128, at most 16 query heads a key/value head)")
-    _need(qkv, "qkv", torch.bfloat16, (n, (n_q + 2 * n_kv) * head_dim))
-    _need(out, "out", torch.bfloat16, (n, n_q * head_dim))
-    _need(table, "table", torch.float32, (None, head_dim // 2, 2))
-    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _need_arrays("attention_decode_fp8_rope", n, qkv.device, seq_slot=seq_slot, seq_kvlen=seq_kvlen, block_table=block_table)
-    _need_here("attention_decode_fp8_rope", qkv, out, table, k_cache, v_cache, k_exp, v_exp)
-    scratch = _decode_fp8_scratch(n_q, n_kv, head_dim, qkv.device)
-    _work(_nbytes(qkv, out) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_rope",
-            [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p])
-    _check(f(qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
-             scratch.data_ptr(), table.data_ptr(), table.shape[0], seq_slot.data_ptr(), seq_kvlen.data_ptr(),
-             block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv, head_dim, float(scale), int(window), int(max_kv_len),
-             _stream()), "attention_decode_fp8_rope")
+        raise KernelError(f"{name}: {n_q} / {n_kv} heads of {head_dim}, {qkv.dtype} are not supported (bfloat16, 64 or 128, at "
+                          "most 16 query heads a key/value head)")
+    index = _index_of(name, qkv)
+    _all_here(name, index, torch.bfloat16, qkv, out)
+    _all_here(name, index, FP8, k_cache, v_cache)
+    _all_here(name, index, torch.int8, k_exp, v_exp)
+    _all_here(name, index, torch.int32, seq_slot, seq_kvlen, block_table)
+    _all_here(name, index, torch.float32, table)
+    n = qkv.shape[0]
+    table_len = table.shape[0]
+    if qkv.shape != (n, (n_q + 2 * n_kv) * head_dim) or out.shape != (n, n_q * head_dim) or table_len < 1 \
+            or table.shape != (table_len, head_dim // 2, 2):
+        raise KernelError(f"{name}: qkv {tuple(qkv.shape)}, out {tuple(out.shape)}, table {tuple(table.shape)} for {n_q} / {n_kv} "
+                          f"heads of {head_dim}")
+    _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
+    if trace.timer is not None:
+        _work(_nbytes(qkv, out) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_rope", _FP8_STEP_ARGS)
+    _with_scratch(name, "attention_decode_fp8", f,
+                  (qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
+                  (table.data_ptr(), table_len, seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(),
+                   block_table.shape[1], n, n_q, n_kv, head_dim, scale, window, max_kv_len, _stream()), (n_q, n_kv, head_dim),
+                  qkv.device)
     return out
 
 
 def attention_prefill_fp8_supported(n_q: int, n_kv: int, head_dim: int, dtype: torch.dtype) -> bool:
     """The sizes attention_prefill_fp8.cu takes (answered without loading the library): bfloat16, head size 64 or 128, at most
     128 query heads a key/value head."""
-    return dtype == torch.bfloat16 and head_dim in (64, 128) and n_kv > 0 and n_q // n_kv <= 128
+    return dtype is torch.bfloat16 and head_dim in (64, 128) and n_kv > 0 and n_q // n_kv <= 128
 
 
 def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot, seq_start, block_table, n_seqs: int,
@@ -1821,31 +1861,33 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     [T, n_q hd] with the sequences packed (cu_q int32 [n + 1]), the cache as in rope_store_fp8 (it holds the step's keys and
     values already), seq_start int32 [n] the tokens each sequence held before this step, window as in attention_paged.
     head_dim 64 or 128, scale > 0. A block whose waits run out leaves NaN in its rows, and check_tc_status raises."""
-    _need_heads("attention_prefill_fp8", n_q, n_kv)
+    name = "attention_prefill_fp8"
+    _need_heads(name, n_q, n_kv)
     if not attention_prefill_fp8_supported(n_q, n_kv, head_dim, q.dtype):
-        raise KernelError(f"attention_prefill_fp8: {n_q} / {n_kv} heads of {head_dim}, {q.dtype} are not supported (bfloat16, "
-                          "64 or 128, at most 128 query heads a key/value head)")
+        raise KernelError(f"{name}: {n_q} / {n_kv} heads of {head_dim}, {q.dtype} are not supported (bfloat16, 64 or 128, at most "
+                          "128 query heads a key/value head)")
     if not scale > 0:
-        raise KernelError(f"attention_prefill_fp8: the scale must be positive, got {scale}")
+        raise KernelError(f"{name}: the scale must be positive, got {scale}")
+    index = _index_of(name, q)
+    _all_here(name, index, torch.bfloat16, q, out)
+    _all_here(name, index, FP8, k_cache, v_cache)
+    _all_here(name, index, torch.int8, k_exp, v_exp)
+    _all_here(name, index, torch.int32, cu_q, seq_slot, seq_start, block_table)
     T = q.shape[0]
-    _need(q, "q", torch.bfloat16, (T, n_q * head_dim))
-    _need(out, "out", torch.bfloat16, (T, n_q * head_dim))
-    _need_fp8_cache(k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _need_arrays("attention_prefill_fp8", n_seqs, q.device, cu_q=cu_q, seq_slot=seq_slot, seq_start=seq_start, block_table=block_table)
-    if cu_q.numel() < n_seqs + 1:
-        raise KernelError(f"attention_prefill_fp8: cu_q has {cu_q.numel()} entries, {n_seqs + 1} are needed")
-    _need_here("attention_prefill_fp8", q, out, k_cache, v_cache, k_exp, v_exp)
-    floats = _fp8_scratch_floats.get(head_dim)
-    if floats is None:
-        f = _fn("attention_prefill_fp8", "llmie_attention_prefill_fp8_scratch", [_c_int], query=True)
-        floats = _fp8_scratch_floats[head_dim] = int(f(head_dim))
-    scratch = torch.empty(floats, dtype=torch.float32, device=q.device)
-    _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_prefill_fp8", "llmie_attention_prefill_fp8", [_c_void_p] * 12 + [_c_int] * 6 + [_c_float, _c_int, _c_void_p])
-    _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
-             scratch.data_ptr(), tc_status_word(q.device).data_ptr(), cu_q.data_ptr(), seq_slot.data_ptr(), seq_start.data_ptr(),
-             block_table.data_ptr(), block_table.shape[1], T, int(n_seqs), n_q, n_kv, head_dim, float(scale), int(window),
-             _stream()), "attention_prefill_fp8")
+    if q.shape != (T, n_q * head_dim) or out.shape != q.shape:
+        raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_q} heads of {head_dim}")
+    _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
+    if n_seqs < 0:
+        raise KernelError(f"{name}: {n_seqs} sequences")
+    _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
+    if trace.timer is not None:
+        _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
+    f = _fn("attention_prefill_fp8", "llmie_attention_prefill_fp8", _FP8_PROMPT_ARGS)
+    _with_scratch(name, "attention_prefill_fp8", f,
+                  (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
+                  (tc_status_word(q.device).data_ptr(), cu_q.data_ptr(), seq_slot.data_ptr(), seq_start.data_ptr(),
+                   block_table.data_ptr(), block_table.shape[1], T, n_seqs, n_q, n_kv, head_dim, scale, window, _stream()),
+                  (head_dim,), q.device)
     return out
 
 
