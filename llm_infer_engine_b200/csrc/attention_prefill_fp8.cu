@@ -3,8 +3,10 @@
 //   o_t = sum_j 2^(s_tj) c_j 2^(ev_j) / sum_j 2^(s_tj),   s_tj = scale log2(e) (q_t . k_j) 2^(ek_j),   j seen by t     (k, c: codes)
 //
 // Rows. A key/value head is read once for all of its query heads: the rows of a 128-row operand are (token, query head) pairs,
-// 128 / G tokens of the G heads that share the key/value head. A block has two such tiles, A and B, with a softmax warpgroup
-// each (a thread a row); while one works on its scores the tensor core is busy with the other's.
+// 128 / G tokens of the G heads that share the key/value head. A block has two such tiles, A and B; while the softmax of one works
+// on its scores the tensor core is busy with the other's. Two threads share a row, half of a key tile's columns each: what a tile
+// costs is mostly latency (tensor memory, barriers, one exponential a score at 16 a clock and SM), which sixteen warps hide
+// better than eight (with a thread a row, all 128 scores in its registers: 55 us where this takes KPF_US).
 //
 // Keys and values become half-precision numbers (exactly) on their way into shared memory: four warps load codes into
 // registers a tile ahead, convert them and write the tensor core's operand layout. Their exponents stay out of the products:
@@ -31,13 +33,18 @@ using namespace tc;
 
 constexpr int kPfRows = 128;         // rows of a tile
 constexpr int kPfKeys = 128;         // keys of a step
-constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B; 8-11: conversion; 12: the tensor core; 13-15 idle
+constexpr int kPfSoftmax = 512;      // warps 0-3, 4-7: softmax of tile A, columns 0-63 and 64-127; 8-11, 12-15: of tile B
+constexpr int kPfThreads = kPfSoftmax + 128 + 128;     // 16-19: conversion; 20, 21: the products of tile A, of tile B; 22, 23: nothing
+// Registers a thread of a softmax, the conversion and the last warpgroup keeps. A block is launched with 80 a thread, six times 80.
+constexpr int kPfLaunchRegs = 80, kPfConvertRegs = 112, kPfIssueRegs = 48;
+static_assert(4 * kPfLaunchRegs + kPfConvertRegs + kPfIssueRegs <= 6 * kPfLaunchRegs, "more than the block has would never be granted");
 constexpr int kPfSub = kPfRows * 128;        // bytes of 128 rows of 64 half-precision numbers
 constexpr int kPfSms = 148;
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
 constexpr int kPfLeast = 4;          // key tiles that a run has at least, on average
 constexpr int kPfSlots = 400;        // partial results at once (see pf_plan)
-constexpr float kPfSlack = 8.f;      // how far scores may outgrow R, in units of log2
+constexpr float kPfTop = 7.f;        // the bound's own weight is 2^7
+constexpr float kPfSlack = 8.f;      // how far scores may outgrow the bound, in units of log2
 
 template <int HD> struct PfCfg {
   static constexpr int kSubs = HD / 64;
@@ -48,18 +55,6 @@ template <int HD> struct PfCfg {
   static constexpr bool kOwnP = HD == 64;                    // tensor memory has room for the weights beside the scores
   static constexpr int kSCol = 0, kOCol = 256, kPCol = 384;  // columns: scores of A and B, sums of A and B, weights
   static constexpr int kRecord = 2 * kPfRows * (HD + 2);     // floats of a partial result: sums, then bounds, then denominators
-};
-
-struct PfShared {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], x_full[4];
-  uint64_t s_full[2], p_ready[2], pv_done[2], last;
-  uint32_t tmem_base;
-  int abort;
-  // Of the key tiles in flight, by step % 4: factors of scores, addends, factors of the denominator's terms, and the step (+ 1)
-  // that last had NaN among its values. x_full: all of them are there. (A step's place is written again four steps on, when
-  // the scores of the step two on are done, which both tiles' softmax has let begin behind its last look at this step.)
-  float k_scale[4][8], v_add[4][8], v_back[4][8];
-  int v_nan[4];
 };
 
 struct PrefillArgs {
@@ -103,6 +98,11 @@ __device__ __forceinline__ void pf_fma2(float& y0, float& y1, float x0, float x1
 __device__ __forceinline__ void pf_add2(uint64_t& acc, float x0, float x1) {
   asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(pf_pair(x0, x1)));
 }
+__device__ __forceinline__ float pf_max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 // D[tmem] (+)= A[tmem] * B[smem], half precision
 __device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -129,56 +129,63 @@ __device__ __forceinline__ void pf_tiles(int start, int t0, int n, int window, i
   lo = first_visible_key(start + t0, window) / kPfKeys;
   count = (start + t0 + n - 1) / kPfKeys - lo + 1;
 }
-// Tiles of tokens of a sequence, and the key tiles of its first and last one.
-__device__ __forceinline__ void pf_sequence(const PrefillArgs& a, int s, int tok, int& tiles, int& first, int& last) {
-  const int len = a.cu_q[s + 1] - a.cu_q[s], start = a.seq_start[s];
-  tiles = (len + tok - 1) / tok;
-  first = last = 0;
-  if (tiles > 0) {
-    int lo;
-    pf_tiles(start, 0, min(tok, len), a.window, lo, first);
-    pf_tiles(start, (tiles - 1) * tok, len - (tiles - 1) * tok, a.window, lo, last);
+// What a lane knows of its sequence: tiles of tokens, the key tiles of the first and the last of them.
+struct PfSequence {
+  int q_begin, q_len, start, slot, tiles, first, last;
+};
+__device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, int tok) {
+  PfSequence q{0, 0, 0, 0, 0, 0, 0};
+  if (s < a.n_seqs) {
+    q.q_begin = a.cu_q[s];
+    q.q_len = a.cu_q[s + 1] - q.q_begin;
+    q.start = a.seq_start[s];
+    q.slot = a.seq_slot[s];
+    q.tiles = (q.q_len + tok - 1) / tok;
+    if (q.tiles > 0) {
+      int lo;
+      pf_tiles(q.start, 0, min(tok, q.q_len), a.window, lo, q.first);
+      pf_tiles(q.start, (q.tiles - 1) * tok, q.q_len - (q.tiles - 1) * tok, a.window, lo, q.last);
+    }
   }
+  return q;
 }
 // Key tiles that a run has on average: a 148th of the step (first and last tile of tokens stand for all of a sequence).
 // All lanes of a warp call it.
 __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok) {
   const int lane = threadIdx.x & 31;
-  long long twice = 0;
+  float twice = 0.f;                 // every block works it out from the same numbers in the same order
   for (int s = lane; s < a.n_seqs; s += 32) {
-    int n, f, l;
-    pf_sequence(a, s, tok, n, f, l);
-    twice += (long long)n * (f + l);
+    const PfSequence q = pf_sequence(a, s, tok);
+    twice += (float)q.tiles * (float)(q.first + q.last);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
-  const long long c = (twice * a.n_kv + 2 * kPfSms - 1) / (2 * kPfSms);
-  return (int)(c < kPfLeast ? kPfLeast : c > (1 << 28) ? (1 << 28) : c);
+  return max(kPfLeast, (int)fminf(ceilf(twice * (float)a.n_kv * (0.5f / kPfSms)), 1e9f));
 }
-// Runs that each of a sequence's tiles of tokens is cut into. A sequence that is cut has last >= 1.5 run, so that runs <= 4/3
-// last / run; and last <= 2 (first + last) / 2: all cut sequences together have at most 8/3 * 148 < kPfSlots runs.
-__device__ __forceinline__ int pf_runs(int last, int run) { return max(1, (int)(((long long)last + run / 2) / run)); }
+// Runs that each of a sequence's tiles of tokens is cut into: last / run, to the nearest. A sequence that is cut has last >= 1.5 run,
+// so that runs <= 4/3 last / run; and last <= 2 (first + last) / 2: all cut sequences together have at most 8/3 * 148 < kPfSlots runs.
+__device__ __forceinline__ int pf_runs(int last, int run) { return max(1, (last + run / 2) / run); }
 
 struct PfWork {
-  int seq, tile, hk, part, parts, slot;          // slot: of the partial result
+  int q_begin, q_len, start, page_row;           // the sequence's rows in the step, what it held, its slot
+  int tile, hk, part, parts, slot;               // slot: of the partial result; parts: 0 where there is no such piece
 };
-// The piece of work of block `index`; false if there is none. All lanes of a warp call it. Late tiles of a sequence, which see
-// the most keys, come first, all heads of one after another.
-__device__ __forceinline__ bool pf_find(const PrefillArgs& a, int tok, long long index, PfWork& w) {
+// Piece `index` of the step's work, or (WHOLE) tile `index` with all its runs. All lanes of a warp call it. Late tiles of a
+// sequence, which see the most keys, come first, all heads of one after another.
+template <bool WHOLE>
+__device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int index) {
   const int lane = threadIdx.x & 31;
   const int run = pf_run(a, tok);
-  long long before = 0, slots = 0;
+  PfWork w{0, 0, 0, 0, 0, 0, 0, 0, 0};
+  int before = 0, slots = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-    int n = 0, f = 0, l = 0, parts = 1;
-    if (s0 + lane < a.n_seqs) {
-      pf_sequence(a, s0 + lane, tok, n, f, l);
-      parts = pf_runs(l, run);
-    }
-    const long long own = (long long)n * parts * a.n_kv, cut = parts > 1 ? own : 0;
-    long long incl = own, cuts = cut;
+    const PfSequence q = pf_sequence(a, s0 + lane, tok);
+    const int parts = pf_runs(q.last, run);
+    const int all = q.tiles * parts * a.n_kv, own = WHOLE ? q.tiles * a.n_kv : all, cut = parts > 1 ? all : 0;
+    int incl = own, cuts = cut;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, incl, o), y = __shfl_up_sync(0xffffffffu, cuts, o);
+      const int x = __shfl_up_sync(0xffffffffu, incl, o), y = __shfl_up_sync(0xffffffffu, cuts, o);
       if (lane >= o) {
         incl += x;
         cuts += y;
@@ -187,21 +194,42 @@ __device__ __forceinline__ bool pf_find(const PrefillArgs& a, int tok, long long
     const unsigned here = __ballot_sync(0xffffffffu, before + incl > index);
     if (here) {
       const int src = __ffs(here) - 1;
-      const int local = (int)(index - before - __shfl_sync(0xffffffffu, incl - own, src));
-      n = __shfl_sync(0xffffffffu, n, src);
+      const int local = index - before - __shfl_sync(0xffffffffu, incl - own, src);
+      w.q_begin = __shfl_sync(0xffffffffu, q.q_begin, src);
+      w.q_len = __shfl_sync(0xffffffffu, q.q_len, src);
+      w.start = __shfl_sync(0xffffffffu, q.start, src);
+      w.page_row = __shfl_sync(0xffffffffu, q.slot, src);
       w.parts = __shfl_sync(0xffffffffu, parts, src);
-      w.slot = (int)(slots + __shfl_sync(0xffffffffu, cuts - cut, src)) + local;
-      w.seq = s0 + src;
-      w.part = local % w.parts;
-      w.hk = local / w.parts % a.n_kv;
-      w.tile = n - 1 - local / w.parts / a.n_kv;
-      return true;
+      const int item = WHOLE ? local : local / w.parts;
+      w.part = WHOLE ? 0 : local - item * w.parts;
+      const int t = item / a.n_kv;
+      w.hk = item - t * a.n_kv;
+      w.tile = __shfl_sync(0xffffffffu, q.tiles, src) - 1 - t;
+      w.slot = slots + __shfl_sync(0xffffffffu, cuts - cut, src) + item * w.parts + w.part;
+      return w;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
     slots += __shfl_sync(0xffffffffu, cuts, 31);
   }
-  return false;
+  return w;
 }
+
+struct PfShared {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], x_full[4];
+  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], last[2];
+  uint32_t tmem_base;
+  int abort;
+  // Of the key tiles in flight, by step % 4: factors of scores, addends, factors of the denominator's terms, and the step (+ 1)
+  // that last had NaN among its values. x_full: all of them are there. (A step's place is written again four steps on, when
+  // the scores of the step two on are done, which both tiles' softmax has let begin behind its last look at this step.)
+  float k_scale[4][8], v_add[4][8], v_back[4][8];
+  int v_nan[4];
+  // the two threads of a row tell each other their numbers here; the two warps that share 32 rows meet at a barrier of their own.
+  // Two buffers in turn: a thread is never more than one exchange ahead.
+  float row_val[2][2][2][kPfRows];
+  PfWork work;
+  uint64_t pair_bar[2][4];
+};
 
 // ------------------------------------------------------------------------------------------ the kernel
 template <int HD>
@@ -214,46 +242,136 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   uint8_t* k_smem = q_smem + 2 * Cfg::kQBytes;
   uint8_t* v_smem = k_smem + Cfg::kStages * Cfg::kKvBytes;
   const int warp = threadIdx.x >> 5;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
 
   const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = 2 * tok_x;      // tokens of a tile, of a block
-  PfWork w;
-  if (!pf_find(a, tok, blockIdx.x, w)) return;               // the whole block alike
-  const int q_begin = a.cu_q[w.seq], q_len = a.cu_q[w.seq + 1] - q_begin, start = a.seq_start[w.seq];
+  // one warp looks for the block's piece of work while others set it up
+  if (warp == 0) {
+    const PfWork found = pf_find<false>(a, tok, blockIdx.x);
+    if (threadIdx.x == 0) sh.work = found;
+  } else if (threadIdx.x == 32) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sh.k_full[s], 128);
+      mbar_init(&sh.k_empty[s], 2);
+      mbar_init(&sh.v_full[s], 128);
+      mbar_init(&sh.v_empty[s], 2);
+      mbar_init(&sh.s_full[s], 1);
+      mbar_init(&sh.s_free[s], 256);
+      mbar_init(&sh.p_ready[s], 256);
+      mbar_init(&sh.pv_done[s], 1);
+      mbar_init(&sh.last[s], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sh.x_full[i], 128);
+      sh.v_nan[i] = 0;
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(&sh.pair_bar[i >> 2][i & 3], 64);
+    sh.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const PfWork w = sh.work;
+  if (w.parts == 0) return;          // the whole block alike
+  if (warp == 20) {
+    tmem_alloc(&sh.tmem_base, 512);
+    tmem_relinquish();
+  }
+  const int q_begin = w.q_begin, q_len = w.q_len, start = w.start;
   const int t0 = w.tile * tok, n_tok = min(tok, q_len - t0);
   int lo_tile, tiles;
   pf_tiles(start, t0, n_tok, a.window, lo_tile, tiles);
   // this run's key tiles: [c0, c1) of the tiles of the block's tokens
-  const int c0 = lo_tile + (int)((long long)tiles * w.part / w.parts), c1 = lo_tile + (int)((long long)tiles * (w.part + 1) / w.parts);
+  const int c0 = lo_tile + tiles * w.part / w.parts, c1 = lo_tile + tiles * (w.part + 1) / w.parts;
   const int last_key = min(start + t0 + n_tok, a.max_pages * kFp8Page) - 1;
   // steps of the two tiles: A's tokens come first and may not see the last key tiles
   const int n_tok_a = min(n_tok, tok_x), n_tok_b = n_tok - n_tok_a;
   const int n_a = max(0, min(c1, (start + t0 + n_tok_a - 1) / kPfKeys + 1) - c0), n_b = n_tok_b > 0 ? c1 - c0 : 0;
   const int n_steps = max(n_a, n_b);
 
-  if (threadIdx.x == 0) {
-    mbar_init(&sh.q_full, 256);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&sh.k_full[s], 128);
-      mbar_init(&sh.k_empty[s], 1);
-      mbar_init(&sh.v_full[s], 128);
-      mbar_init(&sh.v_empty[s], 1);
-      mbar_init(&sh.s_full[s], 1);
-      mbar_init(&sh.p_ready[s], 128);
-      mbar_init(&sh.pv_done[s], 1);
+  // What needs no barrier begins before the block meets: the rows' queries go to shared memory, the first codes are asked for.
+  const bool softmax = warp < 16;
+  const int x = warp >> 3 & 1, half = warp >> 2 & 1, r = threadIdx.x & 127;    // tile, half and row of a softmax thread
+  const int first_tok = t0 + x * tok_x, n_tok_x = x ? n_tok_b : n_tok_a;
+  const int rt = r / G, rh = r - rt * G;                     // token of the tile, query head of the group
+  const bool there = softmax && rt < n_tok_x;
+  const size_t row_off = ((size_t)(q_begin + first_tok + rt) * a.n_q + w.hk * G + rh) * HD;
+  float f = 0.f;                                             // of the row's scores: scale log2(e) and the row's power of two
+  constexpr int kPer = HD / 16;                              // pieces of 16 codes a row, and pieces that a converting thread has
+  constexpr int kStep = 128 / kPer;                          // its rows: row0, row0 + kStep, ...
+  const int ct = threadIdx.x & 127, piece = ct % kPer, row0 = ct / kPer;
+  const int* pages = a.block_table + (size_t)w.page_row * a.max_pages;
+  uint4 kr[kPer], vr[kPer];
+  // Everything is asked for well before it is looked at: a tile's pages a step before its codes, its codes and exponents a step
+  // before they are written out. (Where an exponent was clamped, or a page's address made, as soon as it was asked for, the
+  // conversion waited for memory twice a tile and the whole kernel for the conversion: 57 us for KPF_US.)
+  int pg0 = 0, pg1 = 0;                                      // pages of the tile to be asked for next
+  signed char ke = 0, ve = 0;                                // a thread's two exponents
+  auto page_at = [&](int lp) { return lp * kFp8Page <= last_key ? pages[lp] : 0; };
+  auto load = [&](uint4 (&reg)[kPer], const unsigned char* cache, int tile) {
+    const unsigned char* at0 = cache + (((size_t)pg0 * a.n_kv + w.hk) * kFp8Page + row0) * HD + piece * 16;
+    const unsigned char* at1 = cache + (((size_t)pg1 * a.n_kv + w.hk) * kFp8Page + row0) * HD + piece * 16;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      reg[i] = make_uint4(0u, 0u, 0u, 0u);                   // rows behind the block's last key: nothing that may be NaN
+      if (tile * kPfKeys + row0 + i * kStep <= last_key)
+        reg[i] = *reinterpret_cast<const uint4*>((i < kPer / 2 ? at0 + i * kStep * HD : at1 + (i - kPer / 2) * kStep * HD));
     }
-    for (int i = 0; i < 4; ++i) {
-      mbar_init(&sh.x_full[i], 128);
-      sh.v_nan[i] = 0;
+  };
+  // Exponents of the tile's eight blocks, a thread a block (one behind the last key: anything, nobody sees its scores).
+  auto load_exps = [&]() {
+    if (ct < 8) {
+      const size_t at = ((size_t)(ct < 4 ? pg0 : pg1) * a.n_kv + w.hk) * kPageExps + (ct & 3);
+      ke = a.k_exp[at];
+      ve = a.v_exp[at];
     }
-    mbar_init(&sh.last, 1);
-    sh.abort = 0;
-    fence_mbar_init();
+  };
+  constexpr int kQ8 = HD / 16;                               // pieces of eight of a row's queries that a thread has: half of them
+  uint4 raw[kQ8];
+  float big = 0.f;
+  if (softmax) {
+#pragma unroll
+    for (int i = 0; i < kQ8; ++i) {
+      raw[i] = there ? *reinterpret_cast<const uint4*>(a.q + row_off + (half * kQ8 + i) * 8) : make_uint4(0u, 0u, 0u, 0u);
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = __bfloat1622float2(h[e]);
+        big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
+      }
+    }
+    sh.row_val[0][x][half][r] = big;
+  } else if (warp < 20 && n_steps > 0) {
+    pg0 = page_at(c0 * 2);
+    pg1 = page_at(c0 * 2 + 1);
+    const int next0 = page_at(c0 * 2 + 2), next1 = page_at(c0 * 2 + 3);
+    load(kr, a.k, c0);
+    load(vr, a.v, c0);
+    load_exps();
+    pg0 = next0;
+    pg1 = next1;
   }
-  if (warp == 12) {
-    tmem_alloc(&sh.tmem_base, 512);
-    tmem_relinquish();
+  __syncthreads();
+  if (softmax) {
+    big = fmaxf(big, sh.row_val[0][x][half ^ 1][r]);
+    const int eb = (int)(__float_as_uint(big) >> 23);
+    const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);         // the largest number into [2^14, 2^15)
+    const float up = pow2_of(shift);
+    f = a.scale2 * pow2_of(-shift);
+    uint8_t* dst = q_smem + x * Cfg::kQBytes;
+#pragma unroll
+    for (int i = 0; i < kQ8; ++i) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+      uint32_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = __bfloat1622float2(h[e]);
+        o[e] = pf_half2(y.x * up, y.y * up);
+      }
+      const int piece8 = half * kQ8 + i;
+      *reinterpret_cast<uint4*>(dst + (piece8 >> 3) * kPfSub + swizzle128_offset(r, piece8 & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    fence_proxy_async_smem();
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -262,58 +380,33 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   volatile int* abort = &sh.abort;
 #define LLMIE_FAIL(code) do { if (!*abort) { *abort = 1; atomicExch(a.status, (code)); } } while (0)
 
-  if (warp < 8) {
-    // ------------------------------------------------------------------ softmax: a thread a row
-    const int x = warp >> 2, r = threadIdx.x & 127;
-    const int n_x = x ? n_b : n_a, first_tok = t0 + x * tok_x, n_tok_x = x ? n_tok_b : n_tok_a;
-    const int rt = r / G, rh = r - rt * G;                   // token of the tile, query head of the group
-    const bool there = rt < n_tok_x;
+  if (softmax) {
+    // ------------------------------------------------------------------ softmax: two threads a row
+    const int n_x = x ? n_b : n_a;
     const int qpos = start + first_tok + min(rt, max(n_tok_x - 1, 0));
     const int lo = first_visible_key(qpos, a.window);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128, o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128);
-    const uint32_t p_addr = Cfg::kOwnP ? tmem + lanes + Cfg::kPCol + x * 64 : s_addr;
-    const int head = w.hk * G + rh;
-    const size_t row_off = ((size_t)(q_begin + first_tok + rt) * a.n_q + head) * HD;
-    float f;                                                 // of a score: scale log2(e) and the power of two of the row
-    {
-      uint4 raw[HD / 8];
-      float big = 0.f;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        raw[i] = there ? *reinterpret_cast<const uint4*>(a.q + row_off + i * 8) : make_uint4(0u, 0u, 0u, 0u);
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 y = __bfloat1622float2(h[e]);
-          big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
-        }
-      }
-      const int eb = (int)(__float_as_uint(big) >> 23);
-      const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);       // the largest number into [2^14, 2^15)
-      const float up = pow2_of(shift);
-      f = a.scale2 * pow2_of(-shift);
-      uint8_t* dst = q_smem + x * Cfg::kQBytes;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 y = __bfloat1622float2(h[e]);
-          o[e] = pf_half2(y.x * up, y.y * up);
-        }
-        *reinterpret_cast<uint4*>(dst + (i >> 3) * kPfSub + swizzle128_offset(r, i & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&sh.q_full);
-    }
+    const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128 + half * 64;
+    const uint32_t o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128) + half * (HD / 2);
+    const uint32_t p_addr = tmem + lanes + (Cfg::kOwnP ? Cfg::kPCol + x * 64 + half * 32 : Cfg::kSCol + x * 128 + half * 64);
+    uint64_t* pair = &sh.pair_bar[x][warp & 3];
+    int n_exchanges = 0;
+    // hands `mine` to the row's other thread and takes its number (the whole warp together)
+    auto exchange = [&](float mine, float& theirs) -> bool {
+      const int buf = n_exchanges & 1;
+      sh.row_val[buf][x][half][r] = mine;
+      mbar_arrive(pair);
+      const bool done = __all_sync(0xffffffffu, mbar_wait(pair, n_exchanges & 1, abort));
+      theirs = sh.row_val[buf][x][half ^ 1][r];
+      ++n_exchanges;
+      return done;
+    };
     // a score's factor is never 0: times -inf, which stands where the row does not look, that would be NaN
     auto factor = [&](float k_scale) { return fminf(fmaxf(f * k_scale, 1.2e-38f), 3.4e38f); };
-    float R = -INFINITY, l = 0.f;
-    uint32_t nan_cols[HD / 32];
+    float R = -INFINITY, l = 0.f;                            // l: over this thread's columns
+    uint32_t nan_cols[HD / 64];
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) nan_cols[i] = 0u;
+    for (int i = 0; i < HD / 64; ++i) nan_cols[i] = 0u;
     bool ok = true;
     // the first and last keys that every row of the tile sees
     const int all_to = start + first_tok, all_from = first_visible_key(start + first_tok + max(n_tok_x - 1, 0), a.window);
@@ -325,13 +418,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         break;
       }
       tc_fence_after_sync();
-      const int kbase = (c0 + j) * kPfKeys, ring = j & 3;
-      const bool edge = kbase + kPfKeys - 1 > all_to || kbase < all_from;
-      // pass 1: the largest s + ev of the row; scores that the row does not see become -inf, in tensor memory too
-      float mx = -INFINITY;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
+      const int kbase = (c0 + j) * kPfKeys + half * 64, ring = j & 3;
+      const float* k_scale = sh.k_scale[ring] + half * 4;
+      const float* v_add = sh.v_add[ring] + half * 4;
+      const float* v_back = sh.v_back[ring] + half * 4;
+      const bool edge = kbase + 63 > all_to || kbase < all_from;
+      const int nan_step = sh.v_nan[ring];
+      // 32 of the row's scores; those that it does not see are -inf
+      auto scores_of = [&](int c, uint32_t (&v)[32]) {
         tmem_ld_32x32(s_addr + c * 32, v);
         tmem_ld_wait();
         if (edge) {
@@ -340,23 +434,36 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if ((unsigned)(i - from) > span) v[i] = 0xff800000u;
-          tmem_st_32x32(s_addr + c * 32, v);
         }
+      };
+      float mx = -INFINITY;          // the largest s + ev of the row
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t v[32];
+        scores_of(c, v);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          float m0 = -INFINITY, m1 = -INFINITY;
+          const uint32_t* y = v + b * 16;
+          float m0 = __uint_as_float(y[0]), m1 = __uint_as_float(y[1]);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            m0 = fmaxf(m0, __uint_as_float(v[b * 16 + i]));
-            m1 = fmaxf(m1, __uint_as_float(v[b * 16 + i + 1]));
+          for (int i = 2; i < 14; i += 4) {
+            m0 = pf_max3(m0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+            m1 = pf_max3(m1, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
           }
-          mx = fmaxf(mx, fmaf(fmaxf(m0, m1), factor(sh.k_scale[ring][c * 2 + b]), sh.v_add[ring][c * 2 + b]));
+          m0 = pf_max3(m0, __uint_as_float(y[14]), __uint_as_float(y[15]));
+          mx = fmaxf(mx, fmaf(fmaxf(m0, m1), factor(k_scale[c * 2 + b]), v_add[c * 2 + b]));
         }
       }
-      if (edge) tmem_st_wait();
+      float other;
+      if (!exchange(mx, other)) {
+        LLMIE_FAIL(kStatusTimeoutMma);
+        ok = false;
+        break;
+      }
+      mx = fmaxf(mx, other);
       const bool grow = mx > R + kPfSlack || R == -INFINITY;
       if (__any_sync(0xffffffffu, grow && j > 0)) {
-        // the sums so far are brought to the new bound (rows that keep theirs: times 1)
+        // the sums so far are brought to the new bound (rows that keep theirs: times 1), this thread's half of the columns
         if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (j - 1) & 1, abort))) {
           LLMIE_FAIL(kStatusTimeoutMma);
           ok = false;
@@ -367,42 +474,40 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         l *= alpha;
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
-          uint32_t v[32];
-          tmem_ld_32x32(o_addr + c * 32, v);
+          uint32_t y[16];
+          tmem_ld_32x16(o_addr + c * 16, y);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-          tmem_st_32x32(o_addr + c * 32, v);
+          for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+          pf_tmem_st16(o_addr + c * 16, y);
         }
         tmem_st_wait();
       }
       if (grow) R = mx;
-      const float shift = (R == -INFINITY ? 0.f : R) - 7.f;
-      // pass 2: the weights
+      const float shift = (R == -INFINITY ? 0.f : R) - kPfTop;
+      // the weights, over the scores they come from or in columns of their own
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t v[32], o[16];
-        tmem_ld_32x32(s_addr + c * 32, v);
-        tmem_ld_wait();
+        scores_of(c, v);
+        if (Cfg::kOwnP && c == 1) {
+          // all of them are in registers: the next scores may be written
+          tc_fence_before_sync();
+          mbar_arrive(&sh.s_free[x]);
+        }
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float fk = factor(sh.k_scale[ring][c * 2 + b]), add = sh.v_add[ring][c * 2 + b] - shift;
-          const uint64_t fk2 = pf_pair(fk, fk), add2 = pf_pair(add, add);
-          uint64_t sum0 = 0ull, sum1 = 0ull;
+          const float fk = factor(k_scale[c * 2 + b]), add = v_add[c * 2 + b] - shift;
+          const uint32_t* y = v + b * 16;
+          float sum[4];
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float x0, x1;
-            pf_fma2(x0, x1, __uint_as_float(v[b * 16 + i]), __uint_as_float(v[b * 16 + i + 1]), fk2, add2);
-            x0 = pf_exp2(x0);
-            x1 = pf_exp2(x1);
-            if (i & 2) pf_add2(sum1, x0, x1);
-            else pf_add2(sum0, x0, x1);
+            const float x0 = pf_exp2(fmaf(__uint_as_float(y[i]), fk, add)), x1 = pf_exp2(fmaf(__uint_as_float(y[i + 1]), fk, add));
+            sum[i & 2] = i < 4 ? x0 : sum[i & 2] + x0;
+            sum[(i & 2) + 1] = i < 4 ? x1 : sum[(i & 2) + 1] + x1;
             o[b * 8 + i / 2] = pf_half2(x0, x1);
           }
-          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum0) : "l"(sum1));
-          float y0, y1;
-          asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(sum0));
-          l = fmaf(y0 + y1, sh.v_back[ring][c * 2 + b], l);
+          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), v_back[c * 2 + b], l);
         }
         if (Cfg::kOwnP && c == 0 && j > 0) {
           // the weights of the tile before have to be through the product before they are written over
@@ -419,13 +524,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(&sh.p_ready[x]);
-      if (sh.v_nan[ring] == j + 1) {
-        // rare: which columns of the values that this row sees are NaN
-        const int* pages = a.block_table + (size_t)a.seq_slot[w.seq] * a.max_pages;
-        for (int p = max(lo, kbase); p <= min(min(qpos, last_key), kbase + kPfKeys - 1); ++p) {
-          const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD);
+      if (nan_step == j + 1) {
+        // rare: which columns of the values that this row sees are NaN (this thread's half of them)
+        const int from = max(lo, (c0 + j) * kPfKeys), to = min(min(qpos, last_key), (c0 + j) * kPfKeys + kPfKeys - 1);
+        for (int p = from; p <= to; ++p) {
+          const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD +
+                                                                  half * (HD / 2));
 #pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
+          for (int i = 0; i < HD / 64; ++i) {
             uint32_t bits = 0u;
 #pragma unroll 1
             for (int e = 0; e < 32; ++e) bits |= ((row[i * 8 + e / 4] >> (e % 4 * 8) & 0x7fu) == 0x7fu ? 1u : 0u) << e;
@@ -441,65 +547,54 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       }
       tc_fence_after_sync();
     }
-    // ---- the row's result: the output, or a partial one. Where a wait gave up: NaN.
+    if (ok) {
+      float other;
+      if (exchange(l, other)) {
+        l += other;                  // both kept theirs relative to the same bounds
+      } else {
+        LLMIE_FAIL(kStatusTimeoutMma);
+        ok = false;
+      }
+    }
+    // ---- the row's result, half of its columns: the output, or a partial one. Where a wait gave up: NaN.
     float* rec = a.part + (size_t)w.slot * Cfg::kRecord;
     const int pr = x * kPfRows + r;
-    if (w.parts > 1 && there) {
+    if (w.parts > 1 && there && half == 0) {
       rec[2 * kPfRows * HD + pr] = R;
       rec[2 * kPfRows * (HD + 1) + pr] = ok ? l : __int_as_float(0x7fffffff);
     }
     const float inv = 1.f / l;
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) {
-      uint32_t v[32];
+    for (int c = 0; c < HD / 64; ++c) {
+      uint32_t y[32];
       if (ok && n_x > 0) {
-        tmem_ld_32x32(o_addr + c * 32, v);
+        tmem_ld_32x32(o_addr + c * 32, y);
         tmem_ld_wait();
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0u;
+        for (int i = 0; i < 32; ++i) y[i] = 0u;
       }
-      if (!there) continue;
-      float y[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) y[i] = (nan_cols[c] >> i & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]);
-      if (w.parts > 1) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(rec + (size_t)pr * HD + c * 32 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
-      } else {
+      if (there) {                   // (reads of tensor memory are warp-wide: only what follows them goes by the row)
+        const int col = half * (HD / 2) + c * 32;
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           float v8[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v8[e] = y[i + e] * inv;
-          store8(a.out + row_off + c * 32 + i, v8);
+          for (int e = 0; e < 8; ++e)
+            v8[e] = (nan_cols[c] >> (i + e) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + e]);
+          if (w.parts > 1) {
+            store8(rec + (size_t)pr * HD + col + i, v8);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v8[e] *= inv;
+            store8(a.out + row_off + col + i, v8);
+          }
         }
       }
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // ------------------------------------------------------------------ conversion: 128 threads, 16 codes at a time
-    constexpr int kPer = HD / 16;                            // pieces of 16 codes a row, and pieces a thread
-    const int ct = threadIdx.x - 256;
-    const int piece = ct % kPer, row0 = ct / kPer;           // rows row0, row0 + 128 / kPer, ...
-    constexpr int kStep = 128 / kPer;
-    const int* pages = a.block_table + (size_t)a.seq_slot[w.seq] * a.max_pages;
-    const int last_page = last_key / kFp8Page;
-    uint4 kr[kPer], vr[kPer];
-    auto page_row = [&](int tile, int half) -> size_t {      // (page, head) of a half of a key tile
-      const int lp = tile * 2 + half;
-      return (size_t)(lp <= last_page ? pages[lp] : 0) * a.n_kv + w.hk;
-    };
-    auto load = [&](uint4 (&reg)[kPer], const unsigned char* cache, int tile) {
-      const size_t p0 = page_row(tile, 0), p1 = page_row(tile, 1);
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int row = row0 + i * kStep;
-        reg[i] = make_uint4(0u, 0u, 0u, 0u);                 // rows behind the block's last key: nothing that may be NaN
-        if (tile * kPfKeys + row <= last_key)
-          reg[i] = *reinterpret_cast<const uint4*>(cache + ((row < 64 ? p0 : p1) * kFp8Page + (row & 63)) * HD + piece * 16);
-      }
-    };
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfConvertRegs));
     auto put = [&](uint8_t* dst, const uint4 (&reg)[kPer]) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -518,22 +613,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         *reinterpret_cast<uint4*>(at + swizzle128_offset(row, ch + 1 - odd)) = odd ? lo4 : hi4;
       }
     };
-    load(kr, a.k, c0);
-    load(vr, a.v, c0);
-    bool ok = true;
-    for (int j = 0; ok && j < n_steps; ++j) {
+    for (int j = 0; j < n_steps; ++j) {
       const int st = j & 1, ring = j & 3;
+      const int next0 = page_at((c0 + j + 2) * 2), next1 = page_at((c0 + j + 2) * 2 + 1);
       if (j >= 2 && !mbar_wait(&sh.k_empty[st], ((j >> 1) - 1) & 1, abort)) {
         LLMIE_FAIL(kStatusTimeoutEmpty);
         break;
       }
       if (ct < 8) {
-        // the exponents of the tile's eight blocks (a block behind the last key: anything, nobody sees its scores)
-        const size_t pr = page_row(c0 + j, ct >> 2);
-        const int ke = clamp_exponent(a.k_exp[pr * kPageExps + (ct & 3)]), ve = clamp_exponent(a.v_exp[pr * kPageExps + (ct & 3)]);
-        sh.k_scale[ring][ct] = pow2_of(ke);
-        sh.v_add[ring][ct] = (float)ve;
-        sh.v_back[ring][ct] = pow2_of(-ve);
+        const int k = clamp_exponent(ke), v = clamp_exponent(ve);
+        sh.k_scale[ring][ct] = pow2_of(k);
+        sh.v_add[ring][ct] = (float)v;
+        sh.v_back[ring][ct] = pow2_of(-v);
       }
       // NaN among the values: such codes become zeros here
       unsigned any = 0u;
@@ -542,7 +633,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         any |= ((vr[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((vr[i].y & 0x7f7f7f7fu) + 0x01010101u) |
                ((vr[i].z & 0x7f7f7f7fu) + 0x01010101u) | ((vr[i].w & 0x7f7f7f7fu) + 0x01010101u);
       put(k_smem + st * Cfg::kKvBytes, kr);
-      if (j + 1 < n_steps) load(kr, a.k, c0 + j + 1);
+      if (j + 1 < n_steps) {
+        load(kr, a.k, c0 + j + 1);
+        load_exps();
+      }
       fence_proxy_async_smem();
       if (any & 0x80808080u) {
         sh.v_nan[ring] = j + 1;
@@ -564,171 +658,153 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       }
       put(v_smem + st * Cfg::kKvBytes, vr);
       if (j + 1 < n_steps) load(vr, a.v, c0 + j + 1);
+      pg0 = next0;
+      pg1 = next1;
       fence_proxy_async_smem();
       mbar_arrive(&sh.v_full[st]);
     }
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------ the tensor core
-    if (elect_one()) {
+  } else {
+    // ------------------------------------------------------------------ the tensor core: a thread a tile, so that neither waits for the other's
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfIssueRegs));
+    if (warp < 22 && elect_one()) {
       constexpr uint32_t idesc_s = pf_instr_desc(kPfRows, kPfKeys, 0), idesc_o = pf_instr_desc(kPfRows, HD, 1);
-      bool ok = mbar_wait(&sh.q_full, 0, abort);
-      if (!ok) LLMIE_FAIL(kStatusTimeoutFull);
-      auto scores = [&](int x, int j) {                      // S = Q K^T of tile x, step j (its keys are there)
-        const uint32_t qa = smem_u32(q_smem + x * Cfg::kQBytes), ka = smem_u32(k_smem + (j & 1) * Cfg::kKvBytes);
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kPfSub + (kk & 3) * 32;
-          mma_bf16_ss(tmem + Cfg::kSCol + x * 128, make_smem_desc(qa + off, 16, 1024), make_smem_desc(ka + off, 16, 1024), idesc_s,
-                      kk > 0 ? 1u : 0u);
-        }
-        mma_commit(&sh.s_full[x]);
-      };
-      auto keys = [&](int j) -> bool {
-        if (mbar_wait(&sh.k_full[j & 1], (j >> 1) & 1, abort)) return true;
-        LLMIE_FAIL(kStatusTimeoutFull);
+      const int tx = warp - 20, n_x = tx ? n_b : n_a;
+      const uint32_t s_col = tmem + Cfg::kSCol + tx * 128, o_col = tmem + Cfg::kOCol + tx * (HD == 64 ? 64 : 128);
+      const uint32_t p_col = Cfg::kOwnP ? tmem + Cfg::kPCol + tx * 64 : s_col;
+      // descriptors of the operands' first 16 columns; the rest lie a fixed number of 16-byte units on
+      const uint64_t q_desc = make_smem_desc(smem_u32(q_smem + tx * Cfg::kQBytes), 16, 1024);
+      const uint64_t k_desc = make_smem_desc(smem_u32(k_smem), 16, 1024), v_desc = make_smem_desc(smem_u32(v_smem), kPfSub, 1024);
+      auto wait_for = [&](uint64_t* bar, uint32_t parity, int code) {
+        if (mbar_wait(bar, parity, abort)) return true;
+        LLMIE_FAIL(code);
         return false;
       };
-      if (ok && n_steps > 0 && (ok = keys(0))) {
+      auto scores = [&](int j) -> bool {                     // S = Q K^T of step j
+        if (!wait_for(&sh.k_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull)) return false;
         tc_fence_after_sync();
-        if (n_a > 0) scores(0, 0);
-        if (n_b > 0) scores(1, 0);
-        mma_commit(&sh.k_empty[0]);
-      }
-      for (int j = 0; ok && j < n_steps; ++j) {
-        if (!mbar_wait(&sh.v_full[j & 1], (j >> 1) & 1, abort)) {
-          LLMIE_FAIL(kStatusTimeoutFull);
-          break;
-        }
-        const uint32_t va = smem_u32(v_smem + (j & 1) * Cfg::kKvBytes);
-        for (int x = 0; ok && x < 2; ++x) {
-          const int n_x = x ? n_b : n_a;
-          if (j < n_x) {
-            if (!mbar_wait(&sh.p_ready[x], j & 1, abort)) {
-              LLMIE_FAIL(kStatusTimeoutMma);
-              ok = false;
-              break;
-            }
-            tc_fence_after_sync();
-            // where the weights have columns of their own the next scores may be written at once
-            if (Cfg::kOwnP && j + 1 < n_x) {
-              if (!(ok = keys(j + 1))) break;
-              tc_fence_after_sync();
-              scores(x, j + 1);
-            }
-            const uint32_t pa = tmem + (Cfg::kOwnP ? Cfg::kPCol + x * 64 : Cfg::kSCol + x * 128);
-            const uint32_t od = tmem + Cfg::kOCol + x * (HD == 64 ? 64 : 128);
+        const uint64_t kd = k_desc + (uint64_t)((j & 1) * (Cfg::kKvBytes >> 4));
 #pragma unroll
-            for (int kk = 0; kk < kPfKeys / 16; ++kk)        // 16 weights are 8 columns; 16 keys are 16 rows of the values
-              pf_mma_ts(od, pa + kk * 8, make_smem_desc(va + kk * 2048, kPfSub, 1024), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-            mma_commit(&sh.pv_done[x]);
-            if (!Cfg::kOwnP && j + 1 < n_x) {
-              // the next scores are written where these weights are read from
-              if (!mbar_wait(&sh.pv_done[x], j & 1, abort)) {
-                LLMIE_FAIL(kStatusTimeoutMma);
-                ok = false;
-                break;
-              }
-              if (!(ok = keys(j + 1))) break;
-              tc_fence_after_sync();
-              scores(x, j + 1);
-            }
-          }
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const int off = ((kk >> 2) * kPfSub + (kk & 3) * 32) >> 4;
+          mma_bf16_ss(s_col, q_desc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
         }
-        if (!ok) break;
+        mma_commit(&sh.s_full[tx]);
+        mma_commit(&sh.k_empty[j & 1]);
+        return true;
+      };
+      auto sums = [&](int j) -> bool {                       // O (+)= W V of step j
+        if (!wait_for(&sh.v_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull)) return false;
+        if (!wait_for(&sh.p_ready[tx], j & 1, kStatusTimeoutMma)) return false;
+        tc_fence_after_sync();
+        const uint64_t vd = v_desc + (uint64_t)((j & 1) * (Cfg::kKvBytes >> 4));
+#pragma unroll
+        for (int kk = 0; kk < kPfKeys / 16; ++kk)            // 16 weights are 8 columns; 16 keys are 16 rows of the values
+          pf_mma_ts(o_col, p_col + (Cfg::kOwnP || kk < 4 ? kk * 8 : 32 + kk * 8), vd + kk * (2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&sh.pv_done[tx]);
         mma_commit(&sh.v_empty[j & 1]);
-        if (j + 1 < n_steps) mma_commit(&sh.k_empty[(j + 1) & 1]);
+        return true;
+      };
+      bool ok = n_x == 0 || scores(0);
+      for (int j = 0; ok && j < n_x; ++j) {
+        // where the weights have columns of their own, the next scores as soon as these are in registers; else they are written
+        // where these weights are read from
+        if (Cfg::kOwnP && j + 1 < n_x) ok = wait_for(&sh.s_free[tx], j & 1, kStatusTimeoutMma) && scores(j + 1);
+        ok = ok && sums(j);
+        if (!Cfg::kOwnP && ok && j + 1 < n_x) ok = wait_for(&sh.pv_done[tx], j & 1, kStatusTimeoutMma) && scores(j + 1);
+      }
+      // steps that are the other tile's alone
+      for (int j = n_x; ok && j < n_steps; ++j) {
+        ok = wait_for(&sh.k_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull);
+        if (ok) mbar_arrive(&sh.k_empty[j & 1]);
+        ok = ok && wait_for(&sh.v_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull);
+        if (ok) mbar_arrive(&sh.v_empty[j & 1]);
       }
       // nothing may be in flight when the tensor memory is given back
-      mma_commit(&sh.last);
-      for (unsigned spin = 0; spin < (1u << 20) && !mbar_test(&sh.last, 0); ++spin) __nanosleep(32);
+      mma_commit(&sh.last[tx]);
+      for (unsigned spin = 0; spin < (1u << 20) && !mbar_test(&sh.last[tx], 0); ++spin) __nanosleep(32);
     }
   }
 #undef LLMIE_FAIL
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
 }
 
-// Joins the runs of the tiles that were cut: a warp a (token, query head). grid (tokens, ceil(n_q / 4)).
-template <int HD> __global__ void __launch_bounds__(128) prefill_fp8_join_kernel(const PrefillArgs a) {
+// Joins the runs of the tiles that were cut. grid (tiles of tokens x key/value heads, 8): an eighth of a tile's rows a block, a warp a row.
+constexpr int kPfJoinWarps = 8, kPfJoinSide = 8;
+template <int HD> __global__ void __launch_bounds__(kPfJoinWarps * 32) prefill_fp8_join_kernel(const PrefillArgs a) {
   pdl_launch_dependents();
-  pdl_wait();
   using Cfg = PfCfg<HD>;
-  const int lane = threadIdx.x & 31, head = blockIdx.y * 4 + (threadIdx.x >> 5), t = blockIdx.x;
-  if (head >= a.n_q) return;
-  const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = 2 * tok_x, hk = head / G;
-  const int run = pf_run(a, tok);
-  long long slots = 0;
-  for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-    int n = 0, f = 0, l = 0, parts = 1, q0 = 0, q1 = 0;
-    if (s0 + lane < a.n_seqs) {
-      pf_sequence(a, s0 + lane, tok, n, f, l);
-      parts = pf_runs(l, run);
-      q0 = a.cu_q[s0 + lane];
-      q1 = a.cu_q[s0 + lane + 1];
-    }
-    const long long cut = parts > 1 ? (long long)n * parts * a.n_kv : 0;
-    long long cuts = cut;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, cuts, o);
-      if (lane >= o) cuts += y;
-    }
-    const unsigned here = __ballot_sync(0xffffffffu, t >= q0 && t < q1);
-    if (!here) {
-      slots += __shfl_sync(0xffffffffu, cuts, 31);
-      continue;
-    }
-    const int src = __ffs(here) - 1;
-    parts = __shfl_sync(0xffffffffu, parts, src);
-    if (parts == 1) return;
-    n = __shfl_sync(0xffffffffu, n, src);
-    const int place = t - __shfl_sync(0xffffffffu, q0, src), tile = place / tok, in = place - tile * tok;
-    const int row = in / tok_x * kPfRows + in % tok_x * G + head % G;
-    const long long slot = slots + __shfl_sync(0xffffffffu, cuts - cut, src) + ((long long)(n - 1 - tile) * a.n_kv + hk) * parts;
-    const float* rec = a.part + slot * Cfg::kRecord;
-    float M = -INFINITY;
-    for (int p = lane; p < parts; p += 32) M = fmaxf(M, __ldcg(rec + (size_t)p * Cfg::kRecord + 2 * kPfRows * HD + row));
-    M = warp_max(M);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    float num[HD / 32], den = 0.f;
+  const int lane = threadIdx.x & 31;
+  const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = 2 * tok_x;
+  const PfWork w = pf_find<true>(a, tok, blockIdx.x);
+  if (w.parts <= 1) return;
+  // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait).
+  pdl_wait();
+  const float* base = a.part + (size_t)w.slot * Cfg::kRecord;
+  for (int row = blockIdx.y * kPfJoinWarps + (threadIdx.x >> 5); row < 2 * kPfRows; row += kPfJoinSide * kPfJoinWarps) {
+    const int x = row / kPfRows, rt = row % kPfRows / G, rh = row % kPfRows - rt * G, t = w.tile * tok + x * tok_x + rt;
+    if (rt >= tok_x || t >= w.q_len) continue;
+    const float* rec = base + (size_t)row * HD + lane * (HD / 32);
+    float M = -INFINITY, den = 0.f, num[HD / 32];
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) num[i] = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += 32) {
-      float fac = 0.f;
-      if (p0 + lane < parts) {
-        const float* r = rec + (size_t)(p0 + lane) * Cfg::kRecord;
-        fac = pf_exp2(__ldcg(r + 2 * kPfRows * HD + row) - Mu);
-        den = fmaf(fac, __ldcg(r + 2 * kPfRows * (HD + 1) + row), den);
-      }
-      const int m = min(32, parts - p0);
-      for (int p = 0; p < m; ++p) {
-        const float g = __shfl_sync(0xffffffffu, fac, p);
-        const float* r = rec + (size_t)(p0 + p) * Cfg::kRecord + (size_t)row * HD;
+    // eight runs at a time, all asked for at once
+    for (int p0 = 0; p0 < w.parts; p0 += 8) {
+      float m[8], l[8], v[8][HD / 32];
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) num[i] = fmaf(g, __ldcg(r + lane + 32 * i), num[i]);
+      for (int p = 0; p < 8; ++p) {
+        const bool there = p0 + p < w.parts;
+        const float* r = base + (size_t)(p0 + p) * Cfg::kRecord;
+        m[p] = there ? __ldcg(r + 2 * kPfRows * HD + row) : -INFINITY;
+        l[p] = there ? __ldcg(r + 2 * kPfRows * (HD + 1) + row) : 0.f;
+        const float* c = rec + (size_t)(there ? p0 + p : 0) * Cfg::kRecord;
+        if (HD == 64) {
+          const float2 y = __ldcg(reinterpret_cast<const float2*>(c));
+          v[p][0] = y.x;
+          v[p][1] = y.y;
+        } else {
+          const float4 y = __ldcg(reinterpret_cast<const float4*>(c));
+          v[p][0] = y.x;
+          v[p][1] = y.y;
+          v[p][HD / 32 - 2] = y.z;
+          v[p][HD / 32 - 1] = y.w;
+        }
       }
+      float M8 = M;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) M8 = fmaxf(M8, m[p]);
+      const float Mu = M8 == -INFINITY ? 0.f : M8, back = M == -INFINITY ? 0.f : pf_exp2(M - Mu);
+      den *= back;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) num[i] *= back;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float f = pf_exp2(m[p] - Mu);
+        den = fmaf(f, l[p], den);
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) num[i] = p0 + p < w.parts ? fmaf(f, v[p][i], num[i]) : num[i];
+      }
+      M = M8;
     }
-    den = warp_sum(den);
-    __nv_bfloat16* o = a.out + ((size_t)t * a.n_q + head) * HD;
+    __nv_bfloat16* o = a.out + ((size_t)(w.q_begin + t) * a.n_q + w.hk * G + rh) * HD + lane * (HD / 32);
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) o[lane + 32 * i] = __float2bfloat16_rn(num[i] / den);
-    return;
+    for (int i = 0; i < HD / 32; ++i) o[i] = __float2bfloat16_rn(num[i] / den);
   }
 }
 
 template <int HD>
-static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, cudaStream_t stream) {
+static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, int max_q_len, cudaStream_t stream) {
   using Cfg = PfCfg<HD>;
   cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return (int)e;
   const int tok = 2 * (kPfRows / (a.n_q / a.n_kv));
   // Pieces of work: the tiles of tokens, and the runs that they may be cut into. The most runs that a tile can have follow from
   // the most keys that the table has room for and the least work that so many tokens are.
-  const long long items = ((long long)n_tokens / tok + a.n_seqs) * a.n_kv;
+  const long long items = max_q_len <= tok ? (long long)a.n_seqs * a.n_kv : ((long long)n_tokens / tok + a.n_seqs) * a.n_kv;
   double least = (double)n_tokens / tok * a.n_kv;
   long long most_tiles = ((long long)a.max_pages * kFp8Page + kPfKeys - 1) / kPfKeys;
   if (a.window == 0) {
@@ -742,12 +818,13 @@ static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, cudaStream_t s
   const long long parts = (most_tiles + run / 2) / run;
   const bool cut = parts > 1;
   if (cut && !a.part) return kPfNeedsScratch;
-  const long long blocks = cut ? min(items * parts, items + kPfSlots) : items;
-  if (blocks > 0x7fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  // (a sequence of one tile: parts - 1 <= last / run, and all of them have 148 runs of keys between them)
+  const long long blocks = cut ? min(items * parts, items + (max_q_len <= tok ? kPfSms : kPfSlots)) : items;
+  if (blocks * most_tiles > 0x3fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
   launch_k(prefill_fp8_kernel<HD>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
   LLMIE_LAUNCH_CHECK();
   if (cut) {
-    launch_k(prefill_fp8_join_kernel<HD>, dim3(n_tokens, (a.n_q + 3) / 4), dim3(128), 0, stream, a);
+    launch_k(prefill_fp8_join_kernel<HD>, dim3((unsigned)items, kPfJoinSide), dim3(kPfJoinWarps * 32), 0, stream, a);
     LLMIE_LAUNCH_CHECK();
   }
   return LLMIE_OK;
@@ -764,20 +841,20 @@ extern "C" int llmie_attention_prefill_fp8_scratch(int hd) {
 
 // q, out bfloat16 [n_tokens, n_q hd], hd 64 or 128, at most 128 query heads a key/value head; sequences packed one after another
 // (cu_q [n_seqs + 1]); caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv, 4]; seq_start[i]: tokens that sequence i
-// held before this step, whose keys are in the cache already. scale > 0. window: as in the other attention kernels.
+// held before this step, whose keys are in the cache already; max_q_len: the most tokens that one brings. scale > 0. window: as in the other attention kernels.
 // scratch: llmie_attention_prefill_fp8_scratch floats, 16-byte aligned; null: a call that needs it launches nothing and returns -5.
 extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, const void* v_cache, const void* k_exp,
                                            const void* v_exp, void* out, float* scratch, int* status, const int* cu_q,
                                            const int* seq_slot, const int* seq_start, const int* block_table, int max_pages,
-                                           int n_tokens, int n_seqs, int n_q, int n_kv, int hd, float scale, int window,
-                                           cudaStream_t stream) {
+                                           int n_tokens, int n_seqs, int max_q_len, int n_q, int n_kv, int hd, float scale,
+                                           int window, cudaStream_t stream) {
   if (n_tokens < 0 || n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || !status) return LLMIE_ERR_BAD_ARG;
   if (!(scale > 0.f)) return LLMIE_ERR_BAD_ARG;              // a row's bound is taken before scores are scaled
-  if ((hd != 64 && hd != 128) || n_q / n_kv > kPfRows || (n_q + 3) / 4 > 65535) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  if ((hd != 64 && hd != 128) || n_q / n_kv > kPfRows) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(scratch)) return LLMIE_ERR_ALIGNMENT;
-  if (n_tokens == 0 || n_seqs == 0) return LLMIE_OK;
+  if (n_tokens == 0 || n_seqs == 0 || max_q_len <= 0) return LLMIE_OK;
   const PrefillArgs a{(const __nv_bfloat16*)q, (const unsigned char*)k_cache, (const unsigned char*)v_cache, (const signed char*)k_exp,
                       (const signed char*)v_exp, (__nv_bfloat16*)out, scratch, status, cu_q, seq_slot, seq_start, block_table,
                       max_pages, n_seqs, n_q, n_kv, scale * 1.4426950408889634f, window};
-  return hd == 64 ? launch_prefill_fp8<64>(a, n_tokens, stream) : launch_prefill_fp8<128>(a, n_tokens, stream);
+  return hd == 64 ? launch_prefill_fp8<64>(a, n_tokens, max_q_len, stream) : launch_prefill_fp8<128>(a, n_tokens, max_q_len, stream);
 }

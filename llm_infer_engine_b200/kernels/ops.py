@@ -1636,7 +1636,7 @@ FP8_BLOCK = 16           # positions that share an exponent
 _FP8_STORE_ARGS = [_c_void_p] * 11 + [_c_int] * 10 + [_c_void_p]
 _FP8_ATTENTION_ARGS = [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
 _FP8_STEP_ARGS = [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
-_FP8_PROMPT_ARGS = [_c_void_p] * 12 + [_c_int] * 6 + [_c_float, _c_int, _c_void_p]
+_FP8_PROMPT_ARGS = [_c_void_p] * 12 + [_c_int] * 7 + [_c_float, _c_int, _c_void_p]
 
 
 def _need_heads(name: str, n_q: int, n_kv: int) -> None:
@@ -1877,8 +1877,8 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     if q.shape != (T, n_q * head_dim) or out.shape != q.shape:
         raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_q} heads of {head_dim}")
     _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    if n_seqs < 0:
-        raise KernelError(f"{name}: {n_seqs} sequences")
+    if n_seqs < 0 or (T > 0 and max_q_len <= 0):
+        raise KernelError(f"{name}: {n_seqs} sequences with at most {max_q_len} new tokens each")
     _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
     if trace.timer is not None:
         _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
@@ -1886,7 +1886,7 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     _with_scratch(name, "attention_prefill_fp8", f,
                   (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
                   (tc_status_word(q.device).data_ptr(), cu_q.data_ptr(), seq_slot.data_ptr(), seq_start.data_ptr(),
-                   block_table.data_ptr(), block_table.shape[1], T, n_seqs, n_q, n_kv, head_dim, scale, window, _stream()),
+                   block_table.data_ptr(), block_table.shape[1], T, n_seqs, max_q_len, n_q, n_kv, head_dim, scale, window, _stream()),
                   (head_dim,), q.device)
     return out
 
