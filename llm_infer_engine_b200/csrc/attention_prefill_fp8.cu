@@ -3,10 +3,9 @@
 //   o_t = sum_j 2^(s_tj) c_j 2^(ev_j) / sum_j 2^(s_tj),   s_tj = scale log2(e) (q_t . k_j) 2^(ek_j),   j seen by t     (k, c: codes)
 //
 // Rows. A key/value head is read once for all of its query heads: the rows of a 128-row operand are (token, query head) pairs,
-// 128 / G tokens of the G heads that share the key/value head. A block has two such tiles, A and B; while the softmax of one works
-// on its scores the tensor core is busy with the other's. Two threads share a row, half of a key tile's columns each: what a tile
-// costs is mostly latency (tensor memory, barriers, one exponential a score at 16 a clock and SM), which sixteen warps hide
-// better than eight (with a thread a row, all 128 scores in its registers: 55 us where this takes KPF_US).
+// 128 / G tokens of the G heads that share the key/value head. A block has two such tiles, A and B, with a softmax warpgroup
+// each (a thread a row, its scores of a step in registers) and an issuing thread each; while one's softmax works, the tensor core is
+// busy with the other's.
 //
 // Keys and values become half-precision numbers (exactly) on their way into shared memory: four warps load codes into
 // registers a tile ahead, convert them and write the tensor core's operand layout. Their exponents stay out of the products:
@@ -33,11 +32,7 @@ using namespace tc;
 
 constexpr int kPfRows = 128;         // rows of a tile
 constexpr int kPfKeys = 128;         // keys of a step
-constexpr int kPfSoftmax = 512;      // warps 0-3, 4-7: softmax of tile A, columns 0-63 and 64-127; 8-11, 12-15: of tile B
-constexpr int kPfThreads = kPfSoftmax + 128 + 128;     // 16-19: conversion; 20, 21: the products of tile A, of tile B; 22, 23: nothing
-// Registers a thread of a softmax, the conversion and the last warpgroup keeps. A block is launched with 80 a thread, six times 80.
-constexpr int kPfLaunchRegs = 80, kPfConvertRegs = 112, kPfIssueRegs = 48;
-static_assert(4 * kPfLaunchRegs + kPfConvertRegs + kPfIssueRegs <= 6 * kPfLaunchRegs, "more than the block has would never be granted");
+constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B; 8-11: conversion; 12, 13: the products of A, of B; 14, 15: nothing
 constexpr int kPfSub = kPfRows * 128;        // bytes of 128 rows of 64 half-precision numbers
 constexpr int kPfSms = 148;
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
@@ -55,6 +50,10 @@ template <int HD> struct PfCfg {
   static constexpr bool kOwnP = HD == 64;                    // tensor memory has room for the weights beside the scores
   static constexpr int kSCol = 0, kOCol = 256, kPCol = 384;  // columns: scores of A and B, sums of A and B, weights
   static constexpr int kRecord = 2 * kPfRows * (HD + 2);     // floats of a partial result: sums, then bounds, then denominators
+  // Registers that a thread of a softmax, the conversion and the last warpgroup keeps of the 128 that it is launched with: a row's
+  // 128 scores stay in registers, a converting thread has a step's codes in them.
+  static constexpr int kSoftmaxRegs = HD == 64 ? 200 : 184, kConvertRegs = HD == 64 ? 80 : 104, kIssueRegs = HD == 64 ? 32 : 40;
+  static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "more than the block has would never be granted");
 };
 
 struct PrefillArgs {
@@ -150,11 +149,11 @@ __device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, i
   return q;
 }
 // Key tiles that a run has on average: a 148th of the step (first and last tile of tokens stand for all of a sequence).
-// All lanes of a warp call it.
-__device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok) {
-  const int lane = threadIdx.x & 31;
-  float twice = 0.f;                 // every block works it out from the same numbers in the same order
-  for (int s = lane; s < a.n_seqs; s += 32) {
+// `mine`: the lane's first sequence. All lanes of a warp call it.
+__device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
+  // every block works it out from the same numbers in the same order
+  float twice = (float)mine.tiles * (float)(mine.first + mine.last);
+  for (int s = (threadIdx.x & 31) + 32; s < a.n_seqs; s += 32) {
     const PfSequence q = pf_sequence(a, s, tok);
     twice += (float)q.tiles * (float)(q.first + q.last);
   }
@@ -175,11 +174,12 @@ struct PfWork {
 template <bool WHOLE>
 __device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int index) {
   const int lane = threadIdx.x & 31;
-  const int run = pf_run(a, tok);
+  const PfSequence mine = pf_sequence(a, lane, tok);
+  const int run = pf_run(a, tok, mine);
   PfWork w{0, 0, 0, 0, 0, 0, 0, 0, 0};
   int before = 0, slots = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-    const PfSequence q = pf_sequence(a, s0 + lane, tok);
+    const PfSequence q = s0 == 0 ? mine : pf_sequence(a, s0 + lane, tok);
     const int parts = pf_runs(q.last, run);
     const int all = q.tiles * parts * a.n_kv, own = WHOLE ? q.tiles * a.n_kv : all, cut = parts > 1 ? all : 0;
     int incl = own, cuts = cut;
@@ -224,11 +224,7 @@ struct PfShared {
   // the scores of the step two on are done, which both tiles' softmax has let begin behind its last look at this step.)
   float k_scale[4][8], v_add[4][8], v_back[4][8];
   int v_nan[4];
-  // the two threads of a row tell each other their numbers here; the two warps that share 32 rows meet at a barrier of their own.
-  // Two buffers in turn: a thread is never more than one exchange ahead.
-  float row_val[2][2][2][kPfRows];
   PfWork work;
-  uint64_t pair_bar[2][4];
 };
 
 // ------------------------------------------------------------------------------------------ the kernel
@@ -257,8 +253,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       mbar_init(&sh.v_full[s], 128);
       mbar_init(&sh.v_empty[s], 2);
       mbar_init(&sh.s_full[s], 1);
-      mbar_init(&sh.s_free[s], 256);
-      mbar_init(&sh.p_ready[s], 256);
+      mbar_init(&sh.s_free[s], 128);
+      mbar_init(&sh.p_ready[s], 128);
       mbar_init(&sh.pv_done[s], 1);
       mbar_init(&sh.last[s], 1);
     }
@@ -266,14 +262,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       mbar_init(&sh.x_full[i], 128);
       sh.v_nan[i] = 0;
     }
-    for (int i = 0; i < 8; ++i) mbar_init(&sh.pair_bar[i >> 2][i & 3], 64);
     sh.abort = 0;
     fence_mbar_init();
   }
   __syncthreads();
   const PfWork w = sh.work;
   if (w.parts == 0) return;          // the whole block alike
-  if (warp == 20) {
+  if (warp == 12) {
     tmem_alloc(&sh.tmem_base, 512);
     tmem_relinquish();
   }
@@ -290,8 +285,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   const int n_steps = max(n_a, n_b);
 
   // What needs no barrier begins before the block meets: the rows' queries go to shared memory, the first codes are asked for.
-  const bool softmax = warp < 16;
-  const int x = warp >> 3 & 1, half = warp >> 2 & 1, r = threadIdx.x & 127;    // tile, half and row of a softmax thread
+  const bool softmax = warp < 8;
+  const int x = warp >> 2 & 1, r = threadIdx.x & 127;        // tile and row of a softmax thread
   const int first_tok = t0 + x * tok_x, n_tok_x = x ? n_tok_b : n_tok_a;
   const int rt = r / G, rh = r - rt * G;                     // token of the tile, query head of the group
   const bool there = softmax && rt < n_tok_x;
@@ -304,7 +299,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   uint4 kr[kPer], vr[kPer];
   // Everything is asked for well before it is looked at: a tile's pages a step before its codes, its codes and exponents a step
   // before they are written out. (Where an exponent was clamped, or a page's address made, as soon as it was asked for, the
-  // conversion waited for memory twice a tile and the whole kernel for the conversion: 57 us for KPF_US.)
+  // conversion waited for memory twice a tile, and the whole kernel for the conversion: 3,500 clocks a step.)
   int pg0 = 0, pg1 = 0;                                      // pages of the tile to be asked for next
   signed char ke = 0, ve = 0;                                // a thread's two exponents
   auto page_at = [&](int lp) { return lp * kFp8Page <= last_key ? pages[lp] : 0; };
@@ -326,13 +321,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       ve = a.v_exp[at];
     }
   };
-  constexpr int kQ8 = HD / 16;                               // pieces of eight of a row's queries that a thread has: half of them
-  uint4 raw[kQ8];
-  float big = 0.f;
   if (softmax) {
+    uint4 raw[HD / 8];
+    float big = 0.f;
 #pragma unroll
-    for (int i = 0; i < kQ8; ++i) {
-      raw[i] = there ? *reinterpret_cast<const uint4*>(a.q + row_off + (half * kQ8 + i) * 8) : make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < HD / 8; ++i) {
+      raw[i] = there ? *reinterpret_cast<const uint4*>(a.q + row_off + i * 8) : make_uint4(0u, 0u, 0u, 0u);
       const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -340,8 +334,24 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
       }
     }
-    sh.row_val[0][x][half][r] = big;
-  } else if (warp < 20 && n_steps > 0) {
+    const int eb = (int)(__float_as_uint(big) >> 23);
+    const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);         // the largest number into [2^14, 2^15)
+    const float up = pow2_of(shift);
+    f = a.scale2 * pow2_of(-shift);
+    uint8_t* dst = q_smem + x * Cfg::kQBytes;
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
+      uint32_t o[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = __bfloat1622float2(h[e]);
+        o[e] = pf_half2(y.x * up, y.y * up);
+      }
+      *reinterpret_cast<uint4*>(dst + (i >> 3) * kPfSub + swizzle128_offset(r, i & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+    fence_proxy_async_smem();
+  } else if (warp < 12 && n_steps > 0) {
     pg0 = page_at(c0 * 2);
     pg1 = page_at(c0 * 2 + 1);
     const int next0 = page_at(c0 * 2 + 2), next1 = page_at(c0 * 2 + 3);
@@ -351,28 +361,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
     pg0 = next0;
     pg1 = next1;
   }
-  __syncthreads();
-  if (softmax) {
-    big = fmaxf(big, sh.row_val[0][x][half ^ 1][r]);
-    const int eb = (int)(__float_as_uint(big) >> 23);
-    const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);         // the largest number into [2^14, 2^15)
-    const float up = pow2_of(shift);
-    f = a.scale2 * pow2_of(-shift);
-    uint8_t* dst = q_smem + x * Cfg::kQBytes;
-#pragma unroll
-    for (int i = 0; i < kQ8; ++i) {
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-      uint32_t o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 y = __bfloat1622float2(h[e]);
-        o[e] = pf_half2(y.x * up, y.y * up);
-      }
-      const int piece8 = half * kQ8 + i;
-      *reinterpret_cast<uint4*>(dst + (piece8 >> 3) * kPfSub + swizzle128_offset(r, piece8 & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    fence_proxy_async_smem();
-  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -381,32 +369,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 #define LLMIE_FAIL(code) do { if (!*abort) { *abort = 1; atomicExch(a.status, (code)); } } while (0)
 
   if (softmax) {
-    // ------------------------------------------------------------------ softmax: two threads a row
+    // ------------------------------------------------------------------ softmax: a thread a row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
     const int n_x = x ? n_b : n_a;
     const int qpos = start + first_tok + min(rt, max(n_tok_x - 1, 0));
     const int lo = first_visible_key(qpos, a.window);
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128 + half * 64;
-    const uint32_t o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128) + half * (HD / 2);
-    const uint32_t p_addr = tmem + lanes + (Cfg::kOwnP ? Cfg::kPCol + x * 64 + half * 32 : Cfg::kSCol + x * 128 + half * 64);
-    uint64_t* pair = &sh.pair_bar[x][warp & 3];
-    int n_exchanges = 0;
-    // hands `mine` to the row's other thread and takes its number (the whole warp together)
-    auto exchange = [&](float mine, float& theirs) -> bool {
-      const int buf = n_exchanges & 1;
-      sh.row_val[buf][x][half][r] = mine;
-      mbar_arrive(pair);
-      const bool done = __all_sync(0xffffffffu, mbar_wait(pair, n_exchanges & 1, abort));
-      theirs = sh.row_val[buf][x][half ^ 1][r];
-      ++n_exchanges;
-      return done;
-    };
+    const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128, o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128);
+    const uint32_t p_addr = Cfg::kOwnP ? tmem + lanes + Cfg::kPCol + x * 64 : s_addr;
     // a score's factor is never 0: times -inf, which stands where the row does not look, that would be NaN
     auto factor = [&](float k_scale) { return fminf(fmaxf(f * k_scale, 1.2e-38f), 3.4e38f); };
-    float R = -INFINITY, l = 0.f;                            // l: over this thread's columns
-    uint32_t nan_cols[HD / 64];
+    float R = -INFINITY, l = 0.f;
+    uint32_t nan_cols[HD / 32];
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) nan_cols[i] = 0u;
+    for (int i = 0; i < HD / 32; ++i) nan_cols[i] = 0u;
     bool ok = true;
     // the first and last keys that every row of the tile sees
     const int all_to = start + first_tok, all_from = first_visible_key(start + first_tok + max(n_tok_x - 1, 0), a.window);
@@ -418,52 +394,45 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         break;
       }
       tc_fence_after_sync();
-      const int kbase = (c0 + j) * kPfKeys + half * 64, ring = j & 3;
-      const float* k_scale = sh.k_scale[ring] + half * 4;
-      const float* v_add = sh.v_add[ring] + half * 4;
-      const float* v_back = sh.v_back[ring] + half * 4;
-      const bool edge = kbase + 63 > all_to || kbase < all_from;
+      const int kbase = (c0 + j) * kPfKeys, ring = j & 3;
+      const bool edge = kbase + kPfKeys - 1 > all_to || kbase < all_from;
       const int nan_step = sh.v_nan[ring];
-      // 32 of the row's scores; those that it does not see are -inf
-      auto scores_of = [&](int c, uint32_t (&v)[32]) {
-        tmem_ld_32x32(s_addr + c * 32, v);
-        tmem_ld_wait();
-        if (edge) {
-          const int from = lo - kbase - c * 32;
-          const unsigned span = (unsigned)(qpos - lo);
+      // the row's scores; those that it does not see are -inf
+      uint32_t v[4][32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if ((unsigned)(i - from) > span) v[i] = 0xff800000u;
-        }
-      };
-      float mx = -INFINITY;          // the largest s + ev of the row
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, v[c]);
+      float fk[8];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t v[32];
-        scores_of(c, v);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const uint32_t* y = v + b * 16;
-          float m0 = __uint_as_float(y[0]), m1 = __uint_as_float(y[1]);
-#pragma unroll
-          for (int i = 2; i < 14; i += 4) {
-            m0 = pf_max3(m0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
-            m1 = pf_max3(m1, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
-          }
-          m0 = pf_max3(m0, __uint_as_float(y[14]), __uint_as_float(y[15]));
-          mx = fmaxf(mx, fmaf(fmaxf(m0, m1), factor(k_scale[c * 2 + b]), v_add[c * 2 + b]));
-        }
+      for (int b = 0; b < 8; ++b) fk[b] = factor(sh.k_scale[ring][b]);
+      tmem_ld_wait();
+      if (Cfg::kOwnP) {
+        // they are in registers: the next scores may be written
+        tc_fence_before_sync();
+        mbar_arrive(&sh.s_free[x]);
       }
-      float other;
-      if (!exchange(mx, other)) {
-        LLMIE_FAIL(kStatusTimeoutMma);
-        ok = false;
-        break;
+      if (edge) {
+        const int from = lo - kbase;
+        const unsigned span = (unsigned)(qpos - lo);
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if ((unsigned)(i - from) > span) v[i >> 5][i & 31] = 0xff800000u;
       }
-      mx = fmaxf(mx, other);
+      float mx = -INFINITY;          // the largest s + ev
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint32_t* y = v[b >> 1] + (b & 1) * 16;
+        float m0 = __uint_as_float(y[0]), m1 = __uint_as_float(y[1]);
+#pragma unroll
+        for (int i = 2; i < 14; i += 4) {
+          m0 = pf_max3(m0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+          m1 = pf_max3(m1, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+        }
+        m0 = pf_max3(m0, __uint_as_float(y[14]), __uint_as_float(y[15]));
+        mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fk[b], sh.v_add[ring][b]));
+      }
       const bool grow = mx > R + kPfSlack || R == -INFINITY;
       if (__any_sync(0xffffffffu, grow && j > 0)) {
-        // the sums so far are brought to the new bound (rows that keep theirs: times 1), this thread's half of the columns
+        // the sums so far are brought to the new bound (rows that keep theirs: times 1)
         if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (j - 1) & 1, abort))) {
           LLMIE_FAIL(kStatusTimeoutMma);
           ok = false;
@@ -473,7 +442,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         const float alpha = !grow ? 1.f : R == -INFINITY ? 0.f : pf_exp2(R - mx);
         l *= alpha;
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
+        for (int c = 0; c < HD / 16; ++c) {
           uint32_t y[16];
           tmem_ld_32x16(o_addr + c * 16, y);
           tmem_ld_wait();
@@ -485,53 +454,44 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       }
       if (grow) R = mx;
       const float shift = (R == -INFINITY ? 0.f : R) - kPfTop;
+      if (Cfg::kOwnP && j > 0) {
+        // the weights of the tile before have to be through the product before they are written over
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (j - 1) & 1, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+      }
       // the weights, over the scores they come from or in columns of their own
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t v[32], o[16];
-        scores_of(c, v);
-        if (Cfg::kOwnP && c == 1) {
-          // all of them are in registers: the next scores may be written
-          tc_fence_before_sync();
-          mbar_arrive(&sh.s_free[x]);
-        }
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[16];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const float fk = factor(k_scale[c * 2 + b]), add = v_add[c * 2 + b] - shift;
-          const uint32_t* y = v + b * 16;
+          const float add = sh.v_add[ring][c * 2 + b] - shift;
+          const uint32_t* y = v[c] + b * 16;
           float sum[4];
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const float x0 = pf_exp2(fmaf(__uint_as_float(y[i]), fk, add)), x1 = pf_exp2(fmaf(__uint_as_float(y[i + 1]), fk, add));
+            const float x0 = pf_exp2(fmaf(__uint_as_float(y[i]), fk[c * 2 + b], add)), x1 = pf_exp2(fmaf(__uint_as_float(y[i + 1]), fk[c * 2 + b], add));
             sum[i & 2] = i < 4 ? x0 : sum[i & 2] + x0;
             sum[(i & 2) + 1] = i < 4 ? x1 : sum[(i & 2) + 1] + x1;
             o[b * 8 + i / 2] = pf_half2(x0, x1);
           }
-          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), v_back[c * 2 + b], l);
-        }
-        if (Cfg::kOwnP && c == 0 && j > 0) {
-          // the weights of the tile before have to be through the product before they are written over
-          if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (j - 1) & 1, abort))) {
-            LLMIE_FAIL(kStatusTimeoutMma);
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
+          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), sh.v_back[ring][c * 2 + b], l);
         }
         pf_tmem_st16(p_addr + c * 16, o);
       }
-      if (!ok) break;
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(&sh.p_ready[x]);
       if (nan_step == j + 1) {
-        // rare: which columns of the values that this row sees are NaN (this thread's half of them)
-        const int from = max(lo, (c0 + j) * kPfKeys), to = min(min(qpos, last_key), (c0 + j) * kPfKeys + kPfKeys - 1);
-        for (int p = from; p <= to; ++p) {
-          const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD +
-                                                                  half * (HD / 2));
+        // rare: which columns of the values that this row sees are NaN
+        for (int p = max(lo, kbase); p <= min(min(qpos, last_key), kbase + kPfKeys - 1); ++p) {
+          const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD);
 #pragma unroll
-          for (int i = 0; i < HD / 64; ++i) {
+          for (int i = 0; i < HD / 32; ++i) {
             uint32_t bits = 0u;
 #pragma unroll 1
             for (int e = 0; e < 32; ++e) bits |= ((row[i * 8 + e / 4] >> (e % 4 * 8) & 0x7fu) == 0x7fu ? 1u : 0u) << e;
@@ -547,25 +507,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       }
       tc_fence_after_sync();
     }
-    if (ok) {
-      float other;
-      if (exchange(l, other)) {
-        l += other;                  // both kept theirs relative to the same bounds
-      } else {
-        LLMIE_FAIL(kStatusTimeoutMma);
-        ok = false;
-      }
-    }
-    // ---- the row's result, half of its columns: the output, or a partial one. Where a wait gave up: NaN.
+    // ---- the row's result: the output, or a partial one. Where a wait gave up: NaN.
     float* rec = a.part + (size_t)w.slot * Cfg::kRecord;
     const int pr = x * kPfRows + r;
-    if (w.parts > 1 && there && half == 0) {
+    if (w.parts > 1 && there) {
       rec[2 * kPfRows * HD + pr] = R;
       rec[2 * kPfRows * (HD + 1) + pr] = ok ? l : __int_as_float(0x7fffffff);
     }
     const float inv = 1.f / l;
 #pragma unroll
-    for (int c = 0; c < HD / 64; ++c) {
+    for (int c = 0; c < HD / 32; ++c) {
       uint32_t y[32];
       if (ok && n_x > 0) {
         tmem_ld_32x32(o_addr + c * 32, y);
@@ -575,7 +526,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         for (int i = 0; i < 32; ++i) y[i] = 0u;
       }
       if (there) {                   // (reads of tensor memory are warp-wide: only what follows them goes by the row)
-        const int col = half * (HD / 2) + c * 32;
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
           float v8[8];
@@ -583,18 +533,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
           for (int e = 0; e < 8; ++e)
             v8[e] = (nan_cols[c] >> (i + e) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + e]);
           if (w.parts > 1) {
-            store8(rec + (size_t)pr * HD + col + i, v8);
+            store8(rec + (size_t)pr * HD + c * 32 + i, v8);
           } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v8[e] *= inv;
-            store8(a.out + row_off + col + i, v8);
+            store8(a.out + row_off + c * 32 + i, v8);
           }
         }
       }
     }
-  } else if (warp < 20) {
+  } else if (warp < 12) {
     // ------------------------------------------------------------------ conversion: 128 threads, 16 codes at a time
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfConvertRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kConvertRegs));
     auto put = [&](uint8_t* dst, const uint4 (&reg)[kPer]) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -665,10 +615,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
     }
   } else {
     // ------------------------------------------------------------------ the tensor core: a thread a tile, so that neither waits for the other's
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfIssueRegs));
-    if (warp < 22 && elect_one()) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kIssueRegs));
+    if (warp < 14 && elect_one()) {
       constexpr uint32_t idesc_s = pf_instr_desc(kPfRows, kPfKeys, 0), idesc_o = pf_instr_desc(kPfRows, HD, 1);
-      const int tx = warp - 20, n_x = tx ? n_b : n_a;
+      const int tx = warp - 12, n_x = tx ? n_b : n_a;
       const uint32_t s_col = tmem + Cfg::kSCol + tx * 128, o_col = tmem + Cfg::kOCol + tx * (HD == 64 ? 64 : 128);
       const uint32_t p_col = Cfg::kOwnP ? tmem + Cfg::kPCol + tx * 64 : s_col;
       // descriptors of the operands' first 16 columns; the rest lie a fixed number of 16-byte units on
@@ -699,7 +649,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         const uint64_t vd = v_desc + (uint64_t)((j & 1) * (Cfg::kKvBytes >> 4));
 #pragma unroll
         for (int kk = 0; kk < kPfKeys / 16; ++kk)            // 16 weights are 8 columns; 16 keys are 16 rows of the values
-          pf_mma_ts(o_col, p_col + (Cfg::kOwnP || kk < 4 ? kk * 8 : 32 + kk * 8), vd + kk * (2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
+          pf_mma_ts(o_col, p_col + kk * 8, vd + kk * (2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
         mma_commit(&sh.pv_done[tx]);
         mma_commit(&sh.v_empty[j & 1]);
         return true;
@@ -727,7 +677,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 #undef LLMIE_FAIL
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 20) {
+  if (warp == 12) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, 512);
   }
