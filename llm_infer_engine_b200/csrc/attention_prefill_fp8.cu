@@ -35,9 +35,10 @@ constexpr int kPfKeys = 128;         // keys of a step
 constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B; 8-11: conversion; 12, 13: the products of A, of B; 14, 15: nothing
 constexpr int kPfSub = kPfRows * 128;        // bytes of 128 rows of 64 half-precision numbers
 constexpr int kPfSms = 148;
+constexpr int kPfRing = 8;
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
 constexpr int kPfLeast = 4;          // key tiles that a run has at least, on average
-constexpr int kPfSlots = 400;        // partial results at once (see pf_plan)
+constexpr int kPfSlots = 400;        // partial results at once (see pf_runs)
 constexpr float kPfTop = 7.f;        // the bound's own weight is 2^7
 constexpr float kPfSlack = 8.f;      // how far scores may outgrow the bound, in units of log2
 
@@ -50,10 +51,16 @@ template <int HD> struct PfCfg {
   static constexpr bool kOwnP = HD == 64;                    // tensor memory has room for the weights beside the scores
   static constexpr int kSCol = 0, kOCol = 256, kPCol = 384;  // columns: scores of A and B, sums of A and B, weights
   static constexpr int kRecord = 2 * kPfRows * (HD + 2);     // floats of a partial result: sums, then bounds, then denominators
-  // Registers that a thread of a softmax, the conversion and the last warpgroup keeps of the 128 that it is launched with: a row's
-  // 128 scores stay in registers, a converting thread has a step's codes in them.
-  static constexpr int kSoftmaxRegs = HD == 64 ? 200 : 184, kConvertRegs = HD == 64 ? 80 : 104, kIssueRegs = HD == 64 ? 32 : 40;
-  static_assert(2 * kSoftmaxRegs + kConvertRegs + kIssueRegs == 4 * 128, "more than the block has would never be granted");
+};
+
+// Registers that a thread of a softmax, the conversion and the last warpgroup keeps of the 128 that it is launched with: a row's 128
+// scores stay in registers, a converting thread has a step's codes in them. (Head size 128, 192 / 176 for the softmax: pieces of 60
+// to 1,500 tokens 84.9 / 87.8 us; where the tiles take turns and the conversion sets the pace, 24 sequences of 2 to 8 tokens, 70.2 / 58.5.)
+template <int HD, bool TURNS> struct PfRegs {
+  static constexpr int kSoftmax = HD == 64 ? 200 : TURNS ? 176 : 192, kConvert = HD == 64 ? 80 : TURNS ? 112 : 88,
+                       kIssue = HD == 64 ? 32 : TURNS ? 48 : 40;
+  static_assert(2 * kSoftmax + kConvert + kIssue == 4 * 128, "more than the block has would never be granted");
+  static_assert(kSoftmax >= 128 && kConvert <= 128 && kIssue <= 128, "inc may only raise, dec only lower");
 };
 
 struct PrefillArgs {
@@ -148,22 +155,37 @@ __device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, i
   }
   return q;
 }
-// Key tiles that a run has on average: a 148th of the step (first and last tile of tokens stand for all of a sequence).
-// `mine`: the lane's first sequence. All lanes of a warp call it.
-__device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
-  // every block works it out from the same numbers in the same order
-  float twice = (float)mine.tiles * (float)(mine.first + mine.last);
-  for (int s = (threadIdx.x & 31) + 32; s < a.n_seqs; s += 32) {
-    const PfSequence q = pf_sequence(a, s, tok);
-    twice += (float)q.tiles * (float)(q.first + q.last);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
-  return max(kPfLeast, (int)fminf(ceilf(twice * (float)a.n_kv * (0.5f / kPfSms)), 1e9f));
-}
 // Runs that each of a sequence's tiles of tokens is cut into: last / run, to the nearest. A sequence that is cut has last >= 1.5 run,
 // so that runs <= 4/3 last / run; and last <= 2 (first + last) / 2: all cut sequences together have at most 8/3 * 148 < kPfSlots runs.
 __device__ __forceinline__ int pf_runs(int last, int run) { return max(1, (last + run / 2) / run); }
+// Key tiles that a run has on average: a 148th of the step (first and last tile of tokens stand for all of a sequence), or more,
+// where there are fewer tiles than SMs but more runs: a run that no SM is left for costs a whole round. (24 sequences of 2 to 8
+// tokens behind 300 to 6,000, 96 tiles: 67 us in 170 runs, KPF_FEW us in 148.) `mine`: the lane's first sequence. All lanes of a
+// warp call it, and every block gets the same answer.
+__device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
+  const int lane = threadIdx.x & 31;
+  float twice = (float)mine.tiles * (float)(mine.first + mine.last);
+  int tiles = mine.tiles;
+  for (int s = lane + 32; s < a.n_seqs; s += 32) {
+    const PfSequence q = pf_sequence(a, s, tok);
+    twice += (float)q.tiles * (float)(q.first + q.last);
+    tiles += q.tiles;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
+  int run = max(kPfLeast, (int)fminf(ceilf(twice * (float)a.n_kv * (0.5f / kPfSms)), 1e9f));
+  if ((int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * a.n_kv > kPfSms) return run;
+  for (int i = 0; i < 16; ++i) {
+    unsigned runs = mine.tiles * pf_runs(mine.last, run);
+    for (int s = lane + 32; s < a.n_seqs; s += 32) {
+      const PfSequence q = pf_sequence(a, s, tok);
+      runs += q.tiles * pf_runs(q.last, run);
+    }
+    if ((int)__reduce_add_sync(0xffffffffu, runs) * a.n_kv <= kPfSms) break;
+    run += max(1, run / 8);
+  }
+  return run;
+}
 
 struct PfWork {
   int q_begin, q_len, start, page_row;           // the sequence's rows in the step, what it held, its slot
@@ -215,20 +237,23 @@ __device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int ind
 }
 
 struct PfShared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], x_full[4];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], x_full[kPfRing];
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], last[2];
   uint32_t tmem_base;
   int abort;
-  // Of the key tiles in flight, by step % 4: factors of scores, addends, factors of the denominator's terms, and the step (+ 1)
-  // that last had NaN among its values. x_full: all of them are there. (A step's place is written again four steps on, when
-  // the scores of the step two on are done, which both tiles' softmax has let begin behind its last look at this step.)
-  float k_scale[4][8], v_add[4][8], v_back[4][8];
-  int v_nan[4];
+  // Of the key tiles in flight, by step % 8: factors of scores, addends, factors of the denominator's terms, and the step (+ 1)
+  // that last had NaN among its values. x_full: all of them are there. (A step's place is written again eight steps on, when the
+  // scores of the step six on are done; and those were let begin behind the softmax's last look at this step.)
+  float k_scale[kPfRing][8], v_add[kPfRing][8], v_back[kPfRing][8];
+  int v_nan[kPfRing];
+  float handed[2][kPfRows];          // where B has A's rows: its bounds and denominators
   PfWork work;
 };
 
 // ------------------------------------------------------------------------------------------ the kernel
-template <int HD>
+// TURNS: every tile's tokens fit into one operand tile; B then has the same rows as A, and the two take the key tiles in turn: two
+// steps are under way at a time, and the results meet at the end.
+template <int HD, bool TURNS>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const PrefillArgs a) {
   using Cfg = PfCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -241,7 +266,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   pdl_wait();
   pdl_launch_dependents();
 
-  const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = 2 * tok_x;      // tokens of a tile, of a block
+  const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = TURNS ? tok_x : 2 * tok_x;      // tokens of a tile, of a block
   // one warp looks for the block's piece of work while others set it up
   if (warp == 0) {
     const PfWork found = pf_find<false>(a, tok, blockIdx.x);
@@ -258,7 +283,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       mbar_init(&sh.pv_done[s], 1);
       mbar_init(&sh.last[s], 1);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kPfRing; ++i) {
       mbar_init(&sh.x_full[i], 128);
       sh.v_nan[i] = 0;
     }
@@ -279,15 +304,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   // this run's key tiles: [c0, c1) of the tiles of the block's tokens
   const int c0 = lo_tile + tiles * w.part / w.parts, c1 = lo_tile + tiles * (w.part + 1) / w.parts;
   const int last_key = min(start + t0 + n_tok, a.max_pages * kFp8Page) - 1;
-  // steps of the two tiles: A's tokens come first and may not see the last key tiles
-  const int n_tok_a = min(n_tok, tok_x), n_tok_b = n_tok - n_tok_a;
-  const int n_a = max(0, min(c1, (start + t0 + n_tok_a - 1) / kPfKeys + 1) - c0), n_b = n_tok_b > 0 ? c1 - c0 : 0;
-  const int n_steps = max(n_a, n_b);
+  // Steps of the two tiles: A's tokens come first and may not see the last key tiles.
+  const int n_tok_a = min(n_tok, tok_x);
+  const int n_tok_b = TURNS ? n_tok_a : n_tok - n_tok_a;
+  const int n_steps = c1 - c0;
+  const int n_a = TURNS ? (n_steps + 1) / 2 : max(0, min(c1, (start + t0 + n_tok_a - 1) / kPfKeys + 1) - c0), n_b = TURNS ? n_steps / 2 : n_tok_b > 0 ? n_steps : 0;
 
   // What needs no barrier begins before the block meets: the rows' queries go to shared memory, the first codes are asked for.
   const bool softmax = warp < 8;
   const int x = warp >> 2 & 1, r = threadIdx.x & 127;        // tile and row of a softmax thread
-  const int first_tok = t0 + x * tok_x, n_tok_x = x ? n_tok_b : n_tok_a;
+  const int first_tok = t0 + (TURNS ? 0 : x * tok_x), n_tok_x = x ? n_tok_b : n_tok_a;
   const int rt = r / G, rh = r - rt * G;                     // token of the tile, query head of the group
   const bool there = softmax && rt < n_tok_x;
   const size_t row_off = ((size_t)(q_begin + first_tok + rt) * a.n_q + w.hk * G + rh) * HD;
@@ -370,7 +396,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 
   if (softmax) {
     // ------------------------------------------------------------------ softmax: a thread a row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kSoftmaxRegs));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kSoftmax));
     const int n_x = x ? n_b : n_a;
     const int qpos = start + first_tok + min(rt, max(n_tok_x - 1, 0));
     const int lo = first_visible_key(qpos, a.window);
@@ -386,15 +412,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
     bool ok = true;
     // the first and last keys that every row of the tile sees
     const int all_to = start + first_tok, all_from = first_visible_key(start + first_tok + max(n_tok_x - 1, 0), a.window);
-    for (int j = 0; j < n_x; ++j) {
+    for (int j = 0; j < n_x; ++j) {            // this tile's j-th step is the block's `step`
+      const int step = TURNS ? 2 * j + x : j;
       // every decision to give up is taken by the whole warp: reads of tensor memory are warp-wide instructions
-      if (!__all_sync(0xffffffffu, mbar_wait(&sh.x_full[j & 3], (j >> 2) & 1, abort) && mbar_wait(&sh.s_full[x], j & 1, abort))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh.x_full[step % kPfRing], (step / kPfRing) & 1, abort) && mbar_wait(&sh.s_full[x], j & 1, abort))) {
         LLMIE_FAIL(kStatusTimeoutMma);
         ok = false;
         break;
       }
       tc_fence_after_sync();
-      const int kbase = (c0 + j) * kPfKeys, ring = j & 3;
+      const int kbase = (c0 + step) * kPfKeys, ring = step % kPfRing;
       const bool edge = kbase + kPfKeys - 1 > all_to || kbase < all_from;
       const int nan_step = sh.v_nan[ring];
       // the row's scores; those that it does not see are -inf
@@ -486,7 +513,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(&sh.p_ready[x]);
-      if (nan_step == j + 1) {
+      if (nan_step == step + 1) {
         // rare: which columns of the values that this row sees are NaN
         for (int p = max(lo, kbase); p <= min(min(qpos, last_key), kbase + kPfKeys - 1); ++p) {
           const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD);
@@ -507,44 +534,95 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       }
       tc_fence_after_sync();
     }
-    // ---- the row's result: the output, or a partial one. Where a wait gave up: NaN.
-    float* rec = a.part + (size_t)w.slot * Cfg::kRecord;
-    const int pr = x * kPfRows + r;
-    if (w.parts > 1 && there) {
-      rec[2 * kPfRows * HD + pr] = R;
-      rec[2 * kPfRows * (HD + 1) + pr] = ok ? l : __int_as_float(0x7fffffff);
-    }
-    const float inv = 1.f / l;
+    if (TURNS) {
+      // B hands its results to A through the place of the keys, which nobody reads any more once both tiles' products are done
+      float* handed = reinterpret_cast<float*>(k_smem) + r * HD;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (x == 1) {
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c) {
-      uint32_t y[32];
-      if (ok && n_x > 0) {
-        tmem_ld_32x32(o_addr + c * 32, y);
-        tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = 0u;
-      }
-      if (there) {                   // (reads of tensor memory are warp-wide: only what follows them goes by the row)
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          float v8[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            v8[e] = (nan_cols[c] >> (i + e) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + e]);
-          if (w.parts > 1) {
-            store8(rec + (size_t)pr * HD + c * 32 + i, v8);
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t y[32];
+          if (ok && n_x > 0) {
+            tmem_ld_32x32(o_addr + c * 32, y);
+            tmem_ld_wait();
           } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v8[e] *= inv;
-            store8(a.out + row_off + c * 32 + i, v8);
+            for (int i = 0; i < 32; ++i) y[i] = 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {          // places of a row shifted by the row: other banks for other rows
+            float4 z;
+            z.x = (nan_cols[c] >> i & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i]);
+            z.y = (nan_cols[c] >> (i + 1) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + 1]);
+            z.z = (nan_cols[c] >> (i + 2) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + 2]);
+            z.w = (nan_cols[c] >> (i + 3) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + 3]);
+            *reinterpret_cast<float4*>(handed + (c * 32 + i + r * 4) % HD) = z;
+          }
+        }
+        sh.handed[0][r] = R;
+        sh.handed[1][r] = l;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    // ---- the row's result: the output, or a partial one. Where a wait gave up: NaN.
+    if (!TURNS || x == 0) {
+      float mine_f = 1.f, b_f = 0.f;
+      if (TURNS) {
+        const float Rb = sh.handed[0][r], M = fmaxf(R, Rb), Mu = M == -INFINITY ? 0.f : M;
+        mine_f = R == -INFINITY ? 0.f : pf_exp2(R - Mu);
+        b_f = Rb == -INFINITY ? 0.f : pf_exp2(Rb - Mu);
+        l = fmaf(l, mine_f, sh.handed[1][r] * b_f);
+        R = M;
+      }
+      const float* handed = reinterpret_cast<const float*>(k_smem) + r * HD;
+      float* rec = a.part + (size_t)w.slot * Cfg::kRecord;
+      const int pr = x * kPfRows + r;
+      if (w.parts > 1 && there) {
+        rec[2 * kPfRows * HD + pr] = R;
+        rec[2 * kPfRows * (HD + 1) + pr] = ok ? l : __int_as_float(0x7fffffff);
+      }
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t y[32];
+        if (ok && n_x > 0) {
+          tmem_ld_32x32(o_addr + c * 32, y);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = 0u;
+        }
+        if (there) {                   // (reads of tensor memory are warp-wide: only what follows them goes by the row)
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float v8[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              v8[e] = (nan_cols[c] >> (i + e) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + e]);
+            if (TURNS) {
+#pragma unroll
+              for (int e = 0; e < 8; e += 4) {
+                const float4 z = *reinterpret_cast<const float4*>(handed + (c * 32 + i + e + r * 4) % HD);
+                v8[e] = fmaf(v8[e], mine_f, z.x * b_f);
+                v8[e + 1] = fmaf(v8[e + 1], mine_f, z.y * b_f);
+                v8[e + 2] = fmaf(v8[e + 2], mine_f, z.z * b_f);
+                v8[e + 3] = fmaf(v8[e + 3], mine_f, z.w * b_f);
+              }
+            }
+            if (w.parts > 1) {
+              store8(rec + (size_t)pr * HD + c * 32 + i, v8);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v8[e] *= inv;
+              store8(a.out + row_off + c * 32 + i, v8);
+            }
           }
         }
       }
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------------ conversion: 128 threads, 16 codes at a time
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kConvertRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kConvert));
     auto put = [&](uint8_t* dst, const uint4 (&reg)[kPer]) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -564,7 +642,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       }
     };
     for (int j = 0; j < n_steps; ++j) {
-      const int st = j & 1, ring = j & 3;
+      const int st = j & 1, ring = j % kPfRing;
       const int next0 = page_at((c0 + j + 2) * 2), next1 = page_at((c0 + j + 2) * 2 + 1);
       if (j >= 2 && !mbar_wait(&sh.k_empty[st], ((j >> 1) - 1) & 1, abort)) {
         LLMIE_FAIL(kStatusTimeoutEmpty);
@@ -615,7 +693,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
     }
   } else {
     // ------------------------------------------------------------------ the tensor core: a thread a tile, so that neither waits for the other's
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kIssueRegs));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kIssue));
     if (warp < 14 && elect_one()) {
       constexpr uint32_t idesc_s = pf_instr_desc(kPfRows, kPfKeys, 0), idesc_o = pf_instr_desc(kPfRows, HD, 1);
       const int tx = warp - 12, n_x = tx ? n_b : n_a;
@@ -629,29 +707,36 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         LLMIE_FAIL(code);
         return false;
       };
-      auto scores = [&](int j) -> bool {                     // S = Q K^T of step j
-        if (!wait_for(&sh.k_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull)) return false;
+      // a stage is free when both tiles have let go of it; where they take steps in turn, the one that has it lets go twice
+      auto let_go = [&](uint64_t* bar) {
+        mma_commit(bar);
+        if (TURNS) mma_commit(bar);
+      };
+      auto scores = [&](int j) -> bool {                     // S = Q K^T of this tile's j-th step
+        const int step = TURNS ? 2 * j + tx : j;
+        if (!wait_for(&sh.k_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull)) return false;
         tc_fence_after_sync();
-        const uint64_t kd = k_desc + (uint64_t)((j & 1) * (Cfg::kKvBytes >> 4));
+        const uint64_t kd = k_desc + (uint64_t)((step & 1) * (Cfg::kKvBytes >> 4));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const int off = ((kk >> 2) * kPfSub + (kk & 3) * 32) >> 4;
           mma_bf16_ss(s_col, q_desc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
         }
         mma_commit(&sh.s_full[tx]);
-        mma_commit(&sh.k_empty[j & 1]);
+        let_go(&sh.k_empty[step & 1]);
         return true;
       };
-      auto sums = [&](int j) -> bool {                       // O (+)= W V of step j
-        if (!wait_for(&sh.v_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull)) return false;
+      auto sums = [&](int j) -> bool {                       // O (+)= W V of it
+        const int step = TURNS ? 2 * j + tx : j;
+        if (!wait_for(&sh.v_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull)) return false;
         if (!wait_for(&sh.p_ready[tx], j & 1, kStatusTimeoutMma)) return false;
         tc_fence_after_sync();
-        const uint64_t vd = v_desc + (uint64_t)((j & 1) * (Cfg::kKvBytes >> 4));
+        const uint64_t vd = v_desc + (uint64_t)((step & 1) * (Cfg::kKvBytes >> 4));
 #pragma unroll
         for (int kk = 0; kk < kPfKeys / 16; ++kk)            // 16 weights are 8 columns; 16 keys are 16 rows of the values
           pf_mma_ts(o_col, p_col + kk * 8, vd + kk * (2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
         mma_commit(&sh.pv_done[tx]);
-        mma_commit(&sh.v_empty[j & 1]);
+        let_go(&sh.v_empty[step & 1]);
         return true;
       };
       bool ok = n_x == 0 || scores(0);
@@ -663,7 +748,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         if (!Cfg::kOwnP && ok && j + 1 < n_x) ok = wait_for(&sh.pv_done[tx], j & 1, kStatusTimeoutMma) && scores(j + 1);
       }
       // steps that are the other tile's alone
-      for (int j = n_x; ok && j < n_steps; ++j) {
+      for (int j = n_x; ok && !TURNS && j < n_steps; ++j) {
         ok = wait_for(&sh.k_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull);
         if (ok) mbar_arrive(&sh.k_empty[j & 1]);
         ok = ok && wait_for(&sh.v_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull);
@@ -685,11 +770,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 
 // Joins the runs of the tiles that were cut. grid (tiles of tokens x key/value heads, 8): an eighth of a tile's rows a block, a warp a row.
 constexpr int kPfJoinWarps = 8, kPfJoinSide = 8;
-template <int HD> __global__ void __launch_bounds__(kPfJoinWarps * 32) prefill_fp8_join_kernel(const PrefillArgs a) {
+template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 32) prefill_fp8_join_kernel(const PrefillArgs a) {
   pdl_launch_dependents();
   using Cfg = PfCfg<HD>;
   const int lane = threadIdx.x & 31;
-  const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = 2 * tok_x;
+  const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = TURNS ? tok_x : 2 * tok_x;
   const PfWork w = pf_find<true>(a, tok, blockIdx.x);
   if (w.parts <= 1) return;
   // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait).
@@ -746,12 +831,12 @@ template <int HD> __global__ void __launch_bounds__(kPfJoinWarps * 32) prefill_f
   }
 }
 
-template <int HD>
+template <int HD, bool TURNS>
 static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, int max_q_len, cudaStream_t stream) {
   using Cfg = PfCfg<HD>;
-  cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<HD, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return (int)e;
-  const int tok = 2 * (kPfRows / (a.n_q / a.n_kv));
+  const int tok = (TURNS ? 1 : 2) * (kPfRows / (a.n_q / a.n_kv));
   // Pieces of work: the tiles of tokens, and the runs that they may be cut into. The most runs that a tile can have follow from
   // the most keys that the table has room for and the least work that so many tokens are.
   const long long items = max_q_len <= tok ? (long long)a.n_seqs * a.n_kv : ((long long)n_tokens / tok + a.n_seqs) * a.n_kv;
@@ -771,10 +856,10 @@ static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, int max_q_len,
   // (a sequence of one tile: parts - 1 <= last / run, and all of them have 148 runs of keys between them)
   const long long blocks = cut ? min(items * parts, items + (max_q_len <= tok ? kPfSms : kPfSlots)) : items;
   if (blocks * most_tiles > 0x3fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
-  launch_k(prefill_fp8_kernel<HD>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
+  launch_k(prefill_fp8_kernel<HD, TURNS>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
   LLMIE_LAUNCH_CHECK();
   if (cut) {
-    launch_k(prefill_fp8_join_kernel<HD>, dim3((unsigned)items, kPfJoinSide), dim3(kPfJoinWarps * 32), 0, stream, a);
+    launch_k(prefill_fp8_join_kernel<HD, TURNS>, dim3((unsigned)items, kPfJoinSide), dim3(kPfJoinWarps * 32), 0, stream, a);
     LLMIE_LAUNCH_CHECK();
   }
   return LLMIE_OK;
@@ -806,5 +891,9 @@ extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, c
   const PrefillArgs a{(const __nv_bfloat16*)q, (const unsigned char*)k_cache, (const unsigned char*)v_cache, (const signed char*)k_exp,
                       (const signed char*)v_exp, (__nv_bfloat16*)out, scratch, status, cu_q, seq_slot, seq_start, block_table,
                       max_pages, n_seqs, n_q, n_kv, scale * 1.4426950408889634f, window};
-  return hd == 64 ? launch_prefill_fp8<64>(a, n_tokens, max_q_len, stream) : launch_prefill_fp8<128>(a, n_tokens, max_q_len, stream);
+  const bool turns = max_q_len <= kPfRows / (n_q / n_kv);
+#define LLMIE_PREFILL(HD) return turns ? launch_prefill_fp8<HD, true>(a, n_tokens, max_q_len, stream) : launch_prefill_fp8<HD, false>(a, n_tokens, max_q_len, stream)
+  if (hd == 64) LLMIE_PREFILL(64);
+  LLMIE_PREFILL(128);
+#undef LLMIE_PREFILL
 }
