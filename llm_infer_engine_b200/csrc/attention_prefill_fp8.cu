@@ -38,7 +38,8 @@ constexpr int kPfSms = 148;
 constexpr int kPfRing = 8;
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
 constexpr int kPfLeast = 4;          // key tiles that a run has at least, on average
-constexpr int kPfSlots = 400;        // partial results at once (see pf_runs)
+constexpr int kPfSlots = 200;        // partial results at once (see pf_run)
+constexpr int kPfFew = 128;          // tiles of tokens that can always be cut into runs for which there are SMs (see pf_run)
 constexpr float kPfTop = 7.f;        // the bound's own weight is 2^7
 constexpr float kPfSlack = 8.f;      // how far scores may outgrow the bound, in units of log2
 
@@ -79,6 +80,7 @@ struct PrefillArgs {
   int max_pages, n_seqs, n_q, n_kv;
   float scale2;
   int window;
+  int run;                           // no run is shorter: what the host counted blocks and scratch by
 };
 
 __device__ __forceinline__ float pf_exp2(float x) {
@@ -89,20 +91,6 @@ __device__ __forceinline__ float pf_exp2(float x) {
 __device__ __forceinline__ uint32_t pf_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint64_t pf_pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-// (y0, y1) = (x0, x1) * b + c, one rounding each
-__device__ __forceinline__ void pf_fma2(float& y0, float& y1, float x0, float x1, uint64_t b, uint64_t c) {
-  uint64_t y;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(pf_pair(x0, x1)), "l"(b), "l"(c));
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(y0), "=f"(y1) : "l"(y));
-}
-__device__ __forceinline__ void pf_add2(uint64_t& acc, float x0, float x1) {
-  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(pf_pair(x0, x1)));
 }
 __device__ __forceinline__ float pf_max3(float a, float b, float c) {
   float y;
@@ -130,10 +118,10 @@ __host__ __device__ constexpr uint32_t pf_instr_desc(int m, int n, int b_mn) {
 }
 
 // ------------------------------------------------------------------------------------------ the cut of the work
-// Key tiles of a sequence's tile of tokens [t0, t0 + n): from `lo` on, `count` of them.
-__device__ __forceinline__ void pf_tiles(int start, int t0, int n, int window, int& lo, int& count) {
-  lo = first_visible_key(start + t0, window) / kPfKeys;
-  count = (start + t0 + n - 1) / kPfKeys - lo + 1;
+// Key tiles of a sequence's tile of tokens [t0, t0 + n): from `lo` on, `count` of them. None behind the table's last page.
+__device__ __forceinline__ void pf_tiles(const PrefillArgs& a, int start, int t0, int n, int& lo, int& count) {
+  lo = first_visible_key(start + t0, a.window) / kPfKeys;
+  count = max((min(start + t0 + n, a.max_pages * kFp8Page) - 1) / kPfKeys - lo + 1, 0);
 }
 // What a lane knows of its sequence: tiles of tokens, the key tiles of the first and the last of them.
 struct PfSequence {
@@ -149,19 +137,22 @@ __device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, i
     q.tiles = (q.q_len + tok - 1) / tok;
     if (q.tiles > 0) {
       int lo;
-      pf_tiles(q.start, 0, min(tok, q.q_len), a.window, lo, q.first);
-      pf_tiles(q.start, (q.tiles - 1) * tok, q.q_len - (q.tiles - 1) * tok, a.window, lo, q.last);
+      pf_tiles(a, q.start, 0, min(tok, q.q_len), lo, q.first);
+      pf_tiles(a, q.start, (q.tiles - 1) * tok, q.q_len - (q.tiles - 1) * tok, lo, q.last);
     }
   }
   return q;
 }
-// Runs that each of a sequence's tiles of tokens is cut into: last / run, to the nearest. A sequence that is cut has last >= 1.5 run,
-// so that runs <= 4/3 last / run; and last <= 2 (first + last) / 2: all cut sequences together have at most 8/3 * 148 < kPfSlots runs.
+// Runs that each of a sequence's tiles of tokens is cut into: last / run, to the nearest.
 __device__ __forceinline__ int pf_runs(int last, int run) { return max(1, (last + run / 2) / run); }
-// Key tiles that a run has on average: a 148th of the step (first and last tile of tokens stand for all of a sequence), or more,
-// where there are fewer tiles than SMs but more runs: a run that no SM is left for costs a whole round. (24 sequences of 2 to 8
-// tokens behind 300 to 6,000, 96 tiles: 67 us in 170 runs, KPF_FEW us in 148.) `mine`: the lane's first sequence. All lanes of a
-// warp call it, and every block gets the same answer.
+// Key tiles that a run has on average. With T the sum of (first + last) / 2 over all tiles of tokens and heads:
+// Where those are no more than the SMs: the least, from T / 148 on, with which every run finds an SM at once, since one that does
+// not costs a whole round (24 sequences of 2 to 8 tokens behind 300 to 6,000, 96 tiles: 67 us in 170 runs, 58 in 148). Where they
+// are more, or no such length is found: 2 T / 148, so that a sequence is cut only if one of its tiles alone would hold up the step.
+// How many runs come of it: a sequence that is cut has last >= 1.5 run, so at most 4/3 last / run runs, and at most last / run of
+// them more than tiles; and last <= first + last, whose sum is 2 T. With run >= 2 T / 148 all cut sequences have 4/3 148 < kPfSlots
+// runs, and 148 more than tiles. The search goes on to 16 T / 148, where there are 18 more than tiles: up to kPfFew it finds one.
+// `mine`: the lane's first sequence. All lanes of a warp call it, and every block gets the same answer.
 __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
   const int lane = threadIdx.x & 31;
   float twice = (float)mine.tiles * (float)(mine.first + mine.last);
@@ -173,18 +164,19 @@ __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSeq
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
-  int run = max(kPfLeast, (int)fminf(ceilf(twice * (float)a.n_kv * (0.5f / kPfSms)), 1e9f));
-  if ((int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * a.n_kv > kPfSms) return run;
-  for (int i = 0; i < 16; ++i) {
+  const float share = twice * (float)a.n_kv / kPfSms;                        // 2 T / 148
+  const int most = max(a.run, max(kPfLeast, (int)fminf(ceilf(share), 1e9f)));
+  if ((int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * a.n_kv > kPfSms) return most;
+  int run = max(a.run, max(kPfLeast, (int)fminf(ceilf(share * 0.5f), 1e9f)));
+  for (int i = 0; i < 24; ++i, run += (run + 7) / 8) {                       // (9/8)^24 > 16
     unsigned runs = mine.tiles * pf_runs(mine.last, run);
     for (int s = lane + 32; s < a.n_seqs; s += 32) {
       const PfSequence q = pf_sequence(a, s, tok);
       runs += q.tiles * pf_runs(q.last, run);
     }
-    if ((int)__reduce_add_sync(0xffffffffu, runs) * a.n_kv <= kPfSms) break;
-    run += max(1, run / 8);
+    if ((int)__reduce_add_sync(0xffffffffu, runs) * a.n_kv <= kPfSms) return run;
   }
-  return run;
+  return most;
 }
 
 struct PfWork {
@@ -300,7 +292,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   const int q_begin = w.q_begin, q_len = w.q_len, start = w.start;
   const int t0 = w.tile * tok, n_tok = min(tok, q_len - t0);
   int lo_tile, tiles;
-  pf_tiles(start, t0, n_tok, a.window, lo_tile, tiles);
+  pf_tiles(a, start, t0, n_tok, lo_tile, tiles);
   // this run's key tiles: [c0, c1) of the tiles of the block's tokens
   const int c0 = lo_tile + tiles * w.part / w.parts, c1 = lo_tile + tiles * (w.part + 1) / w.parts;
   const int last_key = min(start + t0 + n_tok, a.max_pages * kFp8Page) - 1;
@@ -832,13 +824,13 @@ template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 3
 }
 
 template <int HD, bool TURNS>
-static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, int max_q_len, cudaStream_t stream) {
+static int launch_prefill_fp8(PrefillArgs a, int n_tokens, int max_q_len, cudaStream_t stream) {
   using Cfg = PfCfg<HD>;
   cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<HD, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return (int)e;
   const int tok = (TURNS ? 1 : 2) * (kPfRows / (a.n_q / a.n_kv));
-  // Pieces of work: the tiles of tokens, and the runs that they may be cut into. The most runs that a tile can have follow from
-  // the most keys that the table has room for and the least work that so many tokens are.
+  // Pieces of work: the tiles of tokens, and the runs that they may be cut into (see pf_run). The most runs that a tile can have
+  // follow from the most keys that the table has room for and the least work that so many tokens are.
   const long long items = max_q_len <= tok ? (long long)a.n_seqs * a.n_kv : ((long long)n_tokens / tok + a.n_seqs) * a.n_kv;
   double least = (double)n_tokens / tok * a.n_kv;
   long long most_tiles = ((long long)a.max_pages * kFp8Page + kPfKeys - 1) / kPfKeys;
@@ -848,13 +840,13 @@ static int launch_prefill_fp8(const PrefillArgs& a, int n_tokens, int max_q_len,
     const long long w = a.window < 0 ? -(long long)a.window : a.window;
     most_tiles = min(most_tiles, (w + tok) / kPfKeys + 2);
   }
-  long long run = (long long)(least / kPfSms);
-  if (run < kPfLeast) run = kPfLeast;
-  const long long parts = (most_tiles + run / 2) / run;
-  const bool cut = parts > 1;
+  // (tokens that do not fill their tiles may leave fewer tiles than SMs after all, where runs may be half as long)
+  long long run = (long long)(least * ((double)n_tokens / tok * a.n_kv > kPfSms ? 2 : 1) / kPfSms);
+  run = min(max(run, (long long)kPfLeast), 1LL << 30);
+  const bool cut = (most_tiles + run / 2) / run > 1;
   if (cut && !a.part) return kPfNeedsScratch;
-  // (a sequence of one tile: parts - 1 <= last / run, and all of them have 148 runs of keys between them)
-  const long long blocks = cut ? min(items * parts, items + (max_q_len <= tok ? kPfSms : kPfSlots)) : items;
+  a.run = (int)run;
+  const long long blocks = !cut ? items : items <= kPfFew ? kPfSms : items + kPfSms;
   if (blocks * most_tiles > 0x3fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
   launch_k(prefill_fp8_kernel<HD, TURNS>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
   LLMIE_LAUNCH_CHECK();
@@ -890,7 +882,7 @@ extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, c
   if (n_tokens == 0 || n_seqs == 0 || max_q_len <= 0) return LLMIE_OK;
   const PrefillArgs a{(const __nv_bfloat16*)q, (const unsigned char*)k_cache, (const unsigned char*)v_cache, (const signed char*)k_exp,
                       (const signed char*)v_exp, (__nv_bfloat16*)out, scratch, status, cu_q, seq_slot, seq_start, block_table,
-                      max_pages, n_seqs, n_q, n_kv, scale * 1.4426950408889634f, window};
+                      max_pages, n_seqs, n_q, n_kv, scale * 1.4426950408889634f, window, 0};
   const bool turns = max_q_len <= kPfRows / (n_q / n_kv);
 #define LLMIE_PREFILL(HD) return turns ? launch_prefill_fp8<HD, true>(a, n_tokens, max_q_len, stream) : launch_prefill_fp8<HD, false>(a, n_tokens, max_q_len, stream)
   if (hd == 64) LLMIE_PREFILL(64);

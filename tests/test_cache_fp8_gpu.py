@@ -463,6 +463,59 @@ def test_prompt_numbers_that_are_not_finite_stay_with_the_rows_that_see_them(hd)
         assert torch.equal(bad, want), window
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_kv,n_short,longs", [(1, 147, [2000]), (1, 130, [2000, 1900]), (1, 128, [2500]), (2, 90, [2000]),
+                                                (1, 20, [2500, 600, 1300]), (4, 30, [2000, 1000, 900])])
+def test_prompt_cut_beside_short_ones(hd, n_kv, n_short, longs):
+    """Some sequences are cut into runs and others are not, with fewer tiles of tokens than SMs, as many, and more."""
+    n_q = 4 * n_kv
+    starts, news = [0] * n_short + longs, [1 + i % 3 for i in range(n_short)] + [5] * len(longs)
+    order = torch.randperm(len(news), generator=torch.Generator().manual_seed(7)).tolist()
+    starts, news = [starts[i] for i in order], [news[i] for i in order]
+    pc = filled([s + m for s, m in zip(starts, news)], n_kv, hd, seed=n_short)
+    q = torch.randn(sum(news), n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = prompt(pc, q, starts, news, n_q, n_kv, hd, hd ** -0.5, 0)
+    check_prompt(pc, out, q, starts, news, n_q, n_kv, hd, hd ** -0.5, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_of_few_tokens_in_a_large_step(hd):
+    """More rows than the sequences have: those behind the last one stay as they were, and how the others' work is cut, which is
+    found by the lengths that are there, has room for its runs whatever the rows made the caller count on."""
+    n_q, n_kv, starts, news = 8, 2, [2500, 0, 700], [3, 40, 200]
+    pc = filled([s + m for s, m in zip(starts, news)], n_kv, hd, seed=5)
+    rows = 40000
+    q = torch.randn(rows, n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    cu = i32([0, 3, 43, 243])
+    for most in (200, 4000):
+        out = torch.full((rows, n_q * hd), 3.0, dtype=BF, device=DEV)
+        ops().attention_prefill_fp8(q.to(DEV), *pc.dev(), out, cu, i32(pc.slots), i32(starts), pc.table.to(DEV), 3, most, n_q, n_kv, hd,
+                                    hd ** -0.5, 0)
+        ops().check_tc_status(DEV)
+        assert bool((out[243:] == 3.0).all())
+        check_prompt(pc, out[:243].cpu().double(), q, starts, news, n_q, n_kv, hd, hd ** -0.5, 0, rows=[0, 1, 2, 39, 63, 64, 128])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_nan_in_one_run_of_several(hd):
+    """A value that is not finite reaches its column of the rows that see it, through the join; a key its rows."""
+    n_q, n_kv, start, new = 4, 1, 2500, 6
+    pc = filled([start + new, start + new], n_kv, hd, seed=9)
+    v = torch.randn(1, n_kv, hd, generator=torch.Generator().manual_seed(2))
+    v[0, 0, 5] = math.inf
+    pc.append(0, 300, torch.zeros(1, n_kv, hd), v)
+    v[0, 0, 5], v[0, 0, hd - 1] = 1.0, math.nan
+    pc.append(0, start + 3, torch.zeros(1, n_kv, hd), v)
+    pc.append(1, start + 2, torch.full((1, n_kv, hd), math.nan), torch.ones(1, n_kv, hd))
+    q = torch.randn(2 * new, n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    bad = torch.isnan(prompt(pc, q, [start, start], [new, new], n_q, n_kv, hd, hd ** -0.5, 0)).view(2, new, n_q, hd)
+    want = torch.zeros(2, new, n_q, hd, dtype=torch.bool)
+    want[0, :, :, 5] = True
+    want[0, 3:, :, hd - 1] = True
+    want[1, 2:] = True
+    assert torch.equal(bad, want)
+
+
 # ------------------------------------------------------------------------------------------ one-token steps in one kernel
 @pytest.mark.parametrize("window", [0, 40, -64])
 @pytest.mark.parametrize("n_q,n_kv,hd", [(4, 4, 64), (12, 4, 64), (32, 8, 128), (7, 1, 128), (16, 1, 64), (32, 2, 128)])
