@@ -254,7 +254,8 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   const size_t q_pitch = (size_t)(ROPE ? a.n_q + 2 * a.n_kv : a.n_q) * HD;
-  if (ROPE && u_end == count && u_begin < count && (count - 1 - u_begin) % kDfWarps == warp)
+  // (a sequence that is longer than its table: there is no place for the position)
+  if (ROPE && u_end == count && u_begin < count && (count - 1 - u_begin) % kDfWarps == warp && a.seq_kvlen[seq] == len)
     df_append<HD>(q + seq * q_pitch, a, st, hk, len, pages[(first + count - 1) >> 1]);            // this warp reads that block itself
   int pg_next;                       // page of the next unit to be asked for
   {
@@ -689,7 +690,6 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
     ahead += s < seq ? c : 0;
   }
   df_units(a, a.seq_kvlen[seq], first, count);
-  if (count == 0) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     all += __shfl_xor_sync(0xffffffffu, all, o);
@@ -697,10 +697,11 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
   }
   const int share = df_share(all * per_seq, blocks);
   const int begin = ahead * per_seq + item * count;
-  const int c0 = begin / share, n = (begin + count - 1) / share - c0 + 1;
-  if (n == 1) return;
-  // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait).
+  const int c0 = begin / share, n = count == 0 ? 0 : (begin + count - 1) / share - c0 + 1;
+  // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait). Blocks with
+  // nothing to join wait too: the kernel behind this one waits for this one alone, and reads what the one in front wrote.
   pdl_wait();
+  if (n <= 1) return;
   // partial result i: the first lies where a piece begins with its item, the others where one goes on
   const float* base = a.part + (size_t)c0 * 2 * Cfg::kRecord;
   auto record = [&](int i) { return base + (size_t)(i == 0 ? 1 : 2 * i) * Cfg::kRecord; };

@@ -27,7 +27,7 @@ attention_paged_fp8_kernel(const T* q, const unsigned char* k_cache, const unsig
   const long long item = (long long)blockIdx.x * kPlainWarps + warp;
   if (item >= n_items) return;       // whole warps: no barrier of the block below
   const int t = (int)(item / n_q), h = (int)(item % n_q), hk = h / (n_q / n_kv);
-  const int pos = tok_pos[t];
+  const int pos = min(tok_pos[t], max_pages * kFp8Page - 1);           // what the table has room for
   const int* pages = block_table + (size_t)seq_slot[tok_seq[t]] * max_pages;
   const int lo = first_visible_key(pos, window);
   float* qs = q_smem[warp];

@@ -768,9 +768,10 @@ template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 3
   const int lane = threadIdx.x & 31;
   const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = TURNS ? tok_x : 2 * tok_x;
   const PfWork w = pf_find<true>(a, tok, blockIdx.x);
-  if (w.parts <= 1) return;
-  // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait).
+  // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait). Blocks with
+  // nothing to join wait too: the kernel behind this one waits for this one alone, and reads what the one in front wrote.
   pdl_wait();
+  if (w.parts <= 1) return;
   const float* base = a.part + (size_t)w.slot * Cfg::kRecord;
   for (int row = blockIdx.y * kPfJoinWarps + (threadIdx.x >> 5); row < 2 * kPfRows; row += kPfJoinSide * kPfJoinWarps) {
     const int x = row / kPfRows, rt = row % kPfRows / G, rh = row % kPfRows - rt * G, t = w.tile * tok + x * tok_x + rt;

@@ -106,6 +106,8 @@ class Engine:
             raise EngineError(f"decode_attention must be 'auto' or 'split', got {decode_attention!r}")
         self.decode_attention = decode_attention
         self.cache_dtype = resolve_cache_dtype(cache_dtype, self.dtype)
+        if decode_attention == "split" and self.cache_dtype != self.dtype:
+            raise EngineError("decode_attention 'split' reads a cache in the engine's own dtype only")
         if nvtx:
             trace.enable_ranges(True)
         self.model, self.config = build_model(model_dir, self.dtype, self.device,

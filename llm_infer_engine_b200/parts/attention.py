@@ -59,7 +59,7 @@ class GroupedQueryAttention(Mixer):
         return self.qkv.nbytes() + self.o.nbytes()
 
     def cache_requests(self):
-        return [KVRequest(self.n_kv_heads, self.head_dim, self.window, eight_bit=True)]
+        return [KVRequest(self.n_kv_heads, self.head_dim, self.window, eight_bit=self.position.eight_bit)]
 
     def forward(self, x, ctx, unit, owns_cache, residual=None):
         kv = unit.kv

@@ -258,6 +258,10 @@ class DeferredBranchAdd:
 
 
 class PositionEncoding(Part):
+    """`eight_bit`: whether encode_and_store can write a cache in 8 bits (codes and exponents, see `KVUnit`)."""
+
+    eight_bit = False
+
     def encode_and_store(self, qkv: torch.Tensor, ctx, kv, n_q: int, n_kv: int, head_dim: int,
                          write_kv: bool) -> torch.Tensor:
         """Takes the packed projections [T, (n_q + 2 n_kv) head_dim], returns position-encoded

@@ -72,6 +72,8 @@ class RotaryEncoding(PositionEncoding):
     (None or {"rope_type": "llama3", factor, low_freq_factor, high_freq_factor,
     original_max_position_embeddings}), exact_angles (bool: the table from double-precision angles, without scaling)."""
 
+    eight_bit = True
+
     def __init__(self, params, runtime):
         super().__init__(params, runtime)
         self.rot_dim = int(params["rot_dim"])
@@ -112,6 +114,8 @@ class RotaryEncoding(PositionEncoding):
 
 class NoEncoding(PositionEncoding):
     """Positions enter nowhere: keys and values are stored as projected."""
+
+    eight_bit = True
 
     def encode_and_store(self, qkv, ctx, kv, n_q, n_kv, head_dim, write_kv):
         q = torch.empty((qkv.shape[0], n_q * head_dim), dtype=qkv.dtype, device=qkv.device)

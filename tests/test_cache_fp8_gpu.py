@@ -558,3 +558,313 @@ def test_step(n_q, n_kv, hd, window):
         err = (outs[0][i].cpu().double().view(1, n_q, hd) - want).abs()
         assert bool((err <= allowed(want, size, BF, True)).all()), (l, float((err / allowed(want, size, BF, True)).max()))
         row += 1
+
+
+# ------------------------------------------------------------------------------------------ calls at the edges
+class FarPages:
+    """A plain cache's pages at the end of a device cache of `pages` pages, whose other pages nobody looks at."""
+
+    def __init__(self, pc, pages):
+        self.pc, self.first = pc, pages - pc.n_pages
+        shape = (pages, pc.n_kv, 64, pc.hd)
+        self.cache = [torch.empty(shape, dtype=F8, device=DEV), torch.empty(shape, dtype=F8, device=DEV),
+                      torch.empty(shape[:2] + (4,), dtype=torch.int8, device=DEV), torch.empty(shape[:2] + (4,), dtype=torch.int8, device=DEV)]
+        for far, near in zip(self.cache, pc.dev()):
+            far.view(torch.uint8)[self.first:] = near.view(torch.uint8)
+        self.table = (pc.table + self.first).to(DEV)
+
+    def back(self):
+        return [t[self.first:] for t in self.cache]
+
+
+def test_pages_behind_the_first_four_billion_codes():
+    """Offsets of codes pass 32 bits: every call on pages at the end of caches of 4.6 GB each."""
+    n_q, n_kv, hd = 16, 8, 128
+    lens, new = [130, 77], [33, 9]
+    pc = PlainCache(lens, n_kv, hd, seed=11)
+    g = torch.Generator().manual_seed(12)
+    starts = [l - m for l, m in zip(lens, new)]
+    for i, st in enumerate(starts):
+        pc.append(i, 0, torch.randn(st, n_kv, hd, generator=g), torch.randn(st, n_kv, hd, generator=g))
+    far = FarPages(pc, 70000)
+    assert far.first * n_kv * 64 * hd > 2 ** 32
+    qkv = torch.randn(sum(new), (n_q + 2 * n_kv) * hd, generator=g).to(BF)
+    table = angles(256, hd)
+    q = torch.empty(sum(new), n_q * hd, dtype=BF, device=DEV)
+    cu = i32([0, new[0], sum(new)])
+    ops().rope_store_fp8(qkv.to(DEV), q, *far.cache, table.to(DEV), cu, i32(pc.slots), i32(starts), far.table, 2, max(new), n_q, n_kv,
+                         hd, hd)
+    assert torch.equal(q.cpu(), plain_store(pc, qkv, table, starts, new, n_q, n_kv, hd, hd))
+    check_cache(pc, far.back())
+    out = torch.empty_like(q)
+    ops().attention_prefill_fp8(q, *far.cache, out, cu, i32(pc.slots), i32(starts), far.table, 2, max(new), n_q, n_kv, hd, hd ** -0.5)
+    check_prompt(pc, out.cpu().double(), q.cpu(), starts, new, n_q, n_kv, hd, hd ** -0.5, 0)
+    plain = torch.empty_like(q)
+    pos = [st + j for st, m in zip(starts, new) for j in range(m)]
+    ops().attention_paged_fp8(q, *far.cache, plain, i32(pos), i32([0] * new[0] + [1] * new[1]), i32(pc.slots), far.table, n_q, n_kv, hd,
+                              hd ** -0.5)
+    check_prompt(pc, plain.cpu().double(), q.cpu(), starts, new, n_q, n_kv, hd, hd ** -0.5, 0)
+    last = q[[new[0] - 1, sum(new) - 1]].contiguous()
+    for max_len in (130, 0):
+        got = torch.empty_like(last)
+        ops().attention_decode_fp8(last, *far.cache, got, i32(pc.slots), i32(lens), far.table, n_q, n_kv, hd, hd ** -0.5, 0, max_len)
+        row = 0
+        for i, l in enumerate(lens):
+            want, size = fp8_cache.attention(last[i:i + 1].cpu().double().view(1, n_q, hd), *pc.held(i, l), [l - 1], hd ** -0.5, 0)
+            assert bool(((got[i].cpu().double().view(1, n_q, hd) - want).abs() <= allowed(want, size, BF, True)).all())
+    step = torch.randn(2, (n_q + 2 * n_kv) * hd, generator=g).to(BF)
+    got = torch.empty_like(last)
+    ops().attention_decode_fp8_rope(step.to(DEV), *far.cache, got, table.to(DEV), i32(pc.slots), i32(lens), far.table, n_q, n_kv, hd,
+                                    hd ** -0.5)
+    plain_store(pc, step, table, [l - 1 for l in lens], [1, 1], n_q, n_kv, hd, hd)
+    check_cache(pc, far.back())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_captured_calls_follow_the_lengths_that_are_there(hd):
+    """A step, a prompt and their joins captured once and replayed with other lengths, tables and tokens: what eager calls give."""
+    n_q, n_kv, n = 8, 2, 6
+    table = angles(4096, hd).to(DEV)
+    longest = [2000, 40, 700, 64, 1, 300]
+    pc = filled(longest, n_kv, hd, seed=4)
+    cache = [t.clone() for t in pc.dev()]
+    fresh = [t.clone() for t in cache]
+    slots, lens, pages = i32(pc.slots), i32([1] * n), pc.table.to(DEV)
+    starts, cu = i32([0] * n), i32([0, 1, 2, 3, 4, 5, 6])
+    qkv = torch.zeros(n, (n_q + 2 * n_kv) * hd, dtype=BF, device=DEV)
+    q = torch.zeros(64, n_q * hd, dtype=BF, device=DEV)
+    outs = [torch.zeros(n, n_q * hd, dtype=BF, device=DEV), torch.zeros(n, n_q * hd, dtype=BF, device=DEV), torch.zeros_like(q)]
+
+    def calls():
+        ops().attention_decode_fp8_rope(qkv, *cache, outs[0], table, slots, lens, pages, n_q, n_kv, hd, hd ** -0.5)
+        ops().attention_decode_fp8(q[:n], *cache, outs[1], slots, lens, pages, n_q, n_kv, hd, hd ** -0.5, 0, 64)
+        ops().attention_prefill_fp8(q, *cache, outs[2], cu, slots, starts, pages, n, 64, n_q, n_kv, hd, hd ** -0.5)
+
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls()
+    g = torch.Generator().manual_seed(5)
+    for held, news in (([2000, 40, 700, 64, 1, 300], [3, 9, 1, 20, 1, 30]), ([5, 1, 0, 33, 1, 0], [1, 1, 0, 33, 1, 0]),
+                       ([1999, 39, 0, 0, 0, 0], [64, 0, 0, 0, 0, 0]), ([0] * 6, [0] * 6)):
+        results = []
+        for run in (graph.replay, calls):
+            for t, f in zip(cache, fresh):
+                t.copy_(f)
+            lens.copy_(torch.tensor(held))
+            starts.copy_(torch.tensor([max(h - m, 0) for h, m in zip(held, news)]))
+            cu.copy_(torch.tensor([sum(news[:i]) for i in range(n + 1)]))
+            g.manual_seed(6)
+            qkv.copy_(torch.randn(qkv.shape, generator=g))
+            q.copy_(torch.randn(q.shape, generator=g))
+            for o in outs:
+                o.fill_(7.0)
+            run()
+            torch.cuda.synchronize()
+            ops().check_tc_status(DEV)
+            results.append([o.clone() for o in outs] + [t.clone() for t in cache])
+        assert all(same_bits(a, b) for a, b in zip(*results))
+        assert bool((results[0][2][sum(news):] == 7.0).all())
+        for i, h in enumerate(held):
+            if h == 0:
+                assert bool((results[0][0][i] == 0).all()) and bool((results[0][1][i] == 0).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_two_streams_at_once(hd):
+    """Calls that need scratch, on two streams and as two captured graphs at once, leave what one call leaves."""
+    n_q, n_kv = 8, 2
+    lens = [6000, 900, 3500, 20, 1, 2000, 700, 64]
+    pc = filled(lens, n_kv, hd, seed=3)
+    cache, slots, held, pages = pc.dev(), i32(pc.slots), i32(lens), pc.table.to(DEV)
+    n = len(lens)
+    starts, cu = i32([l - 1 for l in lens]), i32(list(range(n + 1)))
+    qs = [torch.randn(n, n_q * hd, generator=torch.Generator().manual_seed(s)).to(BF).to(DEV) for s in (1, 2)]
+
+    def calls(q):
+        a, b = torch.empty_like(q), torch.empty_like(q)
+        ops().attention_decode_fp8(q, *cache, a, slots, held, pages, n_q, n_kv, hd, hd ** -0.5)
+        ops().attention_prefill_fp8(q, *cache, b, cu, slots, starts, pages, n, 1, n_q, n_kv, hd, hd ** -0.5)
+        return a, b
+
+    want = [calls(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    graphs, graph_outs = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            graph_outs.append(calls(q))
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls(qs[i]))
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    ops().check_tc_status(DEV)
+    for i in range(2):
+        for pair in got[i] + [graph_outs[i]]:
+            assert torch.equal(pair[0], want[i][0]) and torch.equal(pair[1], want[i][1])
+
+
+def test_more_tokens_than_the_table_has_room_for():
+    """Lengths beyond the table (a caller's mistake): nothing is written or read outside the sequence's pages."""
+    n_q, n_kv, hd = 8, 2, 64
+    pc = filled([128, 128], n_kv, hd, seed=2)
+    table = pc.table[:, :2].contiguous()               # two pages a sequence
+    cache = pc.dev()
+    before = [t.clone() for t in cache]
+    qkv = torch.randn(2, (n_q + 2 * n_kv) * hd, generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    angle = angles(64, hd).to(DEV)                     # and fewer angles than positions
+    out = torch.empty(2, n_q * hd, dtype=BF, device=DEV)
+    ops().attention_decode_fp8_rope(qkv, *cache, out, angle, i32(pc.slots), i32([129, 1000]), table.to(DEV), n_q, n_kv, hd, hd ** -0.5)
+    assert all(same_bits(a, b) for a, b in zip(before, cache))
+    q = torch.zeros(2, n_q * hd, dtype=BF, device=DEV)
+    ops().rope_store_fp8(qkv, q, *cache, angle, i32([0, 1, 2]), i32(pc.slots), i32([128, 999]), table.to(DEV), 2, 1, n_q, n_kv, hd, hd)
+    assert all(same_bits(a, b) for a, b in zip(before, cache))
+    x = torch.randn(2, n_q * hd, generator=torch.Generator().manual_seed(3)).to(BF)
+    want = torch.cat([fp8_cache.attention(x[i:i + 1].double().view(1, n_q, hd), *pc.held(i, 128), [127], hd ** -0.5, 0)[0] for i in range(2)])
+    for call in ("decode", "prefill", "plain"):
+        out.fill_(math.nan)
+        if call == "decode":
+            ops().attention_decode_fp8(x.to(DEV), *cache, out, i32(pc.slots), i32([129, 1000]), table.to(DEV), n_q, n_kv, hd, hd ** -0.5)
+        elif call == "prefill":
+            ops().attention_prefill_fp8(x.to(DEV), *cache, out, i32([0, 1, 2]), i32(pc.slots), i32([128, 999]), table.to(DEV), 2, 1, n_q,
+                                        n_kv, hd, hd ** -0.5)
+        else:
+            ops().attention_paged_fp8(x.to(DEV), *cache, out, i32([128, 999]), i32([0, 1]), i32(pc.slots), table.to(DEV), n_q, n_kv, hd,
+                                      hd ** -0.5)
+        err = (out[0].cpu().double().view(n_q, hd) - want[0]).abs()
+        assert float(err.max()) < 0.1, call            # every key that there is, where the call can tell
+
+
+def test_calls_with_nothing_to_do():
+    n_q, n_kv, hd = 4, 2, 64
+    pc = PlainCache([10], n_kv, hd)
+    cache, none = pc.dev(), torch.empty(0, n_q * hd, dtype=BF, device=DEV)
+    before = [t.clone() for t in cache]
+    empty = torch.empty(0, dtype=torch.int32, device=DEV)
+    pages = pc.table.to(DEV)
+    ops().rope_store_fp8(torch.empty(0, (n_q + 2 * n_kv) * hd, dtype=BF, device=DEV), none, *cache, None, i32([0]), empty, empty, pages, 0, 0,
+                         n_q, n_kv, hd, 0)
+    ops().attention_paged_fp8(none, *cache, none, empty, empty, empty, pages, n_q, n_kv, hd, 0.1)
+    ops().attention_decode_fp8(none, *cache, none, empty, empty, pages, n_q, n_kv, hd, 0.1)
+    ops().attention_decode_fp8_rope(torch.empty(0, (n_q + 2 * n_kv) * hd, dtype=BF, device=DEV), *cache, none, angles(8, hd).to(DEV), empty,
+                                    empty, pages, n_q, n_kv, hd, 0.1)
+    ops().attention_prefill_fp8(none, *cache, none, i32([0]), empty, empty, pages, 0, 0, n_q, n_kv, hd, 0.1)
+    torch.cuda.synchronize()
+    assert all(same_bits(a, b) for a, b in zip(before, cache))
+
+
+def good_call(name):
+    """Arguments of a call that is taken, by name."""
+    n_q, n_kv, hd, n = 4, 2, 64, 2
+    pc = filled([20, 30], n_kv, hd, seed=1)
+    k, v, ke, ve = pc.dev()
+    a = dict(k_cache=k, v_cache=v, k_exp=ke, v_exp=ve, seq_slot=i32(pc.slots), block_table=pc.table.to(DEV), n_q=n_q, n_kv=n_kv,
+             head_dim=hd)
+    q, qkv = torch.zeros(n, n_q * hd, dtype=BF, device=DEV), torch.zeros(n, (n_q + 2 * n_kv) * hd, dtype=BF, device=DEV)
+    packed = dict(cu_q=i32([0, 1, 2]), seq_start=i32([19, 29]), n_seqs=2, max_q_len=1)
+    if name == "rope_store_fp8":
+        return dict(a, qkv=qkv, q_out=q, table=angles(64, hd).to(DEV), rot_dim=hd, **packed)
+    if name == "attention_paged_fp8":
+        return dict(a, q=q, out=torch.zeros_like(q), tok_pos=i32([19, 29]), tok_seq=i32([0, 1]), scale=0.1)
+    if name == "attention_decode_fp8":
+        return dict(a, q=q, out=torch.zeros_like(q), seq_kvlen=i32([20, 30]), scale=0.1)
+    if name == "attention_decode_fp8_rope":
+        return dict(a, qkv=qkv, out=q, table=angles(64, hd).to(DEV), seq_kvlen=i32([20, 30]), scale=0.1)
+    return dict(a, q=q, out=torch.zeros_like(q), scale=0.1, **packed)
+
+
+def shifted(t):
+    """The same numbers, contiguous, one element behind an aligned address."""
+    room = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+    room.view(torch.uint8)[t.element_size():] = t.reshape(-1).view(torch.uint8)
+    return room[1:].view(t.shape)
+
+
+CALLS = ["rope_store_fp8", "attention_paged_fp8", "attention_decode_fp8", "attention_decode_fp8_rope", "attention_prefill_fp8"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_refusals(name):
+    """Each wrong argument alone makes the call fail before anything is launched; the right ones pass."""
+    op, good = getattr(ops(), name), good_call(name)
+    rows = "qkv" if "qkv" in good else "q"
+    out = "q_out" if "q_out" in good else "out"
+    wrong = [dict(k_cache=good["k_cache"].view(torch.uint8)), dict(v_cache=good["v_cache"].to(BF)),
+             dict(k_exp=good["k_exp"].to(torch.int32)), dict(k_cache=good["k_cache"][:, :, :32].contiguous()),
+             dict(v_cache=good["v_cache"][:-1]), dict(v_exp=good["v_exp"][:, :, :3].contiguous()),
+             dict(k_cache=good["k_cache"].transpose(1, 2).contiguous().transpose(1, 2)), dict(k_cache=good["k_cache"].cpu()),
+             dict(block_table=good["block_table"].long()), dict(block_table=good["block_table"][0].contiguous()),
+             dict(seq_slot=good["seq_slot"].float()), dict([(rows, good[rows].to(torch.float16))]),
+             dict([(rows, good[rows][:, :-64].contiguous())]), dict([(rows, torch.cat([good[rows]] * 2, 1)[:, ::2])]),
+             dict([(out, good[out][:1])]), dict([(out, good[out].float())]), dict(n_q=5), dict(n_q=0), dict(head_dim=32),
+             dict(k_cache=shifted(good["k_cache"]))]
+    if "seq_start" in good:
+        wrong += [dict(cu_q=good["cu_q"][:2]), dict(seq_start=good["seq_start"][:1]), dict(max_q_len=0), dict(n_seqs=-1),
+                  dict(seq_slot=good["seq_slot"][:1])]
+    if "seq_kvlen" in good:
+        wrong += [dict(seq_kvlen=good["seq_kvlen"][:1]), dict(seq_kvlen=good["seq_kvlen"].long()), dict(k_exp=shifted(good["k_exp"]))]
+    if "table" in good:
+        wrong += [dict(table=good["table"].to(BF)), dict(table=good["table"][:, :16].contiguous()), dict(table=good["table"][:0])]
+    if "tok_pos" in good:
+        wrong += [dict(tok_pos=good["tok_pos"][:1]), dict(tok_seq=good["tok_seq"].long())]
+    if name == "attention_prefill_fp8":
+        wrong += [dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(q=shifted(good["q"]))]
+    before = [t.clone() for t in (good["k_cache"], good["v_cache"], good["k_exp"], good["v_exp"], good[out])]
+    for w in wrong:
+        with pytest.raises(ops().KernelError):
+            op(**dict(good, **w))
+    torch.cuda.synchronize()
+    after = (good["k_cache"], good["v_cache"], good["k_exp"], good["v_exp"], good[out])
+    assert all(same_bits(a, b) for a, b in zip(before, after))
+    op(**good)
+    torch.cuda.synchronize()
+
+
+def test_exponents_at_any_address_where_the_call_takes_them():
+    """Appends, the plain kernel and prompts read exponents byte by byte."""
+    for name in ("rope_store_fp8", "attention_paged_fp8", "attention_prefill_fp8"):
+        results = []
+        for place in (lambda t: t, shifted):
+            good = good_call(name)
+            good["k_exp"], good["v_exp"] = place(good["k_exp"]), place(good["v_exp"])
+            good["qkv" if "qkv" in good else "q"].fill_(0.25)
+            out = getattr(ops(), name)(**good)
+            results.append((out, good["k_exp"].clone(), good["v_exp"].clone(), good["k_cache"]))
+        assert all(same_bits(a, b) for a, b in zip(*results)), name
+
+
+@pytest.mark.parametrize("n_q,n_kv,hd", [(128, 1, 64), (128, 1, 128), (64, 1, 128)])
+def test_prompt_of_the_widest_groups(n_q, n_kv, hd):
+    starts, news = [0, 300, 60], [3, 2, 5]
+    pc = filled([s + m for s, m in zip(starts, news)], n_kv, hd, seed=hd + n_q)
+    q = torch.randn(sum(news), n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = prompt(pc, q, starts, news, n_q, n_kv, hd, hd ** -0.5, 0)
+    check_prompt(pc, out, q, starts, news, n_q, n_kv, hd, hd ** -0.5, 0)
+
+
+def test_many_sequences_in_a_step():
+    """More sequences than a warp looks at in one go, most of them short, some empty, more items than thread blocks."""
+    n_q, n_kv, hd = 8, 2, 64
+    g = torch.Generator().manual_seed(9)
+    lens = torch.randint(0, 90, (1500,), generator=g).tolist()
+    pc = filled(lens, n_kv, hd, seed=9)
+    n = len(lens)
+    q = torch.randn(n, n_q * hd, generator=g).to(BF)
+    out = torch.full((n, n_q * hd), math.nan, dtype=BF, device=DEV)
+    ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5, 0, 90)
+    two = torch.full((n, n_q * hd), math.nan, dtype=BF, device=DEV)
+    some = [i for i, l in enumerate(lens) if l]
+    ops().attention_prefill_fp8(q[some].to(DEV), *pc.dev(), two[:len(some)], i32(list(range(len(some) + 1))), i32([pc.slots[i] for i in some]),
+                                i32([lens[i] - 1 for i in some]), pc.table.to(DEV), len(some), 1, n_q, n_kv, hd, hd ** -0.5)
+    ops().check_tc_status(DEV)
+    for row, i in enumerate(some):
+        want, size = fp8_cache.attention(q[i:i + 1].double().view(1, n_q, hd), *pc.held(i, lens[i]), [lens[i] - 1], hd ** -0.5, 0)
+        bound = allowed(want, size, BF, True)
+        assert bool(((out[i].cpu().double().view(1, n_q, hd) - want).abs() <= bound).all()), i
+        assert bool(((two[row].cpu().double().view(1, n_q, hd) - want).abs() <= bound).all()), i
+    assert all(bool((out[i] == 0).all()) for i, l in enumerate(lens) if l == 0)

@@ -35,6 +35,17 @@ def test_mixers_that_do_not_know_it_are_refused(req):
     Cache([[req]], 2, 128, 128, torch.bfloat16, "cpu")
 
 
+def test_a_position_encoding_that_writes_the_cache_itself_is_asked():
+    from llm_infer_engine_b200.parts.attention import GroupedQueryAttention
+    from llm_infer_engine_b200.parts.base import PositionEncoding
+    from llm_infer_engine_b200.parts.rope import NoEncoding, RotaryEncoding
+    layer = GroupedQueryAttention.__new__(GroupedQueryAttention)
+    layer.n_kv_heads, layer.head_dim, layer.window = 2, 64, 0
+    for position, knows in ((RotaryEncoding, True), (NoEncoding, True), (PositionEncoding, False)):
+        layer.position = position
+        assert layer.cache_requests() == [KVRequest(2, 64)] and layer.cache_requests()[0].eight_bit is knows
+
+
 def test_other_types_are_refused():
     with pytest.raises(ValueError, match="held in"):
         Cache([[KVRequest(2, 64, eight_bit=True)]], 2, 128, 128, torch.bfloat16, "cpu", torch.float16)
