@@ -64,7 +64,7 @@ class StepContext:
         plan = self.kernels
         if plan is not None and plan.attention(self, q, kv, out, n_q, n_kv, head_dim, options, gate):
             return
-        if kv.k_exp is not None:
+        if getattr(kv, "k_exp", None) is not None:
             if not options.plain:
                 raise ops.KernelError("attention over a cache in 8 bits knows a scale, a window and chunks, no other option")
             ops.attention_paged_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, self.tok_pos, self.tok_seq, self.seq_slot,

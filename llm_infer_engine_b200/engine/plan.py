@@ -43,7 +43,7 @@ class KernelPlan:
         size exists. Returns False (and does nothing) otherwise; the caller then rotates and stores first."""
         if not write_kv:
             return False       # a borrowed cache already holds the owner's new key: it must be read, not replaced
-        if kv.k_exp is not None:
+        if getattr(kv, "k_exp", None) is not None:
             # the same over a cache in 8 bits (where query heads do not need two passes over a key/value head)
             if not (ctx.decode and table is not None and options.plain
                     and ops.attention_decode_fp8_rope_supported(n_q, n_kv, head_dim, qkv.dtype)):
@@ -67,7 +67,7 @@ class KernelPlan:
         every option (scale, window, kept first keys, sink, gate); the CUDA-core split-KV kernel knows scale and
         window. A value head size that differs from the key head size is the plain kernel's alone."""
         scale, window = options.scale, options.reach
-        if kv.k_exp is not None:
+        if getattr(kv, "k_exp", None) is not None:
             return self._attention_fp8(ctx, q, kv, out, n_q, n_kv, head_dim, options, gate)
         if options.sigmoid_bias is not None:
             return self._sigmoid_attention(ctx, q, kv, out, n_q, n_kv, head_dim, options, gate)

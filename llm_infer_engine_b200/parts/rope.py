@@ -104,7 +104,7 @@ class RotaryEncoding(PositionEncoding):
         """`v_head_dim`: the size of a value head where it differs from head_dim (the packed row then ends with
         n_kv * v_head_dim value columns)."""
         q = torch.empty((qkv.shape[0], n_q * head_dim), dtype=qkv.dtype, device=qkv.device)
-        if kv is not None and kv.k_exp is not None:
+        if getattr(kv, "k_exp", None) is not None:
             return _store_fp8(qkv, q, ctx, kv, self.table, n_q, n_kv, head_dim, self.rot_dim, write_kv)
         ops.rope_store(qkv, q, kv.k if kv is not None else None, kv.v if kv is not None else None, self.table,
                        ctx.tok_pos, ctx.tok_seq, ctx.seq_slot, kv.block_table, kv.page_size, n_q, n_kv, head_dim,
@@ -119,7 +119,7 @@ class NoEncoding(PositionEncoding):
 
     def encode_and_store(self, qkv, ctx, kv, n_q, n_kv, head_dim, write_kv):
         q = torch.empty((qkv.shape[0], n_q * head_dim), dtype=qkv.dtype, device=qkv.device)
-        if kv.k_exp is not None:
+        if getattr(kv, "k_exp", None) is not None:
             return _store_fp8(qkv, q, ctx, kv, None, n_q, n_kv, head_dim, 0, write_kv)
         ops.rope_store(qkv, q, kv.k, kv.v, None, ctx.tok_pos, ctx.tok_seq, ctx.seq_slot, kv.block_table,
                        kv.page_size, n_q, n_kv, head_dim, 0, write_kv)
