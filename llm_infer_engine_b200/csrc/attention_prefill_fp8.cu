@@ -16,9 +16,15 @@
 // multiplied by 2^(R - R') in few tiles only. Queries are brought to half precision with a power of two a row, which keeps
 // every digit of bfloat16. Weights go back to tensor memory as the second product's first operand.
 //
-// Work. A block takes one (sequence, tile of tokens, key/value head), or one of several equal runs of its key tiles where the
-// step has too few of them for the GPU: how many runs a sequence's tiles are cut into is worked out on the device from the
-// lengths that are there, so that a run is about a 148th of the step. Runs leave partial results, which a second kernel joins in order.
+// Work. A piece is a (sequence, tile of tokens, key/value head), or one of several equal runs of its key tiles where the step has
+// too few of them for the GPU: how many runs a sequence's tiles are cut into is worked out on the device from the lengths that
+// are there. Runs leave partial results, which a second kernel joins in order. A block per piece is launched, and a block that is
+// about to be done takes over the piece of one that has not begun (cluster launch control): keys of the next piece are converted
+// while this one's last scores are worked on, its queries are brought while its last product runs. (6 sequences of 60 to 1,500 tokens,
+// head size 128, 376 pieces: 76.4 us with a block a piece, which spent 26,000 of 42,000 clocks on finding, bringing and writing.)
+//
+// Code. What a block does once is written in loops that stay loops, and each search for work is there once: a kernel of 140 to 250 KB
+// of instructions, as the compiler lays them out by itself, spends thousands of clocks a piece on fetching them.
 //
 // Numbers that are not finite: a score that is NaN makes its row NaN by itself. A value that is NaN must reach the rows that see it
 // and no other, and a product with a zero weight would spread it; so such codes enter the product as zeros, the tile is marked,
@@ -36,6 +42,8 @@ constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B
 constexpr int kPfSub = kPfRows * 128;        // bytes of 128 rows of 64 half-precision numbers
 constexpr int kPfSms = 148;
 constexpr int kPfRing = 8;
+constexpr int kPfAhead = 4;          // places for pieces of work
+constexpr int kPfReaders = 14;       // who reads one: eight softmax warps, four converting ones, two issuing threads
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
 constexpr int kPfLeast = 4;          // key tiles that a run has at least, on average
 constexpr int kPfSlots = 200;        // partial results at once (see pf_run)
@@ -48,18 +56,19 @@ template <int HD> struct PfCfg {
   static constexpr int kQBytes = kSubs * kPfSub;             // one tile of queries
   static constexpr int kKvBytes = kSubs * kPfSub;            // 128 keys, or values
   static constexpr int kStages = 2;
-  static constexpr int kSmem = 2 * kQBytes + 2 * kStages * kKvBytes + 1024;
+  static constexpr int kOutBytes = 8 * 2048;                 // a warp turns 32 rows of 32 numbers at a time
+  static constexpr int kSmem = 2 * kQBytes + 2 * kStages * kKvBytes + kOutBytes + 1024;
   static constexpr bool kOwnP = HD == 64;                    // tensor memory has room for the weights beside the scores
   static constexpr int kSCol = 0, kOCol = 256, kPCol = 384;  // columns: scores of A and B, sums of A and B, weights
-  static constexpr int kRecord = 2 * kPfRows * (HD + 2);     // floats of a partial result: sums, then bounds, then denominators
+  static constexpr int kRecord = 2 * kPfRows * (HD + 2);     // floats of a partial result: sums [HD / 4][rows][4], then bounds, then denominators
 };
 
 // Registers that a thread of a softmax, the conversion and the last warpgroup keeps of the 128 that it is launched with: a row's 128
-// scores stay in registers, a converting thread has a step's codes in them. (Head size 128, 192 / 176 for the softmax: pieces of 60
-// to 1,500 tokens 84.9 / 87.8 us; where the tiles take turns and the conversion sets the pace, 24 sequences of 2 to 8 tokens, 70.2 / 58.5.)
+// scores stay in registers. (Head size 128, 184 + 96 or 200 + 64 for the softmax and the conversion: pieces of 60 to 1,500 tokens 73.7
+// or 68.2 us; where the tiles take turns, 24 sequences of 2 to 8 tokens, 56.2 or 60.4.)
 template <int HD, bool TURNS> struct PfRegs {
-  static constexpr int kSoftmax = HD == 64 ? 200 : TURNS ? 176 : 192, kConvert = HD == 64 ? 80 : TURNS ? 112 : 88,
-                       kIssue = HD == 64 ? 32 : TURNS ? 48 : 40;
+  static constexpr int kSoftmax = HD == 64 ? 192 : TURNS ? 184 : 200, kConvert = HD == 64 ? 72 : TURNS ? 96 : 64,
+                       kIssue = HD == 64 ? 56 : 48;
   static_assert(2 * kSoftmax + kConvert + kIssue == 4 * 128, "more than the block has would never be granted");
   static_assert(kSoftmax >= 128 && kConvert <= 128 && kIssue <= 128, "inc may only raise, dec only lower");
 };
@@ -96,6 +105,18 @@ __device__ __forceinline__ float pf_max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
+}
+// mbar_wait in few instructions.
+__device__ __forceinline__ bool pf_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  unsigned spin = 0;
+#pragma unroll 1
+  while (!mbar_test(bar, parity)) {
+    if (++spin > 64) {
+      __nanosleep(spin > 4096 ? 256 : 32);
+      if (*abort || spin > kSpinLimit) return false;
+    }
+  }
+  return true;
 }
 // D[tmem] (+)= A[tmem] * B[smem], half precision
 __device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
@@ -157,6 +178,7 @@ __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSeq
   const int lane = threadIdx.x & 31;
   float twice = (float)mine.tiles * (float)(mine.first + mine.last);
   int tiles = mine.tiles;
+#pragma unroll 1
   for (int s = lane + 32; s < a.n_seqs; s += 32) {
     const PfSequence q = pf_sequence(a, s, tok);
     twice += (float)q.tiles * (float)(q.first + q.last);
@@ -168,8 +190,10 @@ __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSeq
   const int most = max(a.run, max(kPfLeast, (int)fminf(ceilf(share), 1e9f)));
   if ((int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * a.n_kv > kPfSms) return most;
   int run = max(a.run, max(kPfLeast, (int)fminf(ceilf(share * 0.5f), 1e9f)));
+#pragma unroll 1
   for (int i = 0; i < 24; ++i, run += (run + 7) / 8) {                       // (9/8)^24 > 16
     unsigned runs = mine.tiles * pf_runs(mine.last, run);
+#pragma unroll 1
     for (int s = lane + 32; s < a.n_seqs; s += 32) {
       const PfSequence q = pf_sequence(a, s, tok);
       runs += q.tiles * pf_runs(q.last, run);
@@ -184,14 +208,13 @@ struct PfWork {
   int tile, hk, part, parts, slot;               // slot: of the partial result; parts: 0 where there is no such piece
 };
 // Piece `index` of the step's work, or (WHOLE) tile `index` with all its runs. All lanes of a warp call it. Late tiles of a
-// sequence, which see the most keys, come first, all heads of one after another.
+// sequence, which see the most keys, come first, all heads of one after another. `mine`: the lane's first sequence; run: pf_run's.
 template <bool WHOLE>
-__device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int index) {
+__device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int index, const PfSequence& mine, int run) {
   const int lane = threadIdx.x & 31;
-  const PfSequence mine = pf_sequence(a, lane, tok);
-  const int run = pf_run(a, tok, mine);
   PfWork w{0, 0, 0, 0, 0, 0, 0, 0, 0};
   int before = 0, slots = 0;
+#pragma unroll 1
   for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
     const PfSequence q = s0 == 0 ? mine : pf_sequence(a, s0 + lane, tok);
     const int parts = pf_runs(q.last, run);
@@ -228,19 +251,85 @@ __device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int ind
   return w;
 }
 
+// What the block's parts need of a piece, worked out by who found it.
+struct PfPiece {
+  int parts, slot, hk, page_row;
+  int row0, pos0;                    // of its first token: row of the step, position
+  int n_tok_a, n_tok_b;              // tokens of the two tiles
+  int c0, n_steps, n_a, n_b;         // its first key tile; its steps and those of either tile
+  int last_key;
+};
+template <bool TURNS> __device__ __forceinline__ PfPiece pf_piece(const PrefillArgs& a, const PfWork& w, int tok_x) {
+  PfPiece p;
+  const int tok = TURNS ? tok_x : 2 * tok_x, t0 = w.tile * tok, n_tok = min(tok, w.q_len - t0), parts = max(w.parts, 1);
+  p.parts = w.parts;
+  p.slot = w.slot;
+  p.hk = w.hk;
+  p.page_row = w.page_row;
+  p.row0 = w.q_begin + t0;
+  p.pos0 = w.start + t0;
+  int lo_tile, tiles;
+  pf_tiles(a, w.start, t0, n_tok, lo_tile, tiles);
+  // this run's key tiles: [c0, c1) of the tiles of the block's tokens
+  p.c0 = lo_tile + tiles * w.part / parts;
+  const int c1 = lo_tile + tiles * (w.part + 1) / parts;
+  p.last_key = min(p.pos0 + n_tok, a.max_pages * kFp8Page) - 1;
+  // Steps of the two tiles: A's tokens come first and may not see the last key tiles.
+  p.n_tok_a = min(n_tok, tok_x);
+  p.n_tok_b = TURNS ? p.n_tok_a : n_tok - p.n_tok_a;
+  p.n_steps = c1 - p.c0;
+  p.n_a = TURNS ? (p.n_steps + 1) / 2 : max(0, min(c1, (p.pos0 + p.n_tok_a - 1) / kPfKeys + 1) - p.c0);
+  p.n_b = TURNS ? p.n_steps / 2 : p.n_tok_b > 0 ? p.n_steps : 0;
+  return p;
+}
+
 struct PfShared {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], x_full[kPfRing];
-  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], last[2];
+  uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready[2], last[2];
+  uint64_t a_scored, b_handed, a_read;             // where the tiles take turns
+  uint64_t work_full[kPfAhead], work_empty[kPfAhead], want, answered, tmem_ready;
   uint32_t tmem_base;
   int abort;
-  // Of the key tiles in flight, by step % 8: factors of scores, addends, factors of the denominator's terms, and the step (+ 1)
-  // that last had NaN among its values. x_full: all of them are there. (A step's place is written again eight steps on, when the
-  // scores of the step six on are done; and those were let begin behind the softmax's last look at this step.)
+  // Of the key tiles in flight, by step % 8 (steps are counted through all the block's pieces): factors of scores, addends, factors of
+  // the denominator's terms, and the step (+ 1) that last had NaN among its values. x_full: all of them are there. (A step's place is
+  // written again eight steps on. By then both tiles' scores of six steps on are done or not wanted, which were let begin behind the
+  // softmax's last look at this step; a piece's first, or its being let go, waits for the softmax to have done with the piece before.)
   float k_scale[kPfRing][8], v_add[kPfRing][8], v_back[kPfRing][8];
   int v_nan[kPfRing];
   float handed[2][kPfRows];          // where B has A's rows: its bounds and denominators
-  PfWork work;
+  PfPiece work[kPfAhead];            // the block's pieces, by their number % 4
+  alignas(16) uint32_t answer[4];    // to the last asking for another
 };
+
+// Asks for a thread block of this launch that has not begun, in whose stead this one works on; false: there is none any more (and
+// nobody may ask again). All lanes of a warp call it; `asked`: how often it has been called.
+__device__ __forceinline__ bool pf_another(PfShared& sh, int asked, int& index, volatile int* abort) {
+  if ((threadIdx.x & 31) == 0) {
+    fence_proxy_async_smem();        // the last answer has been read
+    mbar_arrive_expect_tx(&sh.answered, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(sh.answer)), "r"(smem_u32(&sh.answered)) : "memory");
+  }
+  __syncwarp();
+  if (!__all_sync(0xffffffffu, pf_wait(&sh.answered, asked & 1, abort))) {
+    if ((threadIdx.x & 31) == 0) *abort = 1;
+    return false;
+  }
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_u32(sh.answer))
+      : "memory");
+  __syncwarp();
+  index = (int)x;
+  return got != 0;
+}
 
 // ------------------------------------------------------------------------------------------ the kernel
 // TURNS: every tile's tokens fit into one operand tile; B then has the same rows as A, and the two take the key tiles in turn: two
@@ -254,15 +343,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   uint8_t* q_smem = base;
   uint8_t* k_smem = q_smem + 2 * Cfg::kQBytes;
   uint8_t* v_smem = k_smem + Cfg::kStages * Cfg::kKvBytes;
+  uint8_t* out_smem = v_smem + Cfg::kStages * Cfg::kKvBytes;
   const int warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_launch_dependents();
 
   const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = TURNS ? tok_x : 2 * tok_x;      // tokens of a tile, of a block
-  // one warp looks for the block's piece of work while others set it up
-  if (warp == 0) {
-    const PfWork found = pf_find<false>(a, tok, blockIdx.x);
-    if (threadIdx.x == 0) sh.work = found;
+  // one warp looks for the block's pieces of work while others set it up
+  PfSequence mine;
+  int run = 0;
+  if (warp == 14) {
+    mine = pf_sequence(a, threadIdx.x & 31, tok);
+    run = pf_run(a, tok, mine);
+    const PfWork found = pf_find<false>(a, tok, blockIdx.x, mine, run);
+    if ((threadIdx.x & 31) == 0) sh.work[0] = pf_piece<TURNS>(a, found, tok_x);
   } else if (threadIdx.x == 32) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sh.k_full[s], 128);
@@ -273,240 +367,144 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       mbar_init(&sh.s_free[s], 128);
       mbar_init(&sh.p_ready[s], 128);
       mbar_init(&sh.pv_done[s], 1);
+      mbar_init(&sh.q_ready[s], 128);
       mbar_init(&sh.last[s], 1);
     }
     for (int i = 0; i < kPfRing; ++i) {
       mbar_init(&sh.x_full[i], 128);
       sh.v_nan[i] = 0;
     }
+    for (int i = 0; i < kPfAhead; ++i) {
+      mbar_init(&sh.work_full[i], 1);
+      mbar_init(&sh.work_empty[i], kPfReaders);
+    }
+    mbar_init(&sh.a_scored, 128);
+    mbar_init(&sh.b_handed, 128);
+    mbar_init(&sh.a_read, 128);
+    mbar_init(&sh.want, 1);
+    mbar_init(&sh.answered, 1);
+    mbar_init(&sh.tmem_ready, 1);
     sh.abort = 0;
     fence_mbar_init();
   }
   __syncthreads();
-  const PfWork w = sh.work;
-  if (w.parts == 0) return;          // the whole block alike
-  if (warp == 12) {
-    tmem_alloc(&sh.tmem_base, 512);
-    tmem_relinquish();
-  }
-  const int q_begin = w.q_begin, q_len = w.q_len, start = w.start;
-  const int t0 = w.tile * tok, n_tok = min(tok, q_len - t0);
-  int lo_tile, tiles;
-  pf_tiles(a, start, t0, n_tok, lo_tile, tiles);
-  // this run's key tiles: [c0, c1) of the tiles of the block's tokens
-  const int c0 = lo_tile + tiles * w.part / w.parts, c1 = lo_tile + tiles * (w.part + 1) / w.parts;
-  const int last_key = min(start + t0 + n_tok, a.max_pages * kFp8Page) - 1;
-  // Steps of the two tiles: A's tokens come first and may not see the last key tiles.
-  const int n_tok_a = min(n_tok, tok_x);
-  const int n_tok_b = TURNS ? n_tok_a : n_tok - n_tok_a;
-  const int n_steps = c1 - c0;
-  const int n_a = TURNS ? (n_steps + 1) / 2 : max(0, min(c1, (start + t0 + n_tok_a - 1) / kPfKeys + 1) - c0), n_b = TURNS ? n_steps / 2 : n_tok_b > 0 ? n_steps : 0;
-
-  // What needs no barrier begins before the block meets: the rows' queries go to shared memory, the first codes are asked for.
-  const bool softmax = warp < 8;
-  const int x = warp >> 2 & 1, r = threadIdx.x & 127;        // tile and row of a softmax thread
-  const int first_tok = t0 + (TURNS ? 0 : x * tok_x), n_tok_x = x ? n_tok_b : n_tok_a;
-  const int rt = r / G, rh = r - rt * G;                     // token of the tile, query head of the group
-  const bool there = softmax && rt < n_tok_x;
-  const size_t row_off = ((size_t)(q_begin + first_tok + rt) * a.n_q + w.hk * G + rh) * HD;
-  float f = 0.f;                                             // of the row's scores: scale log2(e) and the row's power of two
-  constexpr int kPer = HD / 16;                              // pieces of 16 codes a row, and pieces that a converting thread has
-  constexpr int kStep = 128 / kPer;                          // its rows: row0, row0 + kStep, ...
-  const int ct = threadIdx.x & 127, piece = ct % kPer, row0 = ct / kPer;
-  const int* pages = a.block_table + (size_t)w.page_row * a.max_pages;
-  uint4 kr[kPer], vr[kPer];
-  // Everything is asked for well before it is looked at: a tile's pages a step before its codes, its codes and exponents a step
-  // before they are written out. (Where an exponent was clamped, or a page's address made, as soon as it was asked for, the
-  // conversion waited for memory twice a tile, and the whole kernel for the conversion: 3,500 clocks a step.)
-  int pg0 = 0, pg1 = 0;                                      // pages of the tile to be asked for next
-  signed char ke = 0, ve = 0;                                // a thread's two exponents
-  auto page_at = [&](int lp) { return lp * kFp8Page <= last_key ? pages[lp] : 0; };
-  auto load = [&](uint4 (&reg)[kPer], const unsigned char* cache, int tile) {
-    const unsigned char* at0 = cache + (((size_t)pg0 * a.n_kv + w.hk) * kFp8Page + row0) * HD + piece * 16;
-    const unsigned char* at1 = cache + (((size_t)pg1 * a.n_kv + w.hk) * kFp8Page + row0) * HD + piece * 16;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      reg[i] = make_uint4(0u, 0u, 0u, 0u);                   // rows behind the block's last key: nothing that may be NaN
-      if (tile * kPfKeys + row0 + i * kStep <= last_key)
-        reg[i] = *reinterpret_cast<const uint4*>((i < kPer / 2 ? at0 + i * kStep * HD : at1 + (i - kPer / 2) * kStep * HD));
-    }
-  };
-  // Exponents of the tile's eight blocks, a thread a block (one behind the last key: anything, nobody sees its scores).
-  auto load_exps = [&]() {
-    if (ct < 8) {
-      const size_t at = ((size_t)(ct < 4 ? pg0 : pg1) * a.n_kv + w.hk) * kPageExps + (ct & 3);
-      ke = a.k_exp[at];
-      ve = a.v_exp[at];
-    }
-  };
-  if (softmax) {
-    uint4 raw[HD / 8];
-    float big = 0.f;
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-      raw[i] = there ? *reinterpret_cast<const uint4*>(a.q + row_off + i * 8) : make_uint4(0u, 0u, 0u, 0u);
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 y = __bfloat1622float2(h[e]);
-        big = fmaxf(big, fmaxf(fabsf(y.x), fabsf(y.y)));
-      }
-    }
-    const int eb = (int)(__float_as_uint(big) >> 23);
-    const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);         // the largest number into [2^14, 2^15)
-    const float up = pow2_of(shift);
-    f = a.scale2 * pow2_of(-shift);
-    uint8_t* dst = q_smem + x * Cfg::kQBytes;
-#pragma unroll
-    for (int i = 0; i < HD / 8; ++i) {
-      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw[i]);
-      uint32_t o[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 y = __bfloat1622float2(h[e]);
-        o[e] = pf_half2(y.x * up, y.y * up);
-      }
-      *reinterpret_cast<uint4*>(dst + (i >> 3) * kPfSub + swizzle128_offset(r, i & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    fence_proxy_async_smem();
-  } else if (warp < 12 && n_steps > 0) {
-    pg0 = page_at(c0 * 2);
-    pg1 = page_at(c0 * 2 + 1);
-    const int next0 = page_at(c0 * 2 + 2), next1 = page_at(c0 * 2 + 3);
-    load(kr, a.k, c0);
-    load(vr, a.v, c0);
-    load_exps();
-    pg0 = next0;
-    pg1 = next1;
-  }
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = sh.tmem_base;
+  if (sh.work[0].parts == 0) return; // the whole block alike
   volatile int* abort = &sh.abort;
 #define LLMIE_FAIL(code) do { if (!*abort) { *abort = 1; atomicExch(a.status, (code)); } } while (0)
+  // Whether there is a piece number n for this block (in sh.work until it is given back): false at the end of the work, or where a
+  // wait gave up. All lanes of a warp call it, or one thread alone.
+  auto piece_there = [&](int n) -> bool {
+    if (!pf_wait(&sh.work_full[n % kPfAhead], (n / kPfAhead) & 1, abort)) {
+      LLMIE_FAIL(kStatusTimeoutFull);
+      return false;
+    }
+    return sh.work[n % kPfAhead].parts > 0;
+  };
 
-  if (softmax) {
+  if (warp < 8) {
     // ------------------------------------------------------------------ softmax: a thread a row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kSoftmax));
-    const int n_x = x ? n_b : n_a;
-    const int qpos = start + first_tok + min(rt, max(n_tok_x - 1, 0));
-    const int lo = first_visible_key(qpos, a.window);
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128, o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128);
-    const uint32_t p_addr = Cfg::kOwnP ? tmem + lanes + Cfg::kPCol + x * 64 : s_addr;
-    // a score's factor is never 0: times -inf, which stands where the row does not look, that would be NaN
-    auto factor = [&](float k_scale) { return fminf(fmaxf(f * k_scale, 1.2e-38f), 3.4e38f); };
-    float R = -INFINITY, l = 0.f;
-    uint32_t nan_cols[HD / 32];
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) nan_cols[i] = 0u;
+    const int x = warp >> 2, r = threadIdx.x & 127;          // tile and row
+    const int rt = r / G, rh = r - rt * G;                   // token of the tile, query head of the group
+    const int lane = threadIdx.x & 31;
+    constexpr int kPieces = HD / 8, kRowsAtOnce = 32 / kPieces, kLoads = 32 / kRowsAtOnce;   // of 16 bytes a row; rows a load of the warp's
+    const uint32_t q_mine = smem_u32(q_smem + x * Cfg::kQBytes) + (lane % kPieces >> 3) * kPfSub;
+    // where the i-th piece that this lane brings lies
+    auto q_place = [&](int i) { return q_mine + swizzle128_offset((warp & 3) * 32 + i * kRowsAtOnce + lane / kPieces, lane & 7); };
+    // which row of the queries and the output is this thread's (-1: none)
+    auto row_of = [&](const PfPiece& p) {
+      return rt < (x ? p.n_tok_b : p.n_tok_a) ? (p.row0 + (TURNS ? 0 : x * tok_x) + rt) * a.n_q + p.hk * G + rh : -1;
+    };
+    // A warp asks for its 32 rows of queries, a row by neighbouring lanes; rows that are not there are zeros.
+    auto ask_for_queries = [&](const PfPiece& p) {
+      const int mine = row_of(p);
+#pragma unroll 4
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = __shfl_sync(0xffffffffu, mine, i * kRowsAtOnce + lane / kPieces);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(q_place(i)), "l"(a.q + (size_t)max(row, 0) * HD + lane % kPieces * 8), "r"(row >= 0 ? 16 : 0) : "memory");
+      }
+    };
+    bool more = __all_sync(0xffffffffu, piece_there(0));
+    if (more) ask_for_queries(sh.work[0]);
+    int gs = 0, gx = 0;              // steps of the block, and of this tile, before this piece
+    int turns = 0;                   // pieces whose results B handed over
     bool ok = true;
-    // the first and last keys that every row of the tile sees
-    const int all_to = start + first_tok, all_from = first_visible_key(start + first_tok + max(n_tok_x - 1, 0), a.window);
-    for (int j = 0; j < n_x; ++j) {            // this tile's j-th step is the block's `step`
-      const int step = TURNS ? 2 * j + x : j;
-      // every decision to give up is taken by the whole warp: reads of tensor memory are warp-wide instructions
-      if (!__all_sync(0xffffffffu, mbar_wait(&sh.x_full[step % kPfRing], (step / kPfRing) & 1, abort) && mbar_wait(&sh.s_full[x], j & 1, abort))) {
-        LLMIE_FAIL(kStatusTimeoutMma);
-        ok = false;
-        break;
-      }
-      tc_fence_after_sync();
-      const int kbase = (c0 + step) * kPfKeys, ring = step % kPfRing;
-      const bool edge = kbase + kPfKeys - 1 > all_to || kbase < all_from;
-      const int nan_step = sh.v_nan[ring];
-      // the row's scores; those that it does not see are -inf
-      uint32_t v[4][32];
+    uint32_t tmem = 0;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+#pragma unroll 1
+    for (int n = 0; more; ++n) {
+      const PfPiece& w = sh.work[n % kPfAhead];
+      const int n_x = x ? w.n_b : w.n_a, c0 = w.c0;
+      const int first = w.pos0 + (TURNS ? 0 : x * tok_x), n_more = max((x ? w.n_tok_b : w.n_tok_a) - 1, 0);
+      const int qpos = first + min(rt, n_more), lo = first_visible_key(qpos, a.window);
+      // the first and last keys that every row of the tile sees
+      const int all_to = first, all_from = first_visible_key(first + n_more, a.window);
+      // Queries become half precision where they lie, a row by its thread, with the power of two that brings its largest number into
+      // [2^14, 2^15).
+      float f;                         // of the row's scores: scale log2(e) and the power of two
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      {
+        const uint32_t row = smem_u32(q_smem + x * Cfg::kQBytes);
+        auto piece_at = [&](int i) { return row + (i >> 3) * kPfSub + swizzle128_offset(r, i & 7); };
+        uint32_t big[4] = {0u, 0u, 0u, 0u};      // the largest magnitudes by their bits, which are ordered as the numbers, what is not finite on top
+#pragma unroll 8
+        for (int i = 0; i < kPieces; ++i) {
+          uint32_t u[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(piece_at(i)) : "memory");
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, v[c]);
-      float fk[8];
-#pragma unroll
-      for (int b = 0; b < 8; ++b) fk[b] = factor(sh.k_scale[ring][b]);
-      tmem_ld_wait();
-      if (Cfg::kOwnP) {
-        // they are in registers: the next scores may be written
-        tc_fence_before_sync();
-        mbar_arrive(&sh.s_free[x]);
-      }
-      if (edge) {
-        const int from = lo - kbase;
-        const unsigned span = (unsigned)(qpos - lo);
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if ((unsigned)(i - from) > span) v[i >> 5][i & 31] = 0xff800000u;
-      }
-      float mx = -INFINITY;          // the largest s + ev
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const uint32_t* y = v[b >> 1] + (b & 1) * 16;
-        float m0 = __uint_as_float(y[0]), m1 = __uint_as_float(y[1]);
-#pragma unroll
-        for (int i = 2; i < 14; i += 4) {
-          m0 = pf_max3(m0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
-          m1 = pf_max3(m1, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+          for (int e = 0; e < 4; ++e) big[e] = max(big[e], max(u[e] & 0x7fffu, u[e] >> 16 & 0x7fffu));
         }
-        m0 = pf_max3(m0, __uint_as_float(y[14]), __uint_as_float(y[15]));
-        mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fk[b], sh.v_add[ring][b]));
-      }
-      const bool grow = mx > R + kPfSlack || R == -INFINITY;
-      if (__any_sync(0xffffffffu, grow && j > 0)) {
-        // the sums so far are brought to the new bound (rows that keep theirs: times 1)
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (j - 1) & 1, abort))) {
-          LLMIE_FAIL(kStatusTimeoutMma);
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-        const float alpha = !grow ? 1.f : R == -INFINITY ? 0.f : pf_exp2(R - mx);
-        l *= alpha;
+        const int eb = (int)(max(max(big[0], big[1]), max(big[2], big[3])) >> 7), shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);
+        const float up = pow2_of(shift);
+        f = a.scale2 * pow2_of(-shift);
+#pragma unroll 4
+        for (int i = 0; i < kPieces; ++i) {
+          uint32_t u[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(piece_at(i)) : "memory");
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-          uint32_t y[16];
-          tmem_ld_32x16(o_addr + c * 16, y);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
-          pf_tmem_st16(o_addr + c * 16, y);
-        }
-        tmem_st_wait();
-      }
-      if (grow) R = mx;
-      const float shift = (R == -INFINITY ? 0.f : R) - kPfTop;
-      if (Cfg::kOwnP && j > 0) {
-        // the weights of the tile before have to be through the product before they are written over
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (j - 1) & 1, abort))) {
-          LLMIE_FAIL(kStatusTimeoutMma);
-          ok = false;
-          break;
-        }
-        tc_fence_after_sync();
-      }
-      // the weights, over the scores they come from or in columns of their own
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[16];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float add = sh.v_add[ring][c * 2 + b] - shift;
-          const uint32_t* y = v[c] + b * 16;
-          float sum[4];
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float x0 = pf_exp2(fmaf(__uint_as_float(y[i]), fk[c * 2 + b], add)), x1 = pf_exp2(fmaf(__uint_as_float(y[i + 1]), fk[c * 2 + b], add));
-            sum[i & 2] = i < 4 ? x0 : sum[i & 2] + x0;
-            sum[(i & 2) + 1] = i < 4 ? x1 : sum[(i & 2) + 1] + x1;
-            o[b * 8 + i / 2] = pf_half2(x0, x1);
+          for (int e = 0; e < 4; ++e) {
+            const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u[e]));
+            u[e] = pf_half2(y.x * up, y.y * up);
           }
-          l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), sh.v_back[ring][c * 2 + b], l);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at(i)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
         }
-        pf_tmem_st16(p_addr + c * 16, o);
       }
-      tmem_st_wait();
-      tc_fence_before_sync();
-      mbar_arrive(&sh.p_ready[x]);
-      if (nan_step == step + 1) {
-        // rare: which columns of the values that this row sees are NaN
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.q_ready[x]);
+      if (n == 0) {
+        if (!__all_sync(0xffffffffu, pf_wait(&sh.tmem_ready, 0, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          break;
+        }
+        tc_fence_after_sync();
+        tmem = sh.tmem_base;
+      }
+      const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128, o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128);
+      const uint32_t p_addr = Cfg::kOwnP ? tmem + lanes + Cfg::kPCol + x * 64 : s_addr;
+      // a score's factor is never 0: times -inf, which stands where the row does not look, that would be NaN
+      auto factor = [&](float k_scale) { return fminf(fmaxf(f * k_scale, 1.2e-38f), 3.4e38f); };
+      float R = -INFINITY, l = 0.f;
+      uint32_t nan_cols[HD / 32];
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) nan_cols[i] = 0u;
+      // Rare: NaN where this row has seen a value that is NaN.
+      auto poison = [&](auto put) {
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) {
+#pragma unroll 1
+          for (uint32_t bits = nan_cols[i]; bits; bits &= bits - 1) put(i * 32 + __ffs(bits) - 1);
+        }
+      };
+      // Of a step whose values are all there. Rare: which columns of the values that this row sees are NaN.
+      auto nan_values = [&](int step) {
+        if (sh.v_nan[step % kPfRing] != step + 1) return;
+        const int kbase = (c0 + step - gs) * kPfKeys;
+      // rare: which columns of the values that this row sees are NaN
+        const int* pages = a.block_table + (size_t)w.page_row * a.max_pages;
+        const int last_key = w.last_key;
+#pragma unroll 1
         for (int p = max(lo, kbase); p <= min(min(qpos, last_key), kbase + kPfKeys - 1); ++p) {
           const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD);
 #pragma unroll
@@ -517,185 +515,426 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
             nan_cols[i] |= bits;
           }
         }
-      }
-    }
-    if (ok && n_x > 0) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&sh.pv_done[x], (n_x - 1) & 1, abort))) {
-        LLMIE_FAIL(kStatusTimeoutMma);
-        ok = false;
-      }
-      tc_fence_after_sync();
-    }
-    if (TURNS) {
-      // B hands its results to A through the place of the keys, which nobody reads any more once both tiles' products are done
-      float* handed = reinterpret_cast<float*>(k_smem) + r * HD;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (x == 1) {
+      };
+#pragma unroll 1
+      for (int j = 0; j < n_x; ++j) {            // this tile's j-th step is the block's `step`
+        const int step = gs + (TURNS ? 2 * j + x : j);
+        // every decision to give up is taken by the whole warp: reads of tensor memory are warp-wide instructions
+        if (!__all_sync(0xffffffffu, pf_wait(&sh.x_full[step % kPfRing], (step / kPfRing) & 1, abort) && pf_wait(&sh.s_full[x], (gx + j) & 1, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const int kbase = (c0 + step - gs) * kPfKeys, ring = step % kPfRing;
+        const bool edge = kbase + kPfKeys - 1 > all_to || kbase < all_from;
+        // the row's scores; those that it does not see are -inf
+        uint32_t v[4][32];
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t y[32];
-          if (ok && n_x > 0) {
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, v[c]);
+        float fk[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) fk[b] = factor(sh.k_scale[ring][b]);
+        tmem_ld_wait();
+        if (Cfg::kOwnP) {
+          // they are in registers: the next scores may be written
+          tc_fence_before_sync();
+          mbar_arrive(&sh.s_free[x]);
+        }
+        if (edge) {
+          const int from = lo - kbase;
+          const unsigned span = (unsigned)(qpos - lo);
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if ((unsigned)(i - from) > span) v[i >> 5][i & 31] = 0xff800000u;
+        }
+        float mx = -INFINITY;          // the largest s + ev
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const uint32_t* y = v[b >> 1] + (b & 1) * 16;
+          float m0 = __uint_as_float(y[0]), m1 = __uint_as_float(y[1]);
+#pragma unroll
+          for (int i = 2; i < 14; i += 4) {
+            m0 = pf_max3(m0, __uint_as_float(y[i]), __uint_as_float(y[i + 1]));
+            m1 = pf_max3(m1, __uint_as_float(y[i + 2]), __uint_as_float(y[i + 3]));
+          }
+          m0 = pf_max3(m0, __uint_as_float(y[14]), __uint_as_float(y[15]));
+          mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fk[b], sh.v_add[ring][b]));
+        }
+        const bool grow = mx > R + kPfSlack || R == -INFINITY;
+        if (__any_sync(0xffffffffu, grow && j > 0)) {
+          // the sums so far are brought to the new bound (rows that keep theirs: times 1)
+          if (!__all_sync(0xffffffffu, pf_wait(&sh.pv_done[x], (gx + j - 1) & 1, abort))) {
+            LLMIE_FAIL(kStatusTimeoutMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const float alpha = !grow ? 1.f : R == -INFINITY ? 0.f : pf_exp2(R - mx);
+          l *= alpha;
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t y[16];
+            tmem_ld_32x16(o_addr + c * 16, y);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * alpha);
+            pf_tmem_st16(o_addr + c * 16, y);
+          }
+          tmem_st_wait();
+        }
+        if (grow) R = mx;
+        const float shift = (R == -INFINITY ? 0.f : R) - kPfTop;
+        if (!Cfg::kOwnP && j > 0) nan_values(step - (TURNS ? 2 : 1));          // its product was done before these scores were begun
+        if (Cfg::kOwnP && j > 0) {
+          // the weights of the tile before have to be through the product before they are written over
+          if (!__all_sync(0xffffffffu, pf_wait(&sh.pv_done[x], (gx + j - 1) & 1, abort))) {
+            LLMIE_FAIL(kStatusTimeoutMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          nan_values(step - (TURNS ? 2 : 1));
+        }
+        // the weights, over the scores they come from or in columns of their own
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[16];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const float add = sh.v_add[ring][c * 2 + b] - shift;
+            const uint32_t* y = v[c] + b * 16;
+            float sum[4];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float x0 = pf_exp2(fmaf(__uint_as_float(y[i]), fk[c * 2 + b], add));
+              const float x1 = pf_exp2(fmaf(__uint_as_float(y[i + 1]), fk[c * 2 + b], add));
+              sum[i & 2] = i < 4 ? x0 : sum[i & 2] + x0;
+              sum[(i & 2) + 1] = i < 4 ? x1 : sum[(i & 2) + 1] + x1;
+              o[b * 8 + i / 2] = pf_half2(x0, x1);
+            }
+            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), sh.v_back[ring][c * 2 + b], l);
+          }
+          pf_tmem_st16(p_addr + c * 16, o);
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(&sh.p_ready[x]);
+      }
+      // the queries of the piece after this one are asked for while the last product runs
+      const int at_end = gs + (TURNS ? 2 * (n_x - 1) + x : n_x - 1);             // this tile's last step
+      gx += n_x;
+      const bool early = ok && __all_sync(0xffffffffu, mbar_test(&sh.work_full[(n + 1) % kPfAhead], ((n + 1) / kPfAhead) & 1));
+      const bool merge = TURNS && w.parts == 1;      // then the place of the queries is wanted first
+      if (early && !merge && sh.work[(n + 1) % kPfAhead].parts > 0) ask_for_queries(sh.work[(n + 1) % kPfAhead]);
+      if (ok && n_x > 0) {
+        if (!__all_sync(0xffffffffu, pf_wait(&sh.pv_done[x], (gx - 1) & 1, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          ok = false;
+        }
+        tc_fence_after_sync();
+        if (ok) nan_values(at_end);
+      }
+      gs += w.n_steps;
+      if (merge) {
+        // B hands its results to A through the place of the queries, which nobody reads any more once both tiles' scores are done
+        // (partial ones are joined later, B's with A's)
+        float* handed = reinterpret_cast<float*>(q_smem) + r * HD;
+        if (x == 0) mbar_arrive(&sh.a_scored);
+        if (!__all_sync(0xffffffffu, x == 0 || pf_wait(&sh.a_scored, turns & 1, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          ok = false;
+        }
+        if (x == 1) {
+#pragma unroll 1
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t y[32];
             tmem_ld_32x32(o_addr + c * 32, y);
             tmem_ld_wait();
-          } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = 0u;
+            for (int i = 0; i < 32; i += 4)            // places of a row shifted by the row: other banks for other rows
+              *reinterpret_cast<uint4*>(handed + (c * 32 + i + r * 4) % HD) =
+                  n_x > 0 ? make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]) : make_uint4(0u, 0u, 0u, 0u);
           }
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {          // places of a row shifted by the row: other banks for other rows
-            float4 z;
-            z.x = (nan_cols[c] >> i & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i]);
-            z.y = (nan_cols[c] >> (i + 1) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + 1]);
-            z.z = (nan_cols[c] >> (i + 2) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + 2]);
-            z.w = (nan_cols[c] >> (i + 3) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + 3]);
-            *reinterpret_cast<float4*>(handed + (c * 32 + i + r * 4) % HD) = z;
-          }
+          poison([&](int d) { handed[(d + r * 4) % HD] = __int_as_float(0x7fffffff); });
+          sh.handed[0][r] = R;
+          sh.handed[1][r] = l;
+          mbar_arrive(&sh.b_handed);
         }
-        sh.handed[0][r] = R;
-        sh.handed[1][r] = l;
+        if (!__all_sync(0xffffffffu, x == 1 || pf_wait(&sh.b_handed, turns & 1, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          ok = false;
+        }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-    }
-    // ---- the row's result: the output, or a partial one. Where a wait gave up: NaN.
-    if (!TURNS || x == 0) {
-      float mine_f = 1.f, b_f = 0.f;
-      if (TURNS) {
-        const float Rb = sh.handed[0][r], M = fmaxf(R, Rb), Mu = M == -INFINITY ? 0.f : M;
-        mine_f = R == -INFINITY ? 0.f : pf_exp2(R - Mu);
-        b_f = Rb == -INFINITY ? 0.f : pf_exp2(Rb - Mu);
-        l = fmaf(l, mine_f, sh.handed[1][r] * b_f);
-        R = M;
-      }
-      const float* handed = reinterpret_cast<const float*>(k_smem) + r * HD;
-      float* rec = a.part + (size_t)w.slot * Cfg::kRecord;
-      const int pr = x * kPfRows + r;
-      if (w.parts > 1 && there) {
-        rec[2 * kPfRows * HD + pr] = R;
-        rec[2 * kPfRows * (HD + 1) + pr] = ok ? l : __int_as_float(0x7fffffff);
-      }
-      const float inv = 1.f / l;
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t y[32];
-        if (ok && n_x > 0) {
+      // ---- the row's result: the output, or a partial one. Where a wait gave up: NaN.
+      if (!merge || x == 0) {
+        float mine_f = 1.f, b_f = 0.f;
+        if (merge) {
+          const float Rb = sh.handed[0][r], M = fmaxf(R, Rb), Mu = M == -INFINITY ? 0.f : M;
+          mine_f = R == -INFINITY ? 0.f : pf_exp2(R - Mu);
+          b_f = Rb == -INFINITY ? 0.f : pf_exp2(Rb - Mu);
+          l = fmaf(l, mine_f, sh.handed[1][r] * b_f);
+        }
+        if (!ok) l = __int_as_float(0x7fffffff);
+        const float* handed = reinterpret_cast<const float*>(q_smem) + r * HD;
+        const int row = row_of(w);
+        const bool cut = w.parts > 1;
+        float* rec = a.part + (size_t)w.slot * Cfg::kRecord + (x * kPfRows + r) * 4;
+        if (cut && row >= 0) {
+          rec[2 * kPfRows * HD - (x * kPfRows + r) * 3] = R;
+          rec[2 * kPfRows * (HD + 1) - (x * kPfRows + r) * 3] = l;
+        }
+        const float by = cut ? 1.f : mine_f / l, b_by = b_f / l;
+        // 32 columns at a time: partial ones lie row beside row, four columns a piece; the output's are turned in shared memory, so that
+        // neighbouring lanes write a row's
+        const uint32_t turn = smem_u32(out_smem) + warp * 2048;
+#pragma unroll 1
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t y[32];
           tmem_ld_32x32(o_addr + c * 32, y);
           tmem_ld_wait();
-        } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = 0u;
-        }
-        if (there) {                   // (reads of tensor memory are warp-wide: only what follows them goes by the row)
+          for (int i = 0; i < 32; ++i) y[i] = n_x > 0 ? __float_as_uint(__uint_as_float(y[i]) * by) : 0u;
+          if (merge) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            float v8[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              v8[e] = (nan_cols[c] >> (i + e) & 1u) || !ok ? __int_as_float(0x7fffffff) : __uint_as_float(y[i + e]);
-            if (TURNS) {
-#pragma unroll
-              for (int e = 0; e < 8; e += 4) {
-                const float4 z = *reinterpret_cast<const float4*>(handed + (c * 32 + i + e + r * 4) % HD);
-                v8[e] = fmaf(v8[e], mine_f, z.x * b_f);
-                v8[e + 1] = fmaf(v8[e + 1], mine_f, z.y * b_f);
-                v8[e + 2] = fmaf(v8[e + 2], mine_f, z.z * b_f);
-                v8[e + 3] = fmaf(v8[e + 3], mine_f, z.w * b_f);
-              }
-            }
-            if (w.parts > 1) {
-              store8(rec + (size_t)pr * HD + c * 32 + i, v8);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v8[e] *= inv;
-              store8(a.out + row_off + c * 32 + i, v8);
+            for (int i = 0; i < 32; i += 4) {
+              const float4 z = *reinterpret_cast<const float4*>(handed + (c * 32 + i + r * 4) % HD);
+              y[i] = __float_as_uint(fmaf(z.x, b_by, __uint_as_float(y[i])));
+              y[i + 1] = __float_as_uint(fmaf(z.y, b_by, __uint_as_float(y[i + 1])));
+              y[i + 2] = __float_as_uint(fmaf(z.z, b_by, __uint_as_float(y[i + 2])));
+              y[i + 3] = __float_as_uint(fmaf(z.w, b_by, __uint_as_float(y[i + 3])));
             }
           }
+          if (cut) {
+            if (row >= 0) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 4)
+                *reinterpret_cast<uint4*>(rec + (size_t)(c * 8 + i / 4) * 8 * kPfRows) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t o[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1]));
+                o[e] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                           ::"r"(turn + lane * 64 + ((i / 8) ^ (lane >> 1 & 3)) * 16), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int of = i * 8 + lane / 4, to = __shfl_sync(0xffffffffu, row, of);
+              uint4 z;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
+                           : "r"(turn + of * 64 + ((lane & 3) ^ (of >> 1 & 3)) * 16) : "memory");
+              if (to >= 0) *reinterpret_cast<uint4*>(a.out + (size_t)to * HD + c * 32 + (lane & 3) * 8) = z;
+            }
+            __syncwarp();
+          }
         }
+        // columns of values that are NaN, or, where B handed them over, were (then they are so already)
+        if (row >= 0 && cut) poison([&](int d) { rec[(size_t)(d / 4) * 8 * kPfRows + d % 4] = __int_as_float(0x7fffffff); });
+        if (row >= 0 && !cut) poison([&](int d) { a.out[(size_t)row * HD + d] = __float2bfloat16_rn(__int_as_float(0x7fffffff)); });
       }
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.work_empty[n % kPfAhead]);
+      more = ok && __all_sync(0xffffffffu, piece_there(n + 1));
+      if (merge) {
+        // the place is the queries' again when all of A's rows have been read
+        if (x == 0) mbar_arrive(&sh.a_read);
+        if (more && !__all_sync(0xffffffffu, pf_wait(&sh.a_read, turns & 1, abort))) {
+          LLMIE_FAIL(kStatusTimeoutMma);
+          ok = false;
+        }
+        ++turns;
+      }
+      if (more && (!early || merge)) ask_for_queries(sh.work[(n + 1) % kPfAhead]);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");         // nothing in flight at the end, where a wait gave up either
   } else if (warp < 12) {
     // ------------------------------------------------------------------ conversion: 128 threads, 16 codes at a time
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kConvert));
-    auto put = [&](uint8_t* dst, const uint4 (&reg)[kPer]) {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int row = row0 + i * kStep;
-        const unsigned c[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[2 * e] = e4m3x2_to_half2((unsigned short)(c[e] & 0xffffu));
-          h[2 * e + 1] = e4m3x2_to_half2((unsigned short)(c[e] >> 16));
-        }
-        uint8_t* at = dst + (piece >> 2) * kPfSub;
-        const int ch = (piece & 3) * 2, odd = piece >> 2 & 1;          // the two 64-column halves of a row in turn: other banks
-        const uint4 lo4 = make_uint4(h[0], h[1], h[2], h[3]), hi4 = make_uint4(h[4], h[5], h[6], h[7]);
-        *reinterpret_cast<uint4*>(at + swizzle128_offset(row, ch + odd)) = odd ? hi4 : lo4;
-        *reinterpret_cast<uint4*>(at + swizzle128_offset(row, ch + 1 - odd)) = odd ? lo4 : hi4;
+    constexpr int kPer = HD / 16;                            // pieces of 16 codes a row, and pieces that a thread has
+    constexpr int kStep = 128 / kPer;                        // its rows: row0, row0 + kStep, ...
+    const int ct = threadIdx.x & 127, piece = ct % kPer, row0 = ct / kPer;
+    uint4 reg[kPer];                 // codes asked for half a step ahead: keys' and values' in turn
+    // Everything is asked for before it is looked at: a tile's pages a step before its codes, its codes and exponents half a step
+    // before they are written out. (Where an exponent was clamped, or a page's address made, as soon as it was asked for, the
+    // conversion waited for memory twice a tile, and the whole kernel for the conversion: 3,500 clocks a step. Codes asked for a whole
+    // step ahead, keys and values side by side, are 64 registers a thread at head size 128, and left too few.)
+    int pg0 = 0, pg1 = 0;            // pages of the tile to be asked for next
+    signed char ke = 0, ve = 0;      // a thread's two exponents
+    int last_key = 0, hk = 0;
+    const int* pages = nullptr;
+    auto page_at = [&](int lp) { return lp * kFp8Page <= last_key ? pages[lp] : 0; };
+    // piece i of a tile's keys, or values. Rows behind the block's last key: zeros, nothing that may be NaN.
+    auto load = [&](int i, const unsigned char* at0, const unsigned char* at1, int first) {
+      reg[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (first + i * kStep <= last_key) reg[i] = *reinterpret_cast<const uint4*>((i < kPer / 2 ? at0 + i * kStep * HD : at1 + (i - kPer / 2) * kStep * HD));
+    };
+    // where this thread's pieces of a page begin
+    auto in_page = [&](int page) { return (((size_t)page * a.n_kv + hk) * kFp8Page + row0) * HD + piece * 16; };
+    // Exponents of the tile's eight blocks, a thread a block (one behind the last key: anything, nobody sees its scores).
+    auto load_exps = [&]() {
+      if (ct < 8) {
+        const size_t at = ((size_t)(ct < 4 ? pg0 : pg1) * a.n_kv + hk) * kPageExps + (ct & 3);
+        ke = a.k_exp[at];
+        ve = a.v_exp[at];
       }
     };
-    for (int j = 0; j < n_steps; ++j) {
-      const int st = j & 1, ring = j % kPfRing;
-      const int next0 = page_at((c0 + j + 2) * 2), next1 = page_at((c0 + j + 2) * 2 + 1);
-      if (j >= 2 && !mbar_wait(&sh.k_empty[st], ((j >> 1) - 1) & 1, abort)) {
-        LLMIE_FAIL(kStatusTimeoutEmpty);
-        break;
-      }
-      if (ct < 8) {
-        const int k = clamp_exponent(ke), v = clamp_exponent(ve);
-        sh.k_scale[ring][ct] = pow2_of(k);
-        sh.v_add[ring][ct] = (float)v;
-        sh.v_back[ring][ct] = pow2_of(-v);
-      }
-      // NaN among the values: such codes become zeros here
-      unsigned any = 0u;
+    auto put = [&](uint8_t* dst, int i) {
+      const int row = row0 + i * kStep;
+      const unsigned c[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
+      uint32_t h[8];
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        any |= ((vr[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((vr[i].y & 0x7f7f7f7fu) + 0x01010101u) |
-               ((vr[i].z & 0x7f7f7f7fu) + 0x01010101u) | ((vr[i].w & 0x7f7f7f7fu) + 0x01010101u);
-      put(k_smem + st * Cfg::kKvBytes, kr);
-      if (j + 1 < n_steps) {
-        load(kr, a.k, c0 + j + 1);
+      for (int e = 0; e < 4; ++e) {
+        h[2 * e] = e4m3x2_to_half2((unsigned short)(c[e] & 0xffffu));
+        h[2 * e + 1] = e4m3x2_to_half2((unsigned short)(c[e] >> 16));
+      }
+      uint8_t* at = dst + (piece >> 2) * kPfSub;
+      const int ch = (piece & 3) * 2, odd = piece >> 2 & 1;            // the two 64-column halves of a row in turn: other banks
+      const uint4 lo4 = make_uint4(h[0], h[1], h[2], h[3]), hi4 = make_uint4(h[4], h[5], h[6], h[7]);
+      *reinterpret_cast<uint4*>(at + swizzle128_offset(row, ch + odd)) = odd ? hi4 : lo4;
+      *reinterpret_cast<uint4*>(at + swizzle128_offset(row, ch + 1 - odd)) = odd ? lo4 : hi4;
+    };
+    int gs = 0;                      // steps so far
+    bool ok = true;
+#pragma unroll 1
+    for (int n = 0; ok && __all_sync(0xffffffffu, piece_there(n)); ++n) {
+      const PfPiece& w = sh.work[n % kPfAhead];
+      const int n_steps = w.n_steps, c0 = w.c0;
+      last_key = w.last_key;
+      hk = w.hk;
+      pages = a.block_table + (size_t)w.page_row * a.max_pages;
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.work_empty[n % kPfAhead]);
+      if (n_steps > 0) {
+        pg0 = page_at(c0 * 2);
+        pg1 = page_at(c0 * 2 + 1);
+        const unsigned char *at0 = a.k + in_page(pg0), *at1 = a.k + in_page(pg1);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) load(i, at0, at1, c0 * kPfKeys + row0);
         load_exps();
+      } else if (ct == 0) {
+        mbar_arrive(&sh.want);
       }
-      fence_proxy_async_smem();
-      if (any & 0x80808080u) {
-        sh.v_nan[ring] = j + 1;
+#pragma unroll 1
+      for (int j = 0; j < n_steps; ++j, ++gs) {
+        const int st = gs & 1, ring = gs % kPfRing;
+        if (ct == 0 && j == max(n_steps - 2, 0)) mbar_arrive(&sh.want);
+        // this step's pages are pg0, pg1; the next one's:
+        const int next0 = page_at((c0 + j + 1) * 2), next1 = page_at((c0 + j + 1) * 2 + 1);
+        if (gs >= 2 && !pf_wait(&sh.k_empty[st], ((gs >> 1) - 1) & 1, abort)) {
+          LLMIE_FAIL(kStatusTimeoutEmpty);
+          ok = false;
+          break;
+        }
+        if (ct < 8) {
+          const int k = clamp_exponent(ke), v = clamp_exponent(ve);
+          sh.k_scale[ring][ct] = pow2_of(k);
+          sh.v_add[ring][ct] = (float)v;
+          sh.v_back[ring][ct] = pow2_of(-v);
+        }
+        const int first = (c0 + j) * kPfKeys + row0;
+        {
+          const unsigned char *at0 = a.v + in_page(pg0), *at1 = a.v + in_page(pg1);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          unsigned* c = reinterpret_cast<unsigned*>(&vr[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned bad = ((c[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-            c[e] &= ~(bad | (bad - (bad >> 7)));             // the whole byte
+          for (int i = 0; i < kPer; ++i) {
+            put(k_smem + st * Cfg::kKvBytes, i);
+            load(i, at0, at1, first);
           }
         }
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.x_full[ring]);
+        mbar_arrive(&sh.k_full[st]);
+        if (gs >= 2 && !pf_wait(&sh.v_empty[st], ((gs >> 1) - 1) & 1, abort)) {
+          LLMIE_FAIL(kStatusTimeoutEmpty);
+          ok = false;
+          break;
+        }
+        // NaN among the values: such codes become zeros here
+        unsigned any = 0u;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          any |= ((reg[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((reg[i].y & 0x7f7f7f7fu) + 0x01010101u) |
+                 ((reg[i].z & 0x7f7f7f7fu) + 0x01010101u) | ((reg[i].w & 0x7f7f7f7fu) + 0x01010101u);
+        if (any & 0x80808080u) {
+          sh.v_nan[ring] = gs + 1;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            unsigned* c = reinterpret_cast<unsigned*>(&reg[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const unsigned bad = ((c[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+              c[e] &= ~(bad | (bad - (bad >> 7)));             // the whole byte
+            }
+          }
+        }
+        pg0 = next0;
+        pg1 = next1;
+        {
+          const int ahead = j + 1 < n_steps ? first + kPfKeys : 0x40000000;      // no tile after the last one
+          const unsigned char *at0 = a.k + in_page(pg0), *at1 = a.k + in_page(pg1);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            put(v_smem + st * Cfg::kKvBytes, i);
+            load(i, at0, at1, ahead);
+          }
+        }
+        if (j + 1 < n_steps) load_exps();
+        fence_proxy_async_smem();
+        mbar_arrive(&sh.v_full[st]);
       }
-      mbar_arrive(&sh.x_full[ring]);
-      mbar_arrive(&sh.k_full[st]);
-      if (j >= 2 && !mbar_wait(&sh.v_empty[st], ((j >> 1) - 1) & 1, abort)) {
-        LLMIE_FAIL(kStatusTimeoutEmpty);
-        break;
-      }
-      put(v_smem + st * Cfg::kKvBytes, vr);
-      if (j + 1 < n_steps) load(vr, a.v, c0 + j + 1);
-      pg0 = next0;
-      pg1 = next1;
-      fence_proxy_async_smem();
-      mbar_arrive(&sh.v_full[st]);
     }
   } else {
     // ------------------------------------------------------------------ the tensor core: a thread a tile, so that neither waits for the other's
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kIssue));
+    if (warp == 12) {
+      tmem_alloc(&sh.tmem_base, 512);
+      tmem_relinquish();
+      tc_fence_before_sync();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.tmem_ready);
+    }
+    if (warp == 14) {
+      // ---------------------------------------------------------------- more work: asked for when the block has two steps left, so that
+      // who is done first goes on with what is left
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.work_full[0]);
+      bool others = true;
+#pragma unroll 1
+      for (int n = 1, asked = 0; others; ++n) {
+        if (!__all_sync(0xffffffffu, pf_wait(&sh.want, (n - 1) & 1, abort))) break;
+        int index;
+        PfWork w{0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 1
+        do {                         // (there are more blocks than pieces: nobody has to begin those behind the last piece)
+          others = pf_another(sh, asked++, index, abort);
+          if (others) w = pf_find<false>(a, tok, index, mine, run);
+        } while (others && w.parts == 0);
+        if (n >= kPfAhead && !__all_sync(0xffffffffu, pf_wait(&sh.work_empty[n % kPfAhead], (n / kPfAhead - 1) & 1, abort))) break;
+        if ((threadIdx.x & 31) == 0) {
+          sh.work[n % kPfAhead] = pf_piece<TURNS>(a, w, tok_x);
+          mbar_arrive(&sh.work_full[n % kPfAhead]);
+        }
+      }
+    }
     if (warp < 14 && elect_one()) {
       constexpr uint32_t idesc_s = pf_instr_desc(kPfRows, kPfKeys, 0), idesc_o = pf_instr_desc(kPfRows, HD, 1);
-      const int tx = warp - 12, n_x = tx ? n_b : n_a;
+      const int tx = warp - 12;
+      bool ok = pf_wait(&sh.tmem_ready, 0, abort);
+      if (!ok) LLMIE_FAIL(kStatusTimeoutMma);
+      tc_fence_after_sync();
+      const uint32_t tmem = sh.tmem_base;
+      int gs = 0, gx = 0;            // steps of the block, and of this tile, before this piece
       const uint32_t s_col = tmem + Cfg::kSCol + tx * 128, o_col = tmem + Cfg::kOCol + tx * (HD == 64 ? 64 : 128);
       const uint32_t p_col = Cfg::kOwnP ? tmem + Cfg::kPCol + tx * 64 : s_col;
       // descriptors of the operands' first 16 columns; the rest lie a fixed number of 16-byte units on
       const uint64_t q_desc = make_smem_desc(smem_u32(q_smem + tx * Cfg::kQBytes), 16, 1024);
       const uint64_t k_desc = make_smem_desc(smem_u32(k_smem), 16, 1024), v_desc = make_smem_desc(smem_u32(v_smem), kPfSub, 1024);
       auto wait_for = [&](uint64_t* bar, uint32_t parity, int code) {
-        if (mbar_wait(bar, parity, abort)) return true;
+        if (pf_wait(bar, parity, abort)) return true;
         LLMIE_FAIL(code);
         return false;
       };
@@ -705,7 +944,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         if (TURNS) mma_commit(bar);
       };
       auto scores = [&](int j) -> bool {                     // S = Q K^T of this tile's j-th step
-        const int step = TURNS ? 2 * j + tx : j;
+        const int step = gs + (TURNS ? 2 * j + tx : j);
         if (!wait_for(&sh.k_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull)) return false;
         tc_fence_after_sync();
         const uint64_t kd = k_desc + (uint64_t)((step & 1) * (Cfg::kKvBytes >> 4));
@@ -719,9 +958,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         return true;
       };
       auto sums = [&](int j) -> bool {                       // O (+)= W V of it
-        const int step = TURNS ? 2 * j + tx : j;
+        const int step = gs + (TURNS ? 2 * j + tx : j);
         if (!wait_for(&sh.v_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull)) return false;
-        if (!wait_for(&sh.p_ready[tx], j & 1, kStatusTimeoutMma)) return false;
+        if (!wait_for(&sh.p_ready[tx], (gx + j) & 1, kStatusTimeoutMma)) return false;
         tc_fence_after_sync();
         const uint64_t vd = v_desc + (uint64_t)((step & 1) * (Cfg::kKvBytes >> 4));
 #pragma unroll
@@ -731,23 +970,37 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         let_go(&sh.v_empty[step & 1]);
         return true;
       };
-      bool ok = n_x == 0 || scores(0);
-      for (int j = 0; ok && j < n_x; ++j) {
-        // where the weights have columns of their own, the next scores as soon as these are in registers; else they are written
-        // where these weights are read from
-        if (Cfg::kOwnP && j + 1 < n_x) ok = wait_for(&sh.s_free[tx], j & 1, kStatusTimeoutMma) && scores(j + 1);
-        ok = ok && sums(j);
-        if (!Cfg::kOwnP && ok && j + 1 < n_x) ok = wait_for(&sh.pv_done[tx], j & 1, kStatusTimeoutMma) && scores(j + 1);
-      }
-      // steps that are the other tile's alone
-      for (int j = n_x; ok && !TURNS && j < n_steps; ++j) {
-        ok = wait_for(&sh.k_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull);
-        if (ok) mbar_arrive(&sh.k_empty[j & 1]);
-        ok = ok && wait_for(&sh.v_full[j & 1], (j >> 1) & 1, kStatusTimeoutFull);
-        if (ok) mbar_arrive(&sh.v_empty[j & 1]);
+#pragma unroll 1
+      for (int n = 0; ok && piece_there(n); ++n) {
+        const int n_x = tx ? sh.work[n % kPfAhead].n_b : sh.work[n % kPfAhead].n_a, n_steps = sh.work[n % kPfAhead].n_steps;
+        mbar_arrive(&sh.work_empty[n % kPfAhead]);
+        // the softmax has done with the piece before, and the queries of this one are there
+        ok = wait_for(&sh.q_ready[tx], n & 1, kStatusTimeoutFull);
+        tc_fence_after_sync();
+        ok = ok && (n_x == 0 || scores(0));
+#pragma unroll 1
+        for (int j = 0; ok && j < n_x; ++j) {
+          // where the weights have columns of their own, the next scores as soon as these are in registers; else they are written
+          // where these weights are read from
+          if (Cfg::kOwnP && j + 1 < n_x) ok = wait_for(&sh.s_free[tx], (gx + j) & 1, kStatusTimeoutMma) && scores(j + 1);
+          ok = ok && sums(j);
+          if (!Cfg::kOwnP && ok && j + 1 < n_x) ok = wait_for(&sh.pv_done[tx], (gx + j) & 1, kStatusTimeoutMma) && scores(j + 1);
+        }
+        // steps that are the other tile's alone
+#pragma unroll 1
+        for (int j = n_x; ok && !TURNS && j < n_steps; ++j) {
+          const int step = gs + j;
+          ok = wait_for(&sh.k_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull);
+          if (ok) mbar_arrive(&sh.k_empty[step & 1]);
+          ok = ok && wait_for(&sh.v_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull);
+          if (ok) mbar_arrive(&sh.v_empty[step & 1]);
+        }
+        gs += n_steps;
+        gx += n_x;
       }
       // nothing may be in flight when the tensor memory is given back
       mma_commit(&sh.last[tx]);
+#pragma unroll 1
       for (unsigned spin = 0; spin < (1u << 20) && !mbar_test(&sh.last[tx], 0); ++spin) __nanosleep(32);
     }
   }
@@ -756,51 +1009,44 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   __syncthreads();
   if (warp == 12) {
     tc_fence_after_sync();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(sh.tmem_base, 512);
   }
 }
 
-// Joins the runs of the tiles that were cut. grid (tiles of tokens x key/value heads, 8): an eighth of a tile's rows a block, a warp a row.
+// Joins the runs of the tiles that were cut. grid (tiles of tokens x key/value heads, 8).
 constexpr int kPfJoinWarps = 8, kPfJoinSide = 8;
 template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 32) prefill_fp8_join_kernel(const PrefillArgs a) {
   pdl_launch_dependents();
   using Cfg = PfCfg<HD>;
-  const int lane = threadIdx.x & 31;
   const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = TURNS ? tok_x : 2 * tok_x;
-  const PfWork w = pf_find<true>(a, tok, blockIdx.x);
+  const PfSequence mine = pf_sequence(a, threadIdx.x & 31, tok);
+  const PfWork w = pf_find<true>(a, tok, blockIdx.x, mine, pf_run(a, tok, mine));
   // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait). Blocks with
   // nothing to join wait too: the kernel behind this one waits for this one alone, and reads what the one in front wrote.
   pdl_wait();
   if (w.parts <= 1) return;
+  // a thread four columns of a row, neighbouring threads neighbouring rows, as the results lie
+  constexpr int kRows = TURNS ? kPfRows : 2 * kPfRows, kHalves = TURNS ? 2 : 1;              // in turns, both halves of a result are of the same rows
+  const int results = w.parts * kHalves;
   const float* base = a.part + (size_t)w.slot * Cfg::kRecord;
-  for (int row = blockIdx.y * kPfJoinWarps + (threadIdx.x >> 5); row < 2 * kPfRows; row += kPfJoinSide * kPfJoinWarps) {
+  for (int it = blockIdx.y * blockDim.x + threadIdx.x; it < kRows * (HD / 4); it += gridDim.y * blockDim.x) {
+    const int row = it % kRows, group = it / kRows;
     const int x = row / kPfRows, rt = row % kPfRows / G, rh = row % kPfRows - rt * G, t = w.tile * tok + x * tok_x + rt;
     if (rt >= tok_x || t >= w.q_len) continue;
-    const float* rec = base + (size_t)row * HD + lane * (HD / 32);
-    float M = -INFINITY, den = 0.f, num[HD / 32];
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) num[i] = 0.f;
+    float M = -INFINITY, den = 0.f, num[4] = {0.f, 0.f, 0.f, 0.f};
     // eight runs at a time, all asked for at once
-    for (int p0 = 0; p0 < w.parts; p0 += 8) {
-      float m[8], l[8], v[8][HD / 32];
+    for (int p0 = 0; p0 < results; p0 += 8) {
+      float m[8], l[8];
+      float4 v[8];
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
-        const bool there = p0 + p < w.parts;
-        const float* r = base + (size_t)(p0 + p) * Cfg::kRecord;
-        m[p] = there ? __ldcg(r + 2 * kPfRows * HD + row) : -INFINITY;
-        l[p] = there ? __ldcg(r + 2 * kPfRows * (HD + 1) + row) : 0.f;
-        const float* c = rec + (size_t)(there ? p0 + p : 0) * Cfg::kRecord;
-        if (HD == 64) {
-          const float2 y = __ldcg(reinterpret_cast<const float2*>(c));
-          v[p][0] = y.x;
-          v[p][1] = y.y;
-        } else {
-          const float4 y = __ldcg(reinterpret_cast<const float4*>(c));
-          v[p][0] = y.x;
-          v[p][1] = y.y;
-          v[p][HD / 32 - 2] = y.z;
-          v[p][HD / 32 - 1] = y.w;
-        }
+        const bool there = p0 + p < results;
+        const int at = there ? p0 + p : 0;
+        const float* r = base + (size_t)(at / kHalves) * Cfg::kRecord;
+        const int in = at % kHalves * kPfRows + row;
+        m[p] = there ? __ldcg(r + 2 * kPfRows * HD + in) : -INFINITY;
+        l[p] = there ? __ldcg(r + 2 * kPfRows * (HD + 1) + in) : 0.f;
+        v[p] = there ? __ldcg(reinterpret_cast<const float4*>(r) + (size_t)group * 2 * kPfRows + in) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       float M8 = M;
 #pragma unroll
@@ -808,19 +1054,25 @@ template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 3
       const float Mu = M8 == -INFINITY ? 0.f : M8, back = M == -INFINITY ? 0.f : pf_exp2(M - Mu);
       den *= back;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) num[i] *= back;
+      for (int i = 0; i < 4; ++i) num[i] *= back;
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
         const float f = pf_exp2(m[p] - Mu);
         den = fmaf(f, l[p], den);
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) num[i] = p0 + p < w.parts ? fmaf(f, v[p][i], num[i]) : num[i];
+        num[0] = fmaf(f, v[p].x, num[0]);
+        num[1] = fmaf(f, v[p].y, num[1]);
+        num[2] = fmaf(f, v[p].z, num[2]);
+        num[3] = fmaf(f, v[p].w, num[3]);
       }
       M = M8;
     }
-    __nv_bfloat16* o = a.out + ((size_t)(w.q_begin + t) * a.n_q + w.hk * G + rh) * HD + lane * (HD / 32);
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) o[i] = __float2bfloat16_rn(num[i] / den);
+    const float inv = 1.f / den;
+    uint2 o;
+    __nv_bfloat162 h = __floats2bfloat162_rn(num[0] * inv, num[1] * inv);
+    o.x = *reinterpret_cast<const uint32_t*>(&h);
+    h = __floats2bfloat162_rn(num[2] * inv, num[3] * inv);
+    o.y = *reinterpret_cast<const uint32_t*>(&h);
+    *reinterpret_cast<uint2*>(a.out + ((size_t)(w.q_begin + t) * a.n_q + w.hk * G + rh) * HD + group * 4) = o;
   }
 }
 

@@ -1860,7 +1860,8 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     """Causal attention of runs of new tokens over a paged cache in 8 bits, on the tcgen05 tensor cores: q, out bfloat16
     [T, n_q hd] with the sequences packed (cu_q int32 [n + 1]), the cache as in rope_store_fp8 (it holds the step's keys and
     values already), seq_start int32 [n] the tokens each sequence held before this step, window as in attention_paged.
-    head_dim 64 or 128, scale > 0. A block whose waits run out leaves NaN in its rows, and check_tc_status raises."""
+    head_dim 64 or 128, scale > 0. max_q_len: no sequence brings more. Rows behind the last sequence stay as they are. Where a block's
+    waits run out, rows are left NaN or as they were, and check_tc_status raises."""
     name = "attention_prefill_fp8"
     _need_heads(name, n_q, n_kv)
     if not attention_prefill_fp8_supported(n_q, n_kv, head_dim, q.dtype):
