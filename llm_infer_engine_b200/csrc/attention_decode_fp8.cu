@@ -87,6 +87,7 @@ __device__ __forceinline__ void df_units(const DecodeArgs& a, int len, int& firs
 __device__ __forceinline__ int df_total(const DecodeArgs& a) {
   const int lane = threadIdx.x & 31;
   int t = 0;
+#pragma unroll 1
   for (int s = lane; s < a.n_seqs; s += 32) {
     int f, c;
     df_units(a, a.seq_kvlen[s], f, c);
@@ -168,6 +169,7 @@ __device__ __forceinline__ void df_append(const __nv_bfloat16* qkv_row, const De
       if (e > before) {
         const float f = lower_factor(before, e);
         unsigned* old = reinterpret_cast<unsigned*>(codes - (size_t)in * HD);
+#pragma unroll 1
         for (int i = lane; i < in * HD / 4; i += 32) old[i] = lower_codes(old[i], f);
       }
     }
@@ -533,8 +535,10 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
   const int end = min(cur + share, total);
   if (blockIdx.x == 0) {
     // sequences that hold nothing: zeros
+#pragma unroll 1
     for (int s = warp; s < a.n_seqs; s += kDfWarps)
       if (a.seq_kvlen[s] <= 0)
+#pragma unroll 1
         for (int i = lane; i < a.n_q * HD; i += 32) a.out[(size_t)s * a.n_q * HD + i] = __float2bfloat16_rn(0.f);
   }
   if (cur >= end) return;
@@ -543,6 +547,7 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
   int begin = 0;                     // where the sequence's units begin on the line
   {
     int before = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
       int f, c = 0;
       if (s0 + lane < a.n_seqs) df_units(a, a.seq_kvlen[s0 + lane], f, c);
@@ -563,6 +568,7 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
   }
+#pragma unroll 1
   while (cur < end) {
     const int len = min(a.seq_kvlen[seq], a.max_pages * kFp8Page);
     df_units(a, len, first, count);
@@ -578,6 +584,7 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
     __syncthreads();
     const bool starts = u_begin == 0, whole = starts && u_end == count;
     float* rec = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Cfg::kRecord;
+#pragma unroll 1
     for (int i = threadIdx.x; i < ng * HD; i += kDfThreads) {
       const int h = i / HD, d = i % HD;
       float M, num, den;
@@ -624,6 +631,7 @@ decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const Deco
   const int u_begin = count * blockIdx.x / gridDim.x, u_end = count * (blockIdx.x + 1) / gridDim.x;
   df_piece<HD, NH, ROPE>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
   __syncthreads();
+#pragma unroll 1
   for (int i = threadIdx.x; i < ng * HD; i += kDfThreads) {
     const int h = i / HD, d = i % HD;
     float M, num, den;
@@ -641,6 +649,7 @@ decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const Deco
   if (gridDim.x == 1) return;
   tc::cluster_sync_all();
   const uint32_t here = (uint32_t)__cvta_generic_to_shared(joined);
+#pragma unroll 1
   for (int i = blockIdx.x * kDfThreads + threadIdx.x; i < ng * HD; i += gridDim.x * kDfThreads) {
     const int h = i / HD;
     float m[8], n[8], l[8], M = -INFINITY;
@@ -683,6 +692,7 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int first, count;
   int all = 0, ahead = 0;
+#pragma unroll 1
   for (int s = lane; s < a.n_seqs; s += 32) {
     int f, c;
     df_units(a, a.seq_kvlen[s], f, c);
@@ -710,6 +720,7 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
   auto column = [](int d) { return (d % 8) * (HD / 8) + (d / 16) * 2 + (d / 8 & 1); };
   if (n <= 4) {
     // few of them (many sequences): a thread a column, everything asked for at once
+#pragma unroll 1
     for (int x = blockIdx.y * kDfSlices * HD + threadIdx.x; x < ng * HD; x += gridDim.y * kDfSlices * HD) {
       const int h = x / HD;
       float m[4], l[4], v[4], M = -INFINITY;
