@@ -20,8 +20,13 @@
 // too few of them for the GPU: how many runs a sequence's tiles are cut into is worked out on the device from the lengths that
 // are there. Runs leave partial results, which a second kernel joins in order. A block per piece is launched, and a block that is
 // about to be done takes over the piece of one that has not begun (cluster launch control): keys of the next piece are converted
-// while this one's last scores are worked on, its queries are brought while its last product runs. (6 sequences of 60 to 1,500 tokens,
-// head size 128, 376 pieces: 76.4 us with a block a piece, which spent 26,000 of 42,000 clocks on finding, bringing and writing.)
+// while this one's last scores are worked on, its queries are brought while its last product runs. (6 sequences of 60 to 1,500
+// tokens, head size 128, 376 pieces: 76.4 us with a block a piece, which spent 26,000 of 42,000 clocks on finding, bringing and
+// writing, 68.0 so.)
+//
+// What bounds it. A step of 128 rows twice and 128 keys is 32,768 exponentials, 2,050 clocks, and takes 4,100 at head size 64 (49 us
+// for a prompt of 2,048 tokens, 32 / 8 heads: 350 TFLOP/s of products) and about 5,000 at 128, where the conversion has 32,768 codes to
+// write. Between pieces some 9,000 clocks pass at head size 128 for results, queries and the first scores.
 //
 // Code. What a block does once is written in loops that stay loops, and each search for work is there once: a kernel of 140 to 250 KB
 // of instructions, as the compiler lays them out by itself, spends thousands of clocks a piece on fetching them.
@@ -37,15 +42,15 @@ namespace llmie {
 using namespace tc;
 
 constexpr int kPfRows = 128;         // rows of a tile
-constexpr int kPfKeys = 128;         // keys of a step
-constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B; 8-11: conversion; 12, 13: the products of A, of B; 14, 15: nothing
+constexpr int kPfThreads = 512;      // warps 0-3, 4-7: softmax of tiles A and B; 8-11: conversion; 12, 13: the products of A, of B; 14: work; 15: nothing
 constexpr int kPfSub = kPfRows * 128;        // bytes of 128 rows of 64 half-precision numbers
 constexpr int kPfSms = 148;
-constexpr int kPfRing = 8;
+constexpr int kPfRing = 16;
+constexpr int kPfStages = 4;         // at most
 constexpr int kPfAhead = 4;          // places for pieces of work
 constexpr int kPfReaders = 14;       // who reads one: eight softmax warps, four converting ones, two issuing threads
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
-constexpr int kPfLeast = 4;          // key tiles that a run has at least, on average
+constexpr int kPfLeast = 512;        // keys that a run has at least, on average
 constexpr int kPfSlots = 200;        // partial results at once (see pf_run)
 constexpr int kPfFew = 128;          // tiles of tokens that can always be cut into runs for which there are SMs (see pf_run)
 constexpr float kPfTop = 7.f;        // the bound's own weight is 2^7
@@ -54,21 +59,27 @@ constexpr float kPfSlack = 8.f;      // how far scores may outgrow the bound, in
 template <int HD> struct PfCfg {
   static constexpr int kSubs = HD / 64;
   static constexpr int kQBytes = kSubs * kPfSub;             // one tile of queries
-  static constexpr int kKvBytes = kSubs * kPfSub;            // 128 keys, or values
-  static constexpr int kStages = 2;
+  // Keys of a step. Where there is room for it in tensor memory, 128: 64 would be the same work with twice the waits (a prompt of 2,048
+  // tokens 53.4 us for 48.8). At head size 128 there is not, and with weights that lay over the scores, the next scores had to
+  // wait for this step's second product (pieces of 60 to 1,500 tokens 68.0 us with 128 keys, 60.5 with 64).
+  static constexpr int kKeys = HD == 64 ? 128 : 64;
+  static constexpr int kKvSub = kKeys * 128;
+  static constexpr int kKvBytes = kSubs * kKvSub;            // a step's keys, or values
+  static constexpr int kStages = 256 / kKeys;
+  static constexpr int kBlocks = kKeys / kExpBlock;          // of the cache, a step
   static constexpr int kOutBytes = 8 * 2048;                 // a warp turns 32 rows of 32 numbers at a time
   static constexpr int kSmem = 2 * kQBytes + 2 * kStages * kKvBytes + kOutBytes + 1024;
-  static constexpr bool kOwnP = HD == 64;                    // tensor memory has room for the weights beside the scores
-  static constexpr int kSCol = 0, kOCol = 256, kPCol = 384;  // columns: scores of A and B, sums of A and B, weights
+  // Columns of tensor memory: sums of A and B, scores of either, weights. There is room for the weights beside the scores, which lets
+  // a step's scores be made while the softmax works on the step before.
+  static constexpr int kOCol = 0, kSCol = 2 * HD, kPCol = kSCol + 2 * kKeys;
+  static_assert(kPCol + kKeys <= 512, "tensor memory has 512 columns");
   static constexpr int kRecord = 2 * kPfRows * (HD + 2);     // floats of a partial result: sums [HD / 4][rows][4], then bounds, then denominators
 };
 
-// Registers that a thread of a softmax, the conversion and the last warpgroup keeps of the 128 that it is launched with: a row's 128
-// scores stay in registers. (Head size 128, 184 + 96 or 200 + 64 for the softmax and the conversion: pieces of 60 to 1,500 tokens 73.7
-// or 68.2 us; where the tiles take turns, 24 sequences of 2 to 8 tokens, 56.2 or 60.4.)
-template <int HD, bool TURNS> struct PfRegs {
-  static constexpr int kSoftmax = HD == 64 ? 192 : TURNS ? 184 : 200, kConvert = HD == 64 ? 72 : TURNS ? 96 : 64,
-                       kIssue = HD == 64 ? 56 : 48;
+// Registers that a thread of a softmax, the conversion and the last warpgroup keeps of the 128 that it is launched with: a row's scores
+// of a step stay in registers.
+template <int HD> struct PfRegs {
+  static constexpr int kSoftmax = HD == 64 ? 192 : 152, kConvert = HD == 64 ? 72 : 120, kIssue = HD == 64 ? 56 : 88;
   static_assert(2 * kSoftmax + kConvert + kIssue == 4 * 128, "more than the block has would never be granted");
   static_assert(kSoftmax >= 128 && kConvert <= 128 && kIssue <= 128, "inc may only raise, dec only lower");
 };
@@ -140,15 +151,15 @@ __host__ __device__ constexpr uint32_t pf_instr_desc(int m, int n, int b_mn) {
 
 // ------------------------------------------------------------------------------------------ the cut of the work
 // Key tiles of a sequence's tile of tokens [t0, t0 + n): from `lo` on, `count` of them. None behind the table's last page.
-__device__ __forceinline__ void pf_tiles(const PrefillArgs& a, int start, int t0, int n, int& lo, int& count) {
-  lo = first_visible_key(start + t0, a.window) / kPfKeys;
-  count = max((min(start + t0 + n, a.max_pages * kFp8Page) - 1) / kPfKeys - lo + 1, 0);
+template <int KEYS> __device__ __forceinline__ void pf_tiles(const PrefillArgs& a, int start, int t0, int n, int& lo, int& count) {
+  lo = first_visible_key(start + t0, a.window) / KEYS;
+  count = max((min(start + t0 + n, a.max_pages * kFp8Page) - 1) / KEYS - lo + 1, 0);
 }
 // What a lane knows of its sequence: tiles of tokens, the key tiles of the first and the last of them.
 struct PfSequence {
   int q_begin, q_len, start, slot, tiles, first, last;
 };
-__device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, int tok) {
+template <int KEYS> __device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, int tok) {
   PfSequence q{0, 0, 0, 0, 0, 0, 0};
   if (s < a.n_seqs) {
     q.q_begin = a.cu_q[s];
@@ -158,47 +169,50 @@ __device__ __forceinline__ PfSequence pf_sequence(const PrefillArgs& a, int s, i
     q.tiles = (q.q_len + tok - 1) / tok;
     if (q.tiles > 0) {
       int lo;
-      pf_tiles(a, q.start, 0, min(tok, q.q_len), lo, q.first);
-      pf_tiles(a, q.start, (q.tiles - 1) * tok, q.q_len - (q.tiles - 1) * tok, lo, q.last);
+      pf_tiles<KEYS>(a, q.start, 0, min(tok, q.q_len), lo, q.first);
+      pf_tiles<KEYS>(a, q.start, (q.tiles - 1) * tok, q.q_len - (q.tiles - 1) * tok, lo, q.last);
     }
   }
   return q;
 }
-// Runs that each of a sequence's tiles of tokens is cut into: last / run, to the nearest.
-__device__ __forceinline__ int pf_runs(int last, int run) { return max(1, (last + run / 2) / run); }
-// Key tiles that a run has on average. With T the sum of (first + last) / 2 over all tiles of tokens and heads:
-// Where those are no more than the SMs: the least, from T / 148 on, with which every run finds an SM at once, since one that does
-// not costs a whole round (24 sequences of 2 to 8 tokens behind 300 to 6,000, 96 tiles: 67 us in 170 runs, 58 in 148). Where they
-// are more, or no such length is found: 2 T / 148, so that a sequence is cut only if one of its tiles alone would hold up the step.
-// How many runs come of it: a sequence that is cut has last >= 1.5 run, so at most 4/3 last / run runs, and at most last / run of
-// them more than tiles; and last <= first + last, whose sum is 2 T. With run >= 2 T / 148 all cut sequences have 4/3 148 < kPfSlots
-// runs, and 148 more than tiles. The search goes on to 16 T / 148, where there are 18 more than tiles: up to kPfFew it finds one.
+// Runs that each of a sequence's tiles of tokens is cut into, by pf_run's answer: none longer than it where all of them find an SM at
+// once (answers below 0), else last / run to the nearest.
+__device__ __forceinline__ int pf_runs(int last, int run) { return run < 0 ? max(1, (last - run - 1) / -run) : max(1, (last + run / 2) / run); }
+// How long runs are, in key tiles. With T the sum of (first + last) / 2 over all tiles of tokens and heads:
+// Where those are no more than the SMs: the least, from T / 148 on, with which every run finds an SM at once and none is longer
+// (answered below 0; 24 sequences of 2 to 8 tokens behind 300 to 6,000, 96 tiles: 52.4 us, and 55.0 where runs are last / run to the
+// nearest, half as long again at worst). Where they are more, or no such length is found: 2 T / 148, so that a sequence is cut only
+// if one of its tiles alone would hold up the step.
+// How many runs come of it: in the first case at most 148. In the second a sequence that is cut has last >= 1.5 run, so at most
+// 4/3 last / run runs, and at most last / run of them more than tiles; and last <= first + last, whose sum is 2 T. So all cut
+// sequences have 4/3 148 < kPfSlots runs, and 148 more than tiles. The search goes on to 16 T / 148, where there are 18 more than
+// tiles: up to kPfFew it finds one.
 // `mine`: the lane's first sequence. All lanes of a warp call it, and every block gets the same answer.
-__device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
+template <int KEYS> __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
   const int lane = threadIdx.x & 31;
   float twice = (float)mine.tiles * (float)(mine.first + mine.last);
   int tiles = mine.tiles;
 #pragma unroll 1
   for (int s = lane + 32; s < a.n_seqs; s += 32) {
-    const PfSequence q = pf_sequence(a, s, tok);
+    const PfSequence q = pf_sequence<KEYS>(a, s, tok);
     twice += (float)q.tiles * (float)(q.first + q.last);
     tiles += q.tiles;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
   const float share = twice * (float)a.n_kv / kPfSms;                        // 2 T / 148
-  const int most = max(a.run, max(kPfLeast, (int)fminf(ceilf(share), 1e9f)));
+  const int most = max(a.run, max(kPfLeast / KEYS, (int)fminf(ceilf(share), 1e9f)));
   if ((int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * a.n_kv > kPfSms) return most;
-  int run = max(a.run, max(kPfLeast, (int)fminf(ceilf(share * 0.5f), 1e9f)));
+  int run = max(a.run, max(kPfLeast / KEYS, (int)fminf(ceilf(share * 0.5f), 1e9f)));
 #pragma unroll 1
   for (int i = 0; i < 24; ++i, run += (run + 7) / 8) {                       // (9/8)^24 > 16
-    unsigned runs = mine.tiles * pf_runs(mine.last, run);
+    unsigned runs = mine.tiles * pf_runs(mine.last, -run);
 #pragma unroll 1
     for (int s = lane + 32; s < a.n_seqs; s += 32) {
-      const PfSequence q = pf_sequence(a, s, tok);
-      runs += q.tiles * pf_runs(q.last, run);
+      const PfSequence q = pf_sequence<KEYS>(a, s, tok);
+      runs += q.tiles * pf_runs(q.last, -run);
     }
-    if ((int)__reduce_add_sync(0xffffffffu, runs) * a.n_kv <= kPfSms) return run;
+    if ((int)__reduce_add_sync(0xffffffffu, runs) * a.n_kv <= kPfSms) return -run;
   }
   return most;
 }
@@ -209,14 +223,14 @@ struct PfWork {
 };
 // Piece `index` of the step's work, or (WHOLE) tile `index` with all its runs. All lanes of a warp call it. Late tiles of a
 // sequence, which see the most keys, come first, all heads of one after another. `mine`: the lane's first sequence; run: pf_run's.
-template <bool WHOLE>
+template <bool WHOLE, int KEYS>
 __device__ __forceinline__ PfWork pf_find(const PrefillArgs& a, int tok, int index, const PfSequence& mine, int run) {
   const int lane = threadIdx.x & 31;
   PfWork w{0, 0, 0, 0, 0, 0, 0, 0, 0};
   int before = 0, slots = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-    const PfSequence q = s0 == 0 ? mine : pf_sequence(a, s0 + lane, tok);
+    const PfSequence q = s0 == 0 ? mine : pf_sequence<KEYS>(a, s0 + lane, tok);
     const int parts = pf_runs(q.last, run);
     const int all = q.tiles * parts * a.n_kv, own = WHOLE ? q.tiles * a.n_kv : all, cut = parts > 1 ? all : 0;
     int incl = own, cuts = cut;
@@ -259,7 +273,7 @@ struct PfPiece {
   int c0, n_steps, n_a, n_b;         // its first key tile; its steps and those of either tile
   int last_key;
 };
-template <bool TURNS> __device__ __forceinline__ PfPiece pf_piece(const PrefillArgs& a, const PfWork& w, int tok_x) {
+template <bool TURNS, int KEYS> __device__ __forceinline__ PfPiece pf_piece(const PrefillArgs& a, const PfWork& w, int tok_x) {
   PfPiece p;
   const int tok = TURNS ? tok_x : 2 * tok_x, t0 = w.tile * tok, n_tok = min(tok, w.q_len - t0), parts = max(w.parts, 1);
   p.parts = w.parts;
@@ -269,7 +283,7 @@ template <bool TURNS> __device__ __forceinline__ PfPiece pf_piece(const PrefillA
   p.row0 = w.q_begin + t0;
   p.pos0 = w.start + t0;
   int lo_tile, tiles;
-  pf_tiles(a, w.start, t0, n_tok, lo_tile, tiles);
+  pf_tiles<KEYS>(a, w.start, t0, n_tok, lo_tile, tiles);
   // this run's key tiles: [c0, c1) of the tiles of the block's tokens
   p.c0 = lo_tile + tiles * w.part / parts;
   const int c1 = lo_tile + tiles * (w.part + 1) / parts;
@@ -278,22 +292,23 @@ template <bool TURNS> __device__ __forceinline__ PfPiece pf_piece(const PrefillA
   p.n_tok_a = min(n_tok, tok_x);
   p.n_tok_b = TURNS ? p.n_tok_a : n_tok - p.n_tok_a;
   p.n_steps = c1 - p.c0;
-  p.n_a = TURNS ? (p.n_steps + 1) / 2 : max(0, min(c1, (p.pos0 + p.n_tok_a - 1) / kPfKeys + 1) - p.c0);
+  p.n_a = TURNS ? (p.n_steps + 1) / 2 : max(0, min(c1, (p.pos0 + p.n_tok_a - 1) / KEYS + 1) - p.c0);
   p.n_b = TURNS ? p.n_steps / 2 : p.n_tok_b > 0 ? p.n_steps : 0;
   return p;
 }
 
 struct PfShared {
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], x_full[kPfRing];
+  uint64_t k_full[kPfStages], k_empty[kPfStages], v_full[kPfStages], v_empty[kPfStages], x_full[kPfRing];
   uint64_t s_full[2], s_free[2], p_ready[2], pv_done[2], q_ready[2], last[2];
   uint64_t a_scored, b_handed, a_read;             // where the tiles take turns
   uint64_t work_full[kPfAhead], work_empty[kPfAhead], want, answered, tmem_ready;
   uint32_t tmem_base;
   int abort;
-  // Of the key tiles in flight, by step % 8 (steps are counted through all the block's pieces): factors of scores, addends, factors of
+  // Of the key tiles in flight, by step % 16 (steps are counted through all the block's pieces): factors of scores, addends, factors of
   // the denominator's terms, and the step (+ 1) that last had NaN among its values. x_full: all of them are there. (A step's place is
-  // written again eight steps on. By then both tiles' scores of six steps on are done or not wanted, which were let begin behind the
-  // softmax's last look at this step; a piece's first, or its being let go, waits for the softmax to have done with the piece before.)
+  // written again sixteen steps on. The conversion is at most four steps ahead of what both tiles have scored or let go of; a tile
+  // lets steps go only behind its softmax's last step of a piece, three at most, and scores a piece's first step only when its
+  // softmax has done with the piece before.)
   float k_scale[kPfRing][8], v_add[kPfRing][8], v_back[kPfRing][8];
   int v_nan[kPfRing];
   float handed[2][kPfRows];          // where B has A's rows: its bounds and denominators
@@ -353,16 +368,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
   PfSequence mine;
   int run = 0;
   if (warp == 14) {
-    mine = pf_sequence(a, threadIdx.x & 31, tok);
-    run = pf_run(a, tok, mine);
-    const PfWork found = pf_find<false>(a, tok, blockIdx.x, mine, run);
-    if ((threadIdx.x & 31) == 0) sh.work[0] = pf_piece<TURNS>(a, found, tok_x);
+    mine = pf_sequence<Cfg::kKeys>(a, threadIdx.x & 31, tok);
+    run = pf_run<Cfg::kKeys>(a, tok, mine);
+    const PfWork found = pf_find<false, Cfg::kKeys>(a, tok, blockIdx.x, mine, run);
+    if ((threadIdx.x & 31) == 0) sh.work[0] = pf_piece<TURNS, Cfg::kKeys>(a, found, tok_x);
   } else if (threadIdx.x == 32) {
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < Cfg::kStages; ++s) {
       mbar_init(&sh.k_full[s], 128);
       mbar_init(&sh.k_empty[s], 2);
       mbar_init(&sh.v_full[s], 128);
       mbar_init(&sh.v_empty[s], 2);
+    }
+    for (int s = 0; s < 2; ++s) {
       mbar_init(&sh.s_full[s], 1);
       mbar_init(&sh.s_free[s], 128);
       mbar_init(&sh.p_ready[s], 128);
@@ -403,7 +420,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 
   if (warp < 8) {
     // ------------------------------------------------------------------ softmax: a thread a row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PfRegs<HD>::kSoftmax));
     const int x = warp >> 2, r = threadIdx.x & 127;          // tile and row
     const int rt = r / G, rh = r - rt * G;                   // token of the tile, query head of the group
     const int lane = threadIdx.x & 31;
@@ -481,8 +498,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         tc_fence_after_sync();
         tmem = sh.tmem_base;
       }
-      const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * 128, o_addr = tmem + lanes + Cfg::kOCol + x * (HD == 64 ? 64 : 128);
-      const uint32_t p_addr = Cfg::kOwnP ? tmem + lanes + Cfg::kPCol + x * 64 : s_addr;
+      const uint32_t s_addr = tmem + lanes + Cfg::kSCol + x * Cfg::kKeys, o_addr = tmem + lanes + Cfg::kOCol + x * HD;
+      const uint32_t p_addr = tmem + lanes + Cfg::kPCol + x * (Cfg::kKeys / 2);
       // a score's factor is never 0: times -inf, which stands where the row does not look, that would be NaN
       auto factor = [&](float k_scale) { return fminf(fmaxf(f * k_scale, 1.2e-38f), 3.4e38f); };
       float R = -INFINITY, l = 0.f;
@@ -500,12 +517,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       // Of a step whose values are all there. Rare: which columns of the values that this row sees are NaN.
       auto nan_values = [&](int step) {
         if (sh.v_nan[step % kPfRing] != step + 1) return;
-        const int kbase = (c0 + step - gs) * kPfKeys;
+        const int kbase = (c0 + step - gs) * Cfg::kKeys;
       // rare: which columns of the values that this row sees are NaN
         const int* pages = a.block_table + (size_t)w.page_row * a.max_pages;
         const int last_key = w.last_key;
 #pragma unroll 1
-        for (int p = max(lo, kbase); p <= min(min(qpos, last_key), kbase + kPfKeys - 1); ++p) {
+        for (int p = max(lo, kbase); p <= min(min(qpos, last_key), kbase + Cfg::kKeys - 1); ++p) {
           const unsigned* row = reinterpret_cast<const unsigned*>(a.v + (((size_t)pages[p / kFp8Page] * a.n_kv + w.hk) * kFp8Page + p % kFp8Page) * HD);
 #pragma unroll
           for (int i = 0; i < HD / 32; ++i) {
@@ -526,31 +543,29 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
           break;
         }
         tc_fence_after_sync();
-        const int kbase = (c0 + step - gs) * kPfKeys, ring = step % kPfRing;
-        const bool edge = kbase + kPfKeys - 1 > all_to || kbase < all_from;
+        const int kbase = (c0 + step - gs) * Cfg::kKeys, ring = step % kPfRing;
+        const bool edge = kbase + Cfg::kKeys - 1 > all_to || kbase < all_from;
         // the row's scores; those that it does not see are -inf
-        uint32_t v[4][32];
+        uint32_t v[Cfg::kKeys / 32][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32(s_addr + c * 32, v[c]);
-        float fk[8];
+        for (int c = 0; c < Cfg::kKeys / 32; ++c) tmem_ld_32x32(s_addr + c * 32, v[c]);
+        float fk[Cfg::kBlocks];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) fk[b] = factor(sh.k_scale[ring][b]);
+        for (int b = 0; b < Cfg::kBlocks; ++b) fk[b] = factor(sh.k_scale[ring][b]);
         tmem_ld_wait();
-        if (Cfg::kOwnP) {
-          // they are in registers: the next scores may be written
-          tc_fence_before_sync();
-          mbar_arrive(&sh.s_free[x]);
-        }
+        // they are in registers: the next scores may be written
+        tc_fence_before_sync();
+        mbar_arrive(&sh.s_free[x]);
         if (edge) {
           const int from = lo - kbase;
           const unsigned span = (unsigned)(qpos - lo);
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
+          for (int i = 0; i < Cfg::kKeys; ++i)
             if ((unsigned)(i - from) > span) v[i >> 5][i & 31] = 0xff800000u;
         }
         float mx = -INFINITY;          // the largest s + ev
 #pragma unroll
-        for (int b = 0; b < 8; ++b) {
+        for (int b = 0; b < Cfg::kBlocks; ++b) {
           const uint32_t* y = v[b >> 1] + (b & 1) * 16;
           float m0 = __uint_as_float(y[0]), m1 = __uint_as_float(y[1]);
 #pragma unroll
@@ -585,8 +600,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         }
         if (grow) R = mx;
         const float shift = (R == -INFINITY ? 0.f : R) - kPfTop;
-        if (!Cfg::kOwnP && j > 0) nan_values(step - (TURNS ? 2 : 1));          // its product was done before these scores were begun
-        if (Cfg::kOwnP && j > 0) {
+        if (j > 0) {
           // the weights of the tile before have to be through the product before they are written over
           if (!__all_sync(0xffffffffu, pf_wait(&sh.pv_done[x], (gx + j - 1) & 1, abort))) {
             LLMIE_FAIL(kStatusTimeoutMma);
@@ -596,9 +610,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
           tc_fence_after_sync();
           nan_values(step - (TURNS ? 2 : 1));
         }
-        // the weights, over the scores they come from or in columns of their own
+        // the weights, in columns of their own
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < Cfg::kKeys / 32; ++c) {
           uint32_t o[16];
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
@@ -756,45 +770,44 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
     asm volatile("cp.async.wait_all;" ::: "memory");         // nothing in flight at the end, where a wait gave up either
   } else if (warp < 12) {
     // ------------------------------------------------------------------ conversion: 128 threads, 16 codes at a time
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kConvert));
-    constexpr int kPer = HD / 16;                            // pieces of 16 codes a row, and pieces that a thread has
-    constexpr int kStep = 128 / kPer;                        // its rows: row0, row0 + kStep, ...
-    const int ct = threadIdx.x & 127, piece = ct % kPer, row0 = ct / kPer;
-    uint4 reg[kPer];                 // codes asked for half a step ahead: keys' and values' in turn
-    // Everything is asked for before it is looked at: a tile's pages a step before its codes, its codes and exponents half a step
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD>::kConvert));
+    constexpr int kPieces = HD / 16, kStep = 128 / kPieces;  // pieces of 16 codes a row; a thread's rows: row0, row0 + kStep, ...
+    constexpr int kPer = Cfg::kKeys / kStep, kPages = Cfg::kKeys / kFp8Page;
+    const int ct = threadIdx.x & 127, piece = ct % kPieces, row0 = ct / kPieces;
+    uint4 kr[kPer], vr[kPer];        // a step's codes
+    // Everything is asked for before it is looked at: a tile's pages a step before its codes, its codes and exponents a step
     // before they are written out. (Where an exponent was clamped, or a page's address made, as soon as it was asked for, the
-    // conversion waited for memory twice a tile, and the whole kernel for the conversion: 3,500 clocks a step. Codes asked for a whole
-    // step ahead, keys and values side by side, are 64 registers a thread at head size 128, and left too few.)
+    // conversion waited for memory twice a tile, and the whole kernel for the conversion: 3,500 clocks a step.)
     int pg0 = 0, pg1 = 0;            // pages of the tile to be asked for next
     signed char ke = 0, ve = 0;      // a thread's two exponents
     int last_key = 0, hk = 0;
     const int* pages = nullptr;
     auto page_at = [&](int lp) { return lp * kFp8Page <= last_key ? pages[lp] : 0; };
     // piece i of a tile's keys, or values. Rows behind the block's last key: zeros, nothing that may be NaN.
-    auto load = [&](int i, const unsigned char* at0, const unsigned char* at1, int first) {
-      reg[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (first + i * kStep <= last_key) reg[i] = *reinterpret_cast<const uint4*>((i < kPer / 2 ? at0 + i * kStep * HD : at1 + (i - kPer / 2) * kStep * HD));
+    auto load = [&](uint4& to, int i, const unsigned char* at0, const unsigned char* at1, int first) {
+      to = make_uint4(0u, 0u, 0u, 0u);
+      if (first + i * kStep <= last_key) to = *reinterpret_cast<const uint4*>((i * kStep < kFp8Page ? at0 + i * kStep * HD : at1 + (i * kStep - kFp8Page) * HD));
     };
     // where this thread's pieces of a page begin
     auto in_page = [&](int page) { return (((size_t)page * a.n_kv + hk) * kFp8Page + row0) * HD + piece * 16; };
     // Exponents of the tile's eight blocks, a thread a block (one behind the last key: anything, nobody sees its scores).
     auto load_exps = [&]() {
-      if (ct < 8) {
+      if (ct < Cfg::kBlocks) {
         const size_t at = ((size_t)(ct < 4 ? pg0 : pg1) * a.n_kv + hk) * kPageExps + (ct & 3);
         ke = a.k_exp[at];
         ve = a.v_exp[at];
       }
     };
-    auto put = [&](uint8_t* dst, int i) {
+    auto put = [&](uint8_t* dst, const uint4& from, int i) {
       const int row = row0 + i * kStep;
-      const unsigned c[4] = {reg[i].x, reg[i].y, reg[i].z, reg[i].w};
+      const unsigned c[4] = {from.x, from.y, from.z, from.w};
       uint32_t h[8];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         h[2 * e] = e4m3x2_to_half2((unsigned short)(c[e] & 0xffffu));
         h[2 * e + 1] = e4m3x2_to_half2((unsigned short)(c[e] >> 16));
       }
-      uint8_t* at = dst + (piece >> 2) * kPfSub;
+      uint8_t* at = dst + (piece >> 2) * Cfg::kKvSub;
       const int ch = (piece & 3) * 2, odd = piece >> 2 & 1;            // the two 64-column halves of a row in turn: other banks
       const uint4 lo4 = make_uint4(h[0], h[1], h[2], h[3]), hi4 = make_uint4(h[4], h[5], h[6], h[7]);
       *reinterpret_cast<uint4*>(at + swizzle128_offset(row, ch + odd)) = odd ? hi4 : lo4;
@@ -812,45 +825,49 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       __syncwarp();
       if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.work_empty[n % kPfAhead]);
       if (n_steps > 0) {
-        pg0 = page_at(c0 * 2);
-        pg1 = page_at(c0 * 2 + 1);
-        const unsigned char *at0 = a.k + in_page(pg0), *at1 = a.k + in_page(pg1);
+        pg0 = page_at(c0 * kPages);
+        if (kPages > 1) pg1 = page_at(c0 * kPages + 1);
+        const int next0 = page_at((c0 + 1) * kPages), next1 = kPages > 1 ? page_at((c0 + 1) * kPages + 1) : 0;
+        const size_t at0 = in_page(pg0), at1 = in_page(pg1);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) load(i, at0, at1, c0 * kPfKeys + row0);
+        for (int i = 0; i < kPer; ++i) load(kr[i], i, a.k + at0, a.k + at1, c0 * Cfg::kKeys + row0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) load(vr[i], i, a.v + at0, a.v + at1, c0 * Cfg::kKeys + row0);
         load_exps();
+        pg0 = next0;
+        pg1 = next1;
       } else if (ct == 0) {
         mbar_arrive(&sh.want);
       }
 #pragma unroll 1
       for (int j = 0; j < n_steps; ++j, ++gs) {
-        const int st = gs & 1, ring = gs % kPfRing;
+        const int st = gs % Cfg::kStages, ring = gs % kPfRing;
         if (ct == 0 && j == max(n_steps - 2, 0)) mbar_arrive(&sh.want);
-        // this step's pages are pg0, pg1; the next one's:
-        const int next0 = page_at((c0 + j + 1) * 2), next1 = page_at((c0 + j + 1) * 2 + 1);
-        if (gs >= 2 && !pf_wait(&sh.k_empty[st], ((gs >> 1) - 1) & 1, abort)) {
+        // the next step's pages are pg0, pg1; those of the one behind it:
+        const int next0 = page_at((c0 + j + 2) * kPages), next1 = kPages > 1 ? page_at((c0 + j + 2) * kPages + 1) : 0;
+        if (gs >= Cfg::kStages && !pf_wait(&sh.k_empty[st], (gs / Cfg::kStages - 1) & 1, abort)) {
           LLMIE_FAIL(kStatusTimeoutEmpty);
           ok = false;
           break;
         }
-        if (ct < 8) {
+        if (ct < Cfg::kBlocks) {
           const int k = clamp_exponent(ke), v = clamp_exponent(ve);
           sh.k_scale[ring][ct] = pow2_of(k);
           sh.v_add[ring][ct] = (float)v;
           sh.v_back[ring][ct] = pow2_of(-v);
         }
-        const int first = (c0 + j) * kPfKeys + row0;
-        {
-          const unsigned char *at0 = a.v + in_page(pg0), *at1 = a.v + in_page(pg1);
+        const int ahead = j + 1 < n_steps ? (c0 + j + 1) * Cfg::kKeys + row0 : 0x40000000;       // no tile after the last one
+        const size_t at0 = in_page(pg0), at1 = in_page(pg1);
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            put(k_smem + st * Cfg::kKvBytes, i);
-            load(i, at0, at1, first);
-          }
+        for (int i = 0; i < kPer; ++i) {
+          put(k_smem + st * Cfg::kKvBytes, kr[i], i);
+          load(kr[i], i, a.k + at0, a.k + at1, ahead);
         }
+        if (j + 1 < n_steps) load_exps();
         fence_proxy_async_smem();
         mbar_arrive(&sh.x_full[ring]);
         mbar_arrive(&sh.k_full[st]);
-        if (gs >= 2 && !pf_wait(&sh.v_empty[st], ((gs >> 1) - 1) & 1, abort)) {
+        if (gs >= Cfg::kStages && !pf_wait(&sh.v_empty[st], (gs / Cfg::kStages - 1) & 1, abort)) {
           LLMIE_FAIL(kStatusTimeoutEmpty);
           ok = false;
           break;
@@ -859,13 +876,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         unsigned any = 0u;
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          any |= ((reg[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((reg[i].y & 0x7f7f7f7fu) + 0x01010101u) |
-                 ((reg[i].z & 0x7f7f7f7fu) + 0x01010101u) | ((reg[i].w & 0x7f7f7f7fu) + 0x01010101u);
+          any |= ((vr[i].x & 0x7f7f7f7fu) + 0x01010101u) | ((vr[i].y & 0x7f7f7f7fu) + 0x01010101u) |
+                 ((vr[i].z & 0x7f7f7f7fu) + 0x01010101u) | ((vr[i].w & 0x7f7f7f7fu) + 0x01010101u);
         if (any & 0x80808080u) {
           sh.v_nan[ring] = gs + 1;
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            unsigned* c = reinterpret_cast<unsigned*>(&reg[i]);
+            unsigned* c = reinterpret_cast<unsigned*>(&vr[i]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const unsigned bad = ((c[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
@@ -873,25 +890,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
             }
           }
         }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          put(v_smem + st * Cfg::kKvBytes, vr[i], i);
+          load(vr[i], i, a.v + at0, a.v + at1, ahead);
+        }
         pg0 = next0;
         pg1 = next1;
-        {
-          const int ahead = j + 1 < n_steps ? first + kPfKeys : 0x40000000;      // no tile after the last one
-          const unsigned char *at0 = a.k + in_page(pg0), *at1 = a.k + in_page(pg1);
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            put(v_smem + st * Cfg::kKvBytes, i);
-            load(i, at0, at1, ahead);
-          }
-        }
-        if (j + 1 < n_steps) load_exps();
         fence_proxy_async_smem();
         mbar_arrive(&sh.v_full[st]);
       }
     }
   } else {
     // ------------------------------------------------------------------ the tensor core: a thread a tile, so that neither waits for the other's
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD, TURNS>::kIssue));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PfRegs<HD>::kIssue));
     if (warp == 12) {
       tmem_alloc(&sh.tmem_base, 512);
       tmem_relinquish();
@@ -911,28 +923,28 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 #pragma unroll 1
         do {                         // (there are more blocks than pieces: nobody has to begin those behind the last piece)
           others = pf_another(sh, asked++, index, abort);
-          if (others) w = pf_find<false>(a, tok, index, mine, run);
+          if (others) w = pf_find<false, Cfg::kKeys>(a, tok, index, mine, run);
         } while (others && w.parts == 0);
         if (n >= kPfAhead && !__all_sync(0xffffffffu, pf_wait(&sh.work_empty[n % kPfAhead], (n / kPfAhead - 1) & 1, abort))) break;
         if ((threadIdx.x & 31) == 0) {
-          sh.work[n % kPfAhead] = pf_piece<TURNS>(a, w, tok_x);
+          sh.work[n % kPfAhead] = pf_piece<TURNS, Cfg::kKeys>(a, w, tok_x);
           mbar_arrive(&sh.work_full[n % kPfAhead]);
         }
       }
     }
     if (warp < 14 && elect_one()) {
-      constexpr uint32_t idesc_s = pf_instr_desc(kPfRows, kPfKeys, 0), idesc_o = pf_instr_desc(kPfRows, HD, 1);
+      constexpr uint32_t idesc_s = pf_instr_desc(kPfRows, Cfg::kKeys, 0), idesc_o = pf_instr_desc(kPfRows, HD, 1);
       const int tx = warp - 12;
       bool ok = pf_wait(&sh.tmem_ready, 0, abort);
       if (!ok) LLMIE_FAIL(kStatusTimeoutMma);
       tc_fence_after_sync();
       const uint32_t tmem = sh.tmem_base;
       int gs = 0, gx = 0;            // steps of the block, and of this tile, before this piece
-      const uint32_t s_col = tmem + Cfg::kSCol + tx * 128, o_col = tmem + Cfg::kOCol + tx * (HD == 64 ? 64 : 128);
-      const uint32_t p_col = Cfg::kOwnP ? tmem + Cfg::kPCol + tx * 64 : s_col;
+      const uint32_t s_col = tmem + Cfg::kSCol + tx * Cfg::kKeys, o_col = tmem + Cfg::kOCol + tx * HD;
+      const uint32_t p_col = tmem + Cfg::kPCol + tx * (Cfg::kKeys / 2);
       // descriptors of the operands' first 16 columns; the rest lie a fixed number of 16-byte units on
       const uint64_t q_desc = make_smem_desc(smem_u32(q_smem + tx * Cfg::kQBytes), 16, 1024);
-      const uint64_t k_desc = make_smem_desc(smem_u32(k_smem), 16, 1024), v_desc = make_smem_desc(smem_u32(v_smem), kPfSub, 1024);
+      const uint64_t k_desc = make_smem_desc(smem_u32(k_smem), 16, 1024), v_desc = make_smem_desc(smem_u32(v_smem), Cfg::kKvSub, 1024);
       auto wait_for = [&](uint64_t* bar, uint32_t parity, int code) {
         if (pf_wait(bar, parity, abort)) return true;
         LLMIE_FAIL(code);
@@ -945,29 +957,29 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       };
       auto scores = [&](int j) -> bool {                     // S = Q K^T of this tile's j-th step
         const int step = gs + (TURNS ? 2 * j + tx : j);
-        if (!wait_for(&sh.k_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull)) return false;
+        if (!wait_for(&sh.k_full[step % Cfg::kStages], (step / Cfg::kStages) & 1, kStatusTimeoutFull)) return false;
         tc_fence_after_sync();
-        const uint64_t kd = k_desc + (uint64_t)((step & 1) * (Cfg::kKvBytes >> 4));
+        const uint64_t kd = k_desc + (uint64_t)((step % Cfg::kStages) * (Cfg::kKvBytes >> 4));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
-          const int off = ((kk >> 2) * kPfSub + (kk & 3) * 32) >> 4;
-          mma_bf16_ss(s_col, q_desc + off, kd + off, idesc_s, kk > 0 ? 1u : 0u);
+          const int q_off = ((kk >> 2) * kPfSub + (kk & 3) * 32) >> 4, k_off = ((kk >> 2) * Cfg::kKvSub + (kk & 3) * 32) >> 4;
+          mma_bf16_ss(s_col, q_desc + q_off, kd + k_off, idesc_s, kk > 0 ? 1u : 0u);
         }
         mma_commit(&sh.s_full[tx]);
-        let_go(&sh.k_empty[step & 1]);
+        let_go(&sh.k_empty[step % Cfg::kStages]);
         return true;
       };
       auto sums = [&](int j) -> bool {                       // O (+)= W V of it
         const int step = gs + (TURNS ? 2 * j + tx : j);
-        if (!wait_for(&sh.v_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull)) return false;
+        if (!wait_for(&sh.v_full[step % Cfg::kStages], (step / Cfg::kStages) & 1, kStatusTimeoutFull)) return false;
         if (!wait_for(&sh.p_ready[tx], (gx + j) & 1, kStatusTimeoutMma)) return false;
         tc_fence_after_sync();
-        const uint64_t vd = v_desc + (uint64_t)((step & 1) * (Cfg::kKvBytes >> 4));
+        const uint64_t vd = v_desc + (uint64_t)((step % Cfg::kStages) * (Cfg::kKvBytes >> 4));
 #pragma unroll
-        for (int kk = 0; kk < kPfKeys / 16; ++kk)            // 16 weights are 8 columns; 16 keys are 16 rows of the values
+        for (int kk = 0; kk < Cfg::kKeys / 16; ++kk)            // 16 weights are 8 columns; 16 keys are 16 rows of the values
           pf_mma_ts(o_col, p_col + kk * 8, vd + kk * (2048 >> 4), idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
         mma_commit(&sh.pv_done[tx]);
-        let_go(&sh.v_empty[step & 1]);
+        let_go(&sh.v_empty[step % Cfg::kStages]);
         return true;
       };
 #pragma unroll 1
@@ -980,20 +992,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         ok = ok && (n_x == 0 || scores(0));
 #pragma unroll 1
         for (int j = 0; ok && j < n_x; ++j) {
-          // where the weights have columns of their own, the next scores as soon as these are in registers; else they are written
-          // where these weights are read from
-          if (Cfg::kOwnP && j + 1 < n_x) ok = wait_for(&sh.s_free[tx], (gx + j) & 1, kStatusTimeoutMma) && scores(j + 1);
+          // the next scores as soon as these are in registers
+          if (j + 1 < n_x) ok = wait_for(&sh.s_free[tx], (gx + j) & 1, kStatusTimeoutMma) && scores(j + 1);
           ok = ok && sums(j);
-          if (!Cfg::kOwnP && ok && j + 1 < n_x) ok = wait_for(&sh.pv_done[tx], (gx + j) & 1, kStatusTimeoutMma) && scores(j + 1);
         }
         // steps that are the other tile's alone
 #pragma unroll 1
         for (int j = n_x; ok && !TURNS && j < n_steps; ++j) {
           const int step = gs + j;
-          ok = wait_for(&sh.k_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull);
-          if (ok) mbar_arrive(&sh.k_empty[step & 1]);
-          ok = ok && wait_for(&sh.v_full[step & 1], (step >> 1) & 1, kStatusTimeoutFull);
-          if (ok) mbar_arrive(&sh.v_empty[step & 1]);
+          ok = wait_for(&sh.k_full[step % Cfg::kStages], (step / Cfg::kStages) & 1, kStatusTimeoutFull);
+          if (ok) mbar_arrive(&sh.k_empty[step % Cfg::kStages]);
+          ok = ok && wait_for(&sh.v_full[step % Cfg::kStages], (step / Cfg::kStages) & 1, kStatusTimeoutFull);
+          if (ok) mbar_arrive(&sh.v_empty[step % Cfg::kStages]);
         }
         gs += n_steps;
         gx += n_x;
@@ -1019,8 +1029,8 @@ template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 3
   pdl_launch_dependents();
   using Cfg = PfCfg<HD>;
   const int G = a.n_q / a.n_kv, tok_x = kPfRows / G, tok = TURNS ? tok_x : 2 * tok_x;
-  const PfSequence mine = pf_sequence(a, threadIdx.x & 31, tok);
-  const PfWork w = pf_find<true>(a, tok, blockIdx.x, mine, pf_run(a, tok, mine));
+  const PfSequence mine = pf_sequence<Cfg::kKeys>(a, threadIdx.x & 31, tok);
+  const PfWork w = pf_find<true, Cfg::kKeys>(a, tok, blockIdx.x, mine, pf_run<Cfg::kKeys>(a, tok, mine));
   // The lengths are older than the kernel that leaves the partial results (it lets this one begin behind its own wait). Blocks with
   // nothing to join wait too: the kernel behind this one waits for this one alone, and reads what the one in front wrote.
   pdl_wait();
@@ -1086,17 +1096,17 @@ static int launch_prefill_fp8(PrefillArgs a, int n_tokens, int max_q_len, cudaSt
   // follow from the most keys that the table has room for and the least work that so many tokens are.
   const long long items = max_q_len <= tok ? (long long)a.n_seqs * a.n_kv : ((long long)n_tokens / tok + a.n_seqs) * a.n_kv;
   double least = (double)n_tokens / tok * a.n_kv;
-  long long most_tiles = ((long long)a.max_pages * kFp8Page + kPfKeys - 1) / kPfKeys;
+  long long most_tiles = ((long long)a.max_pages * kFp8Page + Cfg::kKeys - 1) / Cfg::kKeys;
   if (a.window == 0) {
-    least *= (1.0 + (double)n_tokens / ((double)kPfKeys * a.n_seqs)) / 2;
+    least *= (1.0 + (double)n_tokens / ((double)Cfg::kKeys * a.n_seqs)) / 2;
   } else {
     const long long w = a.window < 0 ? -(long long)a.window : a.window;
-    most_tiles = min(most_tiles, (w + tok) / kPfKeys + 2);
+    most_tiles = min(most_tiles, (w + tok) / Cfg::kKeys + 2);
   }
-  // (tokens that do not fill their tiles may leave fewer tiles than SMs after all, where runs may be half as long)
-  long long run = (long long)(least * ((double)n_tokens / tok * a.n_kv > kPfSms ? 2 : 1) / kPfSms);
-  run = min(max(run, (long long)kPfLeast), 1LL << 30);
-  const bool cut = (most_tiles + run / 2) / run > 1;
+  const bool many = (double)n_tokens / tok * a.n_kv > kPfSms;                // more tiles than SMs whatever the sequences' lengths
+  long long run = (long long)(least * (many ? 2 : 1) / kPfSms);
+  run = min(max(run, (long long)kPfLeast / Cfg::kKeys), 1LL << 30);
+  const bool cut = many ? (most_tiles + run / 2) / run > 1 : most_tiles > run;
   if (cut && !a.part) return kPfNeedsScratch;
   a.run = (int)run;
   const long long blocks = !cut ? items : items <= kPfFew ? kPfSms : items + kPfSms;
@@ -1104,7 +1114,8 @@ static int launch_prefill_fp8(PrefillArgs a, int n_tokens, int max_q_len, cudaSt
   launch_k(prefill_fp8_kernel<HD, TURNS>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
   LLMIE_LAUNCH_CHECK();
   if (cut) {
-    launch_k(prefill_fp8_join_kernel<HD, TURNS>, dim3((unsigned)items, kPfJoinSide), dim3(kPfJoinWarps * 32), 0, stream, a);
+    const unsigned side = (unsigned)max(1LL, min((long long)kPfJoinSide, 8LL * kPfSms / items));
+    launch_k(prefill_fp8_join_kernel<HD, TURNS>, dim3((unsigned)items, side), dim3(kPfJoinWarps * 32), 0, stream, a);
     LLMIE_LAUNCH_CHECK();
   }
   return LLMIE_OK;
