@@ -50,7 +50,8 @@ constexpr int kPfStages = 4;         // at most
 constexpr int kPfAhead = 4;          // places for pieces of work
 constexpr int kPfReaders = 14;       // who reads one: eight softmax warps, four converting ones, two issuing threads
 constexpr int kPfNeedsScratch = -5;  // the answer to a call without scratch that cannot do without
-constexpr int kPfLeast = 512;        // keys that a run has at least, on average
+constexpr int kPfLeast = 256;        // keys that a run has at least, on average
+constexpr int kPfWhole = 768;        // a step is not cut where no token sees more keys
 constexpr int kPfSlots = 200;        // partial results at once (see pf_run)
 constexpr int kPfFew = 128;          // tiles of tokens that can always be cut into runs for which there are SMs (see pf_run)
 constexpr float kPfTop = 7.f;        // the bound's own weight is 2^7
@@ -178,7 +179,9 @@ template <int KEYS> __device__ __forceinline__ PfSequence pf_sequence(const Pref
 // Runs that each of a sequence's tiles of tokens is cut into, by pf_run's answer: none longer than it where all of them find an SM at
 // once (answers below 0), else last / run to the nearest.
 __device__ __forceinline__ int pf_runs(int last, int run) { return run < 0 ? max(1, (last - run - 1) / -run) : max(1, (last + run / 2) / run); }
-// How long runs are, in key tiles. With T the sum of (first + last) / 2 over all tiles of tokens and heads:
+// How long runs are, in key tiles. A step whose tokens see at most kPfWhole keys is left whole: the join takes about as long as it would
+// save (2 sequences of 600 tokens, 16 heads: 25 us whole, 30.5 in runs of 256 keys; 6 of up to 50 behind up to 800 13.9 and 18.5;
+// 4 of up to 156 behind up to 1,592 38.9 and 27.8). With T the sum of (first + last) / 2 over all tiles of tokens and heads:
 // Where those are no more than the SMs: the least, from T / 148 on, with which every run finds an SM at once and none is longer
 // (answered below 0; 24 sequences of 2 to 8 tokens behind 300 to 6,000, 96 tiles: 52.4 us, and 55.0 where runs are last / run to the
 // nearest, half as long again at worst). Where they are more, or no such length is found: 2 T / 148, so that a sequence is cut only
@@ -191,13 +194,15 @@ __device__ __forceinline__ int pf_runs(int last, int run) { return run < 0 ? max
 template <int KEYS> __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
   const int lane = threadIdx.x & 31;
   float twice = (float)mine.tiles * (float)(mine.first + mine.last);
-  int tiles = mine.tiles;
+  int tiles = mine.tiles, longest = mine.last;
 #pragma unroll 1
   for (int s = lane + 32; s < a.n_seqs; s += 32) {
     const PfSequence q = pf_sequence<KEYS>(a, s, tok);
     twice += (float)q.tiles * (float)(q.first + q.last);
     tiles += q.tiles;
+    longest = max(longest, q.last);
   }
+  if (__reduce_max_sync(0xffffffffu, longest) <= kPfWhole / KEYS) return 1 << 30;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
   const float share = twice * (float)a.n_kv / kPfSms;                        // 2 T / 148
@@ -1106,7 +1111,7 @@ static int launch_prefill_fp8(PrefillArgs a, int n_tokens, int max_q_len, cudaSt
   const bool many = (double)n_tokens / tok * a.n_kv > kPfSms;                // more tiles than SMs whatever the sequences' lengths
   long long run = (long long)(least * (many ? 2 : 1) / kPfSms);
   run = min(max(run, (long long)kPfLeast / Cfg::kKeys), 1LL << 30);
-  const bool cut = many ? (most_tiles + run / 2) / run > 1 : most_tiles > run;
+  const bool cut = most_tiles > kPfWhole / Cfg::kKeys && (many ? (most_tiles + run / 2) / run > 1 : most_tiles > run);
   if (cut && !a.part) return kPfNeedsScratch;
   a.run = (int)run;
   const long long blocks = !cut ? items : items <= kPfFew ? kPfSms : items + kPfSms;
