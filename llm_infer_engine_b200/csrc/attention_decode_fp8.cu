@@ -26,7 +26,7 @@
 
 namespace llmie {
 
-constexpr int kDfWarps = 4;
+constexpr int kDfWarps = 4;          // of a block (of a large one, where an item has its blocks to itself: twice as many)
 constexpr int kDfUnit = 2 * kExpBlock;
 constexpr int kDfThreads = kDfWarps * 32;
 constexpr int kSms = 148;
@@ -109,8 +109,11 @@ template <int HD, int NH> struct DfCfg {
   static constexpr int kPitch = HD + 4;                          // floats between two heads' sums: lanes 4 banks apart
   static constexpr int kRecord = kHeads * (HD + 2);              // floats of a partial result: sums, then bounds and denominators
 };
-// Thread blocks that an SM holds at once.
-template <int HD, int NH> __host__ __device__ constexpr int df_per_sm() { return HD == 64 ? (NH == 1 ? 5 : 3) : NH == 1 ? 3 : 2; }
+// Thread blocks that an SM holds at once. (Head size 64, five instead of four, 102 registers a thread: 64 sequences of 700 to 3,900 keys
+// 34.9 us instead of 29.3; one of 517 4.75 instead of 4.4. Head size 128, two instead of three: 48 of 1,000 to 16,000 100 instead of 92.5,
+// with a third stage 94.)
+template <int HD, int NH> __host__ __device__ constexpr int df_per_sm() { return HD == 64 ? (NH == 1 ? 4 : 3) : NH == 1 ? 3 : 2; }
+template <int HD, int NH> __host__ __device__ constexpr int df_large_per_sm() { return HD == 64 && NH == 1 ? 2 : 1; }
 template <int HD, int NH> constexpr int df_blocks() { return kSms * df_per_sm<HD, NH>(); }
 // Where column d of a head stands among a head's sums: as the second product's accumulators hold them.
 template <int HD> __device__ __forceinline__ int df_place(int d) {
@@ -203,7 +206,7 @@ template <int HD> __device__ __forceinline__ int df_at(int r, int p) {
   const int l = r * (HD / 16) + p, line = l >> 3;
   return line * 128 + ((l & 7) ^ df_swizzle<HD>(line)) * 16;
 }
-template <int HD, int NH> struct DfPipe {
+template <int HD, int NH, int W = kDfWarps> struct DfPipe {
   static constexpr int kStages = 2;
   static constexpr int kHalf = kDfUnit * HD;                 // bytes of a unit's keys, or values
   static constexpr int kUnit = 2 * kHalf + 128;              // and the exponents; whole lines
@@ -211,7 +214,7 @@ template <int HD, int NH> struct DfPipe {
   static constexpr int kWarp = kStages * kUnit;
   static constexpr int kSums = DfCfg<HD, NH>::kHeads * (DfCfg<HD, NH>::kPitch + 2) * 4;        // a warp's results, in the same place afterwards
   static constexpr int kPerWarp = ((kWarp > kSums ? kWarp : kSums) + 127) / 128 * 128;
-  static constexpr int kSmem = kDfWarps * kPerWarp;
+  static constexpr int kSmem = W * kPerWarp;
 };
 __device__ __forceinline__ void df_copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -223,7 +226,7 @@ __device__ __forceinline__ void df_copy4(uint32_t dst, const void* src) {
 // A piece of an item: units [u_begin, u_end) of the `count` that sequence seq's newest token sees (unit 0 of them is `first`),
 // KV head hk, ng query heads from g0 of its group on. All warps of the block; each leaves its sums (df_place), bounds and
 // denominators in its own part of shared memory: [heads][pitch], [heads], [heads] floats.
-template <int HD, int NH, bool ROPE>
+template <int HD, int NH, bool ROPE, int W>
 __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArgs& a, const DecodeStep& st, unsigned char* smem, int seq,
                                          int len, int hk, int g0, int ng, int first, int count, int u_begin, int u_end) {
   using Cfg = DfCfg<HD, NH>;
@@ -257,15 +260,15 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
   };
   const size_t q_pitch = (size_t)(ROPE ? a.n_q + 2 * a.n_kv : a.n_q) * HD;
   // (a sequence that is longer than its table: there is no place for the position)
-  if (ROPE && u_end == count && u_begin < count && (count - 1 - u_begin) % kDfWarps == warp && a.seq_kvlen[seq] == len)
+  if (ROPE && u_end == count && u_begin < count && (count - 1 - u_begin) % W == warp && a.seq_kvlen[seq] == len)
     df_append<HD>(q + seq * q_pitch, a, st, hk, len, pages[(first + count - 1) >> 1]);            // this warp reads that block itself
   int pg_next;                       // page of the next unit to be asked for
   {
     int pg[Pipe::kStages];
 #pragma unroll
-    for (int i = 0; i < Pipe::kStages; ++i) pg[i] = page_of(u + i * kDfWarps);
+    for (int i = 0; i < Pipe::kStages; ++i) pg[i] = page_of(u + i * W);
 #pragma unroll
-    for (int i = 0; i < Pipe::kStages - 1; ++i) issue(u + i * kDfWarps, pg[i], i);
+    for (int i = 0; i < Pipe::kStages - 1; ++i) issue(u + i * W, pg[i], i);
     pg_next = pg[Pipe::kStages - 1];
   }
 
@@ -330,11 +333,11 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
   }
 
   int stage = 0, ahead = Pipe::kStages - 1;                  // where this unit lies, and where the one to be asked for goes
-  for (; u < u_stop; u += kDfWarps) {
+  for (; u < u_stop; u += W) {
     asm volatile("cp.async.wait_group %0;" ::"n"(Pipe::kStages - 2) : "memory");
     __syncwarp();                    // everyone's share of the unit is there, and everyone has read the unit before
-    issue(u + (Pipe::kStages - 1) * kDfWarps, pg_next, ahead);
-    pg_next = page_of(u + Pipe::kStages * kDfWarps);
+    issue(u + (Pipe::kStages - 1) * W, pg_next, ahead);
+    pg_next = page_of(u + Pipe::kStages * W);
     const unsigned char* at = mine + stage * Pipe::kUnit;
     ahead = stage;
     stage = stage + 1 == Pipe::kStages ? 0 : stage + 1;
@@ -501,19 +504,19 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
 }
 
 // One number of a block's result: head h, place `at` of its sums; its bound and denominator with it. Behind a barrier.
-template <int HD, int NH>
+template <int HD, int NH, int W>
 __device__ __forceinline__ void df_of_warps(const unsigned char* smem, int h, int at, float& M, float& num, float& den) {
   using Cfg = DfCfg<HD, NH>;
-  const float* s[kDfWarps];
+  const float* s[W];
 #pragma unroll
-  for (int w = 0; w < kDfWarps; ++w) s[w] = reinterpret_cast<const float*>(smem + w * DfPipe<HD, NH>::kPerWarp);
+  for (int w = 0; w < W; ++w) s[w] = reinterpret_cast<const float*>(smem + w * DfPipe<HD, NH>::kPerWarp);
   M = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kDfWarps; ++w) M = fmaxf(M, s[w][Cfg::kHeads * Cfg::kPitch + h]);
+  for (int w = 0; w < W; ++w) M = fmaxf(M, s[w][Cfg::kHeads * Cfg::kPitch + h]);
   const float Mu = M == -INFINITY ? 0.f : M;
   num = den = 0.f;
 #pragma unroll
-  for (int w = 0; w < kDfWarps; ++w) {
+  for (int w = 0; w < W; ++w) {
     const float f = df_exp2(s[w][Cfg::kHeads * Cfg::kPitch + h] - Mu);
     num = fmaf(f, s[w][h * Cfg::kPitch + at], num);
     den = fmaf(f, s[w][Cfg::kHeads * (Cfg::kPitch + 1) + h], den);
@@ -580,7 +583,7 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
     const int u_begin = cur - begin - item * count;
     const int u_end = min(count, u_begin + (end - cur));
     const int hk = item / chunks, g0 = item % chunks * Cfg::kHeads, ng = min(Cfg::kHeads, G - g0);
-    df_piece<HD, NH, ROPE>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
+    df_piece<HD, NH, ROPE, kDfWarps>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
     __syncthreads();
     const bool starts = u_begin == 0, whole = starts && u_end == count;
     float* rec = a.part + ((size_t)blockIdx.x * 2 + (starts ? 1 : 0)) * Cfg::kRecord;
@@ -588,7 +591,7 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
     for (int i = threadIdx.x; i < ng * HD; i += kDfThreads) {
       const int h = i / HD, d = i % HD;
       float M, num, den;
-      df_of_warps<HD, NH>(df_smem, h, whole ? df_place<HD>(d) : d, M, num, den);      // a partial result stays in the order of the sums
+      df_of_warps<HD, NH, kDfWarps>(df_smem, h, whole ? df_place<HD>(d) : d, M, num, den);      // a partial result stays in the order of the sums
       if (whole) {
         a.out[((size_t)seq * a.n_q + hk * G + g0 + h) * HD + d] = __float2bfloat16_rn(num / den);
       } else {
@@ -610,8 +613,8 @@ decode_fp8_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep s
 
 // Few short sequences: an item is one cluster's, its units in equal runs over the cluster's blocks, which read one another's
 // results from shared memory. grid (blocks of a cluster, items of a sequence, sequences). One launch, no partial results.
-template <int HD, int NH, bool ROPE>
-__global__ void __launch_bounds__(kDfThreads, df_per_sm<HD, NH>())
+template <int HD, int NH, bool ROPE, int W>
+__global__ void __launch_bounds__(W * 32, W > kDfWarps ? df_large_per_sm<HD, NH>() : df_per_sm<HD, NH>())
 decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const DecodeStep st) {
   pdl_launch_dependents();
   pdl_wait();
@@ -625,17 +628,17 @@ decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const Deco
   df_units(a, len, first, count);
   __nv_bfloat16* out = a.out + ((size_t)seq * a.n_q + hk * G + g0) * HD;
   if (count == 0) {                  // the whole cluster alike
-    for (int i = blockIdx.x * kDfThreads + threadIdx.x; i < ng * HD; i += gridDim.x * kDfThreads) out[i] = __float2bfloat16_rn(0.f);
+    for (int i = blockIdx.x * W * 32 + threadIdx.x; i < ng * HD; i += gridDim.x * W * 32) out[i] = __float2bfloat16_rn(0.f);
     return;
   }
   const int u_begin = count * blockIdx.x / gridDim.x, u_end = count * (blockIdx.x + 1) / gridDim.x;
-  df_piece<HD, NH, ROPE>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
+  df_piece<HD, NH, ROPE, W>(q, a, st, df_smem, seq, len, hk, g0, ng, first, count, u_begin, u_end);
   __syncthreads();
 #pragma unroll 1
-  for (int i = threadIdx.x; i < ng * HD; i += kDfThreads) {
+  for (int i = threadIdx.x; i < ng * HD; i += W * 32) {
     const int h = i / HD, d = i % HD;
     float M, num, den;
-    df_of_warps<HD, NH>(df_smem, h, df_place<HD>(d), M, num, den);
+    df_of_warps<HD, NH, W>(df_smem, h, df_place<HD>(d), M, num, den);
     if (gridDim.x == 1) {
       out[i] = __float2bfloat16_rn(num / den);
       continue;
@@ -650,7 +653,7 @@ decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const Deco
   tc::cluster_sync_all();
   const uint32_t here = (uint32_t)__cvta_generic_to_shared(joined);
 #pragma unroll 1
-  for (int i = blockIdx.x * kDfThreads + threadIdx.x; i < ng * HD; i += gridDim.x * kDfThreads) {
+  for (int i = blockIdx.x * W * 32 + threadIdx.x; i < ng * HD; i += gridDim.x * W * 32) {
     const int h = i / HD;
     float m[8], n[8], l[8], M = -INFINITY;
 #pragma unroll
@@ -796,6 +799,17 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
   }
 }
 
+template <int HD, int NH, bool ROPE, int W>
+static int launch_cluster(const void* q, const DecodeArgs& a, const DecodeStep& st, int items_of_seq, int cluster, cudaStream_t stream) {
+  constexpr int smem = DfPipe<HD, NH, W>::kSmem;
+  cudaError_t e = cudaFuncSetAttribute(decode_fp8_cluster_kernel<HD, NH, ROPE, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return (int)e;
+  launch_k_cluster(decode_fp8_cluster_kernel<HD, NH, ROPE, W>, dim3(cluster, items_of_seq, a.n_seqs), dim3(W * 32), smem, stream, cluster,
+                   (const __nv_bfloat16*)q, a, st);
+  LLMIE_LAUNCH_CHECK();
+  return LLMIE_OK;
+}
+
 template <int HD, int NH, bool ROPE>
 static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& st, int max_kv_len, cudaStream_t stream) {
   constexpr int smem = DfPipe<HD, NH>::kSmem;
@@ -806,15 +820,15 @@ static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& s
   if (a.window > 0 && a.window + kDfUnit < units) units = a.window + kDfUnit;
   if (a.window < 0 && -(long long)a.window < units) units = -(long long)a.window;
   units = (units + kDfUnit - 1) / kDfUnit;
-  int cluster = 1;
+  int cluster = 1;                   // blocks that share an item
   while (cluster < 8 && 2 * cluster * items <= df_blocks<HD, NH>() && 2 * cluster * kDfWarps <= units) cluster *= 2;
   if (units <= (long long)cluster * kDfWarps * kDfFew && items <= df_blocks<HD, NH>() && items <= 65535) {
-    cudaError_t e = cudaFuncSetAttribute(decode_fp8_cluster_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return (int)e;
-    launch_k_cluster(decode_fp8_cluster_kernel<HD, NH, ROPE>, dim3(cluster, a.n_kv * chunks, a.n_seqs), dim3(kDfThreads), smem, stream,
-                     cluster, (const __nv_bfloat16*)q, a, st);
-    LLMIE_LAUNCH_CHECK();
-    return LLMIE_OK;
+    // Where these blocks would share SMs, half as many large ones, or one instead of two that have to meet (37 sequences, window of
+    // 1,024, 148 items: 14.1 us with two blocks an item, 10.8 with one; 18 of 1,050 keys, head size 64: 10.7 and 7.7. One sequence of
+    // 517: 4.4 with four blocks an item, 4.9 with two).
+    if (cluster > 1 && items * cluster > kSms && items * (cluster / 2) <= kSms * df_large_per_sm<HD, NH>())
+      return launch_cluster<HD, NH, ROPE, 2 * kDfWarps>(q, a, st, a.n_kv * chunks, cluster / 2, stream);
+    return launch_cluster<HD, NH, ROPE, kDfWarps>(q, a, st, a.n_kv * chunks, cluster, stream);
   }
   if (!a.part) return kNeedsScratch;
   cudaError_t e = cudaFuncSetAttribute(decode_fp8_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
