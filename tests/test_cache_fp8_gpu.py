@@ -264,6 +264,48 @@ def test_decode(n_q, n_kv, hd, window):
         assert bool((err <= allowed(want, size, BF, True)).all()), (l, float((err / allowed(want, size, BF, True)).max()))
 
 
+@pytest.mark.parametrize("n,n_q,n_kv,hd", [(18, 32, 8, 64), (20, 14, 2, 64), (18, 40, 4, 64), (37, 28, 4, 128), (18, 48, 4, 128),
+                                           (18, 32, 8, 128), (40, 32, 8, 128), (80, 32, 8, 64)])
+@pytest.mark.parametrize("longest", [70, 1100])
+def test_decode_of_some_dozen_sequences(n, n_q, n_kv, hd, longest):
+    """Between a few items, which have several blocks each, and many, which share blocks: large blocks, alone or in pairs. With the
+    longest length named and not; a step on top of it leaves what appending and attending leaves."""
+    g = torch.Generator().manual_seed(n + hd)
+    lens = torch.randint(1, longest, (n,), generator=g).tolist()
+    lens[3], lens[5] = longest, 0
+    pc = filled(lens, n_kv, hd, seed=n)
+    q = torch.randn(n, n_q * hd, generator=g).to(BF)
+    outs = []
+    for max_len in (longest, 0):
+        out = torch.full((n, n_q * hd), math.nan, dtype=BF, device=DEV)
+        ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5, 0,
+                                   max_len)
+        outs.append(out)
+        for i, l in enumerate(lens):
+            if l == 0:
+                assert bool((out[i] == 0).all())
+                continue
+            want, size = fp8_cache.attention(q[i:i + 1].double().view(1, n_q, hd), *pc.held(i, l), [l - 1], hd ** -0.5, 0)
+            err = (out[i].cpu().double().view(1, n_q, hd) - want).abs()
+            assert bool((err <= allowed(want, size, BF, True)).all()), (i, l, float((err / allowed(want, size, BF, True)).max()))
+    # the step of the last tokens, whose keys and values are in place already: an append of the same numbers
+    starts, news = [max(l - 1, 0) for l in lens], [min(l, 1) for l in lens]
+    qkv = torch.randn(n, (n_q + 2 * n_kv) * hd, generator=g).to(BF)
+    table = angles(longest, hd)
+    rows = torch.tensor([i for i, m in enumerate(news) if m])
+    rotated, after = store(pc, qkv[rows], table, starts, news, n_q, n_kv, hd, hd)
+    for max_len in (longest, 0):
+        stepped, out = pc.dev(), torch.zeros(n, n_q * hd, dtype=BF, device=DEV)
+        ops().attention_decode_fp8_rope(qkv.to(DEV), *stepped, out, table.to(DEV), i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv,
+                                        hd, hd ** -0.5, 0, max_len)
+        assert all(same_bits(a, b) for a, b in zip(stepped, after))
+        whole = torch.zeros(n, n_q * hd, dtype=BF, device=DEV)
+        x = torch.zeros(n, n_q * hd, dtype=BF, device=DEV)
+        x[rows.to(DEV)] = rotated
+        ops().attention_decode_fp8(x, *after, whole, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5, 0, max_len)
+        assert torch.equal(out, whole)
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("case", ["large keys", "small queries", "large queries", "values apart", "zero values", "negative scale"])
 def test_decode_far_ranges(hd, case):
