@@ -193,6 +193,61 @@ def test_captured_generation_is_eager_generation(tag, dtype):
     assert all(len(o) == 30 for o in out[True][0])
 
 
+@pytest.mark.parametrize("which", ["zemivik", "burinex", "rogizen", "selinex"])
+def test_models_whose_mixers_do_not_know_it_are_refused(which, tmp_path):
+    import importlib
+    from llm_infer_engine_b200 import Engine, EngineError, write_random_model
+    cfg = importlib.import_module("plain_zemivik").TINY_A if which == "zemivik" else importlib.import_module(f"test_{which}_host").CFG
+    write_random_model(cfg, str(tmp_path), seed=1)
+    with pytest.raises(EngineError, match="8 bits"):
+        Engine(str(tmp_path), max_batch=2, max_seq_len=64, cache_dtype="float8_e4m3")
+    Engine(str(tmp_path), max_batch=2, max_seq_len=64, cuda_graph=False)
+
+
+@pytest.mark.parametrize("which", ["a join with nothing to join", "a join", "one launch", "prompt", "prompt in runs", "append"])
+def test_the_kernel_behind_reads_finished_rows(which):
+    """Launches that may begin early, bit for bit as launches that may not: what a call leaves goes straight into the next kernel,
+    forty times through the same buffer."""
+    from llm_infer_engine_b200.kernels import ops
+    n_q, n_kv, hd = 16, 4, 128
+    n, held = {"a join with nothing to join": (111, 1920), "a join": (5, 9000), "one launch": (12, 300), "prompt": (40, 90),
+               "prompt in runs": (6, 3000), "append": (40, 90)}[which]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)                                # noqa: E731
+    pages = -(-held // 64)
+    shape = (n * pages, n_kv, 64, hd)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randint(0, 120, shape, generator=g, device=DEV).to(torch.uint8).view(F8) for _ in range(2))
+    exps = torch.full(shape[:2] + (4,), -7, dtype=torch.int8, device=DEV)
+    table = torch.arange(n * pages, dtype=torch.int32, device=DEV).view(n, pages)
+    slots, lens, starts, cu = i32(list(range(n))), i32([held] * n), i32([held - 1] * n), i32(list(range(n + 1)))
+    qs = torch.randn(40, n, n_q * hd, generator=g, device=DEV).to(torch.bfloat16)
+
+    def run():
+        buf, half, outs = torch.zeros(n, n_q * hd, dtype=torch.bfloat16, device=DEV), torch.empty_like(qs[0][:, :8 * hd]), []
+        half, cache = half.contiguous(), [t.clone() for t in (k, v, exps, exps)]
+        for q in qs:
+            if which.startswith("prompt"):
+                ops.attention_prefill_fp8(q, k, v, exps, exps, buf, cu, slots, starts, table, n, 1, n_q, n_kv, hd, hd ** -0.5)
+            elif which == "append":
+                ops.rope_store_fp8(q, half, *cache, None, cu, slots, starts, table, n, 1, 8, n_kv, hd, 0)
+                ops.attention_decode_fp8(q, *cache, buf, slots, lens, table, n_q, n_kv, hd, hd ** -0.5, 0, held)
+            else:
+                ops.attention_decode_fp8(q, k, v, exps, exps, buf, slots, lens, table, n_q, n_kv, hd, hd ** -0.5, 0, held)
+            outs.append(torch.empty(n, 8 * hd, dtype=torch.bfloat16, device=DEV))
+            ops.rope_store_fp8(buf, outs[-1], k, v, exps, exps, None, cu, slots, starts, table, n, 1, 8, n_kv, hd, 0, False)
+        torch.cuda.synchronize()
+        return torch.stack(outs)
+
+    early = [run() for _ in range(3)]
+    ops.set_pdl(False)
+    try:
+        late = run()
+    finally:
+        ops.set_pdl(True)
+    for e in early:
+        assert torch.equal(e, late)
+
+
 def test_options_that_do_not_go_together():
     from llm_infer_engine_b200 import Engine, EngineError
     folder = helpers.model_folder("c")
