@@ -801,18 +801,17 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
 
 template <int HD, int NH, bool ROPE, int W>
 static int launch_cluster(const void* q, const DecodeArgs& a, const DecodeStep& st, int items_of_seq, int cluster, cudaStream_t stream) {
-  constexpr int smem = DfPipe<HD, NH, W>::kSmem;
-  cudaError_t e = cudaFuncSetAttribute(decode_fp8_cluster_kernel<HD, NH, ROPE, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(decode_fp8_cluster_kernel<HD, NH, ROPE, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       DfPipe<HD, NH, W>::kSmem);
   if (e != cudaSuccess) return (int)e;
-  launch_k_cluster(decode_fp8_cluster_kernel<HD, NH, ROPE, W>, dim3(cluster, items_of_seq, a.n_seqs), dim3(W * 32), smem, stream, cluster,
-                   (const __nv_bfloat16*)q, a, st);
+  launch_k_cluster(decode_fp8_cluster_kernel<HD, NH, ROPE, W>, dim3(cluster, items_of_seq, a.n_seqs), dim3(W * 32), DfPipe<HD, NH, W>::kSmem,
+                   stream, cluster, (const __nv_bfloat16*)q, a, st);
   LLMIE_LAUNCH_CHECK();
   return LLMIE_OK;
 }
 
 template <int HD, int NH, bool ROPE>
 static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& st, int max_kv_len, cudaStream_t stream) {
-  constexpr int smem = DfPipe<HD, NH>::kSmem;
   const int G = a.n_q / a.n_kv, chunks = (G + 8 * NH - 1) / (8 * NH);
   const long long items = (long long)a.n_seqs * a.n_kv * chunks;
   // units of the longest sequence, as far as the caller knows
@@ -831,10 +830,11 @@ static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& s
     return launch_cluster<HD, NH, ROPE, kDfWarps>(q, a, st, a.n_kv * chunks, cluster, stream);
   }
   if (!a.part) return kNeedsScratch;
-  cudaError_t e = cudaFuncSetAttribute(decode_fp8_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(decode_fp8_kernel<HD, NH, ROPE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       DfPipe<HD, NH>::kSmem);
   if (e != cudaSuccess) return (int)e;
   constexpr int blocks = df_blocks<HD, NH>();
-  launch_k(decode_fp8_kernel<HD, NH, ROPE>, dim3(blocks), dim3(kDfThreads), smem, stream, (const __nv_bfloat16*)q, a, st);
+  launch_k(decode_fp8_kernel<HD, NH, ROPE>, dim3(blocks), dim3(kDfThreads), DfPipe<HD, NH>::kSmem, stream, (const __nv_bfloat16*)q, a, st);
   LLMIE_LAUNCH_CHECK();
   const int side = (int)max(1LL, min((long long)min(G, 8 * NH), 4 * kSms / items));
   launch_k(decode_fp8_join_kernel<HD, NH>, dim3((unsigned)items, side), dim3(kDfSlices * HD), 0, stream, a, blocks);
