@@ -127,9 +127,10 @@ rope_store_fp8_kernel(const T* qkv, T* __restrict__ q_out, const float2* LLMIE_W
 
 // Head size 64 or 128, the whole head rotated (or none), rows on 16 bytes: a thread has eight neighbouring columns and their
 // partners half a head on, of one position, for all the heads there are; the angles are read once for all of them.
-// (2,048 tokens: 47 MB in 13.7 us, 3.4 TB/s, of which about 4 us are what a launch and four loads that wait for one another take.)
+// (2,048 tokens: 47 MB in 12.2 us, 3.9 TB/s, of which about 4 us are what a launch and four loads that wait for one another take. Four
+// blocks an SM: three 13.6, 9 pieces of 3 to 700 tokens 6.5 and 6.2; 256 threads a block 15.7 and 7.0.)
 template <typename T, int HD>
-__global__ void __launch_bounds__(kStoreThreads)
+__global__ void __launch_bounds__(kStoreThreads, 4)
 rope_store_fp8_vec_kernel(const T* qkv, T* __restrict__ q_out, const float4* LLMIE_WEIGHT table, const StoreArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -185,8 +186,8 @@ rope_store_fp8_vec_kernel(const T* qkv, T* __restrict__ q_out, const float4* LLM
   }
   if (active) {
     T* dst = q_out + (size_t)(b.tok0 + row) * a.n_q * HD + lane * 8;
-    // four heads are asked for before one is worked on (2,048 tokens, 32 / 8 heads of 128: 14.5 us one by one, 13.7 so; a token of each
-    // of 64 sequences 4.4 and 4.0; with 256 threads a block 15.7 and 6.3)
+    // four heads are asked for before one is worked on (2,048 tokens, 32 / 8 heads of 128: 14.5 us one by one, 12.2 so, with two 12.9; a
+    // token of each of 64 sequences 4.4, 4.0, 4.3)
 #pragma unroll 1
     for (int g0 = part; g0 < G; g0 += 4 * kParts) {
       float u[4][8], v[4][8];
