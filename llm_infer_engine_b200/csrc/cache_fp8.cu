@@ -26,6 +26,7 @@ struct StoreArgs {
   const int* seq_start;
   const int* block_table;
   int max_pages, n_q, n_kv, hd, rot_dim, table_len, write_kv;
+  int n_seqs, packed;                // packed: a block's place in the line of all sequences' blocks of 16, instead of one in its sequence's
 };
 
 // What a thread block works on: positions [p0, p1) of sequence `seq`, all in one block of 16.
@@ -35,10 +36,51 @@ struct StoreBlock {
   size_t row;                        // page * n_kv + head, the page that holds the block
   int in_page;                       // row of the block's first position in its page
 };
+// Blocks of 16 that a sequence's new positions lie in.
+__device__ __forceinline__ int store_blocks(const StoreArgs& a, int seq) {
+  const int n_new = a.cu_q[seq + 1] - a.cu_q[seq], start = a.seq_start[seq];
+  return n_new > 0 ? (start + n_new - 1) / kExpBlock - start / kExpBlock + 1 : 0;
+}
+// Finds the sequence whose blocks the block's place in the line lies among, a sequence a thread at a time, and `at`, its place there.
+__device__ __forceinline__ bool store_find(const StoreArgs& a, int& seq, int& at) {
+  __shared__ int total[kStoreThreads / 32], found[2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, index = blockIdx.x;
+  int before = 0;
+  if (threadIdx.x == 0) found[0] = -1;
+#pragma unroll 1
+  for (int s0 = 0; s0 < a.n_seqs; s0 += kStoreThreads) {
+    const int s = s0 + threadIdx.x, own = s < a.n_seqs ? store_blocks(a, s) : 0;
+    int incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    if (lane == 31) total[warp] = incl;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kStoreThreads / 32; ++w) {
+      if (w < warp) incl += total[w];
+      all += total[w];
+    }
+    if (before + incl > index && before + incl - own <= index) {
+      found[0] = s;
+      found[1] = index - before - (incl - own);
+    }
+    __syncthreads();
+    before += all;
+    if (before > index) break;
+  }
+  seq = found[0];
+  at = found[1];
+  return seq >= 0;
+}
 __device__ __forceinline__ bool store_block(const StoreArgs& a, int hk, StoreBlock& b) {
-  const int seq = blockIdx.z;
+  int seq = blockIdx.z, at = blockIdx.x;
+  if (a.packed && !store_find(a, seq, at)) return false;
   const int start = a.seq_start[seq], t0 = a.cu_q[seq], n_new = a.cu_q[seq + 1] - t0;
-  const int first = (start / kExpBlock + (int)blockIdx.x) * kExpBlock;
+  const int first = (start / kExpBlock + at) * kExpBlock;
   b.p0 = max(start, first);
   b.p1 = min(start + n_new, first + kExpBlock);
   if (b.p0 >= b.p1 || first / kFp8Page >= a.max_pages) return false;
@@ -250,21 +292,20 @@ rope_store_fp8_vec_kernel(const T* qkv, T* __restrict__ q_out, const float4* LLM
 }
 
 template <typename T>
-static int launch_store(const void* qkv, void* q_out, const float2* table, const StoreArgs& a, int blocks, int n_seqs,
-                        cudaStream_t stream) {
+static int launch_store(const void* qkv, void* q_out, const float2* table, const StoreArgs& a, dim3 grid, cudaStream_t stream) {
   const bool vec = (a.rot_dim == a.hd || !table) && aligned16(qkv) && aligned16(q_out) && aligned16(table);
   if (vec && (a.hd == 64 || a.hd == 128)) {
     if (a.hd == 64)
-      launch_k(rope_store_fp8_vec_kernel<T, 64>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), 0, stream, (const T*)qkv,
+      launch_k(rope_store_fp8_vec_kernel<T, 64>, grid, dim3(kStoreThreads), 0, stream, (const T*)qkv,
                (T*)q_out, (const float4*)table, a);
     else
-      launch_k(rope_store_fp8_vec_kernel<T, 128>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), 0, stream, (const T*)qkv,
+      launch_k(rope_store_fp8_vec_kernel<T, 128>, grid, dim3(kStoreThreads), 0, stream, (const T*)qkv,
                (T*)q_out, (const float4*)table, a);
     LLMIE_LAUNCH_CHECK();
     return LLMIE_OK;
   }
   const size_t smem = (size_t)2 * kExpBlock * a.hd * sizeof(float);
-  launch_k(rope_store_fp8_kernel<T>, dim3(blocks, a.n_kv, n_seqs), dim3(kStoreThreads), smem, stream, (const T*)qkv, (T*)q_out,
+  launch_k(rope_store_fp8_kernel<T>, grid, dim3(kStoreThreads), smem, stream, (const T*)qkv, (T*)q_out,
            table, a);
   LLMIE_LAUNCH_CHECK();
   return LLMIE_OK;
@@ -276,23 +317,28 @@ using namespace llmie;
 
 // qkv [T, (n_q + 2 n_kv) hd], q_out [T, n_q hd] of one type; caches e4m3 [pages, n_kv, 64, hd] with exponents int8 [pages, n_kv,
 // 4]; table float32 [table_len, rot_dim / 2, 2] or null (no rotation). cu_q [n_seqs + 1], seq_slot, seq_start [n_seqs]:
-// sequence i brings rows cu_q[i] .. cu_q[i + 1] - 1, at positions from seq_start[i] on. max_q_len: the most that one brings.
+// sequence i brings rows cu_q[i] .. cu_q[i + 1] - 1, at positions from seq_start[i] on. n_tokens: rows of qkv; max_q_len: the most that one brings.
 extern "C" int llmie_rope_store_fp8(const void* qkv, void* q_out, void* k_cache, void* v_cache, void* k_exp, void* v_exp,
                                     const float* table, const int* cu_q, const int* seq_slot, const int* seq_start,
-                                    const int* block_table, int max_pages, int n_seqs, int max_q_len, int n_q, int n_kv,
-                                    int hd, int rot_dim, int table_len, int write_kv, int dtype, cudaStream_t stream) {
-  if (n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0) return LLMIE_ERR_BAD_ARG;
+                                    const int* block_table, int max_pages, int n_tokens, int n_seqs, int max_q_len, int n_q,
+                                    int n_kv, int hd, int rot_dim, int table_len, int write_kv, int dtype, cudaStream_t stream) {
+  if (n_tokens < 0 || n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0) return LLMIE_ERR_BAD_ARG;
   if (hd < 16 || hd > 256 || hd % 16) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (table && (rot_dim <= 0 || rot_dim % 2 || rot_dim > hd || table_len <= 0)) return LLMIE_ERR_BAD_ARG;
   if (write_kv && (!aligned16(k_cache) || !aligned16(v_cache))) return LLMIE_ERR_ALIGNMENT;
   if (table && (reinterpret_cast<uintptr_t>(table) & 7u)) return LLMIE_ERR_ALIGNMENT;
-  if (n_seqs == 0 || max_q_len <= 0) return LLMIE_OK;
-  if (n_seqs > 65535 || n_kv > 65535) return LLMIE_ERR_UNSUPPORTED_SIZE;
-  const StoreArgs a{(unsigned char*)k_cache, (unsigned char*)v_cache, (signed char*)k_exp, (signed char*)v_exp, cu_q, seq_slot,
-                    seq_start, block_table, max_pages, n_q, n_kv, hd, table ? rot_dim : 0, table_len, write_kv ? 1 : 0};
-  // a run of L positions lies in at most (L + 14) / 16 + 1 blocks of 16
-  const int blocks = (max_q_len + kExpBlock - 2) / kExpBlock + 1;
-  if (dtype == LLMIE_F32) return launch_store<float>(qkv, q_out, (const float2*)table, a, blocks, n_seqs, stream);
-  if (dtype == LLMIE_BF16) return launch_store<__nv_bfloat16>(qkv, q_out, (const float2*)table, a, blocks, n_seqs, stream);
+  if (n_tokens == 0 || n_seqs == 0 || max_q_len <= 0) return LLMIE_OK;
+  if (n_kv > 65535) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  StoreArgs a{(unsigned char*)k_cache, (unsigned char*)v_cache, (signed char*)k_exp, (signed char*)v_exp, cu_q, seq_slot,
+                    seq_start, block_table, max_pages, n_q, n_kv, hd, table ? rot_dim : 0, table_len, write_kv ? 1 : 0, n_seqs, 0};
+  // A run of L positions lies in at most (L + 14) / 16 + 1 blocks of 16. A block finds its sequence by its index, or, where most
+  // sequences bring much less than the longest, by the lengths. (A prompt of 2,048 tokens
+  // beside 63 single ones, 32 / 8 heads of 128: 75.9 us by index, 14.2 by the lengths; 9 pieces of 3 to 700 tokens 6.95 and 6.66.)
+  const long long longest = (max_q_len + kExpBlock - 2) / kExpBlock + 1, line = (long long)n_tokens / kExpBlock + 2LL * n_seqs;
+  a.packed = longest * n_seqs > 2 * line || n_seqs > 65535 ? 1 : 0;
+  if (line > 0x7fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  const dim3 grid = a.packed ? dim3((unsigned)line, n_kv, 1) : dim3((unsigned)longest, n_kv, n_seqs);
+  if (dtype == LLMIE_F32) return launch_store<float>(qkv, q_out, (const float2*)table, a, grid, stream);
+  if (dtype == LLMIE_BF16) return launch_store<__nv_bfloat16>(qkv, q_out, (const float2*)table, a, grid, stream);
   return LLMIE_ERR_DTYPE;
 }

@@ -1633,7 +1633,7 @@ FP8_PAGE = 64            # positions of a page
 FP8_BLOCK = 16           # positions that share an exponent
 
 
-_FP8_STORE_ARGS = [_c_void_p] * 11 + [_c_int] * 10 + [_c_void_p]
+_FP8_STORE_ARGS = [_c_void_p] * 11 + [_c_int] * 11 + [_c_void_p]
 _FP8_ATTENTION_ARGS = [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
 _FP8_STEP_ARGS = [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
 _FP8_PROMPT_ARGS = [_c_void_p] * 12 + [_c_int] * 7 + [_c_float, _c_int, _c_void_p]
@@ -1725,8 +1725,8 @@ def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_
     f = _fn("cache_fp8", "llmie_rope_store_fp8", _FP8_STORE_ARGS)
     _check(f(qkv.data_ptr(), q_out.data_ptr(), k_cache.data_ptr() if write_kv else None, v_cache.data_ptr() if write_kv else None,
              k_exp.data_ptr() if write_kv else None, v_exp.data_ptr() if write_kv else None, _ptr(table), cu_q.data_ptr(),
-             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], n_seqs, max_q_len, n_q, n_kv,
-             head_dim, rot_dim, table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()), name)
+             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, n_seqs, max_q_len, n_q,
+             n_kv, head_dim, rot_dim, table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()), name)
     return q_out
 
 

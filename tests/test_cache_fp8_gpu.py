@@ -157,6 +157,33 @@ def test_append_in_pieces(hd):
 
 
 @pytest.mark.parametrize("hd", [48, 64, 128])
+@pytest.mark.parametrize("n_single", [1, 40, 300])
+def test_append_of_a_prompt_beside_single_tokens(hd, n_single):
+    """Steps in which one or two sequences bring much more than the others, some of which bring nothing, with rows behind the last."""
+    n_q, n_kv = 4, 2
+    g = torch.Generator().manual_seed(n_single)
+    news = [1 - (i % 7 == 3) for i in range(n_single)] + [333, 0, 90]
+    starts = torch.randint(0, 40, (len(news),), generator=g).tolist()
+    order = torch.randperm(len(news), generator=g).tolist()
+    news, starts = [news[i] for i in order], [starts[i] for i in order]
+    pc = PlainCache([s + m for s, m in zip(starts, news)], n_kv, hd, seed=hd)
+    for i, st in enumerate(starts):
+        if st:
+            pc.append(i, 0, torch.randn(st, n_kv, hd, generator=g), torch.randn(st, n_kv, hd, generator=g))
+    total = sum(news)
+    qkv = torch.randn(total + 5, (n_q + 2 * n_kv) * hd, generator=g).to(BF)
+    table = angles(512, hd)
+    cache = pc.dev()
+    q = torch.full((total + 5, n_q * hd), 7.0, dtype=BF, device=DEV)
+    cu = [sum(news[:i]) for i in range(len(news) + 1)]
+    ops().rope_store_fp8(qkv.to(DEV), q, *cache, table.to(DEV), i32(cu), i32(pc.slots), i32(starts), pc.table.to(DEV), len(news), max(news),
+                         n_q, n_kv, hd, hd)
+    assert torch.equal(q[:total].cpu(), plain_store(pc, qkv[:total], table, starts, news, n_q, n_kv, hd, hd))
+    assert bool((q[total:] == 7.0).all())
+    check_cache(pc, cache)
+
+
+@pytest.mark.parametrize("hd", [48, 64, 128])
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_append_of_extreme_numbers(hd, dtype):
     """Zeros, the smallest and largest numbers of the type, and numbers that are not finite, each in a block of its own and next
