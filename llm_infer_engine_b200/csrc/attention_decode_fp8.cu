@@ -901,3 +901,38 @@ extern "C" int llmie_attention_decode_fp8_rope(const void* qkv, void* k_cache, v
   return decode_fp8_entry(qkv, k_cache, v_cache, k_exp, v_exp, out, scratch, rope, table_len, seq_slot, seq_kvlen, block_table,
                           max_pages, n_seqs, n_q, n_kv, hd, scale, window, max_kv_len, stream);
 }
+
+// Both by one address, with the arguments one behind another as they are above: a caller from another language converts one
+// argument instead of some twenty, which takes as long as the launch.
+struct DecodeCall {
+  const void *q, *k_cache, *v_cache, *k_exp, *v_exp;
+  void* out;
+  float* scratch;
+  const int *seq_slot, *seq_kvlen, *block_table;
+  int max_pages, n_seqs, n_q, n_kv, hd;
+  float scale;
+  int window, max_kv_len;
+  cudaStream_t stream;
+};
+extern "C" int llmie_attention_decode_fp8_call(const DecodeCall* c) {
+  return llmie_attention_decode_fp8(c->q, c->k_cache, c->v_cache, c->k_exp, c->v_exp, c->out, c->scratch, c->seq_slot, c->seq_kvlen,
+                                    c->block_table, c->max_pages, c->n_seqs, c->n_q, c->n_kv, c->hd, c->scale, c->window,
+                                    c->max_kv_len, c->stream);
+}
+struct DecodeRopeCall {
+  const void* qkv;
+  void *k_cache, *v_cache, *k_exp, *v_exp, *out;
+  float* scratch;
+  const float* rope;
+  int table_len;
+  const int *seq_slot, *seq_kvlen, *block_table;
+  int max_pages, n_seqs, n_q, n_kv, hd;
+  float scale;
+  int window, max_kv_len;
+  cudaStream_t stream;
+};
+extern "C" int llmie_attention_decode_fp8_rope_call(const DecodeRopeCall* c) {
+  return llmie_attention_decode_fp8_rope(c->qkv, c->k_cache, c->v_cache, c->k_exp, c->v_exp, c->out, c->scratch, c->rope, c->table_len,
+                                         c->seq_slot, c->seq_kvlen, c->block_table, c->max_pages, c->n_seqs, c->n_q, c->n_kv, c->hd,
+                                         c->scale, c->window, c->max_kv_len, c->stream);
+}

@@ -1158,3 +1158,22 @@ extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, c
   LLMIE_PREFILL(128);
 #undef LLMIE_PREFILL
 }
+
+// The same by one address, with the arguments one behind another as they are above: a caller from another language converts one
+// argument instead of 22, which takes as long as the launch.
+struct PrefillCall {
+  const void *q, *k_cache, *v_cache, *k_exp, *v_exp;
+  void* out;
+  float* scratch;
+  int* status;
+  const int *cu_q, *seq_slot, *seq_start, *block_table;
+  int max_pages, n_tokens, n_seqs, max_q_len, n_q, n_kv, hd;
+  float scale;
+  int window;
+  cudaStream_t stream;
+};
+extern "C" int llmie_attention_prefill_fp8_call(const PrefillCall* c) {
+  return llmie_attention_prefill_fp8(c->q, c->k_cache, c->v_cache, c->k_exp, c->v_exp, c->out, c->scratch, c->status, c->cu_q, c->seq_slot,
+                                     c->seq_start, c->block_table, c->max_pages, c->n_tokens, c->n_seqs, c->max_q_len, c->n_q, c->n_kv,
+                                     c->hd, c->scale, c->window, c->stream);
+}

@@ -342,3 +342,19 @@ extern "C" int llmie_rope_store_fp8(const void* qkv, void* q_out, void* k_cache,
   if (dtype == LLMIE_BF16) return launch_store<__nv_bfloat16>(qkv, q_out, (const float2*)table, a, grid, stream);
   return LLMIE_ERR_DTYPE;
 }
+
+// The same by one address, with the arguments one behind another as they are above: a caller from another language converts one
+// argument instead of 23, which takes as long as the launch.
+struct RopeStoreCall {
+  const void* qkv;
+  void *q_out, *k_cache, *v_cache, *k_exp, *v_exp;
+  const float* table;
+  const int *cu_q, *seq_slot, *seq_start, *block_table;
+  int max_pages, n_tokens, n_seqs, max_q_len, n_q, n_kv, hd, rot_dim, table_len, write_kv, dtype;
+  cudaStream_t stream;
+};
+extern "C" int llmie_rope_store_fp8_call(const RopeStoreCall* c) {
+  return llmie_rope_store_fp8(c->qkv, c->q_out, c->k_cache, c->v_cache, c->k_exp, c->v_exp, c->table, c->cu_q, c->seq_slot, c->seq_start,
+                              c->block_table, c->max_pages, c->n_tokens, c->n_seqs, c->max_q_len, c->n_q, c->n_kv, c->hd, c->rot_dim,
+                              c->table_len, c->write_kv, c->dtype, c->stream);
+}

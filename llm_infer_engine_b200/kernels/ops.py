@@ -9,6 +9,7 @@ raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -1633,10 +1634,30 @@ FP8_PAGE = 64            # positions of a page
 FP8_BLOCK = 16           # positions that share an exponent
 
 
-_FP8_STORE_ARGS = [_c_void_p] * 11 + [_c_int] * 11 + [_c_void_p]
 _FP8_ATTENTION_ARGS = [_c_void_p] * 10 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
-_FP8_STEP_ARGS = [_c_void_p] * 8 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 5 + [_c_float, _c_int, _c_int, _c_void_p]
-_FP8_PROMPT_ARGS = [_c_void_p] * 12 + [_c_int] * 7 + [_c_float, _c_int, _c_void_p]
+# the arguments of the calls below, as `struct` lays them out like C does
+_FP8_STORE_CALL = "11P11iP"
+_FP8_STEP_CALL = "10P5ifiiP"
+_FP8_STEP_ROPE_CALL = "8Pi3P5ifiiP"
+_FP8_PROMPT_CALL = "12P7ifiP"
+
+
+def _fn_by_address(family: str, name: str, layout: str):
+    """The exported function `name`, which takes the address of its arguments, laid out by `layout`: converting some twenty
+    arguments one by one takes 2 us, as long as a launch."""
+    key = (family, name)
+    f = _fn_cache.get(key)
+    if f is None:
+        raw = getattr(build.load(family), name)
+        raw.argtypes, raw.restype = [ctypes.c_char_p], _c_int
+        _apply_pdl(family)
+
+        def f(*args, _raw=raw, _pack=struct.Struct(layout).pack, _name=name[6:-5]):
+            call, t = _pack(*args), trace.timer
+            return _raw(call) if t is None else t.run(_name, _raw, (call,))
+
+        _fn_cache[key] = f
+    return f
 
 
 def _need_heads(name: str, n_q: int, n_kv: int) -> None:
@@ -1722,9 +1743,9 @@ def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_
         _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
     if trace.timer is not None:
         _work(_nbytes(qkv, q_out) + (2 * T * n_kv * head_dim if write_kv else 0))
-    f = _fn("cache_fp8", "llmie_rope_store_fp8", _FP8_STORE_ARGS)
-    _check(f(qkv.data_ptr(), q_out.data_ptr(), k_cache.data_ptr() if write_kv else None, v_cache.data_ptr() if write_kv else None,
-             k_exp.data_ptr() if write_kv else None, v_exp.data_ptr() if write_kv else None, _ptr(table), cu_q.data_ptr(),
+    f = _fn_by_address("cache_fp8", "llmie_rope_store_fp8_call", _FP8_STORE_CALL)
+    _check(f(qkv.data_ptr(), q_out.data_ptr(), k_cache.data_ptr() if write_kv else 0, v_cache.data_ptr() if write_kv else 0,
+             k_exp.data_ptr() if write_kv else 0, v_exp.data_ptr() if write_kv else 0, 0 if table is None else table.data_ptr(), cu_q.data_ptr(),
              seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, n_seqs, max_q_len, n_q,
              n_kv, head_dim, rot_dim, table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()), name)
     return q_out
@@ -1773,7 +1794,7 @@ _fp8_scratch_floats = {}
 def _with_scratch(name: str, family: str, f, args_before, args_after, key, device) -> None:
     """A launch that needs scratch for partial results where its work is cut, which the launcher decides: asked without scratch
     first, since small calls, where a microsecond counts, do not need any."""
-    status = f(*args_before, None, *args_after)
+    status = f(*args_before, 0, *args_after)
     if status == _NEEDS_SCRATCH:
         floats = _fp8_scratch_floats.get((family, key))
         if floats is None:
@@ -1805,7 +1826,7 @@ def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_k
     _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
     if trace.timer is not None:
         _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8", _FP8_ATTENTION_ARGS)
+    f = _fn_by_address("attention_decode_fp8", "llmie_attention_decode_fp8_call", _FP8_STEP_CALL)
     _with_scratch(name, "attention_decode_fp8", f,
                   (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
                   (seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv,
@@ -1840,7 +1861,7 @@ def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, s
     _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
     if trace.timer is not None:
         _work(_nbytes(qkv, out) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_decode_fp8", "llmie_attention_decode_fp8_rope", _FP8_STEP_ARGS)
+    f = _fn_by_address("attention_decode_fp8", "llmie_attention_decode_fp8_rope_call", _FP8_STEP_ROPE_CALL)
     _with_scratch(name, "attention_decode_fp8", f,
                   (qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
                   (table.data_ptr(), table_len, seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(),
@@ -1883,7 +1904,7 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
     if trace.timer is not None:
         _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
-    f = _fn("attention_prefill_fp8", "llmie_attention_prefill_fp8", _FP8_PROMPT_ARGS)
+    f = _fn_by_address("attention_prefill_fp8", "llmie_attention_prefill_fp8_call", _FP8_PROMPT_CALL)
     _with_scratch(name, "attention_prefill_fp8", f,
                   (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
                   (tc_status_word(q.device).data_ptr(), cu_q.data_ptr(), seq_slot.data_ptr(), seq_start.data_ptr(),
