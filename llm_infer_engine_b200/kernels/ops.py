@@ -1699,13 +1699,17 @@ def _fp8_shapes(name: str, k_cache, v_cache, k_exp, v_exp, n_kv: int, head_dim: 
                           f"{FP8_PAGE // FP8_BLOCK}] are expected")
 
 
-def _fp8_arrays(name: str, block_table, *counted) -> None:
-    """block_table [slots, pages of a sequence]; `counted`: an index array and the entries it must have, in turn."""
-    if block_table.dim() != 2 or block_table.shape[1] < 1:
-        raise KernelError(f"{name}: block_table has shape {tuple(block_table.shape)}, [slots, pages of a sequence] is expected")
-    for t, n in zip(counted[::2], counted[1::2]):
-        if t.dim() != 1 or t.shape[0] < n:
-            raise KernelError(f"{name}: an index array of shape {tuple(t.shape)}, {n} entries are needed")
+def _fp8_arrays(name: str, block_table, *counted) -> int:
+    """block_table [slots, pages of a sequence]; `counted`: an index array and the entries it must have, in turn. Returns the pages."""
+    shape = block_table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise KernelError(f"{name}: block_table has shape {tuple(shape)}, [slots, pages of a sequence] is expected")
+    pairs = iter(counted)
+    for t in pairs:
+        n, own = next(pairs), t.shape
+        if len(own) != 1 or own[0] < n:
+            raise KernelError(f"{name}: an index array of shape {tuple(own)}, {n} entries are needed")
+    return shape[1]
 
 
 def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_slot, seq_start, block_table, n_seqs: int,
@@ -1726,7 +1730,7 @@ def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_
     T = qkv.shape[0]
     if qkv.shape != (T, (n_q + 2 * n_kv) * head_dim) or q_out.shape != (T, n_q * head_dim):
         raise KernelError(f"{name}: qkv {tuple(qkv.shape)}, q_out {tuple(q_out.shape)} for {n_q} / {n_kv} heads of {head_dim}")
-    _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
+    max_pages = _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
     if n_seqs < 0 or (T > 0 and max_q_len <= 0):
         raise KernelError(f"{name}: {n_seqs} sequences with at most {max_q_len} new tokens each")
     if head_dim % 16 or not 16 <= head_dim <= 256:
@@ -1746,7 +1750,7 @@ def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_
     f = _fn_by_address("cache_fp8", "llmie_rope_store_fp8_call", _FP8_STORE_CALL)
     _check(f(qkv.data_ptr(), q_out.data_ptr(), k_cache.data_ptr() if write_kv else 0, v_cache.data_ptr() if write_kv else 0,
              k_exp.data_ptr() if write_kv else 0, v_exp.data_ptr() if write_kv else 0, 0 if table is None else table.data_ptr(), cu_q.data_ptr(),
-             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, n_seqs, max_q_len, n_q,
+             seq_slot.data_ptr(), seq_start.data_ptr(), block_table.data_ptr(), max_pages, T, n_seqs, max_q_len, n_q,
              n_kv, head_dim, rot_dim, table_len, 1 if write_kv else 0, _dt(qkv, "qkv"), _stream()), name)
     return q_out
 
@@ -1766,13 +1770,13 @@ def attention_paged_fp8(q, k_cache, v_cache, k_exp, v_exp, out, tok_pos, tok_seq
     if q.shape != (T, n_q * head_dim) or out.shape != q.shape:
         raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_q} heads of {head_dim}")
     _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _fp8_arrays(name, block_table, tok_pos, T, tok_seq, T, seq_slot, 0)
+    max_pages = _fp8_arrays(name, block_table, tok_pos, T, tok_seq, T, seq_slot, 0)
     if head_dim % 16 or not 16 <= head_dim <= 256:
         raise KernelError(f"{name}: head_dim {head_dim} is not supported (multiples of 16 up to 256)")
     _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
     f = _fn("attention_fp8", "llmie_attention_paged_fp8", _FP8_ATTENTION_ARGS)
     _check(f(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr(),
-             tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), block_table.data_ptr(), block_table.shape[1], T, n_q,
+             tok_pos.data_ptr(), tok_seq.data_ptr(), seq_slot.data_ptr(), block_table.data_ptr(), max_pages, T, n_q,
              n_kv, head_dim, scale, window, _dt(q, "q"), _stream()), name)
     return out
 
@@ -1823,13 +1827,13 @@ def attention_decode_fp8(q, k_cache, v_cache, k_exp, v_exp, out, seq_slot, seq_k
     if q.shape != (n, n_q * head_dim) or out.shape != q.shape:
         raise KernelError(f"{name}: q {tuple(q.shape)}, out {tuple(out.shape)} for {n_q} heads of {head_dim}")
     _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
+    max_pages = _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
     if trace.timer is not None:
         _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
     f = _fn_by_address("attention_decode_fp8", "llmie_attention_decode_fp8_call", _FP8_STEP_CALL)
     _with_scratch(name, "attention_decode_fp8", f,
                   (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
-                  (seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), block_table.shape[1], n, n_q, n_kv,
+                  (seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(), max_pages, n, n_q, n_kv,
                    head_dim, scale, window, max_kv_len, _stream()), (n_q, n_kv, head_dim), q.device)
     return out
 
@@ -1858,14 +1862,14 @@ def attention_decode_fp8_rope(qkv, k_cache, v_cache, k_exp, v_exp, out, table, s
         raise KernelError(f"{name}: qkv {tuple(qkv.shape)}, out {tuple(out.shape)}, table {tuple(table.shape)} for {n_q} / {n_kv} "
                           f"heads of {head_dim}")
     _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
-    _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
+    max_pages = _fp8_arrays(name, block_table, seq_slot, n, seq_kvlen, n)
     if trace.timer is not None:
         _work(_nbytes(qkv, out) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
     f = _fn_by_address("attention_decode_fp8", "llmie_attention_decode_fp8_rope_call", _FP8_STEP_ROPE_CALL)
     _with_scratch(name, "attention_decode_fp8", f,
                   (qkv.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
                   (table.data_ptr(), table_len, seq_slot.data_ptr(), seq_kvlen.data_ptr(), block_table.data_ptr(),
-                   block_table.shape[1], n, n_q, n_kv, head_dim, scale, window, max_kv_len, _stream()), (n_q, n_kv, head_dim),
+                   max_pages, n, n_q, n_kv, head_dim, scale, window, max_kv_len, _stream()), (n_q, n_kv, head_dim),
                   qkv.device)
     return out
 
@@ -1901,14 +1905,14 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     _fp8_shapes(name, k_cache, v_cache, k_exp, v_exp, n_kv, head_dim)
     if n_seqs < 0 or (T > 0 and max_q_len <= 0):
         raise KernelError(f"{name}: {n_seqs} sequences with at most {max_q_len} new tokens each")
-    _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
+    max_pages = _fp8_arrays(name, block_table, cu_q, n_seqs + 1, seq_slot, n_seqs, seq_start, n_seqs)
     if trace.timer is not None:
         _work(2 * _nbytes(q) + 2.0 * STEP_HINT["kv_total"] * n_kv * head_dim, 4.0 * n_q * head_dim * STEP_HINT["pairs"])
     f = _fn_by_address("attention_prefill_fp8", "llmie_attention_prefill_fp8_call", _FP8_PROMPT_CALL)
     _with_scratch(name, "attention_prefill_fp8", f,
                   (q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), out.data_ptr()),
                   (tc_status_word(q.device).data_ptr(), cu_q.data_ptr(), seq_slot.data_ptr(), seq_start.data_ptr(),
-                   block_table.data_ptr(), block_table.shape[1], T, n_seqs, max_q_len, n_q, n_kv, head_dim, scale, window, _stream()),
+                   block_table.data_ptr(), max_pages, T, n_seqs, max_q_len, n_q, n_kv, head_dim, scale, window, _stream()),
                   (head_dim,), q.device)
     return out
 
