@@ -101,7 +101,7 @@ struct PrefillArgs {
   int max_pages, n_seqs, n_q, n_kv;
   float scale2;
   int window;
-  int run;                           // no run is shorter: what the host counted blocks and scratch by
+  int run;                           // no run is shorter: what the host counted blocks and scratch by; 0: it counted on whole tiles
 };
 
 __device__ __forceinline__ float pf_exp2(float x) {
@@ -190,6 +190,8 @@ __device__ __forceinline__ int pf_runs(int last, int run) { return run < 0 ? max
 // 4/3 last / run runs, and at most last / run of them more than tiles; and last <= first + last, whose sum is 2 T. So all cut
 // sequences have 4/3 148 < kPfSlots runs, and 148 more than tiles. The search goes on to 16 T / 148, where there are 18 more than
 // tiles: up to kPfFew it finds one.
+// Where the host has counted on whole tiles (a.run 0), they stay whole, whatever the lengths are: there is no scratch then, no join, and a
+// block for each tile. It judges by the rows of the step, of which the sequences may have few.
 // `mine`: the lane's first sequence. All lanes of a warp call it, and every block gets the same answer.
 template <int KEYS> __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
   const int lane = threadIdx.x & 31;
@@ -202,7 +204,7 @@ template <int KEYS> __device__ __forceinline__ int pf_run(const PrefillArgs& a, 
     tiles += q.tiles;
     longest = max(longest, q.last);
   }
-  if (__reduce_max_sync(0xffffffffu, longest) <= kPfWhole / KEYS) return 1 << 30;
+  if (a.run == 0 || __reduce_max_sync(0xffffffffu, longest) <= kPfWhole / KEYS) return 1 << 30;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) twice += __shfl_xor_sync(0xffffffffu, twice, o);
   const float share = twice * (float)a.n_kv / kPfSms;                        // 2 T / 148
@@ -1091,36 +1093,50 @@ template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 3
   }
 }
 
-template <int HD, bool TURNS>
-static int launch_prefill_fp8(PrefillArgs a, int n_tokens, int max_q_len, cudaStream_t stream) {
+// What the host settles of a call before it launches. Nothing of the lengths is known but that they are n_tokens together at most.
+struct PfPlan {
+  int run;                           // PrefillArgs::run
+  bool cut;                          // whether tiles of tokens may be cut into runs: scratch, and a join
+  long long items, blocks;           // tiles of tokens x key/value heads at most; thread blocks of the kernel
+  long long most_tiles;              // key tiles that a token may see
+};
+template <int HD> static PfPlan pf_plan(int n_tokens, int n_seqs, int max_q_len, int max_pages, int n_q, int n_kv, int window) {
   using Cfg = PfCfg<HD>;
-  cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<HD, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
-  if (e != cudaSuccess) return (int)e;
-  const int tok = (TURNS ? 1 : 2) * (kPfRows / (a.n_q / a.n_kv));
+  PfPlan p;
+  const int tok_x = kPfRows / (n_q / n_kv), tok = (max_q_len <= tok_x ? 1 : 2) * tok_x;
   // Pieces of work: the tiles of tokens, and the runs that they may be cut into (see pf_run). The most runs that a tile can have
   // follow from the most keys that the table has room for and the least work that so many tokens are.
-  const long long items = max_q_len <= tok ? (long long)a.n_seqs * a.n_kv : ((long long)n_tokens / tok + a.n_seqs) * a.n_kv;
-  double least = (double)n_tokens / tok * a.n_kv;
-  long long most_tiles = ((long long)a.max_pages * kFp8Page + Cfg::kKeys - 1) / Cfg::kKeys;
-  if (a.window == 0) {
-    least *= (1.0 + (double)n_tokens / ((double)Cfg::kKeys * a.n_seqs)) / 2;
+  p.items = max_q_len <= tok ? (long long)n_seqs * n_kv : ((long long)n_tokens / tok + n_seqs) * n_kv;
+  double least = (double)n_tokens / tok * n_kv;
+  p.most_tiles = ((long long)max_pages * kFp8Page + Cfg::kKeys - 1) / Cfg::kKeys;
+  if (window == 0) {
+    least *= (1.0 + (double)n_tokens / ((double)Cfg::kKeys * n_seqs)) / 2;
   } else {
-    const long long w = a.window < 0 ? -(long long)a.window : a.window;
-    most_tiles = min(most_tiles, (w + tok) / Cfg::kKeys + 2);
+    const long long w = window < 0 ? -(long long)window : window;
+    p.most_tiles = min(p.most_tiles, (w + tok) / Cfg::kKeys + 2);
   }
-  const bool many = (double)n_tokens / tok * a.n_kv > kPfSms;                // more tiles than SMs whatever the sequences' lengths
+  const bool many = (double)n_tokens / tok * n_kv > kPfSms;                  // more tiles than SMs whatever the sequences' lengths
   long long run = (long long)(least * (many ? 2 : 1) / kPfSms);
   run = min(max(run, (long long)kPfLeast / Cfg::kKeys), 1LL << 30);
-  const bool cut = most_tiles > kPfWhole / Cfg::kKeys && (many ? (most_tiles + run / 2) / run > 1 : most_tiles > run);
-  if (cut && !a.part) return kPfNeedsScratch;
-  a.run = (int)run;
-  const long long blocks = !cut ? items : items <= kPfFew ? kPfSms : items + kPfSms;
-  if (blocks * most_tiles > 0x3fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
-  launch_k(prefill_fp8_kernel<HD, TURNS>, dim3((unsigned)blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
+  p.cut = p.most_tiles > kPfWhole / Cfg::kKeys && (many ? (p.most_tiles + run / 2) / run > 1 : p.most_tiles > run);
+  p.run = p.cut ? (int)run : 0;
+  p.blocks = !p.cut ? p.items : p.items <= kPfFew ? kPfSms : p.items + kPfSms;
+  return p;
+}
+
+template <int HD, bool TURNS>
+static int launch_prefill_fp8(PrefillArgs a, const PfPlan& plan, cudaStream_t stream) {
+  using Cfg = PfCfg<HD>;
+  if (plan.cut && !a.part) return kPfNeedsScratch;
+  if (plan.blocks * plan.most_tiles > 0x3fffffffLL) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<HD, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  if (e != cudaSuccess) return (int)e;
+  a.run = plan.run;
+  launch_k(prefill_fp8_kernel<HD, TURNS>, dim3((unsigned)plan.blocks), dim3(kPfThreads), Cfg::kSmem, stream, a);
   LLMIE_LAUNCH_CHECK();
-  if (cut) {
-    const unsigned side = (unsigned)max(1LL, min((long long)kPfJoinSide, 8LL * kPfSms / items));
-    launch_k(prefill_fp8_join_kernel<HD, TURNS>, dim3((unsigned)items, side), dim3(kPfJoinWarps * 32), 0, stream, a);
+  if (plan.cut) {
+    const unsigned side = (unsigned)max(1LL, min((long long)kPfJoinSide, 8LL * kPfSms / plan.items));
+    launch_k(prefill_fp8_join_kernel<HD, TURNS>, dim3((unsigned)plan.items, side), dim3(kPfJoinWarps * 32), 0, stream, a);
     LLMIE_LAUNCH_CHECK();
   }
   return LLMIE_OK;
@@ -1153,10 +1169,31 @@ extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, c
                       (const signed char*)v_exp, (__nv_bfloat16*)out, scratch, status, cu_q, seq_slot, seq_start, block_table,
                       max_pages, n_seqs, n_q, n_kv, scale * 1.4426950408889634f, window, 0};
   const bool turns = max_q_len <= kPfRows / (n_q / n_kv);
-#define LLMIE_PREFILL(HD) return turns ? launch_prefill_fp8<HD, true>(a, n_tokens, max_q_len, stream) : launch_prefill_fp8<HD, false>(a, n_tokens, max_q_len, stream)
-  if (hd == 64) LLMIE_PREFILL(64);
+#define LLMIE_PREFILL(HD)                                                                                    \
+  const PfPlan plan = pf_plan<HD>(n_tokens, n_seqs, max_q_len, max_pages, n_q, n_kv, window);               \
+  return turns ? launch_prefill_fp8<HD, true>(a, plan, stream) : launch_prefill_fp8<HD, false>(a, plan, stream)
+  if (hd == 64) {
+    LLMIE_PREFILL(64);
+  }
   LLMIE_PREFILL(128);
 #undef LLMIE_PREFILL
+}
+
+// How such a call is laid out, on the host: plan[0] the length of a run that the device's cut goes by, in key tiles of 128 (head size 64) or 64
+// (128) keys, plan[1] whether tiles may be cut (scratch and a join), plan[2] thread blocks, plan[3] the partial results that there is room for.
+extern "C" int llmie_attention_prefill_fp8_plan(int n_tokens, int n_seqs, int max_q_len, int max_pages, int n_q, int n_kv, int hd,
+                                                int window, long long* plan) {
+  if (n_tokens <= 0 || n_seqs <= 0 || max_q_len <= 0 || max_pages <= 0 || n_kv <= 0 || n_q % n_kv || n_q / n_kv < 1 ||
+      n_q / n_kv > kPfRows)
+    return LLMIE_ERR_BAD_ARG;
+  if (hd != 64 && hd != 128) return LLMIE_ERR_UNSUPPORTED_SIZE;
+  const PfPlan p = hd == 64 ? pf_plan<64>(n_tokens, n_seqs, max_q_len, max_pages, n_q, n_kv, window)
+                            : pf_plan<128>(n_tokens, n_seqs, max_q_len, max_pages, n_q, n_kv, window);
+  plan[0] = p.run;
+  plan[1] = p.cut;
+  plan[2] = p.blocks;
+  plan[3] = kPfSlots;
+  return LLMIE_OK;
 }
 
 // The same by one address, with the arguments one behind another as they are above: a caller from another language converts one
