@@ -1804,7 +1804,9 @@ def _with_scratch(name: str, family: str, f, args_before, args_after, key, devic
         if floats is None:
             ask = _fn(family, f"llmie_{family}_scratch", [_c_int] * len(key), query=True)
             floats = _fp8_scratch_floats[family, key] = int(ask(*key))
-        status = f(*args_before, torch.empty(floats, dtype=torch.float32, device=device).data_ptr(), *args_after)
+        # held until the launch is in the stream: memory given back before that may be another host thread's by then
+        scratch = torch.empty(floats, dtype=torch.float32, device=device)
+        status = f(*args_before, scratch.data_ptr(), *args_after)
     _check(status, name)
 
 

@@ -115,3 +115,28 @@ def test_the_plain_exponent_is_the_smallest_that_fits():
                    (1e-30, -64), (2.0 ** 127, 119), (448.0 * 2.0 ** -64, -64), (float("inf"), -64)):
         assert fp8_cache.exponent_of(torch.tensor([big, -big / 3])) == (fp8_cache.exponent_of(torch.tensor([0.0]))
                                                                        if big == float("inf") else e), big
+
+
+def test_scratch_is_held_until_the_launch_is_in_the_stream(monkeypatch):
+    """Given back before the call, its memory could go to another host thread, or be unmapped, before the kernel is launched."""
+    import weakref
+    made = []
+
+    def empty(*shape, **kw):
+        t = torch.zeros(*shape, **kw)
+        made.append(weakref.ref(t))
+        return t
+
+    calls = []
+
+    def launch(*args):
+        calls.append(args)
+        if not args[1]:
+            return ops._NEEDS_SCRATCH
+        assert made[-1]() is not None and made[-1]().data_ptr() == args[1]
+        return 0
+
+    monkeypatch.setattr(ops.torch, "empty", empty)
+    monkeypatch.setitem(ops._fp8_scratch_floats, ("some_family", (1, 2)), 64)
+    ops._with_scratch("some_call", "some_family", launch, ("before",), ("after",), (1, 2), "cpu")
+    assert [c[0] for c in calls] == ["before"] * 2 and [c[2] for c in calls] == ["after"] * 2 and len(made) == 1
