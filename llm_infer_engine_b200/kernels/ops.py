@@ -1654,7 +1654,7 @@ def _fn_by_address(family: str, name: str, layout: str):
 
         def f(*args, _raw=raw, _pack=struct.Struct(layout).pack, _name=name[6:-5]):
             call, t = _pack(*args), trace.timer
-            return _raw(call) if t is None else t.run(_name, _raw, (call,))
+            return _raw(call) if t is None else t.run(_name, _raw, (call,), _NEEDS_SCRATCH)
 
         _fn_cache[key] = f
     return f

@@ -75,12 +75,17 @@ class KernelTimer:
         """What the next launch has to read and write (bytes) and compute (flops), as the caller counts it."""
         self._pending = (float(nbytes), float(flops))
 
-    def run(self, name: str, fn, args):
+    def run(self, name: str, fn, args, refusal: Optional[int] = None):
+        """`refusal`: what `fn` answers where it has launched nothing and is asked again, differently: no record, and what was
+        noted is left for the next time."""
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-        nbytes, flops = self._pending
+        nbytes, flops = noted = self._pending
         self._pending = (0.0, 0.0)
         start.record()
         out = fn(*args)
+        if refusal is not None and out == refusal:
+            self._pending = noted
+            return out
         end.record()
         self.records.append((name, generic_stage(), start, end, nbytes, flops))
         return out

@@ -140,3 +140,40 @@ def test_scratch_is_held_until_the_launch_is_in_the_stream(monkeypatch):
     monkeypatch.setitem(ops._fp8_scratch_floats, ("some_family", (1, 2)), 64)
     ops._with_scratch("some_call", "some_family", launch, ("before",), ("after",), (1, 2), "cpu")
     assert [c[0] for c in calls] == ["before"] * 2 and [c[2] for c in calls] == ["after"] * 2 and len(made) == 1
+
+
+def test_a_timer_counts_a_call_that_is_asked_again_with_scratch_once(monkeypatch):
+    from llm_infer_engine_b200.kernels import trace
+    marks = []
+
+    class Event:
+        def __init__(self, **kw):
+            pass
+
+        def record(self):
+            marks.append(self)
+
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    timer = trace.KernelTimer()
+    answers = [ops._NEEDS_SCRATCH, 0, 0]
+    monkeypatch.setattr(trace, "timer", timer)
+
+    class Raw:
+        argtypes = restype = None
+
+        def __call__(self, call):
+            return answers.pop(0)
+
+    class Library:
+        llmie_some_call = Raw()
+
+    monkeypatch.setattr(ops.build, "load", lambda family: Library())
+    monkeypatch.setattr(ops, "_apply_pdl", lambda family: None)
+    monkeypatch.setitem(ops._fp8_scratch_floats, ("some_family", (1, 2)), 64)
+    monkeypatch.setattr(ops, "_fn_cache", {})
+    f = ops._fn_by_address("some_family", "llmie_some_call", "3P")
+    timer.note(100.0, 7.0)
+    ops._with_scratch("some_call", "some_family", f, (1,), (2,), (1, 2), "cpu")
+    assert [r[0] for r in timer.records] == ["some"] and timer.records[0][4:] == (100.0, 7.0)
+    ops._with_scratch("some_call", "some_family", f, (1,), (2,), (1, 2), "cpu")
+    assert len(timer.records) == 2 and timer.records[1][4:] == (0.0, 0.0) and not answers
