@@ -307,9 +307,10 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
     }
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // the exponent that brings the largest number into [2^14, 2^15); a head that is not finite stays as it is
+    // The exponent that brings the largest number into [2^14, 2^15): 141 - eb, -113 at least. (Below 2^-112 it stays lower, in [2^-7, 2^14):
+    // half precision has all digits of bfloat16 there too.) A head that is not finite stays as it is.
     const int eb = (int)(__float_as_uint(big) >> 23);
-    const int shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);
+    const int shift = eb == 255 ? 0 : min(141 - eb, 126);
     const float f = pow2_of(shift);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       // the first and last keys that every row of the tile sees
       const int all_to = first, all_from = first_visible_key(first + n_more, a.window);
       // Queries become half precision where they lie, a row by its thread, with the power of two that brings its largest number into
-      // [2^14, 2^15).
+      // [2^14, 2^15): 2^-113 at least, 2^126 at most (numbers below 2^-112 end up from 2^-7 on, with all digits of bfloat16).
       float f;                         // of the row's scores: scale log2(e) and the power of two
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
 #pragma unroll
           for (int e = 0; e < 4; ++e) big[e] = max(big[e], max(u[e] & 0x7fffu, u[e] >> 16 & 0x7fffu));
         }
-        const int eb = (int)(max(max(big[0], big[1]), max(big[2], big[3])) >> 7), shift = eb == 255 ? 0 : min(max(141 - eb, -100), 100);
+        const int eb = (int)(max(max(big[0], big[1]), max(big[2], big[3])) >> 7), shift = eb == 255 ? 0 : min(141 - eb, 126);
         const float up = pow2_of(shift);
         f = a.scale2 * pow2_of(-shift);
 #pragma unroll 4

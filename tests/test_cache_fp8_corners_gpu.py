@@ -1,12 +1,9 @@
 """The kernels of a cache in 8 bits at corners that their documentation allows, against tests/fp8_cache.py. Bounds: see test_cache_fp8_gpu.py."""
-import math
-
 import pytest
 import torch
 
 import fp8_cache
-from fp8_cache import F8, PlainCache
-from test_cache_fp8_gpu import BF, DEV, F32, allowed, angles, check_cache, check_prompt, filled, i32, ops, plain_store, prompt, same_bits, store
+from test_cache_fp8_gpu import BF, DEV, allowed, check_prompt, filled, i32, ops, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +26,27 @@ def test_prompt_with_many_rows_behind_its_one_sequence(hd, start, new, rows, max
         ops().check_tc_status(DEV)
         assert bool((out[new:] == 3.0).all())
         check_prompt(pc, out[:new].cpu().double(), q, [start], [new], n_q, n_kv, hd, hd ** -0.5, 0, rows=[0, 1, 17, 31, 32])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("power", [116, 124, -100, -112, -126])
+def test_queries_near_the_ends_of_their_range(hd, power):
+    """Queries of 2^power with a scale that makes ordinary scores of them: half precision inside has room for every finite bfloat16. (2^-126:
+    most are subnormal.)"""
+    n_q, n_kv, starts, news = 8, 2, [150, 0], [40, 200]
+    lens = [s + m for s, m in zip(starts, news)]
+    pc = filled(lens, n_kv, hd, seed=5, spread=0.3)
+    q = (torch.randn(sum(news), n_q * hd, generator=torch.Generator().manual_seed(3)) * 2.0 ** power).to(BF)
+    assert bool(torch.isfinite(q).all()) and float(q.abs().max()) > 2.0 ** power
+    scale = 2.0 ** (-power - 3)
+    out = prompt(pc, q, starts, news, n_q, n_kv, hd, scale, 0)
+    check_prompt(pc, out, q, starts, news, n_q, n_kv, hd, scale, 0, rows=[0, 1, 17, 100, 128])
+    last = q[[news[0] - 1, sum(news) - 1]].contiguous()
+    got = torch.empty_like(last, device=DEV)
+    for max_len in (200, 0):
+        ops().attention_decode_fp8(last.to(DEV), *pc.dev(), got, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, scale, 0, max_len)
+        for i, l in enumerate(lens):
+            want, size = fp8_cache.attention(last[i:i + 1].double().view(1, n_q, hd), *pc.held(i, l), [l - 1], scale, 0)
+            bound = allowed(want, size, BF, True)
+            err = (got[i].cpu().double().view(1, n_q, hd) - want).abs()
+            assert bool((err <= bound).all()), float((err / bound).max())
