@@ -57,6 +57,12 @@ __device__ __forceinline__ unsigned df_half2(float a, float b) {
 }
 __device__ __forceinline__ unsigned df_lo(unsigned w) { return e4m3x2_to_half2((unsigned short)(w & 0xffffu)); }
 __device__ __forceinline__ unsigned df_hi(unsigned w) { return e4m3x2_to_half2((unsigned short)(w >> 16)); }
+// What is beyond float32 as its largest number (NaN stays): infinity times a product that is zero would be NaN.
+__device__ __forceinline__ float df_finite(float x) {
+  float y;
+  asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f7f7fffff;\n\tmax.NaN.f32 %0, t, 0fff7fffff;\n\t}" : "=f"(y) : "f"(x));
+  return y;
+}
 struct DecodeArgs {
   const unsigned char* k;            // [pages, n_kv, 64, HD] codes
   const unsigned char* v;
@@ -380,7 +386,7 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
       const int p = p0 + b * kExpBlock + g;
 #pragma unroll
       for (int nh = 0; nh < NH; ++nh) {
-        const float f0 = q_scale[nh][0] * kf, f1 = q_scale[nh][1] * kf;
+        const float f0 = df_finite(q_scale[nh][0] * kf), f1 = df_finite(q_scale[nh][1] * kf);
         float* x = s[b][nh];
         x[0] = fmaf(x[0], f0, add);
         x[1] = fmaf(x[1], f1, add);

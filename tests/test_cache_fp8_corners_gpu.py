@@ -50,3 +50,29 @@ def test_queries_near_the_ends_of_their_range(hd, power):
             bound = allowed(want, size, BF, True)
             err = (got[i].cpu().double().view(1, n_q, hd) - want).abs()
             assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_large_queries_that_large_keys_are_orthogonal_to(hd, sign):
+    """A block of keys near the largest number, queries as large, and products that are all zero: every score is 0, and an ordinary mean of
+    the values comes out, although the factor of such a block's scores is beyond float32. (Prompts take no negative scale.)"""
+    n_q, n_kv, l = 4, 2, 100
+    g = torch.Generator().manual_seed(6)
+    pc = fp8_cache.PlainCache([l], n_kv, hd, seed=4, nan_stale=True)
+    k = torch.randn(l, n_kv, hd, generator=g)
+    k[:, :, 1::2] = 0.0
+    k[32:48] *= 1e37
+    pc.append(0, 0, k, torch.randn(l, n_kv, hd, generator=g))
+    q = torch.zeros(6, n_q, hd)
+    q[:, :, 1::2] = torch.randn(6, n_q, hd // 2, generator=g) * 1e37
+    q = q.reshape(6, -1).to(BF)
+    if sign > 0:
+        out = prompt(pc, q, [l - 6], [6], n_q, n_kv, hd, hd ** -0.5, 0)
+        check_prompt(pc, out, q, [l - 6], [6], n_q, n_kv, hd, hd ** -0.5, 0)
+    got = torch.empty(1, n_q * hd, dtype=BF, device=DEV)
+    for max_len in (l, 0):
+        ops().attention_decode_fp8(q[:1].to(DEV), *pc.dev(), got, i32(pc.slots), i32([l]), pc.table.to(DEV), n_q, n_kv, hd, sign * hd ** -0.5, 0,
+                                   max_len)
+        want, size = fp8_cache.attention(q[:1].double().view(1, n_q, hd), *pc.held(0, l), [l - 1], sign * hd ** -0.5, 0)
+        assert bool(((got.cpu().double().view(1, n_q, hd) - want).abs() <= allowed(want, size, BF, True)).all())
