@@ -151,10 +151,12 @@ __host__ __device__ constexpr uint32_t pf_instr_desc(int m, int n, int b_mn) {
 }
 
 // ------------------------------------------------------------------------------------------ the cut of the work
-// Key tiles of a sequence's tile of tokens [t0, t0 + n): from `lo` on, `count` of them. None behind the table's last page.
+// Key tiles of a sequence's tile of tokens [t0, t0 + n): from `lo` on, `count` of them. None behind the table's last page: tokens at
+// positions that the table has no room for (a caller's mistake) see what one at its last position sees.
 template <int KEYS> __device__ __forceinline__ void pf_tiles(const PrefillArgs& a, int start, int t0, int n, int& lo, int& count) {
-  lo = first_visible_key(start + t0, a.window) / KEYS;
-  count = max((min(start + t0 + n, a.max_pages * kFp8Page) - 1) / KEYS - lo + 1, 0);
+  const int room = a.max_pages * kFp8Page;
+  lo = first_visible_key(min(start + t0, room - 1), a.window) / KEYS;
+  count = max((min(start + t0 + n, room) - 1) / KEYS - lo + 1, 0);
 }
 // What a lane knows of its sequence: tiles of tokens, the key tiles of the first and the last of them.
 struct PfSequence {
@@ -461,9 +463,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       const PfPiece& w = sh.work[n % kPfAhead];
       const int n_x = x ? w.n_b : w.n_a, c0 = w.c0;
       const int first = w.pos0 + (TURNS ? 0 : x * tok_x), n_more = max((x ? w.n_tok_b : w.n_tok_a) - 1, 0);
-      const int qpos = first + min(rt, n_more), lo = first_visible_key(qpos, a.window);
+      const int end = a.max_pages * kFp8Page - 1;            // the last position that the table has room for
+      const int qpos = min(first + min(rt, n_more), end), lo = first_visible_key(qpos, a.window);
       // the first and last keys that every row of the tile sees
-      const int all_to = first, all_from = first_visible_key(first + n_more, a.window);
+      const int all_to = min(first, end), all_from = first_visible_key(min(first + n_more, end), a.window);
       // Queries become half precision where they lie, a row by its thread, with the power of two that brings its largest number into
       // [2^14, 2^15): 2^-113 at least, 2^126 at most (numbers below 2^-112 end up from 2^-7 on, with all digits of bfloat16).
       float f;                         // of the row's scores: scale log2(e) and the power of two

@@ -76,3 +76,34 @@ def test_large_queries_that_large_keys_are_orthogonal_to(hd, sign):
                                    max_len)
         want, size = fp8_cache.attention(q[:1].double().view(1, n_q, hd), *pc.held(0, l), [l - 1], sign * hd ** -0.5, 0)
         assert bool(((got.cpu().double().view(1, n_q, hd) - want).abs() <= allowed(want, size, BF, True)).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("pages", [1, 2, 3, 15])
+@pytest.mark.parametrize("window", [0, 40, -48])
+def test_prompts_longer_than_their_table(hd, pages, window):
+    """Tokens behind the table's last page (a caller's mistake) see what one at its last position sees, as the plain kernel has it: no key
+    that is not there, however many pages a step of the kernel has."""
+    n_q, n_kv, room = 8, 2, 64 * pages
+    starts, news = [room - 20, room + 30, max(room - 70, 0), 0], [40, 3, 90, room + 5]
+    pc = filled([room + 64] * 4, n_kv, hd, seed=pages)
+    table = pc.table[:, :pages].contiguous().to(DEV)
+    q = torch.randn(sum(news), n_q * hd, generator=torch.Generator().manual_seed(2)).to(BF)
+    cu = [sum(news[:i]) for i in range(5)]
+    out = torch.full((sum(news), n_q * hd), float("nan"), dtype=BF, device=DEV)
+    ops().attention_prefill_fp8(q.to(DEV), *pc.dev(), out, i32(cu), i32(pc.slots), i32(starts), table, 4, max(news), n_q, n_kv, hd,
+                                hd ** -0.5, window)
+    ops().check_tc_status(DEV)
+    plain = torch.empty_like(out)
+    pos = [s + j for s, m in zip(starts, news) for j in range(m)]
+    ops().attention_paged_fp8(q.to(DEV), *pc.dev(), plain, i32(pos), i32([i for i, m in enumerate(news) for _ in range(m)]), i32(pc.slots),
+                              table, n_q, n_kv, hd, hd ** -0.5, window)
+    for i, (st, m) in enumerate(zip(starts, news)):
+        k, v = pc.held(i, room)
+        pick = sorted({0, m // 2, max(room - st - 1, 0), min(max(room - st, 0), m - 1), m - 1} & set(range(m)))
+        want, size = fp8_cache.attention(q[cu[i]:cu[i] + m].double().view(m, n_q, hd)[pick], k, v, [min(st + r, room - 1) for r in pick],
+                                         hd ** -0.5, window)
+        for got, tensor_cores in ((out, True), (plain, False)):
+            err = (got[cu[i]:cu[i] + m].cpu().double().view(m, n_q, hd)[pick] - want).abs()
+            bound = allowed(want, size, BF, tensor_cores)
+            assert bool((err <= bound).all()), (i, tensor_cores, float((err / bound).max()))

@@ -35,7 +35,7 @@ def device_cut(run, starts, news, max_q_len, max_pages, n_q, n_kv, hd, window):
     tok = tok_x if max_q_len <= tok_x else 2 * tok_x
 
     def tiles_of(start, t0, n):
-        lo = first_visible(start + t0, window) // keys
+        lo = first_visible(min(start + t0, max_pages * 64 - 1), window) // keys
         return max((min(start + t0 + n, max_pages * 64) - 1) // keys - lo + 1, 0)
 
     seqs = []                                                 # tiles of tokens, key tiles of the first and the last of them
@@ -104,6 +104,6 @@ def test_cuts_have_room(host_plan, hd, padded):
         rows = sum(news) + (between(1, 40000) if padded else 0)
         max_q_len = max(news) if rng.random() < 0.8 else min(rows, max(news) + between(1, 500))
         need = -(-max(s + m for s, m in zip(starts, news)) // 64)
-        max_pages = need if rng.random() < 0.5 else between(need, 4 * need)
+        max_pages = need if rng.random() < 0.5 else between(need, 4 * need) if rng.random() < 0.8 else max(1, need // 2)
         window = rng.choice([0, 0, 0, between(1, 20000), -between(1, 20000)])
         check(host_plan, starts, news, rows, max_q_len, max_pages, n_q, n_kv, hd, window)
