@@ -823,7 +823,7 @@ static int launch_decode(const void* q, const DecodeArgs& a, const DecodeStep& s
   const long long items = (long long)a.n_seqs * a.n_kv * chunks;
   // units of the longest sequence, as far as the caller knows
   long long units = max_kv_len > 0 ? max_kv_len : (long long)a.max_pages * kFp8Page;
-  if (a.window > 0 && a.window + kDfUnit < units) units = a.window + kDfUnit;
+  if (a.window > 0 && (long long)a.window + kDfUnit < units) units = (long long)a.window + kDfUnit;
   if (a.window < 0 && -(long long)a.window < units) units = -(long long)a.window;
   units = (units + kDfUnit - 1) / kDfUnit;
   int cluster = 1;                   // blocks that share an item

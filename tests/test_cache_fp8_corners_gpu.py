@@ -107,3 +107,16 @@ def test_prompts_longer_than_their_table(hd, pages, window):
             err = (got[cu[i]:cu[i] + m].cpu().double().view(m, n_q, hd)[pick] - want).abs()
             bound = allowed(want, size, BF, tensor_cores)
             assert bool((err <= bound).all()), (i, tensor_cores, float((err / bound).max()))
+
+
+def test_a_window_as_wide_as_32_bits_is_no_window():
+    """The kernel is chosen by what a window leaves to be read: with the widest one the same as without, to the bit."""
+    n_q, n_kv, hd, lens = 8, 2, 64, [30000, 40]
+    pc = filled(lens, n_kv, hd, seed=3, spread=0.2)
+    q = torch.randn(2, n_q * hd, generator=torch.Generator().manual_seed(2)).to(BF).to(DEV)
+    outs = []
+    for window in (0, 2 ** 31 - 1, 30000, -2 ** 31 + 1):
+        out = torch.empty_like(q)
+        ops().attention_decode_fp8(q, *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5, window, 30000)
+        outs.append(out.cpu())
+    assert all(torch.equal(o, outs[0]) for o in outs)
