@@ -870,7 +870,11 @@ static int decode_fp8_entry(const void* q, const void* k_cache, const void* v_ca
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache)) return LLMIE_ERR_ALIGNMENT;
   if ((reinterpret_cast<uintptr_t>(k_exp) | reinterpret_cast<uintptr_t>(v_exp)) & 3u) return LLMIE_ERR_ALIGNMENT;   // a page's four at once
   if (n_seqs == 0) return LLMIE_OK;
-  if ((double)n_seqs * n_q * max_pages * 2 > 1.0e9) return LLMIE_ERR_UNSUPPORTED_SIZE;       // the line of units is counted in 32 bits
+  // The line of units is counted in 32 bits: of a (sequence, KV head, chunk of 8 or 16 query heads) as many as its table has room for, or as
+  // its window or chunk can touch.
+  const long long chunks = n_q / n_kv <= 8 ? 1 : (n_q / n_kv + 15) / 16, back = window < 0 ? -(long long)window : window;
+  const long long units = back ? min(2LL * max_pages, back / kDfUnit + 2) : 2LL * max_pages;
+  if ((double)n_seqs * n_kv * chunks * units > 2.0e9) return LLMIE_ERR_UNSUPPORTED_SIZE;
   const DecodeArgs a{(const unsigned char*)k_cache, (const unsigned char*)v_cache, (const signed char*)k_exp, (const signed char*)v_exp,
                      (__nv_bfloat16*)out, scratch, seq_slot, seq_kvlen, block_table, max_pages, n_seqs, n_q, n_kv,
                      scale * 1.4426950408889634f, window};

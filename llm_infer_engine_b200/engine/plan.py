@@ -46,7 +46,8 @@ class KernelPlan:
         if getattr(kv, "k_exp", None) is not None:
             # the same over a cache in 8 bits (where query heads do not need two passes over a key/value head)
             if not (ctx.decode and table is not None and options.plain
-                    and ops.attention_decode_fp8_rope_supported(n_q, n_kv, head_dim, qkv.dtype)):
+                    and ops.attention_decode_fp8_rope_supported(n_q, n_kv, head_dim, qkv.dtype)
+                    and ops.attention_decode_fp8_counts(ctx.n_seqs, n_q, n_kv, kv.block_table.shape[1])):
                 return False
             ops.attention_decode_fp8_rope(qkv, kv.k, kv.v, kv.k_exp, kv.v_exp, out, table, ctx.seq_slot, ctx.seq_kvlen,
                                           kv.block_table, n_q, n_kv, head_dim, options.scale, options.reach, ctx.max_kv_len)
@@ -125,10 +126,12 @@ class KernelPlan:
 
     def _attention_fp8(self, ctx, q, kv, out, n_q, n_kv, head_dim, options, gate) -> bool:
         """A cache in 8 bits: bfloat16 with head size 64 or 128 has kernels of its own for one-token steps and for prompts;
-        other sizes and float32 are the plain kernel's."""
+        other sizes, float32 and steps with too many long tables to be counted in 32 bits are the plain kernel's."""
         if not options.plain or not ops.attention_decode_fp8_supported(head_dim, q.dtype):
             return False
         if ctx.decode:
+            if not ops.attention_decode_fp8_counts(ctx.n_seqs, n_q, n_kv, kv.block_table.shape[1]):
+                return False
             ops.attention_decode_fp8(q, kv.k, kv.v, kv.k_exp, kv.v_exp, out, ctx.seq_slot, ctx.seq_kvlen, kv.block_table, n_q,
                                      n_kv, head_dim, options.scale, options.reach, ctx.max_kv_len)
         elif options.scale > 0 and ops.attention_prefill_fp8_supported(n_q, n_kv, head_dim, q.dtype):

@@ -1791,6 +1791,12 @@ def attention_decode_fp8_rope_supported(n_q: int, n_kv: int, head_dim: int, dtyp
     return attention_decode_fp8_supported(head_dim, dtype) and n_kv > 0 and n_q // n_kv <= 16
 
 
+def attention_decode_fp8_counts(n_seqs: int, n_q: int, n_kv: int, max_pages: int) -> bool:
+    """Whether the kernel can count the positions of a step in its 32 bits, were every sequence as long as its table has room for."""
+    heads = n_q // n_kv
+    return n_seqs * n_kv * (1 if heads <= 8 else (heads + 15) // 16) * 2 * max_pages <= 2_000_000_000
+
+
 _NEEDS_SCRATCH = -5          # a launcher's answer to a call without scratch whose work is cut: nothing was launched
 _fp8_scratch_floats = {}
 

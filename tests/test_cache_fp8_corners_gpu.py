@@ -120,3 +120,39 @@ def test_a_window_as_wide_as_32_bits_is_no_window():
         ops().attention_decode_fp8(q, *pc.dev(), out, i32(pc.slots), i32(lens), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5, window, 30000)
         outs.append(out.cpu())
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("n_q,n_kv,window", [(64, 4, 0), (64, 4, 100), (80, 2, 0), (64, 4, -100)])
+def test_many_lanes_with_many_query_heads_and_room_for_a_million_positions(n_q, n_kv, window):
+    """512 lanes over tables of 16,384 pages: the positions of their KV heads are counted, not those of their query heads."""
+    hd, n, held = 64, 512, [1, 40, 70, 200]
+    pc = filled(held, n_kv, hd, seed=1)
+    table = torch.full((pc.table.shape[0], 16384), pc.n_pages - 1, dtype=torch.int32)
+    table[:, :pc.table.shape[1]] = pc.table
+    table, cache = table.to(DEV), pc.dev()
+    who = [i % 4 for i in range(n)]
+    q = torch.randn(n, n_q * hd, generator=torch.Generator().manual_seed(2)).to(BF)
+    for max_len in (200, 0):
+        out = torch.empty(n, n_q * hd, dtype=BF, device=DEV)
+        ops().attention_decode_fp8(q.to(DEV), *cache, out, i32([pc.slots[i] for i in who]), i32([held[i] for i in who]), table, n_q, n_kv, hd,
+                                   hd ** -0.5, window, max_len)
+        for row in list(range(8)) + [255, 510, 511]:
+            i = who[row]
+            want, size = fp8_cache.attention(q[row:row + 1].double().view(1, n_q, hd), *pc.held(i, held[i]), [held[i] - 1], hd ** -0.5, window)
+            bound = allowed(want, size, BF, True)
+            assert bool(((out[row].cpu().double().view(1, n_q, hd) - want).abs() <= bound).all()), row
+
+
+def test_a_step_beyond_32_bits_of_positions_is_refused():
+    n_q = n_kv = 64
+    hd, n = 64, 954
+    pc = filled([3], n_kv, hd, seed=1)
+    table = torch.zeros(pc.table.shape[0], 16384, dtype=torch.int32, device=DEV)
+    table[:, :pc.table.shape[1]] = pc.table.to(DEV)
+    q = torch.zeros(n, n_q * hd, dtype=BF, device=DEV)
+    args = (i32(pc.slots * n), i32([3] * n), table, n_q, n_kv, hd, 0.125)
+    cache = pc.dev()
+    with pytest.raises(ops().KernelError, match="not supported"):
+        ops().attention_decode_fp8(q, *cache, q, *args)
+    ops().attention_decode_fp8(q, *cache, q, *args, 1000)             # as many as a window can touch are few
+    torch.cuda.synchronize()

@@ -177,3 +177,28 @@ def test_a_timer_counts_a_call_that_is_asked_again_with_scratch_once(monkeypatch
     assert [r[0] for r in timer.records] == ["some"] and timer.records[0][4:] == (100.0, 7.0)
     ops._with_scratch("some_call", "some_family", f, (1,), (2,), (1, 2), "cpu")
     assert len(timer.records) == 2 and timer.records[1][4:] == (0.0, 0.0) and not answers
+
+
+def test_one_token_steps_that_cannot_be_counted_go_to_the_plain_kernel(monkeypatch):
+    """The decode kernel counts a step's positions in 32 bits, by items of a KV head, not of a query head; a step beyond that is refused by
+    the kernels of its own, and the caller goes on with append and plain attention."""
+    from types import SimpleNamespace
+    from llm_infer_engine_b200.engine.plan import KernelPlan
+    from llm_infer_engine_b200.parts.base import AttentionOptions
+    assert ops.attention_decode_fp8_counts(512, 64, 8, 16384) and ops.attention_decode_fp8_counts(512, 64, 4, 16384)
+    assert ops.attention_decode_fp8_counts(953, 64, 64, 16384) and not ops.attention_decode_fp8_counts(954, 64, 64, 16384)
+    assert not ops.attention_decode_fp8_counts(954, 64 * 8, 64, 16384)
+    assert not ops.attention_decode_fp8_counts(954, 64 * 17, 32, 16384)         # two chunks of query heads
+    called = []
+    monkeypatch.setattr(ops, "attention_decode_fp8", lambda *a: called.append("decode"))
+    monkeypatch.setattr(ops, "attention_decode_fp8_rope", lambda *a: called.append("step"))
+    plan = KernelPlan(SimpleNamespace(dtype=torch.bfloat16, decode_attention="auto"))
+    x = torch.zeros(1, 1, dtype=torch.bfloat16)
+    for lanes, pages, taken in ((512, 16384, True), (954, 16384, False)):
+        kv = SimpleNamespace(k=None, v=None, k_exp=x, v_exp=x, block_table=torch.empty(1, pages, dtype=torch.int32))
+        ctx = SimpleNamespace(decode=True, n_seqs=lanes, seq_slot=None, seq_kvlen=None, max_kv_len=10)
+        options = AttentionOptions(scale=0.125)
+        assert plan.attention(ctx, x, kv, x, 64, 64, 64, options) is taken
+        assert plan.attention_with_rope(ctx, x, x, kv, x, 64, 64, 64, options, True) is taken
+        assert called == (["decode", "step"] if taken else [])
+        called.clear()
