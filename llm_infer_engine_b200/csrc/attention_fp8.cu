@@ -111,6 +111,7 @@ extern "C" int llmie_attention_paged_fp8(const void* q, const void* k_cache, con
                                          const int* seq_slot, const int* block_table, int max_pages, int n_tokens, int n_q,
                                          int n_kv, int hd, float scale, int window, int dtype, cudaStream_t stream) {
   if (n_tokens < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0) return LLMIE_ERR_BAD_ARG;
+  if (max_pages > kMostPages) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (hd < 16 || hd > kPlainHd || hd % 16) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(k_cache) || !aligned16(v_cache)) return LLMIE_ERR_ALIGNMENT;
   if (n_tokens == 0) return LLMIE_OK;

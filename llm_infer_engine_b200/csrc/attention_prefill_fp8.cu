@@ -1164,6 +1164,7 @@ extern "C" int llmie_attention_prefill_fp8(const void* q, const void* k_cache, c
                                            int n_tokens, int n_seqs, int max_q_len, int n_q, int n_kv, int hd, float scale,
                                            int window, cudaStream_t stream) {
   if (n_tokens < 0 || n_seqs < 0 || n_q <= 0 || n_kv <= 0 || n_q % n_kv || max_pages <= 0 || !status) return LLMIE_ERR_BAD_ARG;
+  if (max_pages > kMostPages) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!(scale > 0.f)) return LLMIE_ERR_BAD_ARG;              // a row's bound is taken before scores are scaled
   if ((hd != 64 && hd != 128) || n_q / n_kv > kPfRows) return LLMIE_ERR_UNSUPPORTED_SIZE;
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(scratch)) return LLMIE_ERR_ALIGNMENT;

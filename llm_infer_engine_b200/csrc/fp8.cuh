@@ -16,6 +16,7 @@ namespace llmie {
 constexpr int kExpBlock = 16;        // positions that share an exponent
 constexpr int kFp8Page = 64;         // positions of a cache page
 constexpr int kPageExps = kFp8Page / kExpBlock;
+constexpr int kMostPages = 0x7fffffff / kFp8Page;            // of a table, that positions can be counted in 32 bits
 constexpr int kExpMin = -64;         // blocks of zeros, and of numbers below 448 * 2^-64
 constexpr int kExpMax = 119;         // numbers above 448 * 2^119 are held as that
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import fp8_cache
-from test_cache_fp8_gpu import BF, DEV, allowed, check_prompt, filled, i32, ops, prompt
+from test_cache_fp8_gpu import BF, DEV, allowed, check_prompt, filled, good_call, i32, ops, prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -155,4 +155,15 @@ def test_a_step_beyond_32_bits_of_positions_is_refused():
     with pytest.raises(ops().KernelError, match="not supported"):
         ops().attention_decode_fp8(q, *cache, q, *args)
     ops().attention_decode_fp8(q, *cache, q, *args, 1000)             # as many as a window can touch are few
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("name", ["attention_paged_fp8", "attention_prefill_fp8", "attention_decode_fp8"])
+def test_tables_whose_positions_pass_32_bits_are_refused(name):
+    """A table of 2^25 pages has room for 2^31 positions."""
+    good = good_call(name)
+    good["block_table"] = torch.zeros(1, 2 ** 25, dtype=torch.int32, device=DEV)
+    good["seq_slot"].zero_()
+    with pytest.raises(ops().KernelError, match="not supported|bad argument"):
+        getattr(ops(), name)(**good)
     torch.cuda.synchronize()
