@@ -35,11 +35,7 @@ constexpr float kDfSlack = 8.f;      // how far scores may outgrow a head's boun
 constexpr float kDfTop = 7.f;        // the bound's own weight is 2^7: none is above 2^15
 constexpr int kDfFew = 12;           // units a warp up to which an item is one cluster's
 
-__device__ __forceinline__ float df_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+__device__ __forceinline__ float df_exp2(float x) { return exp2_ftz(x); }
 __device__ __forceinline__ void df_mma(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -486,13 +482,62 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
   __syncwarp();                      // no lane reads its units any more: the place becomes the results'
   float* sums = reinterpret_cast<float*>(mine);
   float* bounds = sums + Cfg::kHeads * Cfg::kPitch;
+  // The denominators of the whole warp, in every lane.
+  auto all_lanes = [&]() {
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) {
+        l[nh][0] += __shfl_xor_sync(0xffffffffu, l[nh][0], d);
+        l[nh][1] += __shfl_xor_sync(0xffffffffu, l[nh][1], d);
+      }
+  };
+  all_lanes();
+  bool small = false;
+#pragma unroll
+  for (int nh = 0; nh < NH; ++nh)
+    small |= (l[nh][0] < kLeastDenominator && R[nh][0] != -INFINITY) || (l[nh][1] < kLeastDenominator && R[nh][1] != -INFINITY);
+  if (__any_sync(0xffffffffu, small)) {
+    // rare: by the scores alone (see fp8.cuh), the warp's units once more, codes straight from the cache
+#pragma unroll
+    for (int nh = 0; nh < NH; ++nh) l[nh][0] = l[nh][1] = 0.f;
+#pragma unroll 1
+    for (int v = first + u_begin + warp; v < u_stop; v += W) {
+      const size_t row = (size_t)pages[v >> 1] * a.n_kv + hk;
+#pragma unroll 1
+      for (int b = 0; b < 2; ++b) {
+        const int in = (v & 1) * 2 + b, p = v * kDfUnit + b * kExpBlock + g;
+        const unsigned char* key = a.k + (row * kFp8Page + in * kExpBlock + g) * HD + t * 16;
+        float x[NH][4];
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) x[nh][0] = x[nh][1] = x[nh][2] = x[nh][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const unsigned ka = *reinterpret_cast<const unsigned*>(key + (ks >> 2) * 64 + (ks & 3) * 4);
+          const unsigned kb = *reinterpret_cast<const unsigned*>(key + 8 * HD + (ks >> 2) * 64 + (ks & 3) * 4);
+#pragma unroll
+          for (int nh = 0; nh < NH; ++nh) df_mma(x[nh], df_lo(ka), df_lo(kb), df_hi(ka), df_hi(kb), qb[nh][ks][0], qb[nh][ks][1]);
+        }
+        const float kf = pow2_of(clamp_exponent(a.k_exp[row * kPageExps + in]));
+#pragma unroll
+        for (int nh = 0; nh < NH; ++nh) {
+          const float f0 = df_finite(q_scale[nh][0] * kf), f1 = df_finite(q_scale[nh][1] * kf);
+          const float c0 = kDfTop - (R[nh][0] == -INFINITY ? 0.f : R[nh][0]), c1 = kDfTop - (R[nh][1] == -INFINITY ? 0.f : R[nh][1]);
+          if (p >= lo && p < len) {
+            l[nh][0] += exp2_term(fmaf(x[nh][0], f0, c0));
+            l[nh][1] += exp2_term(fmaf(x[nh][1], f1, c1));
+          }
+          if (p + 8 >= lo && p + 8 < len) {
+            l[nh][0] += exp2_term(fmaf(x[nh][2], f0, c0));
+            l[nh][1] += exp2_term(fmaf(x[nh][3], f1, c1));
+          }
+        }
+      }
+    }
+    all_lanes();
+  }
 #pragma unroll
   for (int nh = 0; nh < NH; ++nh) {
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) {
-      l[nh][0] += __shfl_xor_sync(0xffffffffu, l[nh][0], d);
-      l[nh][1] += __shfl_xor_sync(0xffffffffu, l[nh][1], d);
-    }
     if (g == 0) {
       bounds[nh * 8 + 2 * t] = R[nh][0];
       bounds[nh * 8 + 2 * t + 1] = R[nh][1];
@@ -524,9 +569,9 @@ __device__ __forceinline__ void df_of_warps(const unsigned char* smem, int h, in
   num = den = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    const float f = df_exp2(s[w][Cfg::kHeads * Cfg::kPitch + h] - Mu);
+    const float d = s[w][Cfg::kHeads * Cfg::kPitch + h] - Mu, f = df_exp2(d);
     num = fmaf(f, s[w][h * Cfg::kPitch + at], num);
-    den = fmaf(f, s[w][Cfg::kHeads * (Cfg::kPitch + 1) + h], den);
+    den = add_times_exp2(s[w][Cfg::kHeads * (Cfg::kPitch + 1) + h], f, d, den);
   }
 }
 
@@ -681,7 +726,7 @@ decode_fp8_cluster_kernel(const __nv_bfloat16* q, const DecodeArgs a, const Deco
       if (b >= gridDim.x) continue;
       const float f = df_exp2(m[b] - Mu);
       num = fmaf(f, n[b], num);
-      den = fmaf(f, l[b], den);
+      den = add_times_exp2(l[b], f, m[b] - Mu, den);
     }
     out[i] = __float2bfloat16_rn(num / den);
   }
@@ -748,7 +793,7 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
       for (int i = 0; i < 4; ++i) {
         const float f = df_exp2(m[i] - Mu);
         num = fmaf(f, v[i], num);
-        den = fmaf(f, l[i], den);
+        den = add_times_exp2(l[i], f, m[i] - Mu, den);
       }
       out[h * HD + column(x % HD)] = __float2bfloat16_rn(num / den);
     }
@@ -776,9 +821,9 @@ __global__ void __launch_bounds__(kDfSlices * HD) decode_fp8_join_kernel(const D
     const float Mu = M == -INFINITY ? 0.f : M;
     float den = 0.f;
     for (int k = threadIdx.x; k < n; k += kDfSlices * HD) {
-      const float f = df_exp2(factor[k] - Mu);
+      const float d = factor[k] - Mu, f = df_exp2(d);
       factor[k] = f;
-      den = fmaf(f, denom[k], den);
+      den = add_times_exp2(denom[k], f, d, den);
     }
     den = warp_sum(den);
     if (lane == 0) part_den[warp] = den;

@@ -104,11 +104,7 @@ struct PrefillArgs {
   int run;                           // no run is shorter: what the host counted blocks and scratch by; 0: it counted on whole tiles
 };
 
-__device__ __forceinline__ float pf_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+__device__ __forceinline__ float pf_exp2(float x) { return exp2_ftz(x); }
 __device__ __forceinline__ uint32_t pf_half2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -543,6 +539,53 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
           }
         }
       };
+      // Rare: the row's denominator by the scores alone (see fp8.cuh), four keys at a time: some 500 clocks a key, and the block waits.
+      auto by_scores = [&]() {
+        const int row = row_of(w);
+        if (row < 0) return;
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(a.q + (size_t)row * HD);
+        uint32_t big = 0u;
+#pragma unroll 1
+        for (int i = 0; i < HD / 2; ++i) big = max(big, max(q[i] & 0x7fffu, q[i] >> 16 & 0x7fffu));
+        const int eb = (int)(big >> 7);
+        const float up = pow2_of(eb == 255 ? 0 : min(141 - eb, 126)), shift = R - kPfTop;
+        const int* pages = a.block_table + (size_t)w.page_row * a.max_pages;
+        l = 0.f;
+#pragma unroll 1
+        for (int j = 0; j < n_x; ++j) {
+          const int kbase = (c0 + (TURNS ? 2 * j + x : j)) * Cfg::kKeys;
+#pragma unroll 1
+          for (int p = max(lo, kbase) & ~3; p <= min(qpos, kbase + Cfg::kKeys - 1); p += 4) {
+            const size_t head = (size_t)pages[p / kFp8Page] * a.n_kv + w.hk;
+            const uint4* k = reinterpret_cast<const uint4*>(a.k + (head * kFp8Page + p % kFp8Page) * HD);
+            const float fk = factor(pow2_of(clamp_exponent(a.k_exp[head * kPageExps + p % kFp8Page / kExpBlock])));
+            float dot[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int i = 0; i < HD / 16; ++i) {
+              uint32_t y[8];
+              *reinterpret_cast<uint4*>(y) = reinterpret_cast<const uint4*>(q)[2 * i];
+              *reinterpret_cast<uint4*>(y + 4) = reinterpret_cast<const uint4*>(q)[2 * i + 1];
+              uint4 z[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) z[e] = k[e * (HD / 16) + i];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const unsigned c[4] = {z[e].x, z[e].y, z[e].z, z[e].w};
+#pragma unroll
+                for (int h = 0; h < 8; ++h) {
+                  const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y[h]));
+                  const float2 o = e4m3x2_to_float2((unsigned short)(c[h >> 1] >> (h & 1) * 16 & 0xffffu));
+                  dot[e] = fmaf(u.x * up, o.x, dot[e]);
+                  dot[e] = fmaf(u.y * up, o.y, dot[e]);
+                }
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (p + e >= lo && p + e <= qpos) l += exp2_term(fmaf(dot[e], fk, -shift));
+          }
+        }
+      };
 #pragma unroll 1
       for (int j = 0; j < n_x; ++j) {            // this tile's j-th step is the block's `step`
         const int step = gs + (TURNS ? 2 * j + x : j);
@@ -645,6 +688,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         tc_fence_before_sync();
         mbar_arrive(&sh.p_ready[x]);
       }
+      if (ok && l < kLeastDenominator && R != -INFINITY) by_scores();
       // the queries of the piece after this one are asked for while the last product runs
       const int at_end = gs + (TURNS ? 2 * (n_x - 1) + x : n_x - 1);             // this tile's last step
       gx += n_x;
@@ -697,7 +741,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
           const float Rb = sh.handed[0][r], M = fmaxf(R, Rb), Mu = M == -INFINITY ? 0.f : M;
           mine_f = R == -INFINITY ? 0.f : pf_exp2(R - Mu);
           b_f = Rb == -INFINITY ? 0.f : pf_exp2(Rb - Mu);
-          l = fmaf(l, mine_f, sh.handed[1][r] * b_f);
+          l = add_times_exp2(l, mine_f, R - Mu, times_exp2(sh.handed[1][r], b_f, Rb - Mu));
         }
         if (!ok) l = __int_as_float(0x7fffffff);
         const float* handed = reinterpret_cast<const float*>(q_smem) + r * HD;
@@ -1072,13 +1116,13 @@ template <int HD, bool TURNS> __global__ void __launch_bounds__(kPfJoinWarps * 3
 #pragma unroll
       for (int p = 0; p < 8; ++p) M8 = fmaxf(M8, m[p]);
       const float Mu = M8 == -INFINITY ? 0.f : M8, back = M == -INFINITY ? 0.f : pf_exp2(M - Mu);
-      den *= back;
+      if (M != -INFINITY) den = times_exp2(den, back, M - Mu);             // (without a bound there is nothing yet, or NaN, which stays)
 #pragma unroll
       for (int i = 0; i < 4; ++i) num[i] *= back;
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
         const float f = pf_exp2(m[p] - Mu);
-        den = fmaf(f, l[p], den);
+        den = add_times_exp2(l[p], f, m[p] - Mu, den);
         num[0] = fmaf(f, v[p].x, num[0]);
         num[1] = fmaf(f, v[p].y, num[1]);
         num[2] = fmaf(f, v[p].z, num[2]);

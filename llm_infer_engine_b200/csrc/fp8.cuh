@@ -36,6 +36,35 @@ __device__ __forceinline__ unsigned finite_magnitude(float v) {
 }
 __device__ __forceinline__ int clamp_exponent(int e) { return min(max(e, kExpMin), kExpMax); }
 
+// Values of very different size. The tensor-core kernels weight a value's codes with w = 2^(s + ev - R + 7), R the largest s + ev so far
+// less a slack of 8 at most, and sum the softmax's denominator from the same numbers, w 2^(-ev). Beside a block of far larger values, w is
+// below float32 while w 2^(-ev) is not: it is nothing for the numerator, and may be all of the denominator (16 values of 1e30 and 16 zeros
+// that are seen alike are 5e29 on average, not 1e30).
+//   What is lost so is below 2^-126 2^64 = 2^-62 a key, and below 2^(15 + 64 - 126) = 2^-47 where a sum was brought to a bound more than
+// 2^126 above; 2^20 keys together lose less than 2^-27. A denominator from 2^-12 on lacks less than 2^-15 of itself. A smaller one is
+// that of R's own value, 2^(7 - ev) at least, with ev > 19 (values above 2e8), or of others as large: it is taken once more by the scores
+// alone, sum_j 2^(s_j - R + 7). Those terms are below 2^(7 + 8 + 64) and the sum is at least 2^(7 - 119); their exponentials are taken 2^20
+// larger, so that those above 2^-34 of it come out normal.
+constexpr float kLeastDenominator = 0x1p-12f;
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp2_term(float x) { return exp2_ftz(x + 20.f) * 0x1p-20f; }
+// l 2^d, and sum + l 2^d, for sums l that are relative to a bound d <= 0 below the common one (f is 2^d): where 2^d alone would be below
+// float32, in two steps.
+__device__ __forceinline__ float times_exp2(float l, float f, float d) {
+  if (!(d < -100.f)) return l * f;
+  const float half = exp2_ftz(0.5f * d);
+  return l * half * half;
+}
+__device__ __forceinline__ float add_times_exp2(float l, float f, float d, float sum) {
+  if (!(d < -100.f)) return fmaf(f, l, sum);
+  const float half = exp2_ftz(0.5f * d);
+  return fmaf(l * half, half, sum);
+}
+
 // Two numbers, scaled, as two codes (a in the low byte); what is not finite becomes NaN.
 __device__ __forceinline__ unsigned short to_e4m3x2(float a, float b) {
   a = (__float_as_uint(a) & 0x7f800000u) == 0x7f800000u ? __int_as_float(0x7fffffff) : a;

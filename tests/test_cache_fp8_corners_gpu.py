@@ -167,3 +167,146 @@ def test_tables_whose_positions_pass_32_bits_are_refused(name):
     with pytest.raises(ops().KernelError, match="not supported|bad argument"):
         getattr(ops(), name)(**good)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [1e26, 1e30, 1e37])
+@pytest.mark.parametrize("back", [0.0, 90.0])
+def test_values_of_very_different_size(hd, size, back):
+    """A block of values near the largest numbers beside zeros, ordinary ones and tiny ones, seen alike or (back > 0) hardly at all: the others
+    count in the softmax's denominator by their scores, whatever their values are. The block stands first, in the middle and last."""
+    n_q, n_kv, new = 8, 2, 40
+    lens = [100, 333, 1700, 1700]
+    at = [0, 160, 1680, 32]
+    g = torch.Generator().manual_seed(6)
+    pc = fp8_cache.PlainCache(lens, n_kv, hd, seed=4, nan_stale=True)
+    q = torch.randn(len(lens) * new, n_q, hd, generator=g) * 0.5
+    q[:, :, 0] = 1.0
+    for i, (l, p) in enumerate(zip(lens, at)):
+        k, v = 0.5 * torch.randn(l, n_kv, hd, generator=g), torch.randn(l, n_kv, hd, generator=g)
+        k[:, :, 0] = 0.0
+        k[p:p + 16, :, 0] = -back * hd ** 0.5
+        v[::2] *= 1e-3
+        v[16 * (l // 48):] *= 1e-12
+        v[16 * (l // 32):] = 0.0
+        v[p:p + 16] = size * torch.randn(16, n_kv, hd, generator=g).clamp(-3, 3)
+        pc.append(i, 0, k, v)
+    q = q.reshape(len(lens) * new, -1).to(BF)
+    cache, table, scale = pc.dev(), pc.table.to(DEV), hd ** -0.5
+    starts = [l - new for l in lens]
+    # prompts: all sequences in a call, and each alone (in turns and in runs where it is long); tiles of 128 / 4 tokens and more
+    for news in ([new] * 4, [7, 7, 7, 7]):
+        pick = [i * new + j for i, m in enumerate(news) for j in range(m)]
+        rows = [0, 1, 6, 20, 39]
+        out = prompt(pc, q[pick], starts, news, n_q, n_kv, hd, scale, 0, cache)
+        check_prompt(pc, out, q[pick], starts, news, n_q, n_kv, hd, scale, 0, rows=rows)
+    for i in range(4):
+        mine = q[i * new:(i + 1) * new]
+        out = torch.empty(new, n_q * hd, dtype=BF, device=DEV)
+        ops().attention_prefill_fp8(mine.to(DEV), *cache, out, i32([0, new]), i32(pc.slots[i:i + 1]), i32(starts[i:i + 1]), table, 1, new, n_q,
+                                    n_kv, hd, scale)
+        want, size_ = fp8_cache.attention(mine.double().view(new, n_q, hd)[[0, 20, 39]], *pc.held(i, lens[i]),
+                                          [starts[i] + r for r in (0, 20, 39)], scale, 0)
+        err = (out.cpu().double().view(new, n_q, hd)[[0, 20, 39]] - want).abs()
+        assert bool((err <= allowed(want, size_, BF, True)).all()), i
+    last = q[new - 1::new].contiguous()
+    got = torch.empty_like(last, device=DEV)
+    for max_len in (1700, 0):
+        for pick in ([0, 1, 2, 3], [0], [2], [3]):
+            part = torch.empty(len(pick), n_q * hd, dtype=BF, device=DEV)
+            ops().attention_decode_fp8(last[pick].to(DEV), *cache, part, i32([pc.slots[i] for i in pick]), i32([lens[i] for i in pick]), table,
+                                       n_q, n_kv, hd, scale, 0, max_len)
+            got[pick] = part
+            for i in pick:
+                want, size_ = fp8_cache.attention(last[i:i + 1].double().view(1, n_q, hd), *pc.held(i, lens[i]), [lens[i] - 1], scale, 0)
+                err = (got[i].cpu().double().view(1, n_q, hd) - want).abs()
+                bound = allowed(want, size_, BF, True)
+                assert bool((err <= bound).all()), (i, max_len, float((err / bound).max()))
+    plain = torch.empty_like(got)
+    ops().attention_paged_fp8(last.to(DEV), *cache, plain, i32([l - 1 for l in lens]), i32([0, 1, 2, 3]), i32(pc.slots), table, n_q, n_kv, hd,
+                              scale)
+    for i in range(4):
+        want, size_ = fp8_cache.attention(last[i:i + 1].double().view(1, n_q, hd), *pc.held(i, lens[i]), [lens[i] - 1], scale, 0)
+        assert bool(((plain[i].cpu().double().view(1, n_q, hd) - want).abs() <= allowed(want, size_, BF, False)).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [1e26, 1e30, 1e37])
+@pytest.mark.parametrize("back", [0.0, 90.0])
+def test_values_of_very_different_size(hd, size, back):
+    """A block of values near the largest numbers beside zeros, ordinary ones and tiny ones, seen alike or (back > 0) hardly at all: the others
+    count in the softmax's denominator by their scores, whatever their values are. The block stands first, in the middle and last."""
+    n_q, n_kv, new = 8, 2, 40
+    lens = [100, 333, 1700, 1700]
+    at = [0, 160, 1680, 32]
+    g = torch.Generator().manual_seed(6)
+    pc = fp8_cache.PlainCache(lens, n_kv, hd, seed=4, nan_stale=True)
+    q = torch.randn(len(lens) * new, n_q, hd, generator=g) * 0.5
+    q[:, :, 0] = 1.0
+    for i, (l, p) in enumerate(zip(lens, at)):
+        k, v = 0.5 * torch.randn(l, n_kv, hd, generator=g), torch.randn(l, n_kv, hd, generator=g)
+        k[:, :, 0] = 0.0
+        k[p:p + 16, :, 0] = -back * hd ** 0.5
+        v[::2] *= 1e-3
+        v[16 * (l // 48):] *= 1e-12
+        v[16 * (l // 32):] = 0.0
+        v[p:p + 16] = size * torch.randn(16, n_kv, hd, generator=g).clamp(-3, 3)
+        pc.append(i, 0, k, v)
+    q = q.reshape(len(lens) * new, -1).to(BF)
+    cache, table, scale = pc.dev(), pc.table.to(DEV), hd ** -0.5
+    starts = [l - new for l in lens]
+    # prompts: all sequences in a call, and each alone (in turns and in runs where it is long); tiles of 128 / 4 tokens and more
+    for news in ([new] * 4, [7, 7, 7, 7]):
+        pick = [i * new + j for i, m in enumerate(news) for j in range(m)]
+        rows = [0, 1, 6, 20, 39]
+        out = prompt(pc, q[pick], starts, news, n_q, n_kv, hd, scale, 0, cache)
+        check_prompt(pc, out, q[pick], starts, news, n_q, n_kv, hd, scale, 0, rows=rows)
+    for i in range(4):
+        mine = q[i * new:(i + 1) * new]
+        out = torch.empty(new, n_q * hd, dtype=BF, device=DEV)
+        ops().attention_prefill_fp8(mine.to(DEV), *cache, out, i32([0, new]), i32(pc.slots[i:i + 1]), i32(starts[i:i + 1]), table, 1, new, n_q,
+                                    n_kv, hd, scale)
+        want, size_ = fp8_cache.attention(mine.double().view(new, n_q, hd)[[0, 20, 39]], *pc.held(i, lens[i]),
+                                          [starts[i] + r for r in (0, 20, 39)], scale, 0)
+        err = (out.cpu().double().view(new, n_q, hd)[[0, 20, 39]] - want).abs()
+        assert bool((err <= allowed(want, size_, BF, True)).all()), i
+    last = q[new - 1::new].contiguous()
+    got = torch.empty_like(last, device=DEV)
+    for max_len in (1700, 0):
+        for pick in ([0, 1, 2, 3], [0], [2], [3]):
+            part = torch.empty(len(pick), n_q * hd, dtype=BF, device=DEV)
+            ops().attention_decode_fp8(last[pick].to(DEV), *cache, part, i32([pc.slots[i] for i in pick]), i32([lens[i] for i in pick]), table,
+                                       n_q, n_kv, hd, scale, 0, max_len)
+            got[pick] = part
+            for i in pick:
+                want, size_ = fp8_cache.attention(last[i:i + 1].double().view(1, n_q, hd), *pc.held(i, lens[i]), [lens[i] - 1], scale, 0)
+                err = (got[i].cpu().double().view(1, n_q, hd) - want).abs()
+                bound = allowed(want, size_, BF, True)
+                assert bool((err <= bound).all()), (i, max_len, float((err / bound).max()))
+    plain = torch.empty_like(got)
+    ops().attention_paged_fp8(last.to(DEV), *cache, plain, i32([l - 1 for l in lens]), i32([0, 1, 2, 3]), i32(pc.slots), table, n_q, n_kv, hd,
+                              scale)
+    for i in range(4):
+        want, size_ = fp8_cache.attention(last[i:i + 1].double().view(1, n_q, hd), *pc.held(i, lens[i]), [lens[i] - 1], scale, 0)
+        assert bool(((plain[i].cpu().double().view(1, n_q, hd) - want).abs() <= allowed(want, size_, BF, False)).all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_values_of_very_different_size_in_a_long_prompt(hd):
+    """300 tokens behind 12,000: many rows whose denominators are taken once more, over many keys, while the rest of the block waits."""
+    n_q, n_kv, start, new = 8, 2, 12000, 300
+    l = start + new
+    g = torch.Generator().manual_seed(7)
+    pc = fp8_cache.PlainCache([l], n_kv, hd, seed=4)
+    v = torch.randn(l, n_kv, hd, generator=g)
+    v[::7] = 0.0
+    v[64:96] = 0.0
+    v[96:112] *= 1e30
+    pc.append(0, 0, torch.randn(l, n_kv, hd, generator=g), v)
+    q = (0.3 * torch.randn(new, n_q * hd, generator=g)).to(BF)
+    out = prompt(pc, q, [start], [new], n_q, n_kv, hd, hd ** -0.5, 0)
+    want, size = fp8_cache.attention(q.double().view(new, n_q, hd)[[0, 150, 299]], *pc.held(0, l), [start + r for r in (0, 150, 299)],
+                                     hd ** -0.5, 0)
+    # 12,300 keys: eight times the keys that `allowed` counts float32 sums for
+    bound = allowed(want, size, BF, True) + 2.0 ** -10 * size
+    assert bool(((out.view(new, n_q, hd)[[0, 150, 299]] - want).abs() <= bound).all())
