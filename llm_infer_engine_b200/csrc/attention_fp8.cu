@@ -5,7 +5,8 @@
 //   o_t = sum_j w_tj v_j / sum_j w_tj,   w_tj = exp(scale q_t . k_j - max_j),   j over the keys that token t sees
 //
 // One warp per (token, query head): a key a lane for the scores, a run of columns a lane for the sum over the values. All in
-// float32; a block's two exponents multiply the score and the weight. Keys that a token does not see are not read.
+// float32; a block's two exponents multiply the score and the weight. Keys that a token does not see are not read. The sums over the
+// values are kept 2^24 smaller: of 2^16 values near the largest number there is, the sum is not infinite where the mean is none.
 #include "fp8.cuh"
 #include <math.h>
 
@@ -13,6 +14,7 @@ namespace llmie {
 
 constexpr int kPlainWarps = 4;
 constexpr int kPlainHd = 256;
+constexpr int kPlainDown = 24;
 
 template <typename T>
 __global__ void __launch_bounds__(kPlainWarps * 32)
@@ -62,7 +64,7 @@ attention_paged_fp8_kernel(const T* q, const unsigned char* k_cache, const unsig
         }
       }
       s = dot * pow2_of(clamp_exponent(k_exp[pr * kPageExps + in / kExpBlock]));
-      ev = pow2_of(clamp_exponent(v_exp[pr * kPageExps + in / kExpBlock]));
+      ev = pow2_of(clamp_exponent(v_exp[pr * kPageExps + in / kExpBlock]) - kPlainDown);
     }
     const float m_new = fmaxf(m, warp_max(s));
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
@@ -94,8 +96,8 @@ attention_paged_fp8_kernel(const T* q, const unsigned char* k_cache, const unsig
   for (int i = 0; i < kAcc / 2; ++i) {
     const int d = 2 * lane + 64 * i;
     if (d < hd) {
-      o[d] = from_f32<T>(none ? 0.f : acc[2 * i] / l);
-      o[d + 1] = from_f32<T>(none ? 0.f : acc[2 * i + 1] / l);
+      o[d] = from_f32<T>(none ? 0.f : acc[2 * i] / l * pow2_of(kPlainDown));
+      o[d + 1] = from_f32<T>(none ? 0.f : acc[2 * i + 1] / l * pow2_of(kPlainDown));
     }
   }
 }

@@ -310,3 +310,32 @@ def test_values_of_very_different_size_in_a_long_prompt(hd):
     # 12,300 keys: eight times the keys that `allowed` counts float32 sums for
     bound = allowed(want, size, BF, True) + 2.0 ** -10 * size
     assert bool(((out.view(new, n_q, hd)[[0, 150, 299]] - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("hd", [48, 64, 128])
+def test_sums_of_the_largest_values(hd, dtype):
+    """Values near the largest number that a block can hold, many of them: their mean is one of them. Tiny ones beside them in other heads."""
+    n_q, n_kv, l = 4, 2, 700
+    g = torch.Generator().manual_seed(3)
+    pc = fp8_cache.PlainCache([l], n_kv, hd, seed=4)
+    v = torch.randn(l, n_kv, hd, generator=g) * 1e-15
+    v[:, 0] = 3e38
+    v[:, 0, 1] = -1e38
+    pc.append(0, 0, 0.1 * torch.randn(l, n_kv, hd, generator=g), v)
+    q = torch.randn(1, n_q * hd, generator=g).to(dtype)
+    want, size = fp8_cache.attention(q.double().view(1, n_q, hd), *pc.held(0, l), [l - 1], hd ** -0.5, 0)
+    outs = []
+    plain = torch.empty_like(q, device=DEV)
+    ops().attention_paged_fp8(q.to(DEV), *pc.dev(), plain, i32([l - 1]), i32([0]), i32(pc.slots), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5)
+    outs.append((plain, False))
+    if dtype is BF and hd != 48:
+        for max_len in (l, 0):
+            out = torch.empty_like(plain)
+            ops().attention_decode_fp8(q.to(DEV), *pc.dev(), out, i32(pc.slots), i32([l]), pc.table.to(DEV), n_q, n_kv, hd, hd ** -0.5, 0, max_len)
+            outs.append((out, True))
+        outs.append((prompt(pc, q, [l - 1], [1], n_q, n_kv, hd, hd ** -0.5, 0), True))
+    for out, tensor_cores in outs:
+        err = (out.cpu().double().view(1, n_q, hd) - want).abs()
+        bound = allowed(want, size, dtype, tensor_cores)
+        assert bool((err <= bound).all()), (tensor_cores, float((err / bound).max()))
