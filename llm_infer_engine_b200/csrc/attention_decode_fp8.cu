@@ -493,11 +493,10 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
       }
   };
   all_lanes();
-  bool small = false;
+  unsigned least = 0xffffffffu;      // by their bits less one: without a key there is no denominator, and none is small
 #pragma unroll
-  for (int nh = 0; nh < NH; ++nh)
-    small |= (l[nh][0] < kLeastDenominator && R[nh][0] != -INFINITY) || (l[nh][1] < kLeastDenominator && R[nh][1] != -INFINITY);
-  if (__any_sync(0xffffffffu, small)) {
+  for (int nh = 0; nh < NH; ++nh) least = min(least, min(__float_as_uint(l[nh][0]) - 1u, __float_as_uint(l[nh][1]) - 1u));
+  if (__any_sync(0xffffffffu, least < __float_as_uint(kLeastDenominator) - 1u)) {
     // rare: by the scores alone (see fp8.cuh), the warp's units once more, codes straight from the cache
 #pragma unroll
     for (int nh = 0; nh < NH; ++nh) l[nh][0] = l[nh][1] = 0.f;

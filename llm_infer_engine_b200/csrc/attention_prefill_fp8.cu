@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
         tc_fence_before_sync();
         mbar_arrive(&sh.p_ready[x]);
       }
-      if (ok && l < kLeastDenominator && R != -INFINITY) by_scores();
+      if (ok && __float_as_uint(l) - 1u < __float_as_uint(kLeastDenominator) - 1u) by_scores();
       // the queries of the piece after this one are asked for while the last product runs
       const int at_end = gs + (TURNS ? 2 * (n_x - 1) + x : n_x - 1);             // this tile's last step
       gx += n_x;
