@@ -14,7 +14,8 @@
 // index stands for which column of a head is free as long as both operands agree: a lane reads 16 neighbouring codes of a key
 // (and 8 or 16 of a value), whole sectors every time, through a ring of asynchronous copies of its own.
 // W^T comes out of S^T's accumulators by one 8x8 transpose between lanes (movmatrix). Queries are brought to half precision
-// with a power of two per head (their largest number in [2^14, 2^15)), which keeps every digit of bfloat16.
+// with a power of two per head (their largest number in [2^14, 2^15)), which keeps every digit of bfloat16 (of what is above 2^-31 of the
+// head's largest number; the rest is off by 2^-39 of that at most).
 //
 // Work is cut by blocks of positions, not by sequences: all (sequence, KV head) items one after another make one line of
 // units, and every thread block takes an equal share of it, wherever it begins and ends. Lengths are read on the device, so
@@ -112,8 +113,8 @@ template <int HD, int NH> struct DfCfg {
   static constexpr int kRecord = kHeads * (HD + 2);              // floats of a partial result: sums, then bounds and denominators
 };
 // Thread blocks that an SM holds at once. (Head size 64, five instead of four, 102 registers a thread: 64 sequences of 700 to 3,900 keys
-// 34.9 us instead of 29.3; one of 517 4.75 instead of 4.4. Head size 128, two instead of three: 48 of 1,000 to 16,000 100 instead of 92.5,
-// with a third stage 94.)
+// 34.9 us where four took 29.3; one of 517 4.75 and 4.4. Head size 128, two instead of three: 48 of 1,000 to 16,000 100 and 92.5, with a
+// third stage 94. The looks at small denominators came later: 30.0 and 93.1 now.)
 template <int HD, int NH> __host__ __device__ constexpr int df_per_sm() { return HD == 64 ? (NH == 1 ? 4 : 3) : NH == 1 ? 3 : 2; }
 template <int HD, int NH> __host__ __device__ constexpr int df_large_per_sm() { return HD == 64 && NH == 1 ? 2 : 1; }
 template <int HD, int NH> constexpr int df_blocks() { return kSms * df_per_sm<HD, NH>(); }

@@ -14,19 +14,21 @@
 // R is a running bound that follows the largest s + ev of the row only when that has grown by more than 8: w stays below
 // 2^15, half precision holds it with 11 digits down to 2^-21 of the row's largest, and the sums in tensor memory have to be
 // multiplied by 2^(R - R') in few tiles only. Queries are brought to half precision with a power of two a row, which keeps
-// every digit of bfloat16. Weights go back to tensor memory as the second product's first operand.
+// every digit of bfloat16 (of what is above 2^-31 of the row's largest number; the rest is off by 2^-39 of that at most). Weights go back
+// to tensor memory as the second product's first operand.
 //
 // Work. A piece is a (sequence, tile of tokens, key/value head), or one of several equal runs of its key tiles where the step has
 // too few of them for the GPU: how many runs a sequence's tiles are cut into is worked out on the device from the lengths that
 // are there. Runs leave partial results, which a second kernel joins in order. A block per piece is launched, and a block that is
 // about to be done takes over the piece of one that has not begun (cluster launch control): keys of the next piece are converted
 // while this one's last scores are worked on, its queries are brought while its last product runs. (6 sequences of 60 to 1,500
-// tokens, head size 128, 376 pieces: 76.4 us with a block a piece, which spent 26,000 of 42,000 clocks on finding, bringing and
-// writing, 68.0 so.)
+// tokens, head size 128, steps of 128 keys: 76.4 us with a block a piece, which spent 26,000 of 42,000 clocks on finding, bringing and
+// writing, 68.0 so. With steps of 64 keys 60.0.)
 //
-// What bounds it. A step of 128 rows twice and 128 keys is 32,768 exponentials, 2,050 clocks, and takes 4,100 at head size 64 (49 us
-// for a prompt of 2,048 tokens, 32 / 8 heads: 350 TFLOP/s of products) and about 5,000 at 128, where the conversion has 32,768 codes to
-// write. Between pieces some 9,000 clocks pass at head size 128 for results, queries and the first scores.
+// What bounds it. At head size 64 a step of 128 rows twice and 128 keys is 32,768 exponentials, 2,050 clocks, and takes 4,100 (48.2 us
+// for a prompt of 2,048 tokens, 32 / 8 heads: 357 TFLOP/s of products); what the other half goes into is not broken down. At 128 a step has 64
+// keys, 16,384 exponentials and as many codes to convert, and takes 2,500. Between pieces some 9,000 clocks pass at head size 128 for
+// results, queries and the first scores.
 //
 // Code. What a block does once is written in loops that stay loops, and each search for work is there once: a kernel of 140 to 250 KB
 // of instructions, as the compiler lays them out by itself, spends thousands of clocks a piece on fetching them.
@@ -186,8 +188,8 @@ __device__ __forceinline__ int pf_runs(int last, int run) { return run < 0 ? max
 // if one of its tiles alone would hold up the step.
 // How many runs come of it: in the first case at most 148. In the second a sequence that is cut has last >= 1.5 run, so at most
 // 4/3 last / run runs, and at most last / run of them more than tiles; and last <= first + last, whose sum is 2 T. So all cut
-// sequences have 4/3 148 < kPfSlots runs, and 148 more than tiles. The search goes on to 16 T / 148, where there are 18 more than
-// tiles: up to kPfFew it finds one.
+// sequences have 4/3 148 < kPfSlots runs, and 148 more than tiles. The search goes on beyond 15 T / 148, where there are 19 more than
+// tiles at most: up to kPfFew it finds one.
 // Where the host has counted on whole tiles (a.run 0), they stay whole, whatever the lengths are: there is no scratch then, no join, and a
 // block for each tile. It judges by the rows of the step, of which the sequences may have few.
 // `mine`: the lane's first sequence. All lanes of a warp call it, and every block gets the same answer.
@@ -210,7 +212,7 @@ template <int KEYS> __device__ __forceinline__ int pf_run(const PrefillArgs& a, 
   if ((int)__reduce_add_sync(0xffffffffu, (unsigned)tiles) * a.n_kv > kPfSms) return most;
   int run = max(a.run, max(kPfLeast / KEYS, (int)fminf(ceilf(share * 0.5f), 1e9f)));
 #pragma unroll 1
-  for (int i = 0; i < 24; ++i, run += (run + 7) / 8) {                       // (9/8)^24 > 16
+  for (int i = 0; i < 24; ++i, run += (run + 7) / 8) {                       // the last is (9/8)^23 > 15 times the first
     unsigned runs = mine.tiles * pf_runs(mine.last, -run);
 #pragma unroll 1
     for (int s = lane + 32; s < a.n_seqs; s += 32) {
@@ -524,7 +526,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
       auto nan_values = [&](int step) {
         if (sh.v_nan[step % kPfRing] != step + 1) return;
         const int kbase = (c0 + step - gs) * Cfg::kKeys;
-      // rare: which columns of the values that this row sees are NaN
         const int* pages = a.block_table + (size_t)w.page_row * a.max_pages;
         const int last_key = w.last_key;
 #pragma unroll 1
@@ -539,7 +540,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_fp8_kernel(const Prefil
           }
         }
       };
-      // Rare: the row's denominator by the scores alone (see fp8.cuh), four keys at a time: some 500 clocks a key, and the block waits.
+      // Rare: the row's denominator by the scores alone (see fp8.cuh), four keys at a time, while the rest of the block waits: 800 clocks a
+      // key at head size 64, 1,300 at 128 (2,048 tokens 0.9 and 2.2 ms; the waits' limit is reached behind more than a million keys).
       auto by_scores = [&]() {
         const int row = row_of(w);
         if (row < 0) return;

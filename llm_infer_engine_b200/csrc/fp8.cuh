@@ -3,10 +3,11 @@
 // A number x of a block is held as the code c = e4m3(x 2^-e), to the nearest and ties to even, and read as c 2^e. The block's
 // exponent e is the smallest in [kExpMin, kExpMax] with (largest finite magnitude of the block) 2^-e <= 448, the largest
 // e4m3 number. Why a power of two: multiplying by 2^-e rounds nothing, so a number is rounded once; a block whose exponent
-// has to rise for a later position keeps its codes' digits (a code shifted down rounds again only where it falls below
-// 2^-6, under 2^-14 of the block's largest number); and attention takes a block's scale as an addend of exponents.
-// The relative error of a number is at most 2^-4 (half a step of 3 digits) as long as it is within 2^-14 of its block's
-// largest. What is not finite is held as the code NaN, so that it shows; it does not enter the block's exponent.
+// has to rise for a later position keeps its codes' digits (a code shifted down rounds a second time only where it falls below
+// 2^-6, the smallest normal one, under 2^-13 of the block's largest number); and attention takes a block's scale as an addend of exponents.
+// The relative error of a number is at most 2^-4 (half a step of 3 digits) as long as it is within 2^-13 of its block's
+// largest, whose code is above 224. A smaller one is off by at most 2^-10 2^e, half the smallest step, and by as much again where an
+// exponent rose over it. What is not finite is held as the code NaN, so that it shows; it does not enter the block's exponent.
 #pragma once
 #include "common.cuh"
 #include <cuda_fp16.h>
@@ -83,7 +84,7 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(unsigned short c) {
   const unsigned h = e4m3x2_to_half2(c);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// Four codes moved from a block exponent to one that is `down` (>= 0) higher.
+// Four codes times `factor`, a power of two of 1 at most: moved to a block exponent that is higher.
 __device__ __forceinline__ unsigned lower_codes(unsigned w, float factor) {
   const float2 a = e4m3x2_to_float2((unsigned short)(w & 0xffffu)), b = e4m3x2_to_float2((unsigned short)(w >> 16));
   return (unsigned)to_e4m3x2(a.x * factor, a.y * factor) | ((unsigned)to_e4m3x2(b.x * factor, b.y * factor) << 16);

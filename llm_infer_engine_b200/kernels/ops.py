@@ -1627,7 +1627,6 @@ def latent_prepare(proj, q_off: int, dkv_off: int, q_out, cache, norm_w, eps: fl
     return q_out
 
 
-# ------------------------------------------------------------------------------------------ attention by rows
 # ------------------------------------------------------------------------------------------ a cache in 8 bits
 FP8 = torch.float8_e4m3fn
 FP8_PAGE = 64            # positions of a page
@@ -1893,8 +1892,9 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     """Causal attention of runs of new tokens over a paged cache in 8 bits, on the tcgen05 tensor cores: q, out bfloat16
     [T, n_q hd] with the sequences packed (cu_q int32 [n + 1]), the cache as in rope_store_fp8 (it holds the step's keys and
     values already), seq_start int32 [n] the tokens each sequence held before this step, window as in attention_paged.
-    head_dim 64 or 128, scale > 0. max_q_len: no sequence brings more. Rows behind the last sequence stay as they are. Where a block's
-    waits run out, rows are left NaN or as they were, and check_tc_status raises."""
+    head_dim 64 or 128, scale > 0. max_q_len: no sequence brings more. Rows behind the last sequence stay as they are, but the work is
+    cut among the SMs as if they were tokens: a step of mostly such rows may take longer than one without. Where a block's waits run
+    out, rows are left NaN or as they were, and check_tc_status raises."""
     name = "attention_prefill_fp8"
     _need_heads(name, n_q, n_kv)
     if not attention_prefill_fp8_supported(n_q, n_kv, head_dim, q.dtype):
@@ -1925,6 +1925,7 @@ def attention_prefill_fp8(q, k_cache, v_cache, k_exp, v_exp, out, cu_q, seq_slot
     return out
 
 
+# ------------------------------------------------------------------------------------------ attention by rows
 def attention_rows_mma_supported(head_dim: int, v_head_dim: int, page_size: int, dtype: torch.dtype,
                                  shared_rows: bool) -> bool:
     """The sizes attention_rows_mma.cu takes (answered without loading the library): bfloat16, a head size that is a
