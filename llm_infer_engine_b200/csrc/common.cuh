@@ -120,10 +120,10 @@ __device__ __forceinline__ float gated_pair(float g, float u, const GateForm& f)
 
 // The first key a token at position `pos` may see, by the `window` argument of the attention kernels: 0 = every earlier
 // key; n > 0 = the last n keys, its own included; -n < 0 = the keys of its own chunk of n positions (chunks counted from
-// position 0 of the sequence).
+// position 0 of the sequence). A position below zero (a lane without a sequence) sees none: the answer is above it, never below 0.
 __device__ __forceinline__ int first_visible_key(int pos, int window) {
   if (window > 0) return max(pos - window + 1, 0);
-  if (window < 0) return pos - pos % -window;
+  if (window < 0) return max(pos - pos % -window, 0);
   return 0;
 }
 

@@ -1757,7 +1757,8 @@ def rope_store_fp8(qkv, q_out, k_cache, v_cache, k_exp, v_exp, table, cu_q, seq_
 def attention_paged_fp8(q, k_cache, v_cache, k_exp, v_exp, out, tok_pos, tok_seq, seq_slot, block_table, n_q: int, n_kv: int,
                         head_dim: int, scale: float, window: int = 0):
     """Plain attention over a paged cache in 8 bits, one warp per (token, query head): q, out [T, n_q hd] float32 or bfloat16,
-    the cache as in rope_store_fp8, the rest as in attention_paged. Every head size that is a multiple of 16 up to 256."""
+    the cache as in rope_store_fp8, the rest as in attention_paged. Every head size that is a multiple of 16 up to 256. A token at a
+    position below 0 sees no key: its rows of out become zeros."""
     name = "attention_paged_fp8"
     _need_heads(name, n_q, n_kv)
     index = _index_of(name, q)

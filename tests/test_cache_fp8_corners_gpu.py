@@ -339,3 +339,18 @@ def test_sums_of_the_largest_values(hd, dtype):
         err = (out.cpu().double().view(1, n_q, hd) - want).abs()
         bound = allowed(want, size, dtype, tensor_cores)
         assert bool((err <= bound).all()), (tensor_cores, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("window", [0, 1, 40, -1, -2, -3, -64])
+def test_positions_below_zero_see_no_key(window):
+    """A lane without a sequence, in the plain kernel: zeros, whatever the window or chunk, and nothing in front of its page is read."""
+    n_q, n_kv, hd, pos = 4, 2, 64, [-1, -2, -6, -64, 5]
+    pc = filled([20], n_kv, hd, seed=1, nan_stale=False)
+    pc.table[pc.slots[0], 0] = 0                       # the first page that there is: before it is nothing
+    q = torch.randn(len(pos), n_q * hd, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = torch.full((len(pos), n_q * hd), float("nan"), dtype=BF, device=DEV)
+    ops().attention_paged_fp8(q.to(DEV), *pc.dev(), out, i32(pos), i32([0] * len(pos)), i32(pc.slots), pc.table.to(DEV), n_q, n_kv, hd, 0.125,
+                              window)
+    assert bool((out[:4] == 0).all())
+    want, size = fp8_cache.attention(q[4:].double().view(1, n_q, hd), *pc.held(0, 20), [5], 0.125, window)
+    assert bool(((out[4:].cpu().double().view(1, n_q, hd) - want).abs() <= allowed(want, size, BF, False)).all())
