@@ -523,15 +523,11 @@ __device__ __forceinline__ void df_piece(const __nv_bfloat16* q, const DecodeArg
         for (int nh = 0; nh < NH; ++nh) {
           const float f0 = df_finite(q_scale[nh][0] * kf), f1 = df_finite(q_scale[nh][1] * kf);
           const float c0 = kDfTop - (R[nh][0] == -INFINITY ? 0.f : R[nh][0]), c1 = kDfTop - (R[nh][1] == -INFINITY ? 0.f : R[nh][1]);
-          if (p >= lo && p < len) {
-            l[nh][0] += exp2_term(fmaf(x[nh][0], f0, c0));
-            l[nh][1] += exp2_term(fmaf(x[nh][1], f1, c1));
-          }
-          if (p + 8 >= lo && p + 8 < len) {
-            l[nh][0] += exp2_term(fmaf(x[nh][2], f0, c0));
-            l[nh][1] += exp2_term(fmaf(x[nh][3], f1, c1));
-          }
+          const bool here = p >= lo && p < len, there = p + 8 >= lo && p + 8 < len;
+          l[nh][0] += (here ? exp2_term(fmaf(x[nh][0], f0, c0)) : 0.f) + (there ? exp2_term(fmaf(x[nh][2], f0, c0)) : 0.f);
+          l[nh][1] += (here ? exp2_term(fmaf(x[nh][1], f1, c1)) : 0.f) + (there ? exp2_term(fmaf(x[nh][3], f1, c1)) : 0.f);
         }
+        __syncwarp();                // the products are the whole warp's
       }
     }
     all_lanes();
