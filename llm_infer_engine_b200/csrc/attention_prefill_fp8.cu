@@ -191,7 +191,7 @@ __device__ __forceinline__ int pf_runs(int last, int run) { return run < 0 ? max
 // sequences have 4/3 148 < kPfSlots runs, and 148 more than tiles. The search goes on beyond 15 T / 148, where there are 19 more than
 // tiles at most: up to kPfFew it finds one.
 // Where the host has counted on whole tiles (a.run 0), they stay whole, whatever the lengths are: there is no scratch then, no join, and a
-// block for each tile. It judges by the rows of the step, of which the sequences may have few.
+// block for each tile. It goes by the rows of the step, of which the sequences may have few.
 // `mine`: the lane's first sequence. All lanes of a warp call it, and every block gets the same answer.
 template <int KEYS> __device__ __forceinline__ int pf_run(const PrefillArgs& a, int tok, const PfSequence& mine) {
   const int lane = threadIdx.x & 31;
